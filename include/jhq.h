@@ -47,7 +47,10 @@ enum {
 enum {
     JHQ_F32 = 0, /* float32                                   */
     JHQ_U8 = 1,  /* uint8, converted to float32 (0..255)      */
-    JHQ_I8 = 2   /* int8, converted to float32 (-128..127)    */
+    JHQ_I8 = 2,  /* int8, converted to float32 (-128..127)    */
+    /* the key/value cache's rows (jhq_k_kv_*), beside JHQ_F32 */
+    JHQ_BF16 = 3, /* bfloat16                                 */
+    JHQ_F16 = 4   /* float16                                  */
 };
 
 typedef struct jhq_index jhq_index;
@@ -347,6 +350,96 @@ int jhq_k_final_topk(const float* d_comp_dists, const int32_t* d_topck_pos,
 int jhq_k_assign_noalloc(const float* d_y, int64_t n, int d, const float* d_cent,
                          const float* d_cent_norms, int nlist, int32_t* d_assign,
                          void* stream);
+
+/* ---- key/value cache of attention, 8 or 4 bits (no counterpart in the
+ * reference) ----
+ *
+ * A paged cache of keys and values: one device buffer of jhq_kv_bytes() bytes
+ * (16-byte aligned, the caller's), cut into num_pages pages of page_size tokens,
+ * each with the keys and values of every key/value head.  A row x (a token's key
+ * or value in one head) is held as head_dim codes and one float32 scale: with
+ * top = 127 (8 bits) or 7 (4 bits) and amax = max |x_d|,
+ *   code_d = round_half_even(top * x_d / amax), scale = amax / top;
+ *   amax < 2^-60: every code and the scale 0;
+ *   x with an infinity or a NaN: every code 0 and the scale NaN (the row reads
+ *   back as NaN and makes NaN of what attends to it, and of nothing else).
+ * For bfloat16 and float16 rows the codes are those of exact arithmetic.
+ *
+ * Inside, a page is kv_heads blocks of
+ *   key codes | value codes | key scales | value scales
+ * and codes stand in groups of 16 tokens: keys as 16-byte pieces of one token,
+ * [piece][token][16], values as 16 tokens of one element, [element][token], so
+ * that matrix instructions take both from memory as they are.  With 4 bits a
+ * byte holds elements e (low) and e + head_dim/2 (high). */
+typedef struct {
+    int     bits;      /* 8 or 4                                              */
+    int     kv_heads;  /* key/value heads, 1 .. 1024                          */
+    int     head_dim;  /* 64, 128 or 256                                      */
+    int     page_size; /* tokens of a page: a power of two, 16 .. 1024        */
+    int64_t num_pages; /* pages in the buffer, at most 2^31 - 1               */
+} jhq_kv_params;
+
+/* The sequences that a call works on.  Sequence b holds kv_len[b] tokens, token
+ * j in page pages[b][j / page_size] at place j % page_size; the last
+ * cu_q[b+1] - cu_q[b] of them are its new tokens, rows cu_q[b] .. of the call's
+ * arrays (cu_q[0] >= 0, ascending, cu_q[n_seq] <= n_tokens).  A sequence may
+ * have no new token, or no token at all.  The arrays are device memory, read
+ * when the kernels run; max_q and max_kv, the host's bounds on the new tokens
+ * and tokens of one sequence, size the launch.
+ * What a bound, the page table or cu_q contradicts is not touched: a token
+ * whose page is none of the buffer's is not written, reads back as NaN and
+ * counts as NaN where it is attended to; a sequence with more tokens than
+ * max_kv or its pages, or more new ones than max_q, is not written and its
+ * rows (the first max_q of them) read back and come out as NaN. */
+typedef struct {
+    int            n_seq;     /* sequences                                     */
+    int            max_pages; /* entries of a row of pages                     */
+    const int32_t* d_pages;   /* [n_seq][max_pages]                            */
+    const int32_t* d_kv_len;  /* [n_seq]                                       */
+    const int32_t* d_cu_q;    /* [n_seq + 1]                                   */
+    int64_t        n_tokens;  /* rows of the call's arrays                     */
+    int            max_q;     /* no sequence has more new tokens               */
+    int            max_kv;    /* no sequence has more tokens                   */
+} jhq_kv_batch;
+
+/* Bytes of a cache; 0 and a message where the parameters are not valid. */
+int64_t jhq_kv_bytes(const jhq_kv_params* p);
+
+/* Quantises the new tokens' keys and values into the cache.  d_k, d_v: element
+ * (t, h, e) at t * tok + h * head + e, strides in elements, dtype JHQ_F32,
+ * JHQ_BF16 or JHQ_F16.  Writes those tokens' codes and scales and nothing else. */
+int jhq_k_kv_write(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, const void* d_k,
+                   int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok, int64_t v_head,
+                   int dtype, void* stream);
+
+/* Reads the new tokens' keys and values back: code * scale in float32, rounded
+ * once to dtype; d_k, d_v [n_tokens][kv_heads][head_dim] contiguous (NULL: not
+ * wanted).  A batch whose new tokens are all tokens (cu_q the running sum of
+ * kv_len) reads whole sequences.  Rows of new tokens before position 0 (more
+ * new tokens than tokens) and rows outside cu_q are left alone. */
+int jhq_k_kv_read(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b, void* d_k,
+                  void* d_v, int dtype, void* stream);
+
+/* Device memory that jhq_k_kv_attend needs for this batch (0: none; -1 and a
+ * message where an argument is not valid). */
+int64_t jhq_kv_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_heads, int window);
+
+/* Attention of the new tokens, which the cache already holds, to their
+ * sequences.  New token i of q in a sequence of n tokens stands at position
+ * n - q + i; it sees every token (causal 0), those up to its own position
+ * (causal 1), or the last `window` of those (causal 1, window > 0; 0: no
+ * window).  Query head h reads key/value head h / (q_heads / kv_heads):
+ *   out = sum_j w_j v_j,  w = softmax_j(scale * <q, k_j>),
+ *   lse = ln sum_j exp(scale * <q, k_j>)
+ * a row that sees nothing gives 0 and -inf.  d_q as d_k above, dtype JHQ_BF16
+ * or JHQ_F16; d_out [n_tokens][q_heads][head_dim] contiguous in the same type;
+ * d_lse [n_tokens][q_heads] float32 or NULL.  d_work: work_bytes >=
+ * jhq_kv_work_bytes() bytes, 16-byte aligned, this call's alone until its
+ * kernels have run (its contents before do not matter). */
+int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
+                    const void* d_q, int64_t q_tok, int64_t q_head, int q_heads, int dtype,
+                    float scale, int causal, int window, void* d_out, float* d_lse, void* d_work,
+                    int64_t work_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,7 +20,7 @@ __all__ = [
     "Params", "JHQGpuIndex", "JHQError", "JHQDeviceError", "JHQNotBuiltError",
     "lib", "lib_path", "k_rotate", "k_primary_encode", "k_residual_encode", "k_assign",
     "k_assign_noalloc", "k_build_lut", "k_scan_topck", "k_refine", "k_final_topk",
-    "STEP_NAMES",
+    "STEP_NAMES", "KVCache", "KVBatch",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -74,9 +74,25 @@ class Params:
                        self.residual_per_subspace)
 
 
+class _KvParams(ctypes.Structure):
+    _fields_ = [
+        ("bits", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+        ("page_size", ctypes.c_int), ("num_pages", ctypes.c_int64),
+    ]
+
+
+class _KvBatch(ctypes.Structure):
+    _fields_ = [
+        ("n_seq", ctypes.c_int), ("max_pages", ctypes.c_int), ("d_pages", ctypes.c_void_p),
+        ("d_kv_len", ctypes.c_void_p), ("d_cu_q", ctypes.c_void_p), ("n_tokens", ctypes.c_int64),
+        ("max_q", ctypes.c_int), ("max_kv", ctypes.c_int),
+    ]
+
+
 _VP = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
+_KVP, _KVB = ctypes.POINTER(_KvParams), ctypes.POINTER(_KvBatch)
 
 _SIGS = {
     "jhq_params_default": (None, [ctypes.POINTER(_Params)]),
@@ -122,6 +138,12 @@ _SIGS = {
     "jhq_k_scan_topck": (_I, [_VP] * 8 + [_I, _I, _I, _I64, _I, _VP]),
     "jhq_k_refine": (_I, [_VP] * 7 + [_I] * 6 + [_VP]),
     "jhq_k_final_topk": (_I, [_VP] * 5 + [_I, _I, _I, _VP]),
+    "jhq_kv_bytes": (_I64, [_KVP]),
+    "jhq_kv_work_bytes": (_I64, [_KVP, _KVB, _I, _I]),
+    "jhq_k_kv_write": (_I, [_KVP, _VP, _KVB, _VP, _I64, _I64, _VP, _I64, _I64, _I, _VP]),
+    "jhq_k_kv_read": (_I, [_KVP, _VP, _KVB, _VP, _VP, _I, _VP]),
+    "jhq_k_kv_attend": (_I, [_KVP, _VP, _KVB, _VP, _I64, _I64, _I, _I, ctypes.c_float, _I, _I, _VP,
+                             _VP, _VP, _I64, _VP]),
 }
 
 
@@ -482,3 +504,6 @@ def k_final_topk(comp, topck_pos, list_ids, final_dists, final_ids, stream=None)
     _check(lib().jhq_k_final_topk(_dptr(comp), _dptr(topck_pos), _dptr(list_ids),
                                   _dptr(final_dists), _dptr(final_ids), int(B), int(ck), k,
                                   _stream(stream)))
+
+
+from .kv import KVBatch, KVCache  # noqa: E402  (after the names it uses)

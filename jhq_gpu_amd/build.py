@@ -35,7 +35,8 @@ def _run(cmd):
 
 def build_engine(verbose=False):
     """Compile kernels.hip, jhq_capi.hip, gemm_chain.hip, insert.hip, kmeans.hip,
-    noalloc.hip, assign_mfma.hip and host_train.cpp into libjhq_amd.so."""
+    noalloc.hip, assign_mfma.hip, kvcache.hip, kv_attend.hip and host_train.cpp
+    into libjhq_amd.so."""
     os.makedirs(BUILD, exist_ok=True)
     jobs = [
         ([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, "kernels.hip"),
@@ -52,6 +53,10 @@ def build_engine(verbose=False):
                                 "-o", os.path.join(BUILD, "noalloc.o")]),
         ([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, "assign_mfma.hip"),
                                 "-o", os.path.join(BUILD, "assign_mfma.o")]),
+        ([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, "kvcache.hip"),
+                                "-o", os.path.join(BUILD, "kvcache.o")]),
+        ([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, "kv_attend.hip"),
+                                "-o", os.path.join(BUILD, "kv_attend.o")]),
         (["g++"] + CXX_FLAGS + ["-c", os.path.join(CSRC, "host_train.cpp"),
                                 "-o", os.path.join(BUILD, "host_train.o")]),
     ]
@@ -72,7 +77,8 @@ def build_engine(verbose=False):
           os.path.join(BUILD, "kernels.o"), os.path.join(BUILD, "jhq_capi.o"),
           os.path.join(BUILD, "gemm_chain.o"),
           os.path.join(BUILD, "insert.o"), os.path.join(BUILD, "kmeans.o"), os.path.join(BUILD, "noalloc.o"),
-          os.path.join(BUILD, "assign_mfma.o"), os.path.join(BUILD, "host_train.o")])
+          os.path.join(BUILD, "assign_mfma.o"), os.path.join(BUILD, "kvcache.o"),
+          os.path.join(BUILD, "kv_attend.o"), os.path.join(BUILD, "host_train.o")])
     os.replace(tmp, LIB)
     return LIB
 

@@ -1,0 +1,617 @@
+// kvcache.hip — the quantised key/value cache: its entry points (jhq_kv_*,
+// jhq_k_kv_*), quantising rows into it and reading them back.
+//
+// Both directions are copies with a few operations per element, bound by HBM.
+// One wave takes a group of 16 tokens (32 where a row has only two 16-byte
+// pieces) of one head, keys or values: LP lanes a token, each with the pieces
+// c, c + LP, ... of its row, so that a row's largest magnitude is a maximum over
+// neighbouring lanes and keys leave as they are, 16 bytes a lane.  Values are
+// stored token-minor ([element][token]); their 16 x 16 byte tiles are turned
+// in LDS (words by 4 x 4 byte transposes), so they also leave 16 bytes a lane.
+#include "kvcache.h"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+// Defined in jhq_capi.hip: sets the thread-local message jhq_last_error returns.
+int jhq_set_error(int code, const char* msg);
+
+namespace jhq {
+namespace {
+
+constexpr int kWaves = 4;          // waves of a workgroup, each on its own
+constexpr int kTilePitch = 272;    // bytes from one 16 x 16 tile to the next: 16 apart in the banks
+constexpr float kFloor = 0x1p-60f; // rows below it are held as zeros
+
+// Lanes per token and tokens per wave for NP 16-byte pieces a row.
+template <int NP>
+struct Lanes {
+    static constexpr int LP = NP < 4 ? NP : 4;
+    static constexpr int TW = 64 / LP;
+    static constexpr int IT = NP / LP;  // pieces per lane
+};
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// The values of 16 elements at src, as float.
+template <int DT, bool VEC>
+__device__ inline void load16(const void* base, int64_t i, float* x) {
+    if constexpr (DT == JHQ_F32) {
+        const float* p = static_cast<const float*>(base) + i;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float4 f = reinterpret_cast<const float4*>(p)[w];
+                x[4 * w] = f.x, x[4 * w + 1] = f.y, x[4 * w + 2] = f.z, x[4 * w + 3] = f.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[j] = p[j];
+        }
+    } else {
+        const uint16_t* p = static_cast<const uint16_t*>(base) + i;
+        uint16_t h[16];
+        if constexpr (VEC) {
+            const u32x4 a = reinterpret_cast<const u32x4*>(p)[0];
+            const u32x4 b = reinterpret_cast<const u32x4*>(p)[1];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                h[2 * j] = a[j] & 0xffff, h[2 * j + 1] = a[j] >> 16;
+                h[8 + 2 * j] = b[j] & 0xffff, h[9 + 2 * j] = b[j] >> 16;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) h[j] = p[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            x[j] = DT == JHQ_BF16 ? __uint_as_float(static_cast<uint32_t>(h[j]) << 16)
+                                  : static_cast<float>(__builtin_bit_cast(_Float16, h[j]));
+    }
+}
+
+template <int DT>
+__device__ inline uint32_t round16(float f) {
+    if constexpr (DT == JHQ_BF16)
+        return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f));
+    else
+        return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
+}
+
+template <int DT, bool VEC>
+__device__ inline void store16(void* base, int64_t i, const float* x) {
+    if constexpr (DT == JHQ_F32) {
+        float* p = static_cast<float*>(base) + i;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int w = 0; w < 4; w++)
+                reinterpret_cast<float4*>(p)[w] =
+                    make_float4(x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) p[j] = x[j];
+        }
+    } else {
+        uint16_t* p = static_cast<uint16_t*>(base) + i;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                u32x4 o;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    o[j] = round16<DT>(x[8 * w + 2 * j]) | round16<DT>(x[8 * w + 2 * j + 1]) << 16;
+                reinterpret_cast<u32x4*>(p)[w] = o;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) p[j] = static_cast<uint16_t>(round16<DT>(x[j]));
+        }
+    }
+}
+
+// Orders a wave's LDS accesses before and after it (one wave: they execute in
+// program order, the compiler only has to keep it).
+__device__ inline void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Row i of m (4 bytes) becomes column i.
+__device__ inline void transpose4(uint32_t m[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(m[1], m[0], 0x05010400);
+    const uint32_t b = __builtin_amdgcn_perm(m[3], m[2], 0x05010400);
+    const uint32_t c = __builtin_amdgcn_perm(m[1], m[0], 0x07030602);
+    const uint32_t d = __builtin_amdgcn_perm(m[3], m[2], 0x07030602);
+    m[0] = __builtin_amdgcn_perm(b, a, 0x05040100);
+    m[1] = __builtin_amdgcn_perm(b, a, 0x07060302);
+    m[2] = __builtin_amdgcn_perm(d, c, 0x05040100);
+    m[3] = __builtin_amdgcn_perm(d, c, 0x07060302);
+}
+
+// Four 16 x 16 byte tiles of a wave, transposed through tile (4 * kTilePitch
+// bytes of LDS, this wave's): lane holds row `in` of tile `tin`, gets row
+// lane % 16 of tile lane / 16 (or the other way round: both are 16-byte rows).
+__device__ inline u32x4 transpose16(uint8_t* tile, int lane, int tin, int rin, int tout, int rout,
+                                    u32x4 w) {
+    *reinterpret_cast<u32x4*>(tile + tin * kTilePitch + rin * 16) = w;
+    wave_lds_fence();
+    uint8_t* const t = tile + (lane >> 4) * kTilePitch;
+    const int r = (lane & 3) * 4, c = ((lane >> 2) & 3) * 4;
+    uint32_t m[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) m[i] = *reinterpret_cast<const uint32_t*>(t + (r + i) * 16 + c);
+    wave_lds_fence();
+    transpose4(m);
+#pragma unroll
+    for (int i = 0; i < 4; i++) *reinterpret_cast<uint32_t*>(t + (c + i) * 16 + r) = m[i];
+    wave_lds_fence();
+    const u32x4 o = *reinterpret_cast<const u32x4*>(tile + tout * kTilePitch + rout * 16);
+    wave_lds_fence();
+    return o;
+}
+
+// What one wave works on: a run of TW tokens from `first`, one head, keys or
+// values.
+struct Unit {
+    KvSeq q;
+    int seq, head, value;
+    int first, lo;  // first token of the run; first new token (not below 0)
+    bool any;
+};
+
+template <int TW>
+__device__ inline Unit unit_of(const KvCache& c, const KvBatch& b, int64_t u, int sets) {
+    Unit r;
+    r.value = static_cast<int>(u & 1);
+    u >>= 1;
+    r.head = static_cast<int>(u % c.H);
+    u /= c.H;
+    const int set = static_cast<int>(u % sets);
+    r.seq = static_cast<int>(u / sets);
+    r.any = r.seq < b.n_seq;
+    if (!r.any) return r;
+    r.q = kv_seq(b, r.seq, c.shift);
+    r.lo = max(r.q.n - r.q.q, 0);
+    r.first = (r.lo / kKvGroup) * kKvGroup + set * TW;
+    r.any = r.q.q > 0 && (r.first < r.q.n || !r.q.ok);
+    return r;
+}
+
+// The page of token j's group (groups do not straddle pages), or -1; the
+// sequence is ok, so every position below n is in the table.
+__device__ inline int group_page(const KvCache& c, const KvBatch& b, const Unit& u, int j) {
+    const int g = j & ~(kKvGroup - 1);
+    return g < u.q.n ? kv_page(b, c, u.seq, g) : -1;
+}
+
+// What a lane of a transposed unit holds: a byte column of piece `piece` (and
+// its later pieces) of token group `group` of the run, and which of that
+// group's tokens are to be moved.
+struct Column {
+    int group, piece;
+    uint32_t mask;
+};
+
+template <int LP>
+__device__ inline Column column_of(int lane, bool live) {
+    Column r;
+    r.group = (lane >> 4) / LP;
+    r.piece = (lane >> 4) % LP;
+    const uint64_t m = __ballot(live);
+    r.mask = 0;
+#pragma unroll
+    for (int t = 0; t < 16; t++)
+        r.mask |= static_cast<uint32_t>(m >> ((r.group * 16 + t) * LP) & 1) << t;
+    return r;
+}
+
+// rne(top x / amax) of one row's elements held by a lane.  x * top is exact
+// for 16-bit x and the quotient, corrected once by its remainder, is within one
+// unit of 2^-24: a quotient half way between codes comes out exactly (it is
+// representable and the remainder is exact), and any other is further from
+// half way than that, both sides of the comparison being 19-bit integers in
+// one unit.  Adding 1.5 * 2^23 rounds half to even and leaves the code in the
+// low bits.
+template <int BITS>
+__device__ inline uint32_t code_of(float x, float topf, float a, float inv) {
+    const float y = x * topf;
+    const float q0 = y * inv;
+    const float q = fmaf(fmaf(-q0, a, y), inv, q0);
+    return __float_as_uint(q + (12582912.0f + (BITS == 8 ? 128.0f : 8.0f)));
+}
+
+// HBM-bound: reads 2 T H D elements, writes half (8 bits) or a quarter of that
+// in 16-bit types.
+template <int BITS, int D, int DT, bool VEC>
+__global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatch b, KvRows kr,
+                                                               KvRows vr, int sets) {
+    constexpr int ROW = D * BITS / 8, NP = ROW / 16;
+    using L = Lanes<NP>;
+    constexpr int E = BITS == 8 ? 16 : 32;  // elements in a piece
+    __shared__ __align__(16) uint8_t lds[kWaves][4 * kTilePitch];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Unit u = unit_of<L::TW>(c, b, static_cast<int64_t>(blockIdx.x) * kWaves + wave, sets);
+    if (!u.any || !u.q.ok) return;  // wave-uniform; the waves share nothing
+    const int t = lane / L::LP, lc = lane % L::LP;
+    const int j = u.first + t;
+    const int page = group_page(c, b, u, j);
+    const bool live = j >= u.lo && j < u.q.n && page >= 0;
+    const KvRows src = u.value ? vr : kr;
+    const int64_t at = (u.q.row + (j - (u.q.n - u.q.q))) * src.tok + u.head * src.head;
+
+    float x[L::IT][E];
+#pragma unroll
+    for (int i = 0; i < L::IT; i++) {
+        const int e = (lc + i * L::LP) * 16;
+#pragma unroll
+        for (int w = 0; w < E; w++) x[i][w] = 0.0f;
+        if (live) {
+            load16<DT, VEC>(src.p, at + e, x[i]);
+            if constexpr (BITS == 4) load16<DT, VEC>(src.p, at + D / 2 + e, x[i] + 16);
+        }
+    }
+    // |x| as an integer: infinities and NaN are the largest
+    int mag = 0;
+#pragma unroll
+    for (int i = 0; i < L::IT; i++)
+#pragma unroll
+        for (int w = 0; w < E; w++) mag = max(mag, __float_as_int(x[i][w]) & 0x7fffffff);
+#pragma unroll
+    for (int o = 1; o < L::LP; o <<= 1) mag = max(mag, __shfl_xor(mag, o));
+    constexpr float top = BITS == 8 ? 127.0f : 7.0f;
+    const float amax = __int_as_float(mag);
+    const bool finite = mag < 0x7f800000, held = finite && amax >= kFloor;
+    // top * x must not overflow: very large rows are scaled by 2^-64 first
+    const float f = amax > 0x1p100f ? 0x1p-64f : 1.0f;
+    const float a = held ? amax * f : 1.0f, inv = 1.0f / a, topf = held ? top * f : 0.0f;
+    const float scale = held ? amax / top : finite ? 0.0f : __uint_as_float(0x7fc00000u);
+
+    uint8_t* const blk = kv_block(c, max(page, 0), u.head);
+    uint8_t* const codes = blk + (u.value ? c.codes : 0);
+    const int in_page = (1 << c.shift) - 1, slot = j & in_page;
+    if (live && lc == 0)
+        reinterpret_cast<float*>(blk + 2 * c.codes)[(u.value << c.shift) + slot] = scale;
+    // Values: after the transpose a lane holds one byte column of 16 tokens, of
+    // which it may write those that are new.
+    const Column o = column_of<L::LP>(lane, live && lc == 0);
+    const int opage = __shfl(page, o.group * 16 * L::LP);
+    uint8_t* const ocodes = kv_block(c, max(opage, 0), u.head) + c.codes +
+                            ((u.first + o.group * 16) & in_page) * ROW;
+#pragma unroll
+    for (int i = 0; i < L::IT; i++) {
+        u32x4 w;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            uint32_t d[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                d[e] = code_of<BITS>(x[i][4 * k + e], topf, a, inv);
+                if constexpr (BITS == 4)
+                    d[e] = (d[e] & 15u) | code_of<4>(x[i][16 + 4 * k + e], topf, a, inv) << 4;
+            }
+            const uint32_t p01 = __builtin_amdgcn_perm(d[1], d[0], 0x0c0c0400);
+            const uint32_t p23 = __builtin_amdgcn_perm(d[3], d[2], 0x0c0c0400);
+            w[k] = finite ? p01 | p23 << 16 : BITS == 8 ? 0x80808080u : 0x88888888u;
+        }
+        if (!u.value) {
+            if (live)
+                *reinterpret_cast<u32x4*>(codes + (slot & ~15) * ROW + (lc + i * L::LP) * 256 +
+                                          (slot & 15) * 16) = w;
+            continue;
+        }
+        w = transpose16(lds[wave], lane, (t >> 4) * L::LP + lc, t & 15, lane >> 4, lane & 15, w);
+        uint8_t* const dst = ocodes + ((o.piece + i * L::LP) * 16 + (lane & 15)) * 16;
+        if (o.mask == 0xffff) {
+            *reinterpret_cast<u32x4*>(dst) = w;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (o.mask >> r & 1) dst[r] = static_cast<uint8_t>(w[r >> 2] >> (8 * (r & 3)));
+        }
+    }
+}
+
+// HBM-bound: the reverse of kv_write_kernel, out rows contiguous.
+template <int BITS, int D, int DT, bool VEC>
+__global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvCache c, KvBatch b, void* ko,
+                                                              void* vo, int sets) {
+    constexpr int ROW = D * BITS / 8, NP = ROW / 16;
+    using L = Lanes<NP>;
+    constexpr int E = BITS == 8 ? 16 : 32;
+    __shared__ __align__(16) uint8_t lds[kWaves][4 * kTilePitch];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Unit u = unit_of<L::TW>(c, b, static_cast<int64_t>(blockIdx.x) * kWaves + wave, sets);
+    void* const out = u.value ? vo : ko;
+    if (!u.any || !out) return;  // wave-uniform; the waves share nothing
+    const int t = lane / L::LP, lc = lane % L::LP;
+    int j = u.first + t, row = j - (u.q.n - u.q.q);
+    bool live = j >= u.lo && j < u.q.n;
+    int page = -1;
+    if (u.q.ok) {
+        page = group_page(c, b, u, j);
+    } else {  // no positions to go by: the run's share of the rows becomes NaN
+        row = j;
+        live = row < u.q.q;
+    }
+    const int in_page = (1 << c.shift) - 1, slot = j & in_page;
+    const uint8_t* const blk = kv_block(c, max(page, 0), u.head);
+    const uint8_t* const codes = blk + (u.value ? c.codes : 0);
+    float scale = __uint_as_float(0x7fc00000u);
+    if (live && page >= 0)
+        scale = reinterpret_cast<const float*>(blk + 2 * c.codes)[(u.value << c.shift) + slot];
+    const Column o = column_of<L::LP>(lane, live && lc == 0);
+    const int opage = __shfl(page, o.group * 16 * L::LP);
+    const uint8_t* const ocodes = kv_block(c, max(opage, 0), u.head) + c.codes +
+                                  ((u.first + o.group * 16) & in_page) * ROW;
+    const int64_t at = ((u.q.row + row) * c.H + u.head) * D;
+#pragma unroll
+    for (int i = 0; i < L::IT; i++) {
+        u32x4 w = {0, 0, 0, 0};
+        if (u.value) {
+            if (o.mask && opage >= 0)
+                w = *reinterpret_cast<const u32x4*>(
+                    ocodes + ((o.piece + i * L::LP) * 16 + (lane & 15)) * 16);
+            w = transpose16(lds[wave], lane, lane >> 4, lane & 15, (t >> 4) * L::LP + lc, t & 15, w);
+        } else if (live && page >= 0) {
+            w = *reinterpret_cast<const u32x4*>(codes + (slot & ~15) * ROW +
+                                                (lc + i * L::LP) * 256 + (slot & 15) * 16);
+        }
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const uint32_t by = w[e >> 2] >> (8 * (e & 3));
+            if constexpr (BITS == 8) {
+                x[e] = (static_cast<float>(by & 255u) - 128.0f) * scale;
+            } else {
+                x[e] = (static_cast<float>(by & 15u) - 8.0f) * scale;
+                x[16 + e] = (static_cast<float>(by >> 4 & 15u) - 8.0f) * scale;
+            }
+        }
+        if (live) {
+            const int e = (lc + i * L::LP) * 16;
+            store16<DT, VEC>(out, at + e, x);
+            if constexpr (BITS == 4) store16<DT, VEC>(out, at + D / 2 + e, x + 16);
+        }
+    }
+}
+
+// The launch's units: per sequence the token runs of max_q tokens (one more
+// than they fill, for a run that starts inside a group), every head, keys and
+// values.  False where they do not fit a launch.
+bool units(const KvBatch& b, const KvCache& c, int TW, int* sets, unsigned* blocks) {
+    const int64_t s = (static_cast<int64_t>(b.max_q) + 15 + TW - 1) / TW;
+    const int64_t n = (s * b.n_seq * c.H * 2 + kWaves - 1) / kWaves;
+    *sets = static_cast<int>(s);
+    *blocks = static_cast<unsigned>(n);
+    return n < (int64_t(1) << 31) / (64 * kWaves) * 2;
+}
+
+// f<BITS, D, DT, VEC> for the run-time values.
+template <template <int, int, int, bool> class F, typename... A>
+hipError_t pick(int bits, int D, int dt, bool vec, A&&... a) {
+#define JHQ_KV_V(B, DD, T) return vec ? F<B, DD, T, true>::run(a...) : F<B, DD, T, false>::run(a...)
+#define JHQ_KV_T(B, DD)                              \
+    switch (dt) {                                    \
+        case JHQ_F32: JHQ_KV_V(B, DD, JHQ_F32);      \
+        case JHQ_BF16: JHQ_KV_V(B, DD, JHQ_BF16);    \
+        default: JHQ_KV_V(B, DD, JHQ_F16);           \
+    }
+#define JHQ_KV_D(B)                    \
+    switch (D) {                       \
+        case 64: JHQ_KV_T(B, 64)       \
+        case 128: JHQ_KV_T(B, 128)     \
+        default: JHQ_KV_T(B, 256)      \
+    }
+    if (bits == 8) JHQ_KV_D(8) else JHQ_KV_D(4)
+#undef JHQ_KV_D
+#undef JHQ_KV_T
+#undef JHQ_KV_V
+}
+
+template <int BITS, int D>
+constexpr int run_tokens() {
+    return Lanes<D * BITS / 128>::TW;
+}
+
+template <int BITS, int D, int DT, bool VEC>
+struct Write {
+    static hipError_t run(const KvCache& c, const KvBatch& b, const KvRows& k, const KvRows& v,
+                          hipStream_t s) {
+        int sets;
+        unsigned blocks;
+        if (!units(b, c, run_tokens<BITS, D>(), &sets, &blocks)) return hipErrorInvalidValue;
+        kv_write_kernel<BITS, D, DT, VEC><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
+        return hipGetLastError();
+    }
+};
+
+template <int BITS, int D, int DT, bool VEC>
+struct Read {
+    static hipError_t run(const KvCache& c, const KvBatch& b, void* k, void* v, hipStream_t s) {
+        int sets;
+        unsigned blocks;
+        if (!units(b, c, run_tokens<BITS, D>(), &sets, &blocks)) return hipErrorInvalidValue;
+        kv_read_kernel<BITS, D, DT, VEC><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
+        return hipGetLastError();
+    }
+};
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+hipError_t kv_write(const KvCache& c, const KvBatch& b, int bits, int D, const KvRows& k,
+                    const KvRows& v, int dtype, hipStream_t s) {
+    // 16-byte loads where every row starts on 16 bytes
+    const int e = dtype == JHQ_F32 ? 4 : 8;
+    const bool vec = aligned16(k.p) && aligned16(v.p) && k.tok % e == 0 && k.head % e == 0 &&
+                     v.tok % e == 0 && v.head % e == 0;
+    return pick<Write>(bits, D, dtype, vec, c, b, k, v, s);
+}
+
+hipError_t kv_read(const KvCache& c, const KvBatch& b, int bits, int D, void* k, void* v, int dtype,
+                   hipStream_t s) {
+    return pick<Read>(bits, D, dtype, aligned16(k) && aligned16(v), c, b, k, v, s);
+}
+
+}  // namespace jhq
+
+// ---------------------------------------------------------------------------
+// C-ABI
+// ---------------------------------------------------------------------------
+
+namespace {
+
+int bad(const std::string& msg) { return jhq_set_error(JHQ_EINVAL, msg.c_str()); }
+
+int launched(const char* what, hipError_t e) {
+    if (e == hipSuccess) return JHQ_OK;
+    (void)hipGetLastError();  // reported here: not the next launch's
+    if (e == hipErrorInvalidValue)
+        return bad(std::string(what) + ": more work than one launch holds");
+    return jhq_set_error(e == hipErrorOutOfMemory ? JHQ_ENOMEM : JHQ_EDEVICE,
+                         (std::string(what) + ": " + hipGetErrorString(e)).c_str());
+}
+
+int check_params(const jhq_kv_params* p) {
+    if (!p) return bad("null parameters");
+    if (p->bits != 8 && p->bits != 4) return bad("bits must be 8 or 4");
+    if (p->kv_heads < 1 || p->kv_heads > 1024) return bad("kv_heads must be 1 .. 1024");
+    if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+        return bad("head_dim must be 64, 128 or 256");
+    if (p->page_size < 16 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)))
+        return bad("page_size must be a power of two, 16 .. 1024");
+    if (p->num_pages < 0 || p->num_pages > INT32_MAX) return bad("num_pages must be 0 .. 2^31 - 1");
+    return JHQ_OK;
+}
+
+int check_batch(const jhq_kv_batch* b) {
+    if (!b) return bad("null batch");
+    if (b->n_seq < 0 || b->max_pages < 0 || b->n_tokens < 0 || b->max_q < 0 || b->max_kv < 0)
+        return bad("negative size in the batch");
+    // positions, and the tile a kernel may step past the end, stay within int
+    if (b->max_kv > (1 << 30) || b->max_q > (1 << 30)) return bad("max_q and max_kv are at most 2^30");
+    if (b->n_seq > 0 && (!b->d_kv_len || !b->d_cu_q || (b->max_pages > 0 && !b->d_pages)))
+        return bad("null array in the batch");
+    return JHQ_OK;
+}
+
+int64_t block_bytes(const jhq_kv_params& p) {
+    return static_cast<int64_t>(p.page_size) * (p.head_dim * p.bits / 8 * 2 + 8);
+}
+
+jhq::KvCache cache_of(const jhq_kv_params& p, const void* base) {
+    jhq::KvCache c;
+    c.base = static_cast<uint8_t*>(const_cast<void*>(base));
+    c.block = block_bytes(p);
+    c.num_pages = static_cast<int32_t>(p.num_pages);
+    c.H = p.kv_heads;
+    c.shift = __builtin_ctz(static_cast<unsigned>(p.page_size));
+    c.codes = p.page_size * p.head_dim * p.bits / 8;
+    return c;
+}
+
+jhq::KvBatch batch_of(const jhq_kv_batch& b) {
+    return {b.d_pages, b.d_kv_len, b.d_cu_q, b.n_tokens, b.n_seq, b.max_pages, b.max_q, b.max_kv};
+}
+
+int check_cache(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b) {
+    int rc = check_params(p);
+    if (rc == JHQ_OK) rc = check_batch(b);
+    if (rc != JHQ_OK) return rc;
+    if (!d_cache && p->num_pages > 0) return bad("null cache");
+    if (!jhq::aligned16(d_cache)) return bad("the cache must be 16-byte aligned");
+    return JHQ_OK;
+}
+
+bool idle(const jhq_kv_batch* b) { return b->n_seq == 0 || b->n_tokens == 0 || b->max_q == 0; }
+
+int check_heads(const jhq_kv_params* p, int q_heads, int window) {
+    if (q_heads < 1 || q_heads % p->kv_heads) return bad("q_heads must be a multiple of kv_heads");
+    if (q_heads > 16384) return bad("q_heads must be at most 16384");
+    if (window < 0) return bad("window must not be negative");
+    return JHQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t jhq_kv_bytes(const jhq_kv_params* p) {
+    if (check_params(p) != JHQ_OK) return 0;
+    // at most 2^31 pages x 2^10 heads x 2^10 tokens x 520 bytes: past 2^60
+    const __int128 n = static_cast<__int128>(p->num_pages) * p->kv_heads * block_bytes(*p);
+    if (n > (int64_t(1) << 50)) {
+        bad("the cache would have more than 2^50 bytes");
+        return 0;
+    }
+    return static_cast<int64_t>(n);
+}
+
+int jhq_k_kv_write(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, const void* d_k,
+                   int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok, int64_t v_head,
+                   int dtype, void* stream) {
+    const int rc = check_cache(p, d_cache, b);
+    if (rc != JHQ_OK) return rc;
+    if (dtype != JHQ_F32 && dtype != JHQ_BF16 && dtype != JHQ_F16)
+        return bad("keys and values must be JHQ_F32, JHQ_BF16 or JHQ_F16");
+    if (idle(b) || p->num_pages == 0) return JHQ_OK;
+    if (!d_k || !d_v) return bad("null keys or values");
+    return launched("kv_write", jhq::kv_write(cache_of(*p, d_cache), batch_of(*b), p->bits,
+                                              p->head_dim, {d_k, k_tok, k_head},
+                                              {d_v, v_tok, v_head}, dtype,
+                                              static_cast<hipStream_t>(stream)));
+}
+
+int jhq_k_kv_read(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b, void* d_k,
+                  void* d_v, int dtype, void* stream) {
+    const int rc = check_cache(p, d_cache, b);
+    if (rc != JHQ_OK) return rc;
+    if (dtype != JHQ_F32 && dtype != JHQ_BF16 && dtype != JHQ_F16)
+        return bad("keys and values must be JHQ_F32, JHQ_BF16 or JHQ_F16");
+    if (idle(b) || (!d_k && !d_v)) return JHQ_OK;
+    return launched("kv_read", jhq::kv_read(cache_of(*p, d_cache), batch_of(*b), p->bits,
+                                            p->head_dim, d_k, d_v, dtype,
+                                            static_cast<hipStream_t>(stream)));
+}
+
+int64_t jhq_kv_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_heads, int window) {
+    if (check_params(p) != JHQ_OK || check_batch(b) != JHQ_OK ||
+        check_heads(p, q_heads, window) != JHQ_OK)
+        return -1;
+    if (idle(b)) return 0;
+    return jhq::kv_attend_work(cache_of(*p, nullptr), batch_of(*b), p->head_dim,
+                               q_heads / p->kv_heads, window);
+}
+
+int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
+                    const void* d_q, int64_t q_tok, int64_t q_head, int q_heads, int dtype,
+                    float scale, int causal, int window, void* d_out, float* d_lse, void* d_work,
+                    int64_t work_bytes, void* stream) {
+    int rc = check_cache(p, d_cache, b);
+    if (rc == JHQ_OK) rc = check_heads(p, q_heads, window);
+    if (rc != JHQ_OK) return rc;
+    if (dtype != JHQ_BF16 && dtype != JHQ_F16) return bad("queries must be JHQ_BF16 or JHQ_F16");
+    if (causal != 0 && causal != 1) return bad("causal must be 0 or 1");
+    if (window && !causal) return bad("a window needs causal = 1");
+    if (!std::isfinite(scale)) return bad("scale must be finite");
+    if (idle(b)) return JHQ_OK;
+    if (!d_q || !d_out) return bad("null queries or output");
+    const int64_t need = jhq_kv_work_bytes(p, b, q_heads, window);
+    if (need < 0) return JHQ_EINVAL;
+    if (need > 0 && !d_work) return bad("null workspace");
+    if (work_bytes < need)
+        return bad("the workspace has " + std::to_string(work_bytes) + " bytes, " +
+                   std::to_string(need) + " are needed (jhq_kv_work_bytes)");
+    if (!jhq::aligned16(d_work)) return bad("the workspace must be 16-byte aligned");
+    const jhq::KvAttend a = {{d_q, q_tok, q_head}, q_heads / p->kv_heads, scale, causal, window,
+                             d_out, d_lse, static_cast<float*>(d_work)};
+    return launched("kv_attend", jhq::kv_attend(cache_of(*p, d_cache), batch_of(*b), p->bits,
+                                                p->head_dim, a, dtype,
+                                                static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"
