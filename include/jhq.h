@@ -376,7 +376,7 @@ typedef struct {
     int     kv_heads;  /* key/value heads, 1 .. 1024                          */
     int     head_dim;  /* 64, 128 or 256                                      */
     int     page_size; /* tokens of a page: a power of two, 16 .. 1024        */
-    int64_t num_pages; /* pages in the buffer, at most 2^31 - 1               */
+    int64_t num_pages; /* pages in the buffer, 1 .. 2^31 - 1                  */
 } jhq_kv_params;
 
 /* The sequences that a call works on.  Sequence b holds kv_len[b] tokens, token

@@ -1,129 +1,825 @@
 // kv_attend.hip — attention of new tokens over the quantised key/value cache.
+//
+// Mathematics.  With codes c and scales of the cache, s_ij = scale * ks_j <q_i,
+// ck_j> and o_i = sum_j w_ij vs_j cv_j / sum_j w_ij, w_ij = exp(s_ij).  Both
+// products run on the matrix cores (f32_16x16x32_f16) on the codes themselves:
+// a code is exact in float16, queries are exact there too once the largest is
+// scaled to 2^14 (only what is 2^-28 of it becomes subnormal), and sums are
+// float32.  The scales go where they cost one operation per score:
+//   a_ij  = S_ij * (scale log2e ks_j) + log2 vs_j
+//   p'_ij = 2^(a_ij - m_i)            = w_ij vs_j 2^-m_i
+//   l_i   = sum_j p'_ij / vs_j          o_i = sum_j p'_ij cv_j / l_i
+// m_i is a running maximum of a_ij, so p' is rounded to float16 relative to the
+// row's largest weighted scale whatever the sizes of the values.  A value scale
+// of 0 (all codes 0) counts as 2^-80, below any scale the cache holds.  m_i moves
+// only when some a_ij passes it by more than 8 (p' <= 2^8): then, and not at
+// every step, sums and accumulators are rescaled.
+//
+// Layout.  Scores are computed transposed, S^T = K Q^T: a lane of the result
+// holds one query row (column lane % 16) and 4 tokens, so a row's statistics
+// live in its lane.  Tile t of a step of 64 tokens takes as its row 4 g + i the
+// token 16 g + 4 t + i.  Then lane group g = lane / 16 ends with the scores of
+// the tokens 16 g .. 16 g + 15 of its rows, which is, in order, what it has to
+// supply to O^T = V^T P^T, and the 16 bytes [element][16 tokens] of the cache's
+// values are what it has to supply of V^T: nothing crosses lanes.
 #include "kvcache.h"
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 namespace jhq {
 namespace {
 
-template <int DT>
-__device__ inline float load_el(const void* p, int64_t i) {
-    if constexpr (DT == JHQ_BF16)
-        return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i]) << 16);
-    else
-        return static_cast<float>(static_cast<const _Float16*>(p)[i]);
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int kStep = 64;          // tokens of a step
+constexpr float kNone = -1e30f;    // running maximum before the first token
+constexpr float kSlack = 8.0f;     // how far a score may pass it
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ inline float nan32() { return __uint_as_float(0x7fc00000u); }
+
+// Sizes that follow from the cache's bits and the head's elements.
+template <int BITS, int D>
+struct Dim {
+    static constexpr int ROW = D * BITS / 8;        // bytes of a row
+    static constexpr int LB = ROW / 4;              // of them in a lane's key operand
+    static constexpr int NU = LB < 16 ? 1 : LB / 16;  // loads that bring them
+    static constexpr int KS = D / 32;               // products along D
+    static constexpr int ET = ROW / 16;             // tiles of value byte columns
+    static constexpr int DT = D / 16;               // tiles of output elements
+    // First byte column of octet o (8 bytes) of lane group g.
+    __device__ static int octet(int o, int g) {
+        return LB == 8 ? g * 8 : ((o >> 1) * 4 + g) * 16 + (o & 1) * 8;
+    }
+};
+
+template <int LB>
+struct KeyReg {
+    typedef u4 type;
+};
+template <>
+struct KeyReg<8> {
+    typedef u2 type;
+};
+
+// 8 bytes of 8-bit codes as float16: 0x6400 | u is 1024 + u.
+__device__ inline h8 half8(uint32_t a, uint32_t b) {
+    const h2 bias = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+    const uint32_t k = 0x64646464u;
+    h2 r[4] = {__builtin_bit_cast(h2, __builtin_amdgcn_perm(a, k, 0x00050004)) + bias,
+               __builtin_bit_cast(h2, __builtin_amdgcn_perm(a, k, 0x00070006)) + bias,
+               __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, k, 0x00050004)) + bias,
+               __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, k, 0x00070006)) + bias};
+    return __builtin_bit_cast(h8, r);
 }
 
-template <int DT>
-__device__ inline void store_el(void* p, int64_t i, float f) {
-    if constexpr (DT == JHQ_BF16)
-        static_cast<__bf16*>(p)[i] = static_cast<__bf16>(f);
-    else
-        static_cast<_Float16*>(p)[i] = static_cast<_Float16>(f);
+// 8 bytes of 4-bit codes: low and high nibbles, in the byte order 0 2 1 3 4 6 5 7.
+__device__ inline void half4(uint32_t a, uint32_t b, h8& lo, h8& hi) {
+    const h2 lob = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
+    const h2 hib = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
+    const h2 sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
+    const uint32_t w[4] = {a, a >> 8, b, b >> 8};
+    h2 l[4], h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        l[i] = __builtin_bit_cast(h2, (w[i] & 0x000f000fu) | 0x64006400u) + lob;
+        // 1024 + 16 n
+        h[i] = __builtin_elementwise_fma(
+            __builtin_bit_cast(h2, (w[i] & 0x00f000f0u) | 0x64006400u), sixteenth, hib);
+    }
+    lo = __builtin_bit_cast(h8, l);
+    hi = __builtin_bit_cast(h8, h);
 }
 
-// One wave per (row, head): a lane scores one token of 64, then sums the byte
-// columns e = lane, lane + 64, ... of the values.
-template <int BITS, int D, int DT>
-__global__ __launch_bounds__(64) void kv_attend_kernel(KvCache c, KvBatch b, KvAttend a) {
-    constexpr int ROW = D * BITS / 8, EC = (ROW + 63) / 64, EL = BITS == 8 ? 1 : 2;
-    __shared__ float qs[D], ps[64];
-    __shared__ int pg[64];
-    const int lane = threadIdx.x, hq = blockIdx.y, seq = blockIdx.z, h = hq / a.G;
-    const int Hq = c.H * a.G;
-    const KvSeq s = kv_seq(b, seq, c.shift);
-    const int i = blockIdx.x;
-    if (i >= s.q) return;
-    const int64_t row = s.row + i, orow = (row * Hq + hq) * D;
-    const int pos = s.n - s.q + i;
-    for (int d = lane; d < D; d += 64)
-        qs[d] = load_el<DT>(a.q.p, row * a.q.tok + hq * a.q.head + d);
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[EC * EL] = {};
-    const int hi = s.ok ? (a.causal ? min(pos + 1, s.n) : s.n) : 0;
-    const int lo = a.window ? max(0, pos - a.window + 1) : 0;
-    for (int j0 = lo & ~63; j0 < hi; j0 += 64) {
-        const int j = j0 + lane, slot = j & ((1 << c.shift) - 1);
-        const bool see = j >= lo && j < hi;
-        const int page = see ? kv_page(b, c, seq, j) : -1;
-        const uint8_t* blk = kv_block(c, max(page, 0), h);
-        const float* sc = reinterpret_cast<const float*>(blk + 2 * c.codes);
-        float ks = 0, vs = 0, dot = 0;
-        if (see) ks = vs = NAN;
-        if (page >= 0) {
-            ks = sc[slot];
-            vs = sc[(1 << c.shift) + slot];
-            const uint8_t* kp = blk + (slot & ~15) * ROW + (slot & 15) * 16;
-            for (int e = 0; e < ROW; e++) {
-                const int by = kp[(e >> 4) * 256 + (e & 15)];
-                if (BITS == 8)
-                    dot = fmaf(qs[e], by - 128.0f, dot);
-                else
-                    dot = fmaf(qs[e], (by & 15) - 8.0f, fmaf(qs[e + D / 2], (by >> 4) - 8.0f, dot));
+// Place of operand element i of an octet within it.
+template <int BITS>
+__device__ constexpr int place(int i) {
+    return BITS == 8 ? i : (i & 4) | ((i & 1) << 1) | ((i >> 1) & 1);
+}
+
+__device__ inline f4 mfma(h8 a, h8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+__device__ inline float value16(const KvAttend& a, uint32_t h) {
+    return a.dtype == JHQ_BF16
+               ? __uint_as_float(h << 16)
+               : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
+}
+
+// How the work is cut; made on the host by plan_of.
+struct Plan {
+    int few;      // NT of the kernel for few rows, 0: the other
+    int nc;       // column tiles of a wave of the other kernel
+    int tile;     // rows of a tile
+    int tiles;    // tiles of a sequence with max_q new tokens
+    int nsplit;   // parts that a tile's tokens may be cut into
+    int chunk;    // tokens of a part, a multiple of kStep
+    int64_t rows; // of the partial results: n_tokens * query heads
+};
+
+// One workgroup's share of the work.
+struct Share {
+    KvSeq s;
+    int seq, head, split;
+    int r0, rn;      // rows of the sequence: token i of head h*G+g is row i*G+g
+    int lo, hi;      // tokens [lo, hi) of the part, lo a multiple of kStep
+    int full_lo, full_hi;  // tokens that every row of the tile sees
+    bool any;
+};
+
+// Positions seen by new token i: [first, last).
+__device__ inline int see_hi(const KvSeq& s, const KvAttend& a, int i) {
+    return a.causal ? max(0, min(s.n - s.q + i + 1, s.n)) : s.n;
+}
+__device__ inline int see_lo(const KvSeq& s, const KvAttend& a, int i) {
+    return a.window ? max(0, s.n - s.q + i + 1 - a.window) : 0;
+}
+
+__device__ inline Share share_of(const KvCache& c, const KvBatch& b, const KvAttend& a,
+                                 const Plan& p) {
+    Share r;
+    // Heads vary fastest (workgroups go round the 8 XCDs, whose L2 caches then
+    // hold few heads each), then sequences, then tiles from the last, which sees
+    // most, then parts.
+    uint32_t w = blockIdx.x;
+    r.head = w % c.H;
+    w /= c.H;
+    r.seq = w % b.n_seq;
+    w /= b.n_seq;
+    const int tile = w % p.tiles;
+    r.split = w / p.tiles;
+    r.s = kv_seq(b, r.seq, c.shift);
+    const int rows = r.s.q * a.G, mine = (rows + p.tile - 1) / p.tile - 1 - tile;
+    r.r0 = mine * p.tile;
+    r.rn = min(p.tile, rows - r.r0);
+    r.any = mine >= 0;
+    if (!r.any) return r;
+    const int i0 = r.r0 / a.G, i1 = (r.r0 + r.rn - 1) / a.G;
+    const int from = see_lo(r.s, a, i0) / kStep * kStep;
+    r.lo = from + r.split * p.chunk;
+    r.hi = see_hi(r.s, a, i1);
+    if (p.nsplit > 1) r.hi = min(r.hi, r.lo + p.chunk);
+    r.full_lo = see_lo(r.s, a, i1);
+    r.full_hi = see_hi(r.s, a, i0);
+    return r;
+}
+
+// Where row r of a share lies: first element of its query, and its output row.
+__device__ inline int64_t row_of(const Share& w, const KvAttend& a, int r, int64_t* q) {
+    const int i = r / a.G, h = w.head * a.G + (r - i * a.G);
+    const int64_t t = w.s.row + i;
+    *q = t * a.q.tok + h * a.q.head;
+    return t * a.heads + h;
+}
+
+// A wave's rows: queries as the second operand of S^T, statistics, sums.
+template <int BITS, int D, int NC>
+struct Rows {
+    using M = Dim<BITS, D>;
+    h8 q[NC][M::KS];
+    f4 o[NC][M::DT];
+    float m[NC], l[NC];
+    int hi[NC], lo[NC];  // the row's tokens
+
+    // Row 16 k + lane % 16 of the wave's, which start at r0 (the share's last row
+    // stands in for rows past it).
+    __device__ static int row_at(const Share& w, int r0, int k, int lane) {
+        return min(r0 + k * 16 + (lane & 15), w.r0 + w.rn - 1);
+    }
+
+    // The 8 elements of operand s of the row whose query starts at `at`.
+    __device__ static void operand(const KvAttend& a, int64_t at, int s, int g, float (&x)[8]) {
+        const int64_t e =
+            at + (BITS == 8 ? M::octet(s, g) : M::octet(s >> 1, g) + (s & 1) * (D / 2));
+        if (a.q16) {
+            const u4 v = *reinterpret_cast<const u4*>(static_cast<const uint16_t*>(a.q.p) + e);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                x[i] = value16(a, v[place<BITS>(i) >> 1] >> (16 * (place<BITS>(i) & 1)) & 0xffff);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                x[i] = value16(a, static_cast<const uint16_t*>(a.q.p)[e + place<BITS>(i)]);
+        }
+    }
+
+    // Sets up the wave's rows; returns the largest finite magnitude of the lane's
+    // query elements.
+    __device__ float start(const Share& w, const KvAttend& a, int r0, int lane) {
+        float big = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NC; k++) {
+            const int r = row_at(w, r0, k, lane);
+            int64_t at;
+            row_of(w, a, r, &at);
+            hi[k] = see_hi(w.s, a, r / a.G);
+            lo[k] = see_lo(w.s, a, r / a.G);
+            m[k] = kNone;
+            l[k] = 0.0f;
+#pragma unroll
+            for (int t = 0; t < M::DT; t++) o[k][t] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < M::KS; s++) {
+                float x[8];
+                operand(a, at, s, lane >> 4, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    big = fabsf(x[i]) < INFINITY ? fmaxf(big, fabsf(x[i])) : big;
             }
         }
-        const float x = see ? dot * ks * a.scale : -INFINITY;
-        float mt = x;
-        for (int k = 1; k < 64; k <<= 1) mt = fmaxf(mt, __shfl_xor(mt, k));
-        const float mn = fmaxf(m, mt);
-        const float p = see ? expf(x - mn) : 0.0f;
-        const float al = mn == -INFINITY ? 1.0f : expf(m - mn);
-        float pl = p;
-        for (int k = 1; k < 64; k <<= 1) pl += __shfl_xor(pl, k);
-        l = l * al + pl;
-        m = mn;
-        __syncthreads();
-        ps[lane] = see ? p * vs : 0.0f;
-        pg[lane] = page;
-        __syncthreads();
-        for (int k = 0; k < EC * EL; k++) o[k] *= al;
-        for (int t = 0; t < 64; t++) {
-            const int sl = (j0 + t) & ((1 << c.shift) - 1);
-            const uint8_t* vb = kv_block(c, max(pg[t], 0), h) + c.codes + (sl & ~15) * ROW + (sl & 15);
-            for (int k = 0; k < EC; k++) {
-                const int e = lane + k * 64;
-                if (e >= ROW) continue;
-                const int by = pg[t] >= 0 ? vb[e * 16] : 0;
-                if (BITS == 8) {
-                    o[k] = fmaf(ps[t], by - 128.0f, o[k]);
-                } else {
-                    o[2 * k] = fmaf(ps[t], (by & 15) - 8.0f, o[2 * k]);
-                    o[2 * k + 1] = fmaf(ps[t], (by >> 4) - 8.0f, o[2 * k + 1]);
+        return big;
+    }
+
+    // Reads the queries, scaled by the power of two that takes big to 2^13 ..
+    // 2^14; returns its inverse, which S has to be multiplied by.
+    __device__ float load(const Share& w, const KvAttend& a, int r0, int lane, float big) {
+        int e = 0;
+        if (big > 0.0f) {
+            frexpf(big, &e);
+            e = max(-126, min(126, 14 - e));
+        }
+        const float f = ldexpf(1.0f, e);
+#pragma unroll
+        for (int k = 0; k < NC; k++) {
+            int64_t at;
+            row_of(w, a, row_at(w, r0, k, lane), &at);
+#pragma unroll
+            for (int s = 0; s < M::KS; s++) {
+                float x[8];
+                operand(a, at, s, lane >> 4, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) q[k][s][i] = static_cast<_Float16>(x[i] * f);
+            }
+        }
+        return ldexpf(1.0f, -e);
+    }
+
+    // Scores of a step to weights.  s[k][t][i]: token j0 + 16 g + 4 t + i.  sc:
+    // the step's kk, lv and iv (64 floats each).
+    __device__ void weigh(f4 (&s)[NC][4], const float* sc, int lane, int j0, bool masked,
+                          h8 (&p)[NC][2]) {
+        const int g = lane >> 4;
+        const f4* kk = reinterpret_cast<const f4*>(sc + g * 16);
+        const f4* lv = reinterpret_cast<const f4*>(sc + 64 + g * 16);
+        const f4* iv = reinterpret_cast<const f4*>(sc + 128 + g * 16);
+        float top[NC];
+#pragma unroll
+        for (int k = 0; k < NC; k++) top[k] = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const f4 x = kk[t], y = lv[t];
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float v = fmaf(s[k][t][i], x[i], y[i]);
+                    if (masked) {
+                        const int j = j0 + g * 16 + t * 4 + i;
+                        v = j < hi[k] && j >= lo[k] ? v : -INFINITY;
+                    }
+                    s[k][t][i] = v;
+                    top[k] = fmaxf(top[k], v);
+                }
+        }
+        bool over = false;
+#pragma unroll
+        for (int k = 0; k < NC; k++) over |= top[k] > m[k] + kSlack;
+        if (__any(over)) {
+#pragma unroll
+            for (int k = 0; k < NC; k++) {
+                float n = fmaxf(m[k], top[k]);
+                n = fmaxf(n, __shfl_xor(n, 16));
+                n = fmaxf(n, __shfl_xor(n, 32));
+                const float f = exp2f(m[k] - n);
+                m[k] = n;
+                l[k] *= f;
+#pragma unroll
+                for (int t = 0; t < M::DT; t++) o[k][t] *= f;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const f4 z = iv[t];
+#pragma unroll
+            for (int k = 0; k < NC; k++) {
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    e[i] = __builtin_amdgcn_exp2f(s[k][t][i] - m[k]);
+                    // a token that this row does not see may have a NaN here
+                    const float d = e[i] * z[i];
+                    l[k] += masked && e[i] == 0.0f ? 0.0f : d;
+                }
+                const int at = (t & 1) * 4;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    p[k][t >> 1][at + i] = static_cast<_Float16>(e[BITS == 8 ? i : place<4>(i)]);
+            }
+        }
+    }
+
+    __device__ void add_values(int e, u4 w, const h8 (&p)[NC][2]) {
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            if constexpr (BITS == 8) {
+                const h8 v = half8(w[2 * kk], w[2 * kk + 1]);
+#pragma unroll
+                for (int k = 0; k < NC; k++) o[k][e] = mfma(v, p[k][kk], o[k][e]);
+            } else {
+                h8 lo8, hi8;
+                half4(w[2 * kk], w[2 * kk + 1], lo8, hi8);
+#pragma unroll
+                for (int k = 0; k < NC; k++) {
+                    o[k][e] = mfma(lo8, p[k][kk], o[k][e]);
+                    o[k][e + M::ET] = mfma(hi8, p[k][kk], o[k][e + M::ET]);
                 }
             }
         }
     }
-    const float r = s.ok ? (l == 0.0f ? 0.0f : 1.0f / l) : NAN;
-    for (int k = 0; k < EC; k++) {
-        const int e = lane + k * 64;
-        if (e >= ROW) continue;
-        store_el<DT>(a.out, orow + e, o[k * EL] * r);
-        if (BITS == 4) store_el<DT>(a.out, orow + e + D / 2, o[2 * k + 1] * r);
+
+    // The lanes' sums of a row, joined.
+    __device__ void join() {
+#pragma unroll
+        for (int k = 0; k < NC; k++) {
+            l[k] += __shfl_xor(l[k], 16);
+            l[k] += __shfl_xor(l[k], 32);
+        }
     }
-    if (a.lse && lane == 0)
-        a.lse[row * Hq + hq] = s.ok ? (l == 0.0f ? -INFINITY : m + logf(l)) : NAN;
+};
+
+// Scores of one tile of 16 tokens.
+template <int BITS, int D, int NC>
+__device__ inline void score_tile(const typename KeyReg<Dim<BITS, D>::LB>::type (&w)[Dim<BITS, D>::NU],
+                                  const Rows<BITS, D, NC>& r, f4 (&s)[NC]) {
+    using M = Dim<BITS, D>;
+#pragma unroll
+    for (int k = 0; k < NC; k++) s[k] = f4{0, 0, 0, 0};
+#pragma unroll
+    for (int o = 0; o < M::LB / 8; o++) {
+        const uint32_t a = w[o >> 1][(o & 1) * 2], b = w[o >> 1][(o & 1) * 2 + 1];
+        if constexpr (BITS == 8) {
+            const h8 x = half8(a, b);
+#pragma unroll
+            for (int k = 0; k < NC; k++) s[k] = mfma(x, r.q[k][o], s[k]);
+        } else {
+            h8 lo, hi;
+            half4(a, b, lo, hi);
+#pragma unroll
+            for (int k = 0; k < NC; k++) {
+                s[k] = mfma(lo, r.q[k][2 * o], s[k]);
+                s[k] = mfma(hi, r.q[k][2 * o + 1], s[k]);
+            }
+        }
+    }
+}
+
+// kk, lv and iv of one token from its scales; dead: past the sequence's end.
+__device__ inline void token_terms(float ks, float vs, float f, bool dead, bool lost, float* sc) {
+    const bool tiny = vs < 0x1p-80f;  // a NaN is not
+    const float kk = ks * f;
+    sc[0] = dead ? 0.0f : lost ? nan32() : kk;
+    sc[64] = dead ? -INFINITY : tiny ? -80.0f : __builtin_amdgcn_logf(vs);
+    sc[128] = dead ? 0.0f : tiny ? 0x1p80f : __builtin_amdgcn_rcpf(vs);
+}
+
+__device__ inline void store4(const KvAttend& a, int64_t i, f4 x) {
+    uint32_t h[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        h[k] = a.dtype == JHQ_BF16 ? __builtin_bit_cast(uint16_t, static_cast<__bf16>(x[k]))
+                                   : __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[k]));
+    uint16_t* const p = static_cast<uint16_t*>(a.out) + i;
+    if (a.out8) {
+        *reinterpret_cast<u2*>(p) = u2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) p[k] = static_cast<uint16_t>(h[k]);
+    }
+}
+
+__device__ inline float lse_of(float m, float l) {
+    return l == 0.0f ? -INFINITY : kLn2 * (m + log2f(l));
+}
+
+// A share whose sequence is not in order: its rows become NaN (part 0 writes them).
+template <int D>
+__device__ void fail_rows(const Share& w, const KvAttend& a, const Plan& p) {
+    if (w.split) return;
+    for (int k = threadIdx.x; k < w.rn * (D / 4); k += blockDim.x) {
+        int64_t q;
+        const int64_t o = row_of(w, a, w.r0 + k / (D / 4), &q);
+        const float x = nan32();
+        store4(a, o * D + k % (D / 4) * 4, f4{x, x, x, x});
+        if (a.lse && k % (D / 4) == 0) a.lse[o] = x;
+    }
+}
+
+// A row's result, or its part of it: o unscaled, m and l.  Lane group g holds
+// the elements 16 t + 4 g ..
+template <int BITS, int D, int NC>
+__device__ void finish(const Share& w, const KvAttend& a, const Plan& p, int r0, int lane,
+                       Rows<BITS, D, NC>& r) {
+    using M = Dim<BITS, D>;
+    const int g = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < NC; k++) {
+        const int row = r0 + k * 16 + (lane & 15);
+        if (row >= w.r0 + w.rn) continue;
+        int64_t q;
+        const int64_t o = row_of(w, a, row, &q);
+        if (p.nsplit == 1) {
+            const float f = r.l[k] == 0.0f ? 0.0f : 1.0f / r.l[k];
+#pragma unroll
+            for (int t = 0; t < M::DT; t++) store4(a, o * D + t * 16 + g * 4, r.o[k][t] * f);
+            if (a.lse && g == 0) a.lse[o] = lse_of(r.m[k], r.l[k]);
+        } else {
+            float* const po = a.work + (w.split * p.rows + o) * D;
+#pragma unroll
+            for (int t = 0; t < M::DT; t++) *reinterpret_cast<f4*>(po + t * 16 + g * 4) = r.o[k][t];
+            if (g == 0) {
+                float* const ml = a.work + p.nsplit * p.rows * D + (w.split * p.rows + o) * 2;
+                ml[0] = r.m[k];
+                ml[1] = r.l[k];
+            }
+        }
+    }
+}
+
+// Few rows (16 NT at most): what bounds it is reading the cache.  Every wave of
+// the workgroup takes all rows and every fourth step of the part's tokens; keys
+// and values go from memory to registers as operands, the next step's loads
+// are issued as soon as this step has used the registers.  The four waves'
+// results are joined through LDS.
+template <int BITS, int D, int NT>
+__global__ __launch_bounds__(256, 2) void kv_few_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
+    using M = Dim<BITS, D>;
+    using K = typename KeyReg<M::LB>::type;
+    constexpr int R = NT * 16, P = D + 4;
+    __shared__ __align__(16) float sc[4][192];
+    __shared__ __align__(16) float acc[R * P];
+    __shared__ float ml[4][R][2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = lane >> 4, r = lane & 15;
+    const Share w = share_of(c, b, a, p);
+    if (!w.any) return;
+    if (!w.s.ok) return fail_rows<D>(w, a, p);
+    if (p.nsplit > 1 && w.lo >= w.hi) return;  // the join knows which parts there are
+
+    Rows<BITS, D, NT> rows;
+    float big = rows.start(w, a, w.r0, lane);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
+    const float f = rows.load(w, a, w.r0, lane, big) * (a.scale * kLog2e);
+    const int in_page = (1 << c.shift) - 1;
+    K kr[4][M::NU];
+    u4 vr[M::ET];
+    float ks, vs;
+    bool dead, lost;
+    // pages of the step at j: of the lane's key group, and of its value group
+    auto pages = [&](int j, int& pk, int& pv) {
+        const int jk = j + (r >> 2) * 16, jv = j + g * 16;
+        pk = jk < w.s.n ? kv_page(b, c, w.seq, jk) : -1;
+        pv = jv < w.s.n ? kv_page(b, c, w.seq, jv) : -1;
+    };
+    auto load_keys = [&](int j, int pk, int pv) {
+        const uint8_t* k = kv_block(c, max(pk, 0), w.head) + ((j + (r >> 2) * 16) & in_page) * M::ROW +
+                           (r & 3) * 16;
+        k += M::LB == 8 ? (g >> 1) * 256 + (g & 1) * 8 : g * 256;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int u = 0; u < M::NU; u++)
+                kr[t][u] = *reinterpret_cast<const K*>(k + t * 64 + u * 1024);
+        const float* s = reinterpret_cast<const float*>(kv_block(c, max(pv, 0), w.head) + 2 * c.codes) +
+                         ((j + lane) & in_page);
+        ks = s[0];
+        vs = s[1 << c.shift];
+        dead = j + lane >= w.s.n;
+        lost = pv < 0;
+    };
+    auto load_values = [&](int j, int pv) {
+        const uint8_t* v = kv_block(c, max(pv, 0), w.head) + c.codes + ((j + g * 16) & in_page) * M::ROW +
+                           r * 16;
+#pragma unroll
+        for (int t = 0; t < M::ET; t++) vr[t] = *reinterpret_cast<const u4*>(v + t * 256);
+    };
+    int j = w.lo + wave * kStep;
+    if (j < w.hi) {
+        int pk, pv, nk, nv;
+        pages(j, pk, pv);
+        load_keys(j, pk, pv);
+        load_values(j, pv);
+        nk = nv = -1;
+        if (j + 4 * kStep < w.hi) pages(j + 4 * kStep, nk, nv);
+        for (; j < w.hi; j += 4 * kStep) {
+            const int next = j + 4 * kStep;
+            token_terms(ks, vs, f, dead, lost, sc[wave] + lane);
+            f4 s[NT][4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                f4 x[NT];
+                score_tile<BITS, D, NT>(kr[t], rows, x);
+#pragma unroll
+                for (int k = 0; k < NT; k++) s[k][t] = x[k];
+            }
+            const int nv0 = nv;
+            if (next < w.hi) {
+                load_keys(next, nk, nv);
+                if (next + 4 * kStep < w.hi) pages(next + 4 * kStep, nk, nv);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            h8 pr[NT][2];
+            const bool masked = j < w.full_lo || j + kStep > w.full_hi;
+            if (masked)
+                rows.weigh(s, sc[wave], lane, j, true, pr);
+            else
+                rows.weigh(s, sc[wave], lane, j, false, pr);
+#pragma unroll
+            for (int t = 0; t < M::ET; t++) rows.add_values(t, vr[t], pr);
+            if (next < w.hi) load_values(next, nv0);
+        }
+    }
+    rows.join();
+    if (g == 0)
+#pragma unroll
+        for (int k = 0; k < NT; k++) {
+            ml[wave][k * 16 + r][0] = rows.m[k];
+            ml[wave][k * 16 + r][1] = rows.l[k];
+        }
+    __syncthreads();
+    float fac[NT];
+#pragma unroll
+    for (int k = 0; k < NT; k++) {
+        float m = kNone, l = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 4; x++) m = fmaxf(m, ml[x][k * 16 + r][0]);
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+            l += ml[x][k * 16 + r][1] * exp2f(ml[x][k * 16 + r][0] - m);
+        fac[k] = exp2f(rows.m[k] - m);
+        rows.m[k] = m;
+        rows.l[k] = l;
+    }
+    // waves 3, 2, 1 add theirs in turn, wave 0 finishes
+#pragma unroll 1
+    for (int x = 3; x >= 0; x--) {
+        if (wave == x) {
+#pragma unroll
+            for (int k = 0; k < NT; k++)
+#pragma unroll
+                for (int t = 0; t < M::DT; t++) {
+                    f4* const at = reinterpret_cast<f4*>(acc + (k * 16 + r) * P + t * 16 + g * 4);
+                    rows.o[k][t] *= fac[k];
+                    if (x < 3) rows.o[k][t] += *at;
+                    if (x > 0) *at = rows.o[k][t];
+                }
+        }
+        __syncthreads();
+    }
+    if (wave == 0) finish<BITS, D, NT>(w, a, p, w.r0, lane, rows);
+}
+
+// Many rows: 64 NC of them, 16 NC a wave.  What bounds it are the matrix cores and
+// the exponentials.  A step's keys and values are turned to float16 once for the
+// workgroup, in LDS in the order in which the operands are read (16 bytes a lane,
+// consecutive), while the next step's bytes are on their way into registers.
+template <int BITS, int D, int NC>
+__global__ __launch_bounds__(256, NC >= 4 ? 1 : 2) void kv_many_kernel(KvCache c, KvBatch b,
+                                                                        KvAttend a, Plan p) {
+    using M = Dim<BITS, D>;
+    using K = typename KeyReg<M::LB>::type;
+    __shared__ __align__(16) h8 kf[2][4 * M::KS * 64];   // [tile][product][lane]
+    __shared__ __align__(16) h8 vf[2][2 * M::DT * 64];   // [half][tile][lane]
+    __shared__ __align__(16) float sc[2][192];
+    __shared__ float bigs[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = lane >> 4, r = lane & 15;
+    const Share w = share_of(c, b, a, p);
+    if (!w.any) return;
+    if (!w.s.ok) return fail_rows<D>(w, a, p);
+    if (p.nsplit > 1 && w.lo >= w.hi) return;
+
+    Rows<BITS, D, NC> rows;
+    const int r0 = w.r0 + wave * NC * 16;
+    float big = rows.start(w, a, r0, lane);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
+    if (lane == 0) bigs[wave] = big;
+    __syncthreads();
+    big = fmaxf(fmaxf(bigs[0], bigs[1]), fmaxf(bigs[2], bigs[3]));
+    const float f = rows.load(w, a, r0, lane, big) * (a.scale * kLog2e);
+    const int in_page = (1 << c.shift) - 1;
+    // A wave stages the key tile `wave` and the value tiles wave, wave + 4, ...
+    constexpr int VT = (M::ET + 3) / 4;
+    K kr[M::NU];
+    u4 vr[VT];
+    float ks = 0, vs = 0;
+    bool dead = true, lost = true;
+    auto fetch = [&](int j) {
+        const int jk = j + (r >> 2) * 16, jv = j + g * 16;
+        const int pk = jk < w.s.n ? kv_page(b, c, w.seq, jk) : -1;
+        const int pv = jv < w.s.n ? kv_page(b, c, w.seq, jv) : -1;
+        const uint8_t* k = kv_block(c, max(pk, 0), w.head) + (jk & in_page) * M::ROW + (r & 3) * 16 +
+                           wave * 64 + (M::LB == 8 ? (g >> 1) * 256 + (g & 1) * 8 : g * 256);
+#pragma unroll
+        for (int u = 0; u < M::NU; u++) kr[u] = *reinterpret_cast<const K*>(k + u * 1024);
+        const uint8_t* const blk = kv_block(c, max(pv, 0), w.head);
+        const uint8_t* v = blk + c.codes + (jv & in_page) * M::ROW + r * 16;
+#pragma unroll
+        for (int t = 0; t < VT; t++)
+            if (M::ET % 4 == 0 || t * 4 + wave < M::ET)
+                vr[t] = *reinterpret_cast<const u4*>(v + (t * 4 + wave) * 256);
+        if (wave == 0) {
+            const float* s = reinterpret_cast<const float*>(blk + 2 * c.codes) + ((j + lane) & in_page);
+            ks = s[0];
+            vs = s[1 << c.shift];
+            dead = j + lane >= w.s.n;
+            lost = pv < 0;
+        }
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int o = 0; o < M::LB / 8; o++) {
+            const uint32_t x = kr[o >> 1][(o & 1) * 2], y = kr[o >> 1][(o & 1) * 2 + 1];
+            if constexpr (BITS == 8) {
+                kf[buf][(wave * M::KS + o) * 64 + lane] = half8(x, y);
+            } else {
+                h8 lo, hi;
+                half4(x, y, lo, hi);
+                kf[buf][(wave * M::KS + 2 * o) * 64 + lane] = lo;
+                kf[buf][(wave * M::KS + 2 * o + 1) * 64 + lane] = hi;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < VT; t++) {
+            const int e = t * 4 + wave;
+            if (M::ET % 4 != 0 && e >= M::ET) continue;
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {
+                if constexpr (BITS == 8) {
+                    vf[buf][(kk * M::DT + e) * 64 + lane] = half8(vr[t][2 * kk], vr[t][2 * kk + 1]);
+                } else {
+                    h8 lo, hi;
+                    half4(vr[t][2 * kk], vr[t][2 * kk + 1], lo, hi);
+                    vf[buf][(kk * M::DT + e) * 64 + lane] = lo;
+                    vf[buf][(kk * M::DT + e + M::ET) * 64 + lane] = hi;
+                }
+            }
+        }
+        if (wave == 0) token_terms(ks, vs, f, dead, lost, sc[buf] + lane);
+    };
+    int buf = 0;
+    if (w.lo < w.hi) {
+        fetch(w.lo);
+        stage(0);
+    }
+    __syncthreads();
+    for (int j = w.lo; j < w.hi; j += kStep, buf ^= 1) {
+        if (j + kStep < w.hi) fetch(j + kStep);
+        f4 s[NC][4];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int q = 0; q < M::KS; q++) {
+                const h8 x = kf[buf][(t * M::KS + q) * 64 + lane];
+#pragma unroll
+                for (int k = 0; k < NC; k++)
+                    s[k][t] = mfma(x, rows.q[k][q], q ? s[k][t] : f4{0, 0, 0, 0});
+            }
+        h8 pr[NC][2];
+        const bool masked = j < w.full_lo || j + kStep > w.full_hi;
+        if (masked)
+            rows.weigh(s, sc[buf], lane, j, true, pr);
+        else
+            rows.weigh(s, sc[buf], lane, j, false, pr);
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+            for (int t = 0; t < M::DT; t++) {
+                const h8 v = vf[buf][(kk * M::DT + t) * 64 + lane];
+#pragma unroll
+                for (int k = 0; k < NC; k++) rows.o[k][t] = mfma(v, pr[k][kk], rows.o[k][t]);
+            }
+        if (j + kStep < w.hi) stage(buf ^ 1);
+        __syncthreads();
+    }
+    rows.join();
+    finish<BITS, D, NC>(w, a, p, r0, lane, rows);
+}
+
+// Joins the parts of a row: one wave per output row.  Which parts there are
+// follows from the row's tile as in share_of.
+template <int D>
+__global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t x = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int per = b.max_q * a.heads;
+    const int seq = static_cast<int>(x / per), in = static_cast<int>(x % per);
+    if (seq >= b.n_seq) return;
+    const int i = in / a.heads, h = in % a.heads;
+    const KvSeq s = kv_seq(b, seq, c.shift);
+    if (i >= s.q || !s.ok) return;  // fail_rows has written the rows of those that are not ok
+    const int64_t o = (s.row + i) * a.heads + h;
+    const int tile = (i * a.G + h % a.G) / p.tile;
+    const int last = min((tile + 1) * p.tile, s.q * a.G) - 1;
+    const int from = see_lo(s, a, tile * p.tile / a.G) / kStep * kStep;
+    const int hi = see_hi(s, a, last / a.G);
+    const int n = hi > from ? (hi - from + p.chunk - 1) / p.chunk : 0;
+    const float* const ml = a.work + p.nsplit * p.rows * D;
+    float m = kNone;
+    for (int k = 0; k < n; k++) m = fmaxf(m, ml[(k * p.rows + o) * 2]);
+    float l = 0.0f;
+    constexpr int E = D / 64;
+    float acc[E] = {};
+    for (int k = 0; k < n; k++) {
+        const float f = exp2f(ml[(k * p.rows + o) * 2] - m);
+        l += ml[(k * p.rows + o) * 2 + 1] * f;
+        const float* const po = a.work + (k * p.rows + o) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[e] += po[e] * f;
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        uint16_t* const out = static_cast<uint16_t*>(a.out) + o * D + lane * E + e;
+        const float v = acc[e] * f;
+        *out = a.dtype == JHQ_BF16 ? __builtin_bit_cast(uint16_t, static_cast<__bf16>(v))
+                                   : __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+    }
+    if (a.lse && lane == 0) a.lse[o] = lse_of(m, l);
+}
+
+Plan plan_of(const KvCache& c, const KvBatch& b, int D, int G, int window) {
+    Plan p;
+    const int64_t rows = static_cast<int64_t>(b.max_q) * G;
+    p.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
+    p.nc = p.few ? 0 : rows <= 64 ? 1 : rows <= 128 || D == 256 ? 2 : 4;
+    p.tile = p.few ? p.few * 16 : p.nc * 64;
+    p.tiles = static_cast<int>((rows + p.tile - 1) / p.tile);
+    p.rows = b.n_tokens * c.H * G;
+    // workgroups without a split: no more tiles than the rows fill
+    const int64_t tiles = std::min<int64_t>(static_cast<int64_t>(b.n_seq) * p.tiles,
+                                            b.n_tokens * G / p.tile + b.n_seq) * c.H;
+    const int64_t span =
+        window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) + p.tile / G + 2 + kStep)
+               : b.max_kv;
+    constexpr int64_t want = 1024;
+    int64_t chunk = std::max<int64_t>(512, span * tiles / want);
+    chunk = (chunk + kStep - 1) / kStep * kStep;
+    p.nsplit = static_cast<int>(std::max<int64_t>(1, (span + chunk - 1) / chunk));
+    p.chunk = p.nsplit == 1 ? 1 << 30 : static_cast<int>(chunk);
+    return p;
+}
+
+template <int BITS, int D>
+hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const Plan& p, hipStream_t s) {
+    const int64_t blocks = static_cast<int64_t>(c.H) * b.n_seq * p.tiles * p.nsplit;
+    const int64_t joins = (static_cast<int64_t>(b.n_seq) * b.max_q * a.heads + 3) / 4;
+    // rows and positions are ints in the kernels
+    if (static_cast<int64_t>(b.max_q) * a.G > 1 << 30) return hipErrorInvalidValue;
+    if (blocks >= 1 << 24 || (p.nsplit > 1 && joins >= 1 << 24)) return hipErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (p.few == 1)
+        kv_few_kernel<BITS, D, 1><<<grid, 256, 0, s>>>(c, b, a, p);
+    else if (p.few == 2)
+        kv_few_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
+    else if (p.nc == 1)
+        kv_many_kernel<BITS, D, 1><<<grid, 256, 0, s>>>(c, b, a, p);
+    else if (p.nc == 2)
+        kv_many_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
+    else if constexpr (D < 256)
+        kv_many_kernel<BITS, D, 4><<<grid, 256, 0, s>>>(c, b, a, p);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && p.nsplit > 1) {
+        kv_join_kernel<D><<<static_cast<unsigned>(joins), 256, 0, s>>>(c, b, a, p);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 }  // namespace
 
-int64_t kv_attend_work(const KvCache&, const KvBatch&, int, int, int) { return 0; }
+int64_t kv_attend_work(const KvCache& c, const KvBatch& b, int D, int G, int window) {
+    const Plan p = plan_of(c, b, D, G, window);
+    return p.nsplit > 1 ? p.nsplit * p.rows * (D + 2) * 4 : 0;
+}
 
 hipError_t kv_attend(const KvCache& c, const KvBatch& b, int bits, int D, const KvAttend& a,
-                     int dtype, hipStream_t s) {
-    if (c.H * a.G > 65535 || b.n_seq > 65535) return hipErrorInvalidValue;
-    const dim3 grid(b.max_q, c.H * a.G, b.n_seq);
-#define JHQ_GO(B, DD)                                                        \
-    if (dtype == JHQ_BF16)                                                   \
-        kv_attend_kernel<B, DD, JHQ_BF16><<<grid, 64, 0, s>>>(c, b, a);      \
-    else                                                                     \
-        kv_attend_kernel<B, DD, JHQ_F16><<<grid, 64, 0, s>>>(c, b, a)
-    if (bits == 8) {
-        if (D == 64) { JHQ_GO(8, 64); } else if (D == 128) { JHQ_GO(8, 128); } else { JHQ_GO(8, 256); }
-    } else {
-        if (D == 64) { JHQ_GO(4, 64); } else if (D == 128) { JHQ_GO(4, 128); } else { JHQ_GO(4, 256); }
-    }
-#undef JHQ_GO
-    return hipGetLastError();
+                     hipStream_t s) {
+    const Plan p = plan_of(c, b, D, a.G, a.window);
+    if (bits == 8)
+        return D == 64 ? launch<8, 64>(c, b, a, p, s)
+                       : D == 128 ? launch<8, 128>(c, b, a, p, s) : launch<8, 256>(c, b, a, p, s);
+    return D == 64 ? launch<4, 64>(c, b, a, p, s)
+                   : D == 128 ? launch<4, 128>(c, b, a, p, s) : launch<4, 256>(c, b, a, p, s);
 }
 
 }  // namespace jhq

@@ -83,15 +83,17 @@ hipError_t kv_read(const KvCache& c, const KvBatch& b, int bits, int D, void* k,
 
 struct KvAttend {
     KvRows q;
-    int G;           // query heads per key/value head
+    int heads, G;    // query heads; of them per key/value head
+    int dtype;       // of q and out: JHQ_BF16 or JHQ_F16
     float scale;
     int causal, window;
     void* out;
+    int q16, out8;   // query rows start on 16 bytes, out on 8
     float* lse;
     float* work;
 };
 int64_t kv_attend_work(const KvCache& c, const KvBatch& b, int D, int G, int window);
 hipError_t kv_attend(const KvCache& c, const KvBatch& b, int bits, int D, const KvAttend& a,
-                     int dtype, hipStream_t s);
+                     hipStream_t s);
 
 }  // namespace jhq

@@ -484,7 +484,7 @@ int check_params(const jhq_kv_params* p) {
         return bad("head_dim must be 64, 128 or 256");
     if (p->page_size < 16 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)))
         return bad("page_size must be a power of two, 16 .. 1024");
-    if (p->num_pages < 0 || p->num_pages > INT32_MAX) return bad("num_pages must be 0 .. 2^31 - 1");
+    if (p->num_pages < 1 || p->num_pages > INT32_MAX) return bad("num_pages must be 1 .. 2^31 - 1");
     return JHQ_OK;
 }
 
@@ -522,7 +522,7 @@ int check_cache(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch*
     int rc = check_params(p);
     if (rc == JHQ_OK) rc = check_batch(b);
     if (rc != JHQ_OK) return rc;
-    if (!d_cache && p->num_pages > 0) return bad("null cache");
+    if (!d_cache) return bad("null cache");
     if (!jhq::aligned16(d_cache)) return bad("the cache must be 16-byte aligned");
     return JHQ_OK;
 }
@@ -558,7 +558,7 @@ int jhq_k_kv_write(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b,
     if (rc != JHQ_OK) return rc;
     if (dtype != JHQ_F32 && dtype != JHQ_BF16 && dtype != JHQ_F16)
         return bad("keys and values must be JHQ_F32, JHQ_BF16 or JHQ_F16");
-    if (idle(b) || p->num_pages == 0) return JHQ_OK;
+    if (idle(b)) return JHQ_OK;
     if (!d_k || !d_v) return bad("null keys or values");
     return launched("kv_write", jhq::kv_write(cache_of(*p, d_cache), batch_of(*b), p->bits,
                                               p->head_dim, {d_k, k_tok, k_head},
@@ -607,11 +607,12 @@ int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_ba
         return bad("the workspace has " + std::to_string(work_bytes) + " bytes, " +
                    std::to_string(need) + " are needed (jhq_kv_work_bytes)");
     if (!jhq::aligned16(d_work)) return bad("the workspace must be 16-byte aligned");
-    const jhq::KvAttend a = {{d_q, q_tok, q_head}, q_heads / p->kv_heads, scale, causal, window,
-                             d_out, d_lse, static_cast<float*>(d_work)};
+    const int q16 = jhq::aligned16(d_q) && q_tok % 8 == 0 && q_head % 8 == 0;
+    const int out8 = (reinterpret_cast<uintptr_t>(d_out) & 7) == 0;
+    const jhq::KvAttend a = {{d_q, q_tok, q_head}, q_heads, q_heads / p->kv_heads, dtype, scale,
+                             causal, window, d_out, q16, out8, d_lse, static_cast<float*>(d_work)};
     return launched("kv_attend", jhq::kv_attend(cache_of(*p, d_cache), batch_of(*b), p->bits,
-                                                p->head_dim, a, dtype,
-                                                static_cast<hipStream_t>(stream)));
+                                                p->head_dim, a, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

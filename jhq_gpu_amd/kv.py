@@ -80,7 +80,7 @@ class KVCache:
         self._ref = ctypes.byref(self._c)
         L = _jg.lib()
         n = int(L.jhq_kv_bytes(self._ref))
-        if n == 0 and int(num_pages) != 0:
+        if n == 0:
             _jg._check(_jg.JHQ_EINVAL)
         torch = _torch()
         self.data = torch.empty(n, dtype=torch.uint8, device=device)
