@@ -27,6 +27,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 
 namespace jhq {
 namespace {
@@ -261,43 +262,51 @@ struct Rows {
         return ldexpf(1.0f, -e);
     }
 
-    // Scores of a step to weights.  s[k][t][i]: token j0 + 16 g + 4 t + i.  sc:
-    // the step's kk, lv and iv (64 floats each).
-    __device__ void weigh(f4 (&s)[NC][4], const float* sc, int lane, int j0, bool masked,
-                          h8 (&p)[NC][2]) {
-        const int g = lane >> 4;
-        const f4* kk = reinterpret_cast<const f4*>(sc + g * 16);
-        const f4* lv = reinterpret_cast<const f4*>(sc + 64 + g * 16);
-        const f4* iv = reinterpret_cast<const f4*>(sc + 128 + g * 16);
-        float top[NC];
+    // Scores of half a step (its tiles 2 hf, 2 hf + 1) to weights.  s[k][t][i]: token
+    // j0 + 16 g + 8 hf + 4 t + i.  sc: the step's kk, lv and iv (64 floats each).
+    __device__ void weigh(f4 (&s)[NC][2], const float* sc, int lane, int j0, int hf, bool masked,
+                          h8 (&p)[NC]) {
+        const int at = (lane >> 4) * 16 + hf * 8;
+        const f4* const kk = reinterpret_cast<const f4*>(sc + at);
+        const f4* const lv = reinterpret_cast<const f4*>(sc + 64 + at);
+        const f4* const iv = reinterpret_cast<const f4*>(sc + 128 + at);
 #pragma unroll
-        for (int k = 0; k < NC; k++) top[k] = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
+        for (int t = 0; t < 2; t++) {
             const f4 x = kk[t], y = lv[t];
 #pragma unroll
             for (int k = 0; k < NC; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float v = fmaf(s[k][t][i], x[i], y[i]);
-                    if (masked) {
-                        const int j = j0 + g * 16 + t * 4 + i;
-                        v = j < hi[k] && j >= lo[k] ? v : -INFINITY;
-                    }
-                    s[k][t][i] = v;
-                    top[k] = fmaxf(top[k], v);
-                }
+                for (int i = 0; i < 4; i++) s[k][t][i] = fmaf(s[k][t][i], x[i], y[i]);
         }
+        if (masked) {
+#pragma unroll
+            for (int k = 0; k < NC; k++) {
+                const int h = hi[k] - j0 - at, l0 = lo[k] - j0 - at;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (t * 4 + i >= h || t * 4 + i < l0) s[k][t][i] = -INFINITY;
+            }
+        }
+        float top[NC];
         bool over = false;
 #pragma unroll
-        for (int k = 0; k < NC; k++) over |= top[k] > m[k] + kSlack;
+        for (int k = 0; k < NC; k++) {
+            top[k] = s[k][0][0];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) top[k] = fmaxf(top[k], s[k][t][i]);
+            over |= top[k] > m[k] + kSlack;
+        }
         if (__any(over)) {
 #pragma unroll
             for (int k = 0; k < NC; k++) {
                 float n = fmaxf(m[k], top[k]);
                 n = fmaxf(n, __shfl_xor(n, 16));
                 n = fmaxf(n, __shfl_xor(n, 32));
-                const float f = exp2f(m[k] - n);
+                const float f = __builtin_amdgcn_exp2f(m[k] - n);
                 m[k] = n;
                 l[k] *= f;
 #pragma unroll
@@ -305,7 +314,7 @@ struct Rows {
             }
         }
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
+        for (int t = 0; t < 2; t++) {
             const f4 z = iv[t];
 #pragma unroll
             for (int k = 0; k < NC; k++) {
@@ -313,33 +322,28 @@ struct Rows {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     e[i] = __builtin_amdgcn_exp2f(s[k][t][i] - m[k]);
-                    // a token that this row does not see may have a NaN here
-                    const float d = e[i] * z[i];
-                    l[k] += masked && e[i] == 0.0f ? 0.0f : d;
+                    l[k] = fmaf(e[i], z[i], l[k]);
                 }
-                const int at = (t & 1) * 4;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    p[k][t >> 1][at + i] = static_cast<_Float16>(e[BITS == 8 ? i : place<4>(i)]);
+                    p[k][t * 4 + i] = static_cast<_Float16>(e[BITS == 8 ? i : place<4>(i)]);
             }
         }
     }
 
-    __device__ void add_values(int e, u4 w, const h8 (&p)[NC][2]) {
+    // O^T += V^T P^T for half a step and one tile of value byte columns.
+    __device__ void add_values(int e, uint32_t w0, uint32_t w1, const h8 (&p)[NC]) {
+        if constexpr (BITS == 8) {
+            const h8 v = half8(w0, w1);
 #pragma unroll
-        for (int kk = 0; kk < 2; kk++) {
-            if constexpr (BITS == 8) {
-                const h8 v = half8(w[2 * kk], w[2 * kk + 1]);
+            for (int k = 0; k < NC; k++) o[k][e] = mfma(v, p[k], o[k][e]);
+        } else {
+            h8 lo8, hi8;
+            half4(w0, w1, lo8, hi8);
 #pragma unroll
-                for (int k = 0; k < NC; k++) o[k][e] = mfma(v, p[k][kk], o[k][e]);
-            } else {
-                h8 lo8, hi8;
-                half4(w[2 * kk], w[2 * kk + 1], lo8, hi8);
-#pragma unroll
-                for (int k = 0; k < NC; k++) {
-                    o[k][e] = mfma(lo8, p[k][kk], o[k][e]);
-                    o[k][e + M::ET] = mfma(hi8, p[k][kk], o[k][e + M::ET]);
-                }
+            for (int k = 0; k < NC; k++) {
+                o[k][e] = mfma(lo8, p[k], o[k][e]);
+                o[k][e + M::ET] = mfma(hi8, p[k], o[k][e + M::ET]);
             }
         }
     }
@@ -386,7 +390,9 @@ __device__ inline void token_terms(float ks, float vs, float f, bool dead, bool 
     const float kk = ks * f;
     sc[0] = dead ? 0.0f : lost ? nan32() : kk;
     sc[64] = dead ? -INFINITY : tiny ? -80.0f : __builtin_amdgcn_logf(vs);
-    sc[128] = dead ? 0.0f : tiny ? 0x1p80f : __builtin_amdgcn_rcpf(vs);
+    // finite also where vs is NaN: a row that does not see the token multiplies it
+    // by 0
+    sc[128] = dead ? 0.0f : tiny ? 0x1p80f : vs <= FLT_MAX ? __builtin_amdgcn_rcpf(vs) : 0.0f;
 }
 
 __device__ inline void store4(const KvAttend& a, int64_t i, f4 x) {
@@ -521,13 +527,13 @@ __global__ __launch_bounds__(256, 2) void kv_few_kernel(KvCache c, KvBatch b, Kv
         for (; j < w.hi; j += 4 * kStep) {
             const int next = j + 4 * kStep;
             token_terms(ks, vs, f, dead, lost, sc[wave] + lane);
-            f4 s[NT][4];
+            f4 s[2][NT][2];
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 f4 x[NT];
                 score_tile<BITS, D, NT>(kr[t], rows, x);
 #pragma unroll
-                for (int k = 0; k < NT; k++) s[k][t] = x[k];
+                for (int k = 0; k < NT; k++) s[t >> 1][k][t & 1] = x[k];
             }
             const int nv0 = nv;
             if (next < w.hi) {
@@ -536,14 +542,15 @@ __global__ __launch_bounds__(256, 2) void kv_few_kernel(KvCache c, KvBatch b, Kv
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            h8 pr[NT][2];
             const bool masked = j < w.full_lo || j + kStep > w.full_hi;
-            if (masked)
-                rows.weigh(s, sc[wave], lane, j, true, pr);
-            else
-                rows.weigh(s, sc[wave], lane, j, false, pr);
 #pragma unroll
-            for (int t = 0; t < M::ET; t++) rows.add_values(t, vr[t], pr);
+            for (int hf = 0; hf < 2; hf++) {
+                h8 pr[NT];
+                rows.weigh(s[hf], sc[wave], lane, j, hf, masked, pr);
+#pragma unroll
+                for (int t = 0; t < M::ET; t++)
+                    rows.add_values(t, vr[t][2 * hf], vr[t][2 * hf + 1], pr);
+            }
             if (next < w.hi) load_values(next, nv0);
         }
     }
@@ -592,7 +599,7 @@ __global__ __launch_bounds__(256, 2) void kv_few_kernel(KvCache c, KvBatch b, Kv
 // workgroup, in LDS in the order in which the operands are read (16 bytes a lane,
 // consecutive), while the next step's bytes are on their way into registers.
 template <int BITS, int D, int NC>
-__global__ __launch_bounds__(256, NC >= 4 ? 1 : 2) void kv_many_kernel(KvCache c, KvBatch b,
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_many_kernel(KvCache c, KvBatch b,
                                                                         KvAttend a, Plan p) {
     using M = Dim<BITS, D>;
     using K = typename KeyReg<M::LB>::type;
@@ -684,30 +691,28 @@ __global__ __launch_bounds__(256, NC >= 4 ? 1 : 2) void kv_many_kernel(KvCache c
     __syncthreads();
     for (int j = w.lo; j < w.hi; j += kStep, buf ^= 1) {
         if (j + kStep < w.hi) fetch(j + kStep);
-        f4 s[NC][4];
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int q = 0; q < M::KS; q++) {
-                const h8 x = kf[buf][(t * M::KS + q) * 64 + lane];
-#pragma unroll
-                for (int k = 0; k < NC; k++)
-                    s[k][t] = mfma(x, rows.q[k][q], q ? s[k][t] : f4{0, 0, 0, 0});
-            }
-        h8 pr[NC][2];
         const bool masked = j < w.full_lo || j + kStep > w.full_hi;
-        if (masked)
-            rows.weigh(s, sc[buf], lane, j, true, pr);
-        else
-            rows.weigh(s, sc[buf], lane, j, false, pr);
 #pragma unroll
-        for (int kk = 0; kk < 2; kk++)
+        for (int hf = 0; hf < 2; hf++) {
+            f4 s[NC][2];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int q = 0; q < M::KS; q++) {
+                    const h8 x = kf[buf][((hf * 2 + t) * M::KS + q) * 64 + lane];
+#pragma unroll
+                    for (int k = 0; k < NC; k++)
+                        s[k][t] = mfma(x, rows.q[k][q], q ? s[k][t] : f4{0, 0, 0, 0});
+                }
+            h8 pr[NC];
+            rows.weigh(s, sc[buf], lane, j, hf, masked, pr);
 #pragma unroll
             for (int t = 0; t < M::DT; t++) {
-                const h8 v = vf[buf][(kk * M::DT + t) * 64 + lane];
+                const h8 v = vf[buf][(hf * M::DT + t) * 64 + lane];
 #pragma unroll
-                for (int k = 0; k < NC; k++) rows.o[k][t] = mfma(v, pr[k][kk], rows.o[k][t]);
+                for (int k = 0; k < NC; k++) rows.o[k][t] = mfma(v, pr[k], rows.o[k][t]);
             }
+        }
         if (j + kStep < w.hi) stage(buf ^ 1);
         __syncthreads();
     }
@@ -761,7 +766,7 @@ Plan plan_of(const KvCache& c, const KvBatch& b, int D, int G, int window) {
     Plan p;
     const int64_t rows = static_cast<int64_t>(b.max_q) * G;
     p.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
-    p.nc = p.few ? 0 : rows <= 64 ? 1 : rows <= 128 || D == 256 ? 2 : 4;
+    p.nc = p.few ? 0 : rows <= 64 ? 1 : 2;
     p.tile = p.few ? p.few * 16 : p.nc * 64;
     p.tiles = static_cast<int>((rows + p.tile - 1) / p.tile);
     p.rows = b.n_tokens * c.H * G;
@@ -793,10 +798,8 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const P
         kv_few_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
     else if (p.nc == 1)
         kv_many_kernel<BITS, D, 1><<<grid, 256, 0, s>>>(c, b, a, p);
-    else if (p.nc == 2)
+    else
         kv_many_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
-    else if constexpr (D < 256)
-        kv_many_kernel<BITS, D, 4><<<grid, 256, 0, s>>>(c, b, a, p);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && p.nsplit > 1) {
         kv_join_kernel<D><<<static_cast<unsigned>(joins), 256, 0, s>>>(c, b, a, p);
