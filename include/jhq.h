@@ -367,9 +367,9 @@ int jhq_k_assign_noalloc(const float* d_y, int64_t n, int d, const float* d_cent
  *
  * Inside, a page is kv_heads blocks of
  *   key codes | value codes | key scales | value scales
- * and codes stand in groups of 16 tokens: keys as 16-byte pieces of one token,
- * [piece][token][16], values as 16 tokens of one element, [element][token], so
- * that matrix instructions take both from memory as they are.  With 4 bits a
+ * and the codes stand as matrix instructions take them from memory: keys in
+ * groups of 4 tokens, [piece][token][16 bytes of a row], values in groups of 16
+ * tokens, [element][token].  With 4 bits a
  * byte holds elements e (low) and e + head_dim/2 (high). */
 typedef struct {
     int     bits;      /* 8 or 4                                              */

@@ -39,6 +39,8 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = 64;          // tokens of a step
+constexpr int kLeast = 2;          // steps of a streaming wave at least
+constexpr int kShortSpan = 1024;   // tokens that one workgroup takes alone
 constexpr float kNone = -1e30f;    // running maximum before the first token
 constexpr float kSlack = 8.0f;     // how far a score may pass it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -116,22 +118,21 @@ __device__ inline float value16(const KvAttend& a, uint32_t h) {
 
 // How the work is cut; made on the host by plan_of.
 struct Plan {
-    int few;      // NT of the kernel for few rows, 0: the other
-    int nc;       // column tiles of a wave of the other kernel
     int tile;     // rows of a tile
     int tiles;    // tiles of a sequence with max_q new tokens
-    int nsplit;   // parts that a tile's tokens may be cut into
+    int workers;  // of the streaming kernel
+    int nsplit;   // parts that a tile's tokens may be cut into (many rows)
     int chunk;    // tokens of a part, a multiple of kStep
     int64_t rows; // of the partial results: n_tokens * query heads
 };
 
-// One workgroup's share of the work.
+// Rows of one head of one sequence, and tokens that they attend to.
 struct Share {
     KvSeq s;
     int seq, head, split;
     int r0, rn;      // rows of the sequence: token i of head h*G+g is row i*G+g
-    int lo, hi;      // tokens [lo, hi) of the part, lo a multiple of kStep
-    int full_lo, full_hi;  // tokens that every row of the tile sees
+    int lo, hi;      // tokens [lo, hi), lo a multiple of kStep
+    int full_lo, full_hi;  // tokens that every row sees
     bool any;
 };
 
@@ -143,6 +144,16 @@ __device__ inline int see_lo(const KvSeq& s, const KvAttend& a, int i) {
     return a.window ? max(0, s.n - s.q + i + 1 - a.window) : 0;
 }
 
+// The tokens that rows [r0, r0 + rn) of a share's sequence attend to.
+__device__ inline void span_of(Share& r, const KvAttend& a) {
+    const int i0 = r.r0 / a.G, i1 = (r.r0 + r.rn - 1) / a.G;
+    r.lo = see_lo(r.s, a, i0) / kStep * kStep;
+    r.hi = see_hi(r.s, a, i1);
+    r.full_lo = see_lo(r.s, a, i1);
+    r.full_hi = see_hi(r.s, a, i0);
+}
+
+// A workgroup's tile of rows and part of their tokens.
 __device__ inline Share share_of(const KvCache& c, const KvBatch& b, const KvAttend& a,
                                  const Plan& p) {
     Share r;
@@ -162,13 +173,9 @@ __device__ inline Share share_of(const KvCache& c, const KvBatch& b, const KvAtt
     r.rn = min(p.tile, rows - r.r0);
     r.any = mine >= 0;
     if (!r.any) return r;
-    const int i0 = r.r0 / a.G, i1 = (r.r0 + r.rn - 1) / a.G;
-    const int from = see_lo(r.s, a, i0) / kStep * kStep;
-    r.lo = from + r.split * p.chunk;
-    r.hi = see_hi(r.s, a, i1);
+    span_of(r, a);
+    r.lo += r.split * p.chunk;
     if (p.nsplit > 1) r.hi = min(r.hi, r.lo + p.chunk);
-    r.full_lo = see_lo(r.s, a, i1);
-    r.full_hi = see_hi(r.s, a, i0);
     return r;
 }
 
@@ -195,26 +202,9 @@ struct Rows {
         return min(r0 + k * 16 + (lane & 15), w.r0 + w.rn - 1);
     }
 
-    // The 8 elements of operand s of the row whose query starts at `at`.
-    __device__ static void operand(const KvAttend& a, int64_t at, int s, int g, float (&x)[8]) {
-        const int64_t e =
-            at + (BITS == 8 ? M::octet(s, g) : M::octet(s >> 1, g) + (s & 1) * (D / 2));
-        if (a.q16) {
-            const u4 v = *reinterpret_cast<const u4*>(static_cast<const uint16_t*>(a.q.p) + e);
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                x[i] = value16(a, v[place<BITS>(i) >> 1] >> (16 * (place<BITS>(i) & 1)) & 0xffff);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                x[i] = value16(a, static_cast<const uint16_t*>(a.q.p)[e + place<BITS>(i)]);
-        }
-    }
-
-    // Sets up the wave's rows; returns the largest finite magnitude of the lane's
-    // query elements.
-    __device__ float start(const Share& w, const KvAttend& a, int r0, int lane) {
-        float big = 0.0f;
+    // Sets up the wave's rows and reads their queries as they are.
+    __device__ void start(const Share& w, const KvAttend& a, int r0, int lane) {
+        const int g = lane >> 4;
 #pragma unroll
         for (int k = 0; k < NC; k++) {
             const int r = row_at(w, r0, k, lane);
@@ -228,19 +218,47 @@ struct Rows {
             for (int t = 0; t < M::DT; t++) o[k][t] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < M::KS; s++) {
-                float x[8];
-                operand(a, at, s, lane >> 4, x);
+                const int64_t e =
+                    at + (BITS == 8 ? M::octet(s, g) : M::octet(s >> 1, g) + (s & 1) * (D / 2));
+                const uint16_t* const src = static_cast<const uint16_t*>(a.q.p) + e;
+                u4 v;
+                if (a.q16) {
+                    v = *reinterpret_cast<const u4*>(src);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    big = fabsf(x[i]) < INFINITY ? fmaxf(big, fabsf(x[i])) : big;
+                    for (int i = 0; i < 4; i++) v[i] = src[2 * i] | static_cast<uint32_t>(src[2 * i + 1]) << 16;
+                }
+                q[k][s] = __builtin_bit_cast(h8, v);
             }
         }
+    }
+
+    __device__ static float element(const KvAttend& a, u4 v, int i) {
+        return value16(a, v[i >> 1] >> (16 * (i & 1)) & 0xffff);
+    }
+
+    // The largest finite magnitude of the wave's query elements.
+    __device__ float largest(const KvAttend& a) const {
+        float big = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NC; k++)
+#pragma unroll
+            for (int s = 0; s < M::KS; s++) {
+                const u4 v = __builtin_bit_cast(u4, q[k][s]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float x = fabsf(element(a, v, i));
+                    big = x < INFINITY ? fmaxf(big, x) : big;
+                }
+            }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
         return big;
     }
 
-    // Reads the queries, scaled by the power of two that takes big to 2^13 ..
-    // 2^14; returns its inverse, which S has to be multiplied by.
-    __device__ float load(const Share& w, const KvAttend& a, int r0, int lane, float big) {
+    // Turns the queries to operands, scaled by the power of two that takes big to
+    // 2^13 .. 2^14; returns its inverse, which S has to be multiplied by.
+    __device__ float scale(const KvAttend& a, float big) {
         int e = 0;
         if (big > 0.0f) {
             frexpf(big, &e);
@@ -248,17 +266,14 @@ struct Rows {
         }
         const float f = ldexpf(1.0f, e);
 #pragma unroll
-        for (int k = 0; k < NC; k++) {
-            int64_t at;
-            row_of(w, a, row_at(w, r0, k, lane), &at);
+        for (int k = 0; k < NC; k++)
 #pragma unroll
             for (int s = 0; s < M::KS; s++) {
-                float x[8];
-                operand(a, at, s, lane >> 4, x);
+                const u4 v = __builtin_bit_cast(u4, q[k][s]);
 #pragma unroll
-                for (int i = 0; i < 8; i++) q[k][s][i] = static_cast<_Float16>(x[i] * f);
+                for (int i = 0; i < 8; i++)
+                    q[k][s][i] = static_cast<_Float16>(element(a, v, place<BITS>(i)) * f);
             }
-        }
         return ldexpf(1.0f, -e);
     }
 
@@ -414,25 +429,22 @@ __device__ inline float lse_of(float m, float l) {
     return l == 0.0f ? -INFINITY : kLn2 * (m + log2f(l));
 }
 
-// A share whose sequence is not in order: its rows become NaN (part 0 writes them).
+// A share whose sequence is not in order: its rows become NaN.
 template <int D>
-__device__ void fail_rows(const Share& w, const KvAttend& a, const Plan& p) {
-    if (w.split) return;
-    for (int k = threadIdx.x; k < w.rn * (D / 4); k += blockDim.x) {
+__device__ void fail_rows(const Share& w, const KvAttend& a, int thread, int threads) {
+    const float x = nan32();
+    for (int k = thread; k < w.rn * (D / 4); k += threads) {
         int64_t q;
         const int64_t o = row_of(w, a, w.r0 + k / (D / 4), &q);
-        const float x = nan32();
         store4(a, o * D + k % (D / 4) * 4, f4{x, x, x, x});
         if (a.lse && k % (D / 4) == 0) a.lse[o] = x;
     }
 }
 
-// A row's result, or its part of it: o unscaled, m and l.  Lane group g holds
-// the elements 16 t + 4 g ..
+// The results of a wave's rows.  Lane group g holds the elements 16 t + 4 g ..
 template <int BITS, int D, int NC>
-__device__ void finish(const Share& w, const KvAttend& a, const Plan& p, int r0, int lane,
-                       Rows<BITS, D, NC>& r) {
-    using M = Dim<BITS, D>;
+__device__ void finish(const Share& w, const KvAttend& a, int r0, int lane,
+                       const Rows<BITS, D, NC>& r) {
     const int g = lane >> 4;
 #pragma unroll
     for (int k = 0; k < NC; k++) {
@@ -440,93 +452,97 @@ __device__ void finish(const Share& w, const KvAttend& a, const Plan& p, int r0,
         if (row >= w.r0 + w.rn) continue;
         int64_t q;
         const int64_t o = row_of(w, a, row, &q);
-        if (p.nsplit == 1) {
-            const float f = r.l[k] == 0.0f ? 0.0f : 1.0f / r.l[k];
+        const float f = r.l[k] == 0.0f ? 0.0f : 1.0f / r.l[k];
 #pragma unroll
-            for (int t = 0; t < M::DT; t++) store4(a, o * D + t * 16 + g * 4, r.o[k][t] * f);
-            if (a.lse && g == 0) a.lse[o] = lse_of(r.m[k], r.l[k]);
-        } else {
-            float* const po = a.work + (w.split * p.rows + o) * D;
+        for (int t = 0; t < D / 16; t++) store4(a, o * D + t * 16 + g * 4, r.o[k][t] * f);
+        if (a.lse && g == 0) a.lse[o] = lse_of(r.m[k], r.l[k]);
+    }
+}
+
+// A part of a wave's rows: 16 NC sums per slot, then every slot's maxima and sums.
+template <int D, int NC>
+__device__ void keep(float* work, int64_t slot, int64_t slots, int lane, const f4 (&o)[NC][D / 16],
+                     const float (&m)[NC], const float (&l)[NC]) {
+    const int g = lane >> 4;
 #pragma unroll
-            for (int t = 0; t < M::DT; t++) *reinterpret_cast<f4*>(po + t * 16 + g * 4) = r.o[k][t];
-            if (g == 0) {
-                float* const ml = a.work + p.nsplit * p.rows * D + (w.split * p.rows + o) * 2;
-                ml[0] = r.m[k];
-                ml[1] = r.l[k];
-            }
+    for (int k = 0; k < NC; k++) {
+        const int64_t row = slot * (NC * 16) + k * 16 + (lane & 15);
+#pragma unroll
+        for (int t = 0; t < D / 16; t++)
+            *reinterpret_cast<f4*>(work + row * D + t * 16 + g * 4) = o[k][t];
+        if (g == 0) {
+            float* const ml = work + slots * (NC * 16) * D + row * 2;
+            ml[0] = m[k];
+            ml[1] = l[k];
         }
     }
 }
 
-// Few rows (16 NT at most): what bounds it is reading the cache.  Every wave of
-// the workgroup takes all rows and every fourth step of the part's tokens; keys
-// and values go from memory to registers as operands, the next step's loads
-// are issued as soon as this step has used the registers.  The four waves'
-// results are joined through LDS.
+// The cache's bytes of one head as a wave with few rows reads them: keys and
+// values go from memory to registers as operands, the next step's loads are
+// issued as soon as this step has used the registers.
 template <int BITS, int D, int NT>
-__global__ __launch_bounds__(256, 2) void kv_few_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
+struct Stream {
     using M = Dim<BITS, D>;
     using K = typename KeyReg<M::LB>::type;
-    constexpr int R = NT * 16, P = D + 4;
-    __shared__ __align__(16) float sc[4][192];
-    __shared__ __align__(16) float acc[R * P];
-    __shared__ float ml[4][R][2];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int g = lane >> 4, r = lane & 15;
-    const Share w = share_of(c, b, a, p);
-    if (!w.any) return;
-    if (!w.s.ok) return fail_rows<D>(w, a, p);
-    if (p.nsplit > 1 && w.lo >= w.hi) return;  // the join knows which parts there are
-
-    Rows<BITS, D, NT> rows;
-    float big = rows.start(w, a, w.r0, lane);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
-    const float f = rows.load(w, a, w.r0, lane, big) * (a.scale * kLog2e);
-    const int in_page = (1 << c.shift) - 1;
+    const KvCache& c;
+    const KvBatch& b;
+    const Share& w;
+    const int lane, g, r;
     K kr[4][M::NU];
     u4 vr[M::ET];
     float ks, vs;
     bool dead, lost;
-    // pages of the step at j: of the lane's key group, and of its value group
-    auto pages = [&](int j, int& pk, int& pv) {
+    int pk, pv;  // pages of the step to be loaded: of the lane's key and value groups
+
+    __device__ Stream(const KvCache& c, const KvBatch& b, const Share& w, int lane)
+        : c(c), b(b), w(w), lane(lane), g(lane >> 4), r(lane & 15) {}
+
+    __device__ void pages(int j) {
         const int jk = j + (r >> 2) * 16, jv = j + g * 16;
         pk = jk < w.s.n ? kv_page(b, c, w.seq, jk) : -1;
         pv = jv < w.s.n ? kv_page(b, c, w.seq, jv) : -1;
-    };
-    auto load_keys = [&](int j, int pk, int pv) {
-        const uint8_t* k = kv_block(c, max(pk, 0), w.head) + ((j + (r >> 2) * 16) & in_page) * M::ROW +
-                           (r & 3) * 16;
-        k += M::LB == 8 ? (g >> 1) * 256 + (g & 1) * 8 : g * 256;
+    }
+    __device__ void load_keys(int j) {
+        const int in_page = (1 << c.shift) - 1;
+        const uint8_t* k = kv_block(c, max(pk, 0), w.head) +
+                           ((j + (r >> 2) * 16) & in_page) * M::ROW + (r & 3) * 16 +
+                           (M::LB == 8 ? (g >> 1) * 64 + (g & 1) * 8 : g * 64);
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int u = 0; u < M::NU; u++)
-                kr[t][u] = *reinterpret_cast<const K*>(k + t * 64 + u * 1024);
-        const float* s = reinterpret_cast<const float*>(kv_block(c, max(pv, 0), w.head) + 2 * c.codes) +
-                         ((j + lane) & in_page);
+                kr[t][u] = *reinterpret_cast<const K*>(k + t * (4 * M::ROW) + u * 256);
+        const float* const s =
+            reinterpret_cast<const float*>(kv_block(c, max(pv, 0), w.head) + 2 * c.codes) +
+            ((j + lane) & in_page);
         ks = s[0];
         vs = s[1 << c.shift];
         dead = j + lane >= w.s.n;
         lost = pv < 0;
-    };
-    auto load_values = [&](int j, int pv) {
-        const uint8_t* v = kv_block(c, max(pv, 0), w.head) + c.codes + ((j + g * 16) & in_page) * M::ROW +
-                           r * 16;
+    }
+    __device__ void load_values(int j, int page) {
+        const uint8_t* const v = kv_block(c, max(page, 0), w.head) + c.codes +
+                                 ((j + g * 16) & ((1 << c.shift) - 1)) * M::ROW + r * 16;
 #pragma unroll
         for (int t = 0; t < M::ET; t++) vr[t] = *reinterpret_cast<const u4*>(v + t * 256);
-    };
-    int j = w.lo + wave * kStep;
-    if (j < w.hi) {
-        int pk, pv, nk, nv;
-        pages(j, pk, pv);
-        load_keys(j, pk, pv);
+    }
+
+    // Issues the first step's loads (at j; nothing where j >= hi).
+    __device__ void open(int j, int stride) {
+        if (j >= w.hi) return;
+        pages(j);
+        load_keys(j);
         load_values(j, pv);
-        nk = nv = -1;
-        if (j + 4 * kStep < w.hi) pages(j + 4 * kStep, nk, nv);
-        for (; j < w.hi; j += 4 * kStep) {
-            const int next = j + 4 * kStep;
-            token_terms(ks, vs, f, dead, lost, sc[wave] + lane);
+        if (j + stride < w.hi) pages(j + stride);
+    }
+
+    // The steps j, j + stride, .. below the share's end; sc: 192 floats of LDS, this
+    // wave's.
+    __device__ void run(Rows<BITS, D, NT>& rows, int j, int stride, float f, float* sc) {
+        for (; j < w.hi; j += stride) {
+            const int next = j + stride;
+            token_terms(ks, vs, f, dead, lost, sc + lane);
             f4 s[2][NT][2];
 #pragma unroll
             for (int t = 0; t < 4; t++) {
@@ -535,63 +551,265 @@ __global__ __launch_bounds__(256, 2) void kv_few_kernel(KvCache c, KvBatch b, Kv
 #pragma unroll
                 for (int k = 0; k < NT; k++) s[t >> 1][k][t & 1] = x[k];
             }
-            const int nv0 = nv;
+            const int vpage = pv;
             if (next < w.hi) {
-                load_keys(next, nk, nv);
-                if (next + 4 * kStep < w.hi) pages(next + 4 * kStep, nk, nv);
+                load_keys(next);
+                if (next + stride < w.hi) pages(next + stride);
             }
+            // one wave: LDS is written and read in order, the compiler has to keep it
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             const bool masked = j < w.full_lo || j + kStep > w.full_hi;
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
                 h8 pr[NT];
-                rows.weigh(s[hf], sc[wave], lane, j, hf, masked, pr);
+                rows.weigh(s[hf], sc, lane, j, hf, masked, pr);
 #pragma unroll
                 for (int t = 0; t < M::ET; t++)
                     rows.add_values(t, vr[t][2 * hf], vr[t][2 * hf + 1], pr);
             }
-            if (next < w.hi) load_values(next, nv0);
+            if (next < w.hi) load_values(next, vpage);
         }
+        rows.join();
     }
-    rows.join();
-    if (g == 0)
+};
+
+// Few rows (16 NT at most) over short contexts: one workgroup has all tokens of a
+// sequence's head, its W waves take every W-th step, and what they have is joined
+// in LDS, so that one launch does it.
+template <int D, int NT>
+constexpr int kShortWaves = 8 * NT * 16 * (D + 4) * 4 <= 140 * 1024 ? 8 : 4;
+
+template <int BITS, int D, int NT, int W>
+__global__ __launch_bounds__(64 * W, W / 4) void kv_short_kernel(KvCache c, KvBatch b, KvAttend a,
+                                                                 Plan p) {
+    using M = Dim<BITS, D>;
+    constexpr int R = NT * 16, P = D + 4;
+    __shared__ __align__(16) float sc[W][192];
+    __shared__ __align__(16) float acc[W][R * P];
+    __shared__ float ml[W][R][2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = lane >> 4, r = lane & 15;
+    const Share w = share_of(c, b, a, p);
+    if (!w.any) return;
+    if (!w.s.ok) return fail_rows<D>(w, a, threadIdx.x, blockDim.x);
+    Rows<BITS, D, NT> rows;
+    Stream<BITS, D, NT> st(c, b, w, lane);
+    const int j = w.lo + wave * kStep;
+    rows.start(w, a, w.r0, lane);
+    st.open(j, W * kStep);
+    const float f = rows.scale(a, rows.largest(a)) * (a.scale * kLog2e);
+    st.run(rows, j, W * kStep, f, sc[wave]);
 #pragma unroll
-        for (int k = 0; k < NT; k++) {
+    for (int k = 0; k < NT; k++) {
+#pragma unroll
+        for (int t = 0; t < M::DT; t++)
+            *reinterpret_cast<f4*>(acc[wave] + (k * 16 + r) * P + t * 16 + g * 4) = rows.o[k][t];
+        if (g == 0) {
             ml[wave][k * 16 + r][0] = rows.m[k];
             ml[wave][k * 16 + r][1] = rows.l[k];
         }
+    }
     __syncthreads();
-    float fac[NT];
-#pragma unroll
-    for (int k = 0; k < NT; k++) {
+    for (int x = threadIdx.x; x < w.rn * (D / 4); x += 64 * W) {
+        const int row = x / (D / 4), e = x % (D / 4) * 4;
         float m = kNone, l = 0.0f;
 #pragma unroll
-        for (int x = 0; x < 4; x++) m = fmaxf(m, ml[x][k * 16 + r][0]);
+        for (int y = 0; y < W; y++) m = fmaxf(m, ml[y][row][0]);
+        f4 o = {0, 0, 0, 0};
 #pragma unroll
-        for (int x = 0; x < 4; x++)
-            l += ml[x][k * 16 + r][1] * exp2f(ml[x][k * 16 + r][0] - m);
-        fac[k] = exp2f(rows.m[k] - m);
-        rows.m[k] = m;
-        rows.l[k] = l;
-    }
-    // waves 3, 2, 1 add theirs in turn, wave 0 finishes
-#pragma unroll 1
-    for (int x = 3; x >= 0; x--) {
-        if (wave == x) {
-#pragma unroll
-            for (int k = 0; k < NT; k++)
-#pragma unroll
-                for (int t = 0; t < M::DT; t++) {
-                    f4* const at = reinterpret_cast<f4*>(acc + (k * 16 + r) * P + t * 16 + g * 4);
-                    rows.o[k][t] *= fac[k];
-                    if (x < 3) rows.o[k][t] += *at;
-                    if (x > 0) *at = rows.o[k][t];
-                }
+        for (int y = 0; y < W; y++) {
+            const float z = __builtin_amdgcn_exp2f(ml[y][row][0] - m);
+            l = fmaf(ml[y][row][1], z, l);
+            o += *reinterpret_cast<const f4*>(acc[y] + row * P + e) * z;
         }
-        __syncthreads();
+        int64_t q;
+        const int64_t at = row_of(w, a, w.r0 + row, &q);
+        store4(a, at * D + e, o * (l == 0.0f ? 0.0f : 1.0f / l));
+        if (a.lse && e == 0) a.lse[at] = lse_of(m, l);
     }
-    if (wave == 0) finish<BITS, D, NT>(w, a, p, w.r0, lane, rows);
+}
+
+// Few rows over longer contexts: what bounds it is reading the cache.  The steps
+// of all sequences and heads are numbered in one row (sequence, head, step) and
+// cut evenly among the waves of the chip, so that ragged batches end together
+// whatever their lengths; a wave works alone, from a step within one head to a
+// step within another.  What it begins or ends in the middle of a head is kept as
+// a part (two at most for a wave: slot 0 where the head began before it, 1 where it
+// goes on after it), and kv_stream_join_kernel adds the parts.
+struct Cut {
+    int64_t total;  // steps of the batch
+    int64_t per;    // of a worker
+};
+
+// Steps of sequence s (a head of it); 0 where it has no new token.
+__device__ inline int steps_of(const KvSeq& s, const KvAttend& a, int* lo, int* hi) {
+    *lo = see_lo(s, a, 0) / kStep * kStep;
+    *hi = see_hi(s, a, s.q - 1);
+    // a sequence whose rows see nothing still has rows to write
+    return s.q == 0 ? 0 : max(1, (*hi - *lo + kStep - 1) / kStep);
+}
+
+// The whole wave: the cut of the batch, and the sequence that `find` (given the cut)
+// falls into, with the number of its first step.
+template <class F>
+__device__ inline Cut cut_of(const KvCache& c, const KvBatch& b, const KvAttend& a, const Plan& p,
+                             int lane, F find, int* seq, int64_t* first) {
+    auto steps = [&](int s) {
+        int lo, hi;
+        return s < b.n_seq ? steps_of(kv_seq(b, s, c.shift), a, &lo, &hi) : 0;
+    };
+    const int own = steps(lane);  // of the first 64 sequences, kept
+    int64_t sum = own;
+    for (int s = lane + 64; s < b.n_seq; s += 64) sum += steps(s);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+    Cut r;
+    r.total = sum * c.H;
+    r.per = max(static_cast<int64_t>(kLeast), (r.total + p.workers - 1) / p.workers);
+    const int64_t at = find(r);
+    *seq = -1;
+    int64_t base = 0;
+    for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
+        const int n = s0 ? steps(s0 + lane) : own;
+        int64_t in = n;  // inclusive sum
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t y = __shfl_up(in, o);
+            if (lane >= o) in += y;
+        }
+        const uint64_t hit = __ballot((base + in) * c.H > at);
+        if (hit) {
+            const int k = __builtin_ctzll(hit);
+            *seq = s0 + k;
+            *first = (base + __shfl(in - n, k)) * c.H;
+            break;
+        }
+        base += __shfl(in, 63);
+    }
+    return r;
+}
+
+// Streaming waves on a SIMD: two hide each other's latencies as long as a wave's
+// sums, operands and loads in flight fit half of its registers.
+template <int D, int NT>
+constexpr int kStreamWaves = D * NT >= 256 ? 1 : 2;
+
+template <int BITS, int D, int NT>
+__global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
+    __shared__ __align__(16) float sc[4][192];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int worker = blockIdx.x * 4 + wave;
+    int seq;
+    int64_t first;
+    const Cut cut = cut_of(
+        c, b, a, p, lane, [&](const Cut& r) { return worker * r.per; }, &seq, &first);
+    int64_t at = worker * cut.per;
+    const int64_t end = min(at + cut.per, cut.total);
+    if (at >= end) return;
+    Share w;
+    w.seq = seq;
+    w.split = 0;
+    w.r0 = 0;
+    w.s = kv_seq(b, seq, c.shift);
+    int lo, hi, n = steps_of(w.s, a, &lo, &hi);
+    w.head = static_cast<int>((at - first) / n);
+    int from = static_cast<int>((at - first) % n);
+    while (true) {
+        const int to = static_cast<int>(min(static_cast<int64_t>(n), from + (end - at)));
+        w.rn = w.s.q * a.G;
+        if (!w.s.ok) {
+            fail_rows<D>(w, a, lane, 64);
+        } else {
+            span_of(w, a);
+            w.lo = lo + from * kStep;
+            w.hi = min(hi, lo + to * kStep);
+            Rows<BITS, D, NT> rows;
+            Stream<BITS, D, NT> st(c, b, w, lane);
+            rows.start(w, a, 0, lane);
+            st.open(w.lo, kStep);
+            const float f = rows.scale(a, rows.largest(a)) * (a.scale * kLog2e);
+            st.run(rows, w.lo, kStep, f, sc[wave]);
+            if (from == 0 && to == n)
+                finish<BITS, D, NT>(w, a, 0, lane, rows);
+            else
+                keep<D, NT>(a.work, 2 * worker + (from == 0), 2 * p.workers, lane, rows.o, rows.m,
+                            rows.l);
+        }
+        at += to - from;
+        if (at >= end) return;
+        from = 0;
+        if (++w.head == c.H) {
+            w.head = 0;
+            do {
+                w.s = kv_seq(b, ++w.seq, c.shift);
+                n = steps_of(w.s, a, &lo, &hi);
+            } while (n == 0);
+        }
+    }
+}
+
+// Adds the parts of a row: one workgroup per row of a head, its waves take every
+// fourth part.
+template <int D, int NT>
+__global__ __launch_bounds__(256) void kv_stream_join_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
+    constexpr int E = D / 64, R = NT * 16;
+    __shared__ __align__(16) float acc[4][D];
+    __shared__ float ls[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int per_seq = b.max_q * a.heads;
+    const int s0 = blockIdx.x / per_seq, in = blockIdx.x % per_seq;
+    const int i = in / a.heads, hq = in % a.heads, head = hq / a.G;
+    const KvSeq s = kv_seq(b, s0, c.shift);
+    if (i >= s.q || !s.ok) return;  // fail_rows has written the rows of those that are not ok
+    int lo, hi;
+    const int n = steps_of(s, a, &lo, &hi);
+    // the number of this sequence's first step
+    int64_t before = 0, all = 0;
+    for (int x = lane; x < b.n_seq; x += 64) {
+        int y, z;
+        const int64_t k = steps_of(kv_seq(b, x, c.shift), a, &y, &z);
+        all += k;
+        if (x < s0) before += k;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        all += __shfl_xor(all, o);
+        before += __shfl_xor(before, o);
+    }
+    const int64_t per = max(static_cast<int64_t>(kLeast), (all * c.H + p.workers - 1) / p.workers);
+    const int64_t first = before * c.H + static_cast<int64_t>(head) * n;
+    const int w0 = static_cast<int>(first / per), w1 = static_cast<int>((first + n - 1) / per);
+    if (w0 == w1) return;  // one wave had it all and has written it
+    const int row = i * a.G + hq - head * a.G;
+    const float* const parts = a.work;
+    const float* const stats = a.work + static_cast<int64_t>(2 * p.workers) * R * D;
+    auto slot = [&](int w) { return static_cast<int64_t>(2 * w + (w == w0)) * R + row; };
+    float m = kNone;
+    for (int w = w0 + lane; w <= w1; w += 64) m = fmaxf(m, stats[slot(w) * 2]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    float l = 0.0f, x[E] = {};
+    for (int w = w0 + wave; w <= w1; w += 4) {
+        const int64_t k = slot(w);
+        const float f = __builtin_amdgcn_exp2f(stats[k * 2] - m);
+        l = fmaf(stats[k * 2 + 1], f, l);
+#pragma unroll
+        for (int e = 0; e < E; e++) x[e] = fmaf(parts[k * D + e * 64 + lane], f, x[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[wave][e * 64 + lane] = x[e];
+    if (lane == 0) ls[wave] = l;
+    __syncthreads();
+    if (threadIdx.x >= D / 4) return;
+    l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    const int e = threadIdx.x * 4;
+    f4 o = {0, 0, 0, 0};
+#pragma unroll
+    for (int y = 0; y < 4; y++) o += *reinterpret_cast<const f4*>(acc[y] + e);
+    const int64_t at = (s.row + i) * a.heads + hq;
+    store4(a, at * D + e, o * (l == 0.0f ? 0.0f : 1.0f / l));
+    if (a.lse && e == 0) a.lse[at] = lse_of(m, l);
 }
 
 // Many rows: 64 NC of them, 16 NC a wave.  What bounds it are the matrix cores and
@@ -611,18 +829,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_many_kernel(KvCache 
     const int g = lane >> 4, r = lane & 15;
     const Share w = share_of(c, b, a, p);
     if (!w.any) return;
-    if (!w.s.ok) return fail_rows<D>(w, a, p);
-    if (p.nsplit > 1 && w.lo >= w.hi) return;
+    if (!w.s.ok) {
+        if (w.split == 0) fail_rows<D>(w, a, threadIdx.x, 256);
+        return;
+    }
+    if (p.nsplit > 1 && w.lo >= w.hi) return;  // the join knows which parts there are
 
     Rows<BITS, D, NC> rows;
     const int r0 = w.r0 + wave * NC * 16;
-    float big = rows.start(w, a, r0, lane);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
+    rows.start(w, a, r0, lane);
+    float big = rows.largest(a);
     if (lane == 0) bigs[wave] = big;
     __syncthreads();
     big = fmaxf(fmaxf(bigs[0], bigs[1]), fmaxf(bigs[2], bigs[3]));
-    const float f = rows.load(w, a, r0, lane, big) * (a.scale * kLog2e);
+    const float f = rows.scale(a, big) * (a.scale * kLog2e);
     const int in_page = (1 << c.shift) - 1;
     // A wave stages the key tile `wave` and the value tiles wave, wave + 4, ...
     constexpr int VT = (M::ET + 3) / 4;
@@ -635,9 +855,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_many_kernel(KvCache 
         const int pk = jk < w.s.n ? kv_page(b, c, w.seq, jk) : -1;
         const int pv = jv < w.s.n ? kv_page(b, c, w.seq, jv) : -1;
         const uint8_t* k = kv_block(c, max(pk, 0), w.head) + (jk & in_page) * M::ROW + (r & 3) * 16 +
-                           wave * 64 + (M::LB == 8 ? (g >> 1) * 256 + (g & 1) * 8 : g * 256);
+                           wave * (4 * M::ROW) + (M::LB == 8 ? (g >> 1) * 64 + (g & 1) * 8 : g * 64);
 #pragma unroll
-        for (int u = 0; u < M::NU; u++) kr[u] = *reinterpret_cast<const K*>(k + u * 1024);
+        for (int u = 0; u < M::NU; u++) kr[u] = *reinterpret_cast<const K*>(k + u * 256);
         const uint8_t* const blk = kv_block(c, max(pv, 0), w.head);
         const uint8_t* v = blk + c.codes + (jv & in_page) * M::ROW + r * 16;
 #pragma unroll
@@ -717,10 +937,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_many_kernel(KvCache 
         __syncthreads();
     }
     rows.join();
-    finish<BITS, D, NC>(w, a, p, r0, lane, rows);
+    if (p.nsplit == 1) return finish<BITS, D, NC>(w, a, r0, lane, rows);
+#pragma unroll
+    for (int k = 0; k < NC; k++) {
+        const int row = r0 + k * 16 + r;
+        if (row >= w.r0 + w.rn) continue;
+        int64_t q;
+        const int64_t o = w.split * p.rows + row_of(w, a, row, &q);
+#pragma unroll
+        for (int t = 0; t < M::DT; t++)
+            *reinterpret_cast<f4*>(a.work + o * D + t * 16 + g * 4) = rows.o[k][t];
+        if (g == 0) {
+            float* const ml = a.work + p.nsplit * p.rows * D + o * 2;
+            ml[0] = rows.m[k];
+            ml[1] = rows.l[k];
+        }
+    }
 }
 
-// Joins the parts of a row: one wave per output row.  Which parts there are
+// Joins the parts of a row of many: one wave per output row.  Which parts there are
 // follows from the row's tile as in share_of.
 template <int D>
 __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
@@ -762,62 +997,107 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAt
     if (a.lse && lane == 0) a.lse[o] = lse_of(m, l);
 }
 
-Plan plan_of(const KvCache& c, const KvBatch& b, int D, int G, int window) {
+// What a call runs: 16 or 32 rows from registers (short or streaming), or tiles of 64 or
+// 128 rows through LDS.
+enum class Path { kShort, kStream, kMany };
+struct Choice {
+    Path path;
+    int nc;  // column tiles of a wave
     Plan p;
+    int64_t work;  // bytes
+};
+
+Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
+    Choice r;
+    Plan& p = r.p;
     const int64_t rows = static_cast<int64_t>(b.max_q) * G;
-    p.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
-    p.nc = p.few ? 0 : rows <= 64 ? 1 : 2;
-    p.tile = p.few ? p.few * 16 : p.nc * 64;
+    const int64_t span = window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) + b.max_q + kStep)
+                                : b.max_kv;
+    r.path = rows > 32 ? Path::kMany : span <= kShortSpan ? Path::kShort : Path::kStream;
+    r.nc = r.path == Path::kMany ? (rows <= 64 ? 1 : 2) : (rows <= 16 ? 1 : 2);
+    p.tile = r.path == Path::kMany ? r.nc * 64 : r.nc * 16;
     p.tiles = static_cast<int>((rows + p.tile - 1) / p.tile);
     p.rows = b.n_tokens * c.H * G;
-    // workgroups without a split: no more tiles than the rows fill
-    const int64_t tiles = std::min<int64_t>(static_cast<int64_t>(b.n_seq) * p.tiles,
-                                            b.n_tokens * G / p.tile + b.n_seq) * c.H;
-    const int64_t span =
-        window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) + p.tile / G + 2 + kStep)
-               : b.max_kv;
-    constexpr int64_t want = 1024;
-    int64_t chunk = std::max<int64_t>(512, span * tiles / want);
-    chunk = (chunk + kStep - 1) / kStep * kStep;
-    p.nsplit = static_cast<int>(std::max<int64_t>(1, (span + chunk - 1) / chunk));
-    p.chunk = p.nsplit == 1 ? 1 << 30 : static_cast<int>(chunk);
-    return p;
+    p.nsplit = 1;
+    p.chunk = 0;
+    p.workers = 0;
+    r.work = 0;
+    if (r.path == Path::kStream) {
+        p.workers = 1024 * (D * r.nc >= 256 ? 1 : 2);  // kStreamWaves on each of the chip's SIMDs
+        r.work = static_cast<int64_t>(2 * p.workers) * p.tile * (D + 2) * 4;
+    } else if (r.path == Path::kMany) {
+        // workgroups without a split: no more tiles than the rows fill
+        const int64_t tiles = std::min<int64_t>(static_cast<int64_t>(b.n_seq) * p.tiles,
+                                                b.n_tokens * G / p.tile + b.n_seq) * c.H;
+        const int64_t seen = window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) +
+                                                                      p.tile / G + 2 + kStep)
+                                    : b.max_kv;
+        constexpr int64_t want = 1024;
+        int64_t chunk = std::max<int64_t>(512, seen * tiles / want);
+        chunk = (chunk + kStep - 1) / kStep * kStep;
+        p.nsplit = static_cast<int>(std::max<int64_t>(1, (seen + chunk - 1) / chunk));
+        if (p.nsplit > 1) {
+            p.chunk = static_cast<int>(chunk);
+            r.work = p.nsplit * p.rows * (D + 2) * 4;
+        }
+    }
+    return r;
 }
 
 template <int BITS, int D>
-hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const Plan& p, hipStream_t s) {
-    const int64_t blocks = static_cast<int64_t>(c.H) * b.n_seq * p.tiles * p.nsplit;
-    const int64_t joins = (static_cast<int64_t>(b.n_seq) * b.max_q * a.heads + 3) / 4;
-    // rows and positions are ints in the kernels
+hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const Choice& ch,
+                  hipStream_t s) {
+    const Plan& p = ch.p;
+    // rows and positions are ints in the kernels, and a launch has 2^32 threads
     if (static_cast<int64_t>(b.max_q) * a.G > 1 << 30) return hipErrorInvalidValue;
-    if (blocks >= 1 << 24 || (p.nsplit > 1 && joins >= 1 << 24)) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(blocks));
-    if (p.few == 1)
-        kv_few_kernel<BITS, D, 1><<<grid, 256, 0, s>>>(c, b, a, p);
-    else if (p.few == 2)
-        kv_few_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
-    else if (p.nc == 1)
-        kv_many_kernel<BITS, D, 1><<<grid, 256, 0, s>>>(c, b, a, p);
-    else
-        kv_many_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess && p.nsplit > 1) {
-        kv_join_kernel<D><<<static_cast<unsigned>(joins), 256, 0, s>>>(c, b, a, p);
-        e = hipGetLastError();
+    const int64_t out = static_cast<int64_t>(b.n_seq) * b.max_q * a.heads;
+    const int64_t blocks = ch.path == Path::kStream ? p.workers / 4
+                                                    : static_cast<int64_t>(c.H) * b.n_seq * p.tiles * p.nsplit;
+    const int64_t joins = ch.path == Path::kStream ? out : p.nsplit > 1 ? (out + 3) / 4 : 0;
+    if (blocks >= 1 << 23 || joins >= 1 << 23) return hipErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>(blocks)), jgrid(static_cast<unsigned>(joins));
+    switch (ch.path) {
+        case Path::kShort:
+            if (ch.nc == 1)
+                kv_short_kernel<BITS, D, 1, kShortWaves<D, 1>>
+                    <<<grid, 64 * kShortWaves<D, 1>, 0, s>>>(c, b, a, p);
+            else
+                kv_short_kernel<BITS, D, 2, kShortWaves<D, 2>>
+                    <<<grid, 64 * kShortWaves<D, 2>, 0, s>>>(c, b, a, p);
+            break;
+        case Path::kStream:
+            if (ch.nc == 1)
+                kv_stream_kernel<BITS, D, 1><<<grid, 256, 0, s>>>(c, b, a, p);
+            else
+                kv_stream_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
+            break;
+        case Path::kMany:
+            if (ch.nc == 1)
+                kv_many_kernel<BITS, D, 1><<<grid, 256, 0, s>>>(c, b, a, p);
+            else
+                kv_many_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
+            break;
     }
-    return e;
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || joins == 0) return e;
+    if (ch.path == Path::kMany)
+        kv_join_kernel<D><<<jgrid, 256, 0, s>>>(c, b, a, p);
+    else if (ch.nc == 1)
+        kv_stream_join_kernel<D, 1><<<jgrid, 256, 0, s>>>(c, b, a, p);
+    else
+        kv_stream_join_kernel<D, 2><<<jgrid, 256, 0, s>>>(c, b, a, p);
+    return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t kv_attend_work(const KvCache& c, const KvBatch& b, int D, int G, int window) {
-    const Plan p = plan_of(c, b, D, G, window);
-    return p.nsplit > 1 ? p.nsplit * p.rows * (D + 2) * 4 : 0;
+    return choose(c, b, D, G, window).work;
 }
 
 hipError_t kv_attend(const KvCache& c, const KvBatch& b, int bits, int D, const KvAttend& a,
                      hipStream_t s) {
-    const Plan p = plan_of(c, b, D, a.G, a.window);
+    const Choice p = choose(c, b, D, a.G, a.window);
     if (bits == 8)
         return D == 64 ? launch<8, 64>(c, b, a, p, s)
                        : D == 128 ? launch<8, 128>(c, b, a, p, s) : launch<8, 256>(c, b, a, p, s);

@@ -14,10 +14,10 @@ constexpr int kKvGroup = 16;
 
 // The cache as kernels see it.  Block (page, head) starts at
 // base + (page * H + head) * block; in it
-//   [0, codes)            key codes: group g, piece p, token r: the 16 bytes at
-//                         (g * 16 * row) + p * 256 + r * 16
-//   [codes, 2 codes)      value codes: group g, byte column e, token r: the byte
-//                         at (g * 16 * row) + e * 16 + r
+//   [0, codes)            key codes, 4 tokens after 4 tokens: piece p of token t: the
+//                         16 bytes at (t / 4) * 4 * row + p * 64 + (t % 4) * 16
+//   [codes, 2 codes)      value codes, 16 tokens after 16 tokens: byte column e of
+//                         token t: the byte at (t / 16) * 16 * row + e * 16 + t % 16
 //   then page_size key scales and page_size value scales (float)
 // with row = D * bits / 8 bytes per token.  A code is stored unsigned, c + 128
 // in 8 bits and c + 8 in 4.  Byte e of a row holds element e in 8 bits, and

@@ -187,6 +187,12 @@ __device__ inline int group_page(const KvCache& c, const KvBatch& b, const Unit&
     return g < u.q.n ? kv_page(b, c, u.seq, g) : -1;
 }
 
+// Where piece p of the token in a slot of its page starts among the key codes.
+template <int ROW>
+__device__ inline int key_at(int slot, int p) {
+    return (slot & ~3) * ROW + p * 64 + (slot & 3) * 16;
+}
+
 // What a lane of a transposed unit holds: a byte column of piece `piece` (and
 // its later pieces) of token group `group` of the run, and which of that
 // group's tokens are to be moved.
@@ -298,8 +304,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatc
         }
         if (!u.value) {
             if (live)
-                *reinterpret_cast<u32x4*>(codes + (slot & ~15) * ROW + (lc + i * L::LP) * 256 +
-                                          (slot & 15) * 16) = w;
+                *reinterpret_cast<u32x4*>(codes + key_at<ROW>(slot, lc + i * L::LP)) = w;
             continue;
         }
         w = transpose16(lds[wave], lane, (t >> 4) * L::LP + lc, t & 15, lane >> 4, lane & 15, w);
@@ -356,8 +361,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvCache c, KvBatch
                     ocodes + ((o.piece + i * L::LP) * 16 + (lane & 15)) * 16);
             w = transpose16(lds[wave], lane, lane >> 4, lane & 15, (t >> 4) * L::LP + lc, t & 15, w);
         } else if (live && page >= 0) {
-            w = *reinterpret_cast<const u32x4*>(codes + (slot & ~15) * ROW +
-                                                (lc + i * L::LP) * 256 + (slot & 15) * 16);
+            w = *reinterpret_cast<const u32x4*>(codes + key_at<ROW>(slot, lc + i * L::LP));
         }
         float x[E];
 #pragma unroll
