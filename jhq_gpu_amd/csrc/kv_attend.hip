@@ -35,6 +35,7 @@ namespace {
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
@@ -44,6 +45,9 @@ constexpr int kShortSpan = 1024;   // tokens that one workgroup takes alone
 constexpr float kNone = -1e30f;    // running maximum before the first token
 constexpr float kSlack = 8.0f;     // how far a score may pass it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// The wave's number in its workgroup, as a value the compiler knows to be uniform.
+__device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 __device__ inline float nan32() { return __uint_as_float(0x7fc00000u); }
 
@@ -120,7 +124,7 @@ __device__ inline float value16(const KvAttend& a, uint32_t h) {
 struct Plan {
     int tile;     // rows of a tile
     int tiles;    // tiles of a sequence with max_q new tokens
-    int workers;  // of the streaming kernel
+    int log_workers;  // of the streaming kernel, a power of two
     int nsplit;   // parts that a tile's tokens may be cut into (many rows)
     int chunk;    // tokens of a part, a multiple of kStep
     int64_t rows; // of the partial results: n_tokens * query heads
@@ -237,23 +241,38 @@ struct Rows {
         return value16(a, v[i >> 1] >> (16 * (i & 1)) & 0xffff);
     }
 
-    // The largest finite magnitude of the wave's query elements.
+    // The largest finite magnitude of the wave's query elements: magnitudes of
+    // either type are in the order of their bits.
     __device__ float largest(const KvAttend& a) const {
-        float big = 0.0f;
+        const uint32_t inf = a.dtype == JHQ_BF16 ? 0x7f80 : 0x7c00;
+        us2 two = {0, 0};
 #pragma unroll
         for (int k = 0; k < NC; k++)
 #pragma unroll
             for (int s = 0; s < M::KS; s++) {
                 const u4 v = __builtin_bit_cast(u4, q[k][s]);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float x = fabsf(element(a, v, i));
-                    big = x < INFINITY ? fmaxf(big, x) : big;
-                }
+                for (int i = 0; i < 4; i++)
+                    two = __builtin_elementwise_max(two, __builtin_bit_cast(us2, v[i] & 0x7fff7fffu));
             }
+        uint32_t big = max(two[0], two[1]);
+        if (__any(big >= inf)) {
+            big = 0;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
-        return big;
+            for (int k = 0; k < NC; k++)
+#pragma unroll
+                for (int s = 0; s < M::KS; s++) {
+                    const u4 v = __builtin_bit_cast(u4, q[k][s]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t x = v[i] & 0x7fff, y = v[i] >> 16 & 0x7fff;
+                        big = max(big, max(x < inf ? x : 0, y < inf ? y : 0));
+                    }
+                }
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), o)));
+        return value16(a, big);
     }
 
     // Turns the queries to operands, scaled by the power of two that takes big to
@@ -461,11 +480,12 @@ __device__ void finish(const Share& w, const KvAttend& a, int r0, int lane,
 
 // A part of a wave's rows: 16 NC sums per slot, then every slot's maxima and sums.
 template <int D, int NC>
-__device__ void keep(float* work, int64_t slot, int64_t slots, int lane, const f4 (&o)[NC][D / 16],
+__device__ void keep(float* work, int64_t slot, int64_t slots, int rows, int lane, const f4 (&o)[NC][D / 16],
                      const float (&m)[NC], const float (&l)[NC]) {
     const int g = lane >> 4;
 #pragma unroll
     for (int k = 0; k < NC; k++) {
+        if (k * 16 + (lane & 15) >= rows) continue;
         const int64_t row = slot * (NC * 16) + k * 16 + (lane & 15);
 #pragma unroll
         for (int t = 0; t < D / 16; t++)
@@ -578,7 +598,7 @@ struct Stream {
 // sequence's head, its W waves take every W-th step, and what they have is joined
 // in LDS, so that one launch does it.
 template <int D, int NT>
-constexpr int kShortWaves = 8 * NT * 16 * (D + 4) * 4 <= 140 * 1024 ? 8 : 4;
+constexpr int kShortWaves = D == 256 ? 4 : 8;
 
 template <int BITS, int D, int NT, int W>
 __global__ __launch_bounds__(64 * W, W / 4) void kv_short_kernel(KvCache c, KvBatch b, KvAttend a,
@@ -588,7 +608,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv_short_kernel(KvCache c, KvBa
     __shared__ __align__(16) float sc[W][192];
     __shared__ __align__(16) float acc[W][R * P];
     __shared__ float ml[W][R][2];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = wave_id();
     const int g = lane >> 4, r = lane & 15;
     const Share w = share_of(c, b, a, p);
     if (!w.any) return;
@@ -636,11 +656,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv_short_kernel(KvCache c, KvBa
 // whatever their lengths; a wave works alone, from a step within one head to a
 // step within another.  What it begins or ends in the middle of a head is kept as
 // a part (two at most for a wave: slot 0 where the head began before it, 1 where it
-// goes on after it), and kv_stream_join_kernel adds the parts.
-struct Cut {
-    int64_t total;  // steps of the batch
-    int64_t per;    // of a worker
-};
+// goes on after it), and kv_join_kernel adds the parts.  The wave that begins a
+// head notes which waves have parts of it.
 
 // Steps of sequence s (a head of it); 0 where it has no new token.
 __device__ inline int steps_of(const KvSeq& s, const KvAttend& a, int* lo, int* hi) {
@@ -650,44 +667,67 @@ __device__ inline int steps_of(const KvSeq& s, const KvAttend& a, int* lo, int* 
     return s.q == 0 ? 0 : max(1, (*hi - *lo + kStep - 1) / kStep);
 }
 
-// The whole wave: the cut of the batch, and the sequence that `find` (given the cut)
-// falls into, with the number of its first step.
-template <class F>
-__device__ inline Cut cut_of(const KvCache& c, const KvBatch& b, const KvAttend& a, const Plan& p,
-                             int lane, F find, int* seq, int64_t* first) {
-    auto steps = [&](int s) {
-        int lo, hi;
-        return s < b.n_seq ? steps_of(kv_seq(b, s, c.shift), a, &lo, &hi) : 0;
-    };
-    const int own = steps(lane);  // of the first 64 sequences, kept
-    int64_t sum = own;
-    for (int s = lane + 64; s < b.n_seq; s += 64) sum += steps(s);
+__device__ inline int wave_sum(int x) {
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+// The lane's sequence of 64, no new token past the last.
+__device__ inline KvSeq lane_seq(const KvCache& c, const KvBatch& b, int s) {
+    if (s < b.n_seq) return kv_seq(b, s, c.shift);
+    return {0, 0, 0, true};
+}
+
+// A wave's first step: where it lies, and how many there are.
+struct Cut {
+    int per, at, end;  // steps of a wave; this wave's
+    int seq, first;    // the sequence of `at`, and the number of its first step
+    KvSeq s;
+};
+
+__device__ inline Cut cut_of(const KvCache& c, const KvBatch& b, const KvAttend& a, const Plan& p,
+                             int worker, int lane) {
+    int lo, hi;
+    const KvSeq s0 = lane_seq(c, b, lane);
+    const int n0 = steps_of(s0, a, &lo, &hi);
+    int sum = n0;
+    for (int s = lane + 64; s < b.n_seq; s += 64) sum += steps_of(lane_seq(c, b, s), a, &lo, &hi);
     Cut r;
-    r.total = sum * c.H;
-    r.per = max(static_cast<int64_t>(kLeast), (r.total + p.workers - 1) / p.workers);
-    const int64_t at = find(r);
-    *seq = -1;
-    int64_t base = 0;
-    for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
-        const int n = s0 ? steps(s0 + lane) : own;
-        int64_t in = n;  // inclusive sum
+    const int total = __builtin_amdgcn_readfirstlane(wave_sum(sum)) * c.H;
+    r.per = max(kLeast, (total + (1 << p.log_workers) - 1) >> p.log_workers);
+    r.at = min(static_cast<int64_t>(worker) * r.per, static_cast<int64_t>(total));
+    r.end = min(r.at + r.per, total);
+    if (r.at >= r.end) return r;
+    int base = 0;
+    for (int x = 0;; x += 64) {
+        const KvSeq s = x ? lane_seq(c, b, x + lane) : s0;
+        const int n = x ? steps_of(s, a, &lo, &hi) : n0;
+        int in = n;  // inclusive sum
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const int64_t y = __shfl_up(in, o);
+            const int y = __shfl_up(in, o);
             if (lane >= o) in += y;
         }
-        const uint64_t hit = __ballot((base + in) * c.H > at);
+        const uint64_t hit = __ballot((base + in) * c.H > r.at);
         if (hit) {
             const int k = __builtin_ctzll(hit);
-            *seq = s0 + k;
-            *first = (base + __shfl(in - n, k)) * c.H;
-            break;
+            r.seq = x + k;
+            r.first = (base + __builtin_amdgcn_readlane(in - n, k)) * c.H;
+            r.s.row = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(s.row), k));
+            r.s.q = __builtin_amdgcn_readlane(s.q, k);
+            r.s.n = __builtin_amdgcn_readlane(s.n, k);
+            r.s.ok = __builtin_amdgcn_readlane(s.ok, k);
+            return r;
         }
-        base += __shfl(in, 63);
+        base += __builtin_amdgcn_readlane(in, 63);
     }
-    return r;
+}
+
+// Per sequence and head: the wave that begins it, and how many more have parts.
+template <int D, int NT>
+__device__ inline int2* joins_of(const KvAttend& a, const Plan& p) {
+    return reinterpret_cast<int2*>(a.work + (int64_t(2) << p.log_workers) * (NT * 16) * (D + 2));
 }
 
 // Streaming waves on a SIMD: two hide each other's latencies as long as a wave's
@@ -698,25 +738,23 @@ constexpr int kStreamWaves = D * NT >= 256 ? 1 : 2;
 template <int BITS, int D, int NT>
 __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
     __shared__ __align__(16) float sc[4][192];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = wave_id();
     const int worker = blockIdx.x * 4 + wave;
-    int seq;
-    int64_t first;
-    const Cut cut = cut_of(
-        c, b, a, p, lane, [&](const Cut& r) { return worker * r.per; }, &seq, &first);
-    int64_t at = worker * cut.per;
-    const int64_t end = min(at + cut.per, cut.total);
-    if (at >= end) return;
+    const Cut cut = cut_of(c, b, a, p, worker, lane);
+    if (cut.at >= cut.end) return;
+    int at = cut.at;
     Share w;
-    w.seq = seq;
+    w.seq = cut.seq;
     w.split = 0;
     w.r0 = 0;
-    w.s = kv_seq(b, seq, c.shift);
+    w.s = cut.s;
     int lo, hi, n = steps_of(w.s, a, &lo, &hi);
-    w.head = static_cast<int>((at - first) / n);
-    int from = static_cast<int>((at - first) % n);
+    w.head = (at - cut.first) / n;
+    int from = (at - cut.first) % n;
     while (true) {
-        const int to = static_cast<int>(min(static_cast<int64_t>(n), from + (end - at)));
+        const int to = min(n, from + (cut.end - at));
+        if (from == 0 && lane == 0)
+            joins_of<D, NT>(a, p)[w.seq * c.H + w.head] = int2{worker, (at + n - 1) / cut.per - worker};
         w.rn = w.s.q * a.G;
         if (!w.s.ok) {
             fail_rows<D>(w, a, lane, 64);
@@ -733,11 +771,11 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
             if (from == 0 && to == n)
                 finish<BITS, D, NT>(w, a, 0, lane, rows);
             else
-                keep<D, NT>(a.work, 2 * worker + (from == 0), 2 * p.workers, lane, rows.o, rows.m,
-                            rows.l);
+                keep<D, NT>(a.work, 2 * worker + (from == 0), 2 << p.log_workers, w.rn, lane,
+                            rows.o, rows.m, rows.l);
         }
         at += to - from;
-        if (at >= end) return;
+        if (at >= cut.end) return;
         from = 0;
         if (++w.head == c.H) {
             w.head = 0;
@@ -747,69 +785,6 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
             } while (n == 0);
         }
     }
-}
-
-// Adds the parts of a row: one workgroup per row of a head, its waves take every
-// fourth part.
-template <int D, int NT>
-__global__ __launch_bounds__(256) void kv_stream_join_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
-    constexpr int E = D / 64, R = NT * 16;
-    __shared__ __align__(16) float acc[4][D];
-    __shared__ float ls[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int per_seq = b.max_q * a.heads;
-    const int s0 = blockIdx.x / per_seq, in = blockIdx.x % per_seq;
-    const int i = in / a.heads, hq = in % a.heads, head = hq / a.G;
-    const KvSeq s = kv_seq(b, s0, c.shift);
-    if (i >= s.q || !s.ok) return;  // fail_rows has written the rows of those that are not ok
-    int lo, hi;
-    const int n = steps_of(s, a, &lo, &hi);
-    // the number of this sequence's first step
-    int64_t before = 0, all = 0;
-    for (int x = lane; x < b.n_seq; x += 64) {
-        int y, z;
-        const int64_t k = steps_of(kv_seq(b, x, c.shift), a, &y, &z);
-        all += k;
-        if (x < s0) before += k;
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        all += __shfl_xor(all, o);
-        before += __shfl_xor(before, o);
-    }
-    const int64_t per = max(static_cast<int64_t>(kLeast), (all * c.H + p.workers - 1) / p.workers);
-    const int64_t first = before * c.H + static_cast<int64_t>(head) * n;
-    const int w0 = static_cast<int>(first / per), w1 = static_cast<int>((first + n - 1) / per);
-    if (w0 == w1) return;  // one wave had it all and has written it
-    const int row = i * a.G + hq - head * a.G;
-    const float* const parts = a.work;
-    const float* const stats = a.work + static_cast<int64_t>(2 * p.workers) * R * D;
-    auto slot = [&](int w) { return static_cast<int64_t>(2 * w + (w == w0)) * R + row; };
-    float m = kNone;
-    for (int w = w0 + lane; w <= w1; w += 64) m = fmaxf(m, stats[slot(w) * 2]);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-    float l = 0.0f, x[E] = {};
-    for (int w = w0 + wave; w <= w1; w += 4) {
-        const int64_t k = slot(w);
-        const float f = __builtin_amdgcn_exp2f(stats[k * 2] - m);
-        l = fmaf(stats[k * 2 + 1], f, l);
-#pragma unroll
-        for (int e = 0; e < E; e++) x[e] = fmaf(parts[k * D + e * 64 + lane], f, x[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < E; e++) acc[wave][e * 64 + lane] = x[e];
-    if (lane == 0) ls[wave] = l;
-    __syncthreads();
-    if (threadIdx.x >= D / 4) return;
-    l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
-    const int e = threadIdx.x * 4;
-    f4 o = {0, 0, 0, 0};
-#pragma unroll
-    for (int y = 0; y < 4; y++) o += *reinterpret_cast<const f4*>(acc[y] + e);
-    const int64_t at = (s.row + i) * a.heads + hq;
-    store4(a, at * D + e, o * (l == 0.0f ? 0.0f : 1.0f / l));
-    if (a.lse && e == 0) a.lse[at] = lse_of(m, l);
 }
 
 // Many rows: 64 NC of them, 16 NC a wave.  What bounds it are the matrix cores and
@@ -825,7 +800,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_many_kernel(KvCache 
     __shared__ __align__(16) h8 vf[2][2 * M::DT * 64];   // [half][tile][lane]
     __shared__ __align__(16) float sc[2][192];
     __shared__ float bigs[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = wave_id();
     const int g = lane >> 4, r = lane & 15;
     const Share w = share_of(c, b, a, p);
     if (!w.any) return;
@@ -955,46 +930,86 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_many_kernel(KvCache 
     }
 }
 
-// Joins the parts of a row of many: one wave per output row.  Which parts there are
-// follows from the row's tile as in share_of.
+// Adds the parts of rows, a thread 4 elements of every fourth part of a row; latency
+// bounds it.  NT > 0: parts of kv_stream_kernel, rows in the order (sequence, head,
+// row); 0: of kv_many_kernel, (sequence, new token, query head).
 template <int D>
+constexpr int kJoinRows = 256 / D;  // rows of a workgroup
+
+template <int D, int NT>
 __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t x = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int per = b.max_q * a.heads;
-    const int seq = static_cast<int>(x / per), in = static_cast<int>(x % per);
-    if (seq >= b.n_seq) return;
-    const int i = in / a.heads, h = in % a.heads;
-    const KvSeq s = kv_seq(b, seq, c.shift);
-    if (i >= s.q || !s.ok) return;  // fail_rows has written the rows of those that are not ok
-    const int64_t o = (s.row + i) * a.heads + h;
-    const int tile = (i * a.G + h % a.G) / p.tile;
-    const int last = min((tile + 1) * p.tile, s.q * a.G) - 1;
-    const int from = see_lo(s, a, tile * p.tile / a.G) / kStep * kStep;
-    const int hi = see_hi(s, a, last / a.G);
-    const int n = hi > from ? (hi - from + p.chunk - 1) / p.chunk : 0;
-    const float* const ml = a.work + p.nsplit * p.rows * D;
-    float m = kNone;
-    for (int k = 0; k < n; k++) m = fmaxf(m, ml[(k * p.rows + o) * 2]);
-    float l = 0.0f;
-    constexpr int E = D / 64;
-    float acc[E] = {};
-    for (int k = 0; k < n; k++) {
-        const float f = exp2f(ml[(k * p.rows + o) * 2] - m);
-        l += ml[(k * p.rows + o) * 2 + 1] * f;
-        const float* const po = a.work + (k * p.rows + o) * D + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; e++) acc[e] += po[e] * f;
+    constexpr int T = D / 4, R = kJoinRows<D>;
+    __shared__ __align__(16) float acc[R][4][D];
+    __shared__ float ml[R][4][2];
+    const int t = threadIdx.x % T, y = threadIdx.x / T % 4, r = threadIdx.x / (4 * T);
+    const int x = blockIdx.x * R + r, per = b.max_q * a.heads;
+    const int seq = x / per, in = x % per;
+    int n = 0;            // parts
+    int64_t row = 0;      // of the output
+    int64_t slot = 0, next = 0;  // the first part's row, and from one to the next
+    int64_t jump = 0;     // added from the second on
+    if (seq < b.n_seq) {
+        const KvSeq s = kv_seq(b, seq, c.shift);
+        if constexpr (NT > 0) {
+            const int rows = b.max_q * a.G, head = in / rows, k = in % rows, i = k / a.G;
+            if (i < s.q && s.ok) {
+                const int2 j = joins_of<D, NT>(a, p)[seq * c.H + head];
+                n = j.y ? j.y + 1 : 0;  // one wave had it all and has written it
+                row = (s.row + i) * a.heads + head * a.G + (k - i * a.G);
+                slot = static_cast<int64_t>(2 * j.x + 1) * (NT * 16) + k;
+                next = 2 * NT * 16;
+                jump = -NT * 16;
+            }
+        } else {
+            const int i = in / a.heads, h = in % a.heads;
+            if (i < s.q && s.ok) {
+                // as in share_of
+                const int tile = (i * a.G + h % a.G) / p.tile;
+                const int last = min((tile + 1) * p.tile, s.q * a.G) - 1;
+                const int from = see_lo(s, a, tile * p.tile / a.G) / kStep * kStep;
+                const int hi = see_hi(s, a, last / a.G);
+                n = max(1, (hi - from + p.chunk - 1) / p.chunk);
+                if (hi <= from) n = -1;  // sees nothing: no part
+                row = slot = (s.row + i) * a.heads + h;
+                next = p.rows;
+            }
+        }
     }
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    const float* const stats = a.work + (NT > 0 ? (int64_t(2) << p.log_workers) * (NT * 16) * D
+                                                : p.nsplit * p.rows * D);
+    float m = kNone, l = 0.0f;
+    f4 o = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int k = y; k < n; k += 4) {
+        const int64_t at = slot + k * next + (k ? jump : 0);
+        const float2 st = *reinterpret_cast<const float2*>(stats + at * 2);
+        const f4 v = *reinterpret_cast<const f4*>(a.work + at * D + t * 4);
+        const float big = fmaxf(m, st.x);
+        const float f0 = __builtin_amdgcn_exp2f(m - big), f1 = __builtin_amdgcn_exp2f(st.x - big);
+        l = fmaf(l, f0, st.y * f1);
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        uint16_t* const out = static_cast<uint16_t*>(a.out) + o * D + lane * E + e;
-        const float v = acc[e] * f;
-        *out = a.dtype == JHQ_BF16 ? __builtin_bit_cast(uint16_t, static_cast<__bf16>(v))
-                                   : __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+        for (int e = 0; e < 4; e++) o[e] = fmaf(o[e], f0, v[e] * f1);
+        m = big;
     }
-    if (a.lse && lane == 0) a.lse[o] = lse_of(m, l);
+    *reinterpret_cast<f4*>(acc[r][y] + t * 4) = o;
+    if (t == 0) {
+        ml[r][y][0] = m;
+        ml[r][y][1] = l;
+    }
+    __syncthreads();
+    if (y || n == 0) return;
+    l = 0.0f;
+    o = f4{0, 0, 0, 0};
+#pragma unroll
+    for (int z = 0; z < 4; z++) m = fmaxf(m, ml[r][z][0]);
+#pragma unroll
+    for (int z = 0; z < 4; z++) {
+        const float f = __builtin_amdgcn_exp2f(ml[r][z][0] - m);
+        l = fmaf(ml[r][z][1], f, l);
+        o += *reinterpret_cast<const f4*>(acc[r][z] + t * 4) * f;
+    }
+    store4(a, row * D + t * 4, o * (l == 0.0f ? 0.0f : 1.0f / l));
+    if (a.lse && t == 0) a.lse[row] = lse_of(m, l);
 }
 
 // What a call runs: 16 or 32 rows from registers (short or streaming), or tiles of 64 or
@@ -1013,18 +1028,22 @@ Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
     const int64_t rows = static_cast<int64_t>(b.max_q) * G;
     const int64_t span = window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) + b.max_q + kStep)
                                 : b.max_kv;
-    r.path = rows > 32 ? Path::kMany : span <= kShortSpan ? Path::kShort : Path::kStream;
+    // the streaming kernel numbers steps with an int
+    const bool counted = static_cast<int64_t>(b.n_seq) * c.H * (span / kStep + 2) < INT32_MAX / 2;
+    r.path = rows > 32 ? Path::kMany
+             : span <= kShortSpan ? Path::kShort : counted ? Path::kStream : Path::kMany;
     r.nc = r.path == Path::kMany ? (rows <= 64 ? 1 : 2) : (rows <= 16 ? 1 : 2);
     p.tile = r.path == Path::kMany ? r.nc * 64 : r.nc * 16;
     p.tiles = static_cast<int>((rows + p.tile - 1) / p.tile);
     p.rows = b.n_tokens * c.H * G;
     p.nsplit = 1;
     p.chunk = 0;
-    p.workers = 0;
+    p.log_workers = 0;
     r.work = 0;
     if (r.path == Path::kStream) {
-        p.workers = 1024 * (D * r.nc >= 256 ? 1 : 2);  // kStreamWaves on each of the chip's SIMDs
-        r.work = static_cast<int64_t>(2 * p.workers) * p.tile * (D + 2) * 4;
+        p.log_workers = D * r.nc >= 256 ? 10 : 11;  // kStreamWaves on each of 1024 SIMDs
+        r.work = (int64_t(2) << p.log_workers) * p.tile * (D + 2) * 4 +
+                 static_cast<int64_t>(b.n_seq) * c.H * 8;
     } else if (r.path == Path::kMany) {
         // workgroups without a split: no more tiles than the rows fill
         const int64_t tiles = std::min<int64_t>(static_cast<int64_t>(b.n_seq) * p.tiles,
@@ -1032,8 +1051,9 @@ Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
         const int64_t seen = window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) +
                                                                       p.tile / G + 2 + kStep)
                                     : b.max_kv;
-        constexpr int64_t want = 1024;
-        int64_t chunk = std::max<int64_t>(512, seen * tiles / want);
+        // no split where the tiles fill the chip (two on each of 256 CUs)
+        const int64_t parts = std::max<int64_t>(1, 512 / tiles);
+        int64_t chunk = std::max<int64_t>(512, (seen + parts - 1) / parts);
         chunk = (chunk + kStep - 1) / kStep * kStep;
         p.nsplit = static_cast<int>(std::max<int64_t>(1, (seen + chunk - 1) / chunk));
         if (p.nsplit > 1) {
@@ -1051,9 +1071,10 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const C
     // rows and positions are ints in the kernels, and a launch has 2^32 threads
     if (static_cast<int64_t>(b.max_q) * a.G > 1 << 30) return hipErrorInvalidValue;
     const int64_t out = static_cast<int64_t>(b.n_seq) * b.max_q * a.heads;
-    const int64_t blocks = ch.path == Path::kStream ? p.workers / 4
+    const int64_t blocks = ch.path == Path::kStream ? (1 << p.log_workers) / 4
                                                     : static_cast<int64_t>(c.H) * b.n_seq * p.tiles * p.nsplit;
-    const int64_t joins = ch.path == Path::kStream ? out : p.nsplit > 1 ? (out + 3) / 4 : 0;
+    const int64_t joins = ch.path == Path::kStream || p.nsplit > 1
+                              ? (out + kJoinRows<D> - 1) / kJoinRows<D> : 0;
     if (blocks >= 1 << 23 || joins >= 1 << 23) return hipErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(blocks)), jgrid(static_cast<unsigned>(joins));
     switch (ch.path) {
@@ -1081,11 +1102,11 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const C
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || joins == 0) return e;
     if (ch.path == Path::kMany)
-        kv_join_kernel<D><<<jgrid, 256, 0, s>>>(c, b, a, p);
+        kv_join_kernel<D, 0><<<jgrid, 256, 0, s>>>(c, b, a, p);
     else if (ch.nc == 1)
-        kv_stream_join_kernel<D, 1><<<jgrid, 256, 0, s>>>(c, b, a, p);
+        kv_join_kernel<D, 1><<<jgrid, 256, 0, s>>>(c, b, a, p);
     else
-        kv_stream_join_kernel<D, 2><<<jgrid, 256, 0, s>>>(c, b, a, p);
+        kv_join_kernel<D, 2><<<jgrid, 256, 0, s>>>(c, b, a, p);
     return hipGetLastError();
 }
 
