@@ -498,6 +498,52 @@ __device__ void keep(float* work, int64_t slot, int64_t slots, int rows, int lan
     }
 }
 
+// Where the bytes of a share's steps lie.  A lane's keys belong to token group
+// (lane % 16) / 4 of the step, its values and its token's scales to group lane / 16;
+// pages of a step or more are looked up once, for the whole wave.
+template <int BITS, int D>
+struct Where {
+    using M = Dim<BITS, D>;
+    const KvCache& c;
+    const KvBatch& b;
+    const Share& w;
+    const int lane;
+    int pk, pv;  // pages of the step that look() was last asked for, -1: none
+
+    __device__ Where(const KvCache& c, const KvBatch& b, const Share& w, int lane)
+        : c(c), b(b), w(w), lane(lane), pk(-1), pv(-1) {}
+
+    __device__ bool wide() const { return (1 << c.shift) >= kStep; }
+    __device__ void look(int j) {
+        if (wide()) {
+            pk = pv = j < w.s.n ? kv_page(b, c, w.seq, j) : -1;
+        } else {
+            const int jk = j + (lane >> 2 & 3) * 16, jv = j + (lane >> 4) * 16;
+            pk = jk < w.s.n ? kv_page(b, c, w.seq, jk) : -1;
+            pv = jv < w.s.n ? kv_page(b, c, w.seq, jv) : -1;
+        }
+    }
+    // Pointers of the step j that was looked up: first key byte of the lane's
+    // operand (tile t, load u at + t * 4 ROW + 256 u), first value byte (tile e at +
+    // 256 e), scales of the lane's token (keys; values a page on).
+    __device__ void find(int j, const uint8_t*& k, const uint8_t*& v, const float*& s) const {
+        const int in_page = (1 << c.shift) - 1, at = j & in_page;
+        const int g = lane >> 4, kg = lane >> 2 & 3;
+        const int klane = (lane & 3) * 16 + (M::LB == 8 ? (g >> 1) * 64 + (g & 1) * 8 : g * 64);
+        if (wide()) {
+            const uint8_t* const x = kv_block(c, max(__builtin_amdgcn_readfirstlane(pk), 0), w.head);
+            k = x + at * M::ROW + (kg * 16 * M::ROW + klane);
+            v = x + (c.codes + at * M::ROW) + (g * 16 * M::ROW + (lane & 15) * 16);
+            s = reinterpret_cast<const float*>(x + (2 * c.codes + at * 4)) + lane;
+        } else {
+            const uint8_t* const y = kv_block(c, max(pv, 0), w.head);
+            k = kv_block(c, max(pk, 0), w.head) + ((j + kg * 16) & in_page) * M::ROW + klane;
+            v = y + c.codes + ((j + g * 16) & in_page) * M::ROW + (lane & 15) * 16;
+            s = reinterpret_cast<const float*>(y + 2 * c.codes) + ((j + lane) & in_page);
+        }
+    }
+};
+
 // The cache's bytes of one head as a wave with few rows reads them: keys and
 // values go from memory to registers as operands, the next step's loads are
 // issued as soon as this step has used the registers.
@@ -506,55 +552,44 @@ struct Stream {
     using M = Dim<BITS, D>;
     using K = typename KeyReg<M::LB>::type;
     const KvCache& c;
-    const KvBatch& b;
     const Share& w;
-    const int lane, g, r;
+    const int lane;
+    Where<BITS, D> where;
     K kr[4][M::NU];
     u4 vr[M::ET];
     float ks, vs;
     bool dead, lost;
-    int pk, pv;  // pages of the step to be loaded: of the lane's key and value groups
+    const uint8_t* vp;  // of the step whose keys are loaded
 
     __device__ Stream(const KvCache& c, const KvBatch& b, const Share& w, int lane)
-        : c(c), b(b), w(w), lane(lane), g(lane >> 4), r(lane & 15) {}
+        : c(c), w(w), lane(lane), where(c, b, w, lane) {}
 
-    __device__ void pages(int j) {
-        const int jk = j + (r >> 2) * 16, jv = j + g * 16;
-        pk = jk < w.s.n ? kv_page(b, c, w.seq, jk) : -1;
-        pv = jv < w.s.n ? kv_page(b, c, w.seq, jv) : -1;
-    }
     __device__ void load_keys(int j) {
-        const int in_page = (1 << c.shift) - 1;
-        const uint8_t* k = kv_block(c, max(pk, 0), w.head) +
-                           ((j + (r >> 2) * 16) & in_page) * M::ROW + (r & 3) * 16 +
-                           (M::LB == 8 ? (g >> 1) * 64 + (g & 1) * 8 : g * 64);
+        const uint8_t* k;
+        const float* s;
+        where.find(j, k, vp, s);
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int u = 0; u < M::NU; u++)
                 kr[t][u] = *reinterpret_cast<const K*>(k + t * (4 * M::ROW) + u * 256);
-        const float* const s =
-            reinterpret_cast<const float*>(kv_block(c, max(pv, 0), w.head) + 2 * c.codes) +
-            ((j + lane) & in_page);
         ks = s[0];
         vs = s[1 << c.shift];
         dead = j + lane >= w.s.n;
-        lost = pv < 0;
+        lost = where.pv < 0;
     }
-    __device__ void load_values(int j, int page) {
-        const uint8_t* const v = kv_block(c, max(page, 0), w.head) + c.codes +
-                                 ((j + g * 16) & ((1 << c.shift) - 1)) * M::ROW + r * 16;
+    __device__ void load_values() {
 #pragma unroll
-        for (int t = 0; t < M::ET; t++) vr[t] = *reinterpret_cast<const u4*>(v + t * 256);
+        for (int t = 0; t < M::ET; t++) vr[t] = *reinterpret_cast<const u4*>(vp + t * 256);
     }
 
     // Issues the first step's loads (at j; nothing where j >= hi).
     __device__ void open(int j, int stride) {
         if (j >= w.hi) return;
-        pages(j);
+        where.look(j);
         load_keys(j);
-        load_values(j, pv);
-        if (j + stride < w.hi) pages(j + stride);
+        load_values();
+        if (j + stride < w.hi) where.look(j + stride);
     }
 
     // The steps j, j + stride, .. below the share's end; sc: 192 floats of LDS, this
@@ -571,10 +606,9 @@ struct Stream {
 #pragma unroll
                 for (int k = 0; k < NT; k++) s[t >> 1][k][t & 1] = x[k];
             }
-            const int vpage = pv;
             if (next < w.hi) {
                 load_keys(next);
-                if (next + stride < w.hi) pages(next + stride);
+                if (next + stride < w.hi) where.look(next + stride);
             }
             // one wave: LDS is written and read in order, the compiler has to keep it
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -588,7 +622,7 @@ struct Stream {
                 for (int t = 0; t < M::ET; t++)
                     rows.add_values(t, vr[t][2 * hf], vr[t][2 * hf + 1], pr);
             }
-            if (next < w.hi) load_values(next, vpage);
+            if (next < w.hi) load_values();
         }
         rows.join();
     }
@@ -787,102 +821,110 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
     }
 }
 
-// Many rows: 64 NC of them, 16 NC a wave.  What bounds it are the matrix cores and
-// the exponentials.  A step's keys and values are turned to float16 once for the
+// Many rows: 16 NC of them a wave, W waves.  What bounds it are the matrix cores
+// and the exponentials.  A step's keys and values are turned to float16 once for the
 // workgroup, in LDS in the order in which the operands are read (16 bytes a lane,
 // consecutive), while the next step's bytes are on their way into registers.
-template <int BITS, int D, int NC>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_many_kernel(KvCache c, KvBatch b,
-                                                                        KvAttend a, Plan p) {
+template <int BITS, int D, int NC, int W>
+__global__ __launch_bounds__(64 * W, W == 8 || D < 256 ? 2 : 1)
+void kv_many_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
     using M = Dim<BITS, D>;
     using K = typename KeyReg<M::LB>::type;
     __shared__ __align__(16) h8 kf[2][4 * M::KS * 64];   // [tile][product][lane]
     __shared__ __align__(16) h8 vf[2][2 * M::DT * 64];   // [half][tile][lane]
     __shared__ __align__(16) float sc[2][192];
-    __shared__ float bigs[4];
+    __shared__ float bigs[W];
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int g = lane >> 4, r = lane & 15;
     const Share w = share_of(c, b, a, p);
     if (!w.any) return;
     if (!w.s.ok) {
-        if (w.split == 0) fail_rows<D>(w, a, threadIdx.x, 256);
+        if (w.split == 0) fail_rows<D>(w, a, threadIdx.x, 64 * W);
         return;
     }
     if (p.nsplit > 1 && w.lo >= w.hi) return;  // the join knows which parts there are
 
+    Where<BITS, D> where(c, b, w, lane);
+    if (w.lo < w.hi) where.look(w.lo);
     Rows<BITS, D, NC> rows;
     const int r0 = w.r0 + wave * NC * 16;
     rows.start(w, a, r0, lane);
-    float big = rows.largest(a);
-    if (lane == 0) bigs[wave] = big;
-    __syncthreads();
-    big = fmaxf(fmaxf(bigs[0], bigs[1]), fmaxf(bigs[2], bigs[3]));
-    const float f = rows.scale(a, big) * (a.scale * kLog2e);
-    const int in_page = (1 << c.shift) - 1;
-    // A wave stages the key tile `wave` and the value tiles wave, wave + 4, ...
+    // Four waves stage a tile of keys and every fourth tile of values each; of eight,
+    // the first four take the keys, the others the values.
     constexpr int VT = (M::ET + 3) / 4;
+    const int part = wave & 3;
+    const bool has_keys = W == 4 || wave < 4, has_values = W == 4 || wave >= 4;
     K kr[M::NU];
     u4 vr[VT];
     float ks = 0, vs = 0;
     bool dead = true, lost = true;
     auto fetch = [&](int j) {
-        const int jk = j + (r >> 2) * 16, jv = j + g * 16;
-        const int pk = jk < w.s.n ? kv_page(b, c, w.seq, jk) : -1;
-        const int pv = jv < w.s.n ? kv_page(b, c, w.seq, jv) : -1;
-        const uint8_t* k = kv_block(c, max(pk, 0), w.head) + (jk & in_page) * M::ROW + (r & 3) * 16 +
-                           wave * (4 * M::ROW) + (M::LB == 8 ? (g >> 1) * 64 + (g & 1) * 8 : g * 64);
+        const uint8_t *k, *v;
+        const float* s;
+        where.find(j, k, v, s);
+        if (has_keys) {
 #pragma unroll
-        for (int u = 0; u < M::NU; u++) kr[u] = *reinterpret_cast<const K*>(k + u * 256);
-        const uint8_t* const blk = kv_block(c, max(pv, 0), w.head);
-        const uint8_t* v = blk + c.codes + (jv & in_page) * M::ROW + r * 16;
+            for (int u = 0; u < M::NU; u++)
+                kr[u] = *reinterpret_cast<const K*>(k + part * (4 * M::ROW) + u * 256);
+        }
+        if (has_values) {
 #pragma unroll
-        for (int t = 0; t < VT; t++)
-            if (M::ET % 4 == 0 || t * 4 + wave < M::ET)
-                vr[t] = *reinterpret_cast<const u4*>(v + (t * 4 + wave) * 256);
-        if (wave == 0) {
-            const float* s = reinterpret_cast<const float*>(blk + 2 * c.codes) + ((j + lane) & in_page);
+            for (int t = 0; t < VT; t++)
+                if (M::ET % 4 == 0 || t * 4 + part < M::ET)
+                    vr[t] = *reinterpret_cast<const u4*>(v + (t * 4 + part) * 256);
+        }
+        if (wave == W - 4) {
             ks = s[0];
             vs = s[1 << c.shift];
             dead = j + lane >= w.s.n;
-            lost = pv < 0;
+            lost = where.pv < 0;
         }
+        if (j + kStep < w.hi) where.look(j + kStep);
     };
+    if (w.lo < w.hi) fetch(w.lo);
+    float big = rows.largest(a);
+    if (lane == 0) bigs[wave] = big;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < W; x++) big = fmaxf(big, bigs[x]);
+    const float f = rows.scale(a, big) * (a.scale * kLog2e);
     auto stage = [&](int buf) {
+        if (has_keys) {
 #pragma unroll
-        for (int o = 0; o < M::LB / 8; o++) {
-            const uint32_t x = kr[o >> 1][(o & 1) * 2], y = kr[o >> 1][(o & 1) * 2 + 1];
-            if constexpr (BITS == 8) {
-                kf[buf][(wave * M::KS + o) * 64 + lane] = half8(x, y);
-            } else {
-                h8 lo, hi;
-                half4(x, y, lo, hi);
-                kf[buf][(wave * M::KS + 2 * o) * 64 + lane] = lo;
-                kf[buf][(wave * M::KS + 2 * o + 1) * 64 + lane] = hi;
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < VT; t++) {
-            const int e = t * 4 + wave;
-            if (M::ET % 4 != 0 && e >= M::ET) continue;
-#pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
+            for (int o = 0; o < M::LB / 8; o++) {
+                const uint32_t x = kr[o >> 1][(o & 1) * 2], y = kr[o >> 1][(o & 1) * 2 + 1];
                 if constexpr (BITS == 8) {
-                    vf[buf][(kk * M::DT + e) * 64 + lane] = half8(vr[t][2 * kk], vr[t][2 * kk + 1]);
+                    kf[buf][(part * M::KS + o) * 64 + lane] = half8(x, y);
                 } else {
                     h8 lo, hi;
-                    half4(vr[t][2 * kk], vr[t][2 * kk + 1], lo, hi);
-                    vf[buf][(kk * M::DT + e) * 64 + lane] = lo;
-                    vf[buf][(kk * M::DT + e + M::ET) * 64 + lane] = hi;
+                    half4(x, y, lo, hi);
+                    kf[buf][(part * M::KS + 2 * o) * 64 + lane] = lo;
+                    kf[buf][(part * M::KS + 2 * o + 1) * 64 + lane] = hi;
                 }
             }
         }
-        if (wave == 0) token_terms(ks, vs, f, dead, lost, sc[buf] + lane);
+        if (has_values) {
+#pragma unroll
+            for (int t = 0; t < VT; t++) {
+                const int e = t * 4 + part;
+                if (M::ET % 4 != 0 && e >= M::ET) continue;
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++) {
+                    if constexpr (BITS == 8) {
+                        vf[buf][(kk * M::DT + e) * 64 + lane] = half8(vr[t][2 * kk], vr[t][2 * kk + 1]);
+                    } else {
+                        h8 lo, hi;
+                        half4(vr[t][2 * kk], vr[t][2 * kk + 1], lo, hi);
+                        vf[buf][(kk * M::DT + e) * 64 + lane] = lo;
+                        vf[buf][(kk * M::DT + e + M::ET) * 64 + lane] = hi;
+                    }
+                }
+            }
+        }
+        if (wave == W - 4) token_terms(ks, vs, f, dead, lost, sc[buf] + lane);
     };
     int buf = 0;
-    if (w.lo < w.hi) {
-        fetch(w.lo);
-        stage(0);
-    }
+    if (w.lo < w.hi) stage(0);
     __syncthreads();
     for (int j = w.lo; j < w.hi; j += kStep, buf ^= 1) {
         if (j + kStep < w.hi) fetch(j + kStep);
@@ -1017,7 +1059,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAt
 enum class Path { kShort, kStream, kMany };
 struct Choice {
     Path path;
-    int nc;  // column tiles of a wave
+    int nc;     // column tiles of a wave
+    int waves;  // of a workgroup of many rows
     Plan p;
     int64_t work;  // bytes
 };
@@ -1033,7 +1076,9 @@ Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
     r.path = rows > 32 ? Path::kMany
              : span <= kShortSpan ? Path::kShort : counted ? Path::kStream : Path::kMany;
     r.nc = r.path == Path::kMany ? (rows <= 64 ? 1 : 2) : (rows <= 16 ? 1 : 2);
-    p.tile = r.path == Path::kMany ? r.nc * 64 : r.nc * 16;
+    r.waves = r.path == Path::kMany && D == 256 && r.nc == 2 ? 8 : 4;
+    if (r.waves == 8) r.nc = 1;
+    p.tile = r.path == Path::kMany ? r.nc * 16 * r.waves : r.nc * 16;
     p.tiles = static_cast<int>((rows + p.tile - 1) / p.tile);
     p.rows = b.n_tokens * c.H * G;
     p.nsplit = 1;
@@ -1093,10 +1138,12 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const C
                 kv_stream_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
             break;
         case Path::kMany:
-            if (ch.nc == 1)
-                kv_many_kernel<BITS, D, 1><<<grid, 256, 0, s>>>(c, b, a, p);
-            else
-                kv_many_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
+            if (ch.waves == 8)
+                kv_many_kernel<BITS, D, D == 256 ? 1 : 2, 8><<<grid, 512, 0, s>>>(c, b, a, p);
+            else if (ch.nc == 1)
+                kv_many_kernel<BITS, D, 1, 4><<<grid, 256, 0, s>>>(c, b, a, p);
+            else if constexpr (D < 256)
+                kv_many_kernel<BITS, D, 2, 4><<<grid, 256, 0, s>>>(c, b, a, p);
             break;
     }
     const hipError_t e = hipGetLastError();
