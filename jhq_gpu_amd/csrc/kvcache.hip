@@ -2,12 +2,13 @@
 // jhq_k_kv_*), quantising rows into it and reading them back.
 //
 // Both directions are copies with a few operations per element, bound by HBM.
-// One wave takes a group of 16 tokens (32 where a row has only two 16-byte
-// pieces) of one head, keys or values: LP lanes a token, each with the pieces
-// c, c + LP, ... of its row, so that a row's largest magnitude is a maximum over
-// neighbouring lanes and keys leave as they are, 16 bytes a lane.  Values are
-// stored token-minor ([element][token]); their 16 x 16 byte tiles are turned
-// in LDS (words by 4 x 4 byte transposes), so they also leave 16 bytes a lane.
+// One wave takes a run of 16 tokens (32 where their codes are fewer than 64 x 16
+// bytes) of one head, keys or values.  On the side of the rows a lane holds 8
+// consecutive elements, D / 8 lanes a row, so that rows move 16 bytes a lane and
+// a row's largest magnitude is a maximum over neighbouring lanes; on the side of
+// the cache a lane holds 16 consecutive code bytes.  Between the two the codes
+// pass through LDS, [piece][token][16 bytes]; values, which the cache holds
+// token-minor, have their 16 x 16 byte tiles turned there.
 #include "kvcache.h"
 
 #include <hip/hip_runtime.h>
@@ -22,52 +23,55 @@ int jhq_set_error(int code, const char* msg);
 namespace jhq {
 namespace {
 
-constexpr int kWaves = 4;          // waves of a workgroup, each on its own
-constexpr int kTilePitch = 272;    // bytes from one 16 x 16 tile to the next: 16 apart in the banks
-constexpr float kFloor = 0x1p-60f; // rows below it are held as zeros
+constexpr int kWaves = 4;           // waves of a workgroup, each on its own
+constexpr int kTilePitch = 272;     // bytes from one 16 x 16 tile to the next: 16 apart in the banks
+constexpr float kFloor = 0x1p-60f;  // rows below it are held as zeros
 
-// Lanes per token and tokens per wave for NP 16-byte pieces a row.
-template <int NP>
-struct Lanes {
-    static constexpr int LP = NP < 4 ? NP : 4;
-    static constexpr int TW = 64 / LP;
-    static constexpr int IT = NP / LP;  // pieces per lane
+// Sizes that follow from the bits and the head's elements.
+template <int BITS, int D>
+struct Run {
+    static constexpr int ROW = D * BITS / 8;           // code bytes of a row
+    static constexpr int NP = ROW / 16;                // pieces of it
+    static constexpr int TW = ROW < 64 ? 32 : 16;      // tokens of a run
+    static constexpr int CL = D / 8;                   // lanes of a row
+    static constexpr int RI = 64 / CL, NI = TW / RI;   // rows at once; times
+    static constexpr int OUT = TW * ROW / 16 / 64;     // 16-byte units of a lane
+    static constexpr int LDS = TW / 16 * NP * kTilePitch;
 };
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// The values of 16 elements at src, as float.
+__device__ inline float nan32() { return __uint_as_float(0x7fc00000u); }
+
+// The values of 8 elements from element i on.
 template <int DT, bool VEC>
-__device__ inline void load16(const void* base, int64_t i, float* x) {
+__device__ inline void load8(const void* base, int64_t i, float* x) {
     if constexpr (DT == JHQ_F32) {
         const float* p = static_cast<const float*>(base) + i;
         if constexpr (VEC) {
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int w = 0; w < 2; w++) {
                 const float4 f = reinterpret_cast<const float4*>(p)[w];
                 x[4 * w] = f.x, x[4 * w + 1] = f.y, x[4 * w + 2] = f.z, x[4 * w + 3] = f.w;
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 16; j++) x[j] = p[j];
+            for (int j = 0; j < 8; j++) x[j] = p[j];
         }
     } else {
         const uint16_t* p = static_cast<const uint16_t*>(base) + i;
-        uint16_t h[16];
+        uint16_t h[8];
         if constexpr (VEC) {
-            const u32x4 a = reinterpret_cast<const u32x4*>(p)[0];
-            const u32x4 b = reinterpret_cast<const u32x4*>(p)[1];
+            const u32x4 a = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                h[2 * j] = a[j] & 0xffff, h[2 * j + 1] = a[j] >> 16;
-                h[8 + 2 * j] = b[j] & 0xffff, h[9 + 2 * j] = b[j] >> 16;
-            }
+            for (int j = 0; j < 4; j++) h[2 * j] = a[j] & 0xffff, h[2 * j + 1] = a[j] >> 16;
         } else {
 #pragma unroll
-            for (int j = 0; j < 16; j++) h[j] = p[j];
+            for (int j = 0; j < 8; j++) h[j] = p[j];
         }
 #pragma unroll
-        for (int j = 0; j < 16; j++)
+        for (int j = 0; j < 8; j++)
             x[j] = DT == JHQ_BF16 ? __uint_as_float(static_cast<uint32_t>(h[j]) << 16)
                                   : static_cast<float>(__builtin_bit_cast(_Float16, h[j]));
     }
@@ -82,32 +86,29 @@ __device__ inline uint32_t round16(float f) {
 }
 
 template <int DT, bool VEC>
-__device__ inline void store16(void* base, int64_t i, const float* x) {
+__device__ inline void store8(void* base, int64_t i, const float* x) {
     if constexpr (DT == JHQ_F32) {
         float* p = static_cast<float*>(base) + i;
         if constexpr (VEC) {
 #pragma unroll
-            for (int w = 0; w < 4; w++)
+            for (int w = 0; w < 2; w++)
                 reinterpret_cast<float4*>(p)[w] =
                     make_float4(x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 16; j++) p[j] = x[j];
+            for (int j = 0; j < 8; j++) p[j] = x[j];
         }
     } else {
         uint16_t* p = static_cast<uint16_t*>(base) + i;
         if constexpr (VEC) {
+            u32x4 o;
 #pragma unroll
-            for (int w = 0; w < 2; w++) {
-                u32x4 o;
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    o[j] = round16<DT>(x[8 * w + 2 * j]) | round16<DT>(x[8 * w + 2 * j + 1]) << 16;
-                reinterpret_cast<u32x4*>(p)[w] = o;
-            }
+            for (int j = 0; j < 4; j++)
+                o[j] = round16<DT>(x[2 * j]) | round16<DT>(x[2 * j + 1]) << 16;
+            *reinterpret_cast<u32x4*>(p) = o;
         } else {
 #pragma unroll
-            for (int j = 0; j < 16; j++) p[j] = static_cast<uint16_t>(round16<DT>(x[j]));
+            for (int j = 0; j < 8; j++) p[j] = static_cast<uint16_t>(round16<DT>(x[j]));
         }
     }
 }
@@ -131,30 +132,22 @@ __device__ inline void transpose4(uint32_t m[4]) {
     m[3] = __builtin_amdgcn_perm(d, c, 0x07060302);
 }
 
-// Four 16 x 16 byte tiles of a wave, transposed through tile (4 * kTilePitch
-// bytes of LDS, this wave's): lane holds row `in` of tile `tin`, gets row
-// lane % 16 of tile lane / 16 (or the other way round: both are 16-byte rows).
-__device__ inline u32x4 transpose16(uint8_t* tile, int lane, int tin, int rin, int tout, int rout,
-                                    u32x4 w) {
-    *reinterpret_cast<u32x4*>(tile + tin * kTilePitch + rin * 16) = w;
-    wave_lds_fence();
-    uint8_t* const t = tile + (lane >> 4) * kTilePitch;
-    const int r = (lane & 3) * 4, c = ((lane >> 2) & 3) * 4;
+// Transposes a 16 x 16 byte tile in LDS in place, 16 lanes a tile: words by 4 x 4
+// bytes.
+__device__ inline void transpose16(uint8_t* tile, int lane) {
+    const int r = (lane & 3) * 4, c = (lane >> 2 & 3) * 4;
     uint32_t m[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) m[i] = *reinterpret_cast<const uint32_t*>(t + (r + i) * 16 + c);
+    for (int i = 0; i < 4; i++) m[i] = *reinterpret_cast<const uint32_t*>(tile + (r + i) * 16 + c);
     wave_lds_fence();
     transpose4(m);
 #pragma unroll
-    for (int i = 0; i < 4; i++) *reinterpret_cast<uint32_t*>(t + (c + i) * 16 + r) = m[i];
+    for (int i = 0; i < 4; i++) *reinterpret_cast<uint32_t*>(tile + (c + i) * 16 + r) = m[i];
     wave_lds_fence();
-    const u32x4 o = *reinterpret_cast<const u32x4*>(tile + tout * kTilePitch + rout * 16);
-    wave_lds_fence();
-    return o;
 }
 
-// What one wave works on: a run of TW tokens from `first`, one head, keys or
-// values.
+// What one wave works on: a run of tokens from `first` (a multiple of 16), one
+// head, keys or values.
 struct Unit {
     KvSeq q;
     int seq, head, value;
@@ -163,70 +156,69 @@ struct Unit {
 };
 
 template <int TW>
-__device__ inline Unit unit_of(const KvCache& c, const KvBatch& b, int64_t u, int sets) {
+__device__ inline Unit unit_of(const KvCache& c, const KvBatch& b, int sets) {
     Unit r;
-    r.value = static_cast<int>(u & 1);
+    uint32_t u = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    r.value = u & 1;
     u >>= 1;
-    r.head = static_cast<int>(u % c.H);
+    r.head = u % c.H;
     u /= c.H;
-    const int set = static_cast<int>(u % sets);
-    r.seq = static_cast<int>(u / sets);
+    const int set = u % sets;
+    r.seq = u / sets;
     r.any = r.seq < b.n_seq;
     if (!r.any) return r;
     r.q = kv_seq(b, r.seq, c.shift);
     r.lo = max(r.q.n - r.q.q, 0);
-    r.first = (r.lo / kKvGroup) * kKvGroup + set * TW;
+    r.first = r.lo / kKvGroup * kKvGroup + set * TW;
     r.any = r.q.q > 0 && (r.first < r.q.n || !r.q.ok);
     return r;
 }
 
-// The page of token j's group (groups do not straddle pages), or -1; the
-// sequence is ok, so every position below n is in the table.
-__device__ inline int group_page(const KvCache& c, const KvBatch& b, const Unit& u, int j) {
-    const int g = j & ~(kKvGroup - 1);
-    return g < u.q.n ? kv_page(b, c, u.seq, g) : -1;
-}
+// The groups of a run: where their codes begin and which of their tokens are to
+// be moved.
+template <int TW>
+struct Groups {
+    uint8_t* block[TW / 16];  // the page's block of the head, null: no such page
+    int slot[TW / 16];        // of the group's first token in its page
+    uint32_t live;            // a bit for each token of the run
 
-// Where piece p of the token in a slot of its page starts among the key codes.
-template <int ROW>
-__device__ inline int key_at(int slot, int p) {
-    return (slot & ~3) * ROW + p * 64 + (slot & 3) * 16;
-}
-
-// What a lane of a transposed unit holds: a byte column of piece `piece` (and
-// its later pieces) of token group `group` of the run, and which of that
-// group's tokens are to be moved.
-struct Column {
-    int group, piece;
-    uint32_t mask;
+    // ok: the sequence's positions below n are all in the table.
+    __device__ Groups(const KvCache& c, const KvBatch& b, const Unit& u) : live(0) {
+#pragma unroll
+        for (int g = 0; g < TW / 16; g++) {
+            const int j = u.first + g * 16;
+            const int page = j < u.q.n ? kv_page(b, c, u.seq, j) : -1;
+            block[g] = page < 0 ? nullptr : kv_block(c, page, u.head);
+            slot[g] = j & ((1 << c.shift) - 1);
+            const int from = min(max(u.lo - j, 0), 16), to = min(max(u.q.n - j, 0), 16);
+            if (from < to) live |= (((1u << to) - 1) & ~((1u << from) - 1)) << (g * 16);
+        }
+    }
+    __device__ uint32_t held() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int g = 0; g < TW / 16; g++)
+            if (block[g]) m |= 0xffffu << (g * 16);
+        return m;
+    }
 };
 
-template <int LP>
-__device__ inline Column column_of(int lane, bool live) {
-    Column r;
-    r.group = (lane >> 4) / LP;
-    r.piece = (lane >> 4) % LP;
-    const uint64_t m = __ballot(live);
-    r.mask = 0;
-#pragma unroll
-    for (int t = 0; t < 16; t++)
-        r.mask |= static_cast<uint32_t>(m >> ((r.group * 16 + t) * LP) & 1) << t;
-    return r;
-}
-
-// rne(top x / amax) of one row's elements held by a lane.  x * top is exact
-// for 16-bit x and the quotient, corrected once by its remainder, is within one
-// unit of 2^-24: a quotient half way between codes comes out exactly (it is
-// representable and the remainder is exact), and any other is further from
-// half way than that, both sides of the comparison being 19-bit integers in
-// one unit.  Adding 1.5 * 2^23 rounds half to even and leaves the code in the
-// low bits.
+// rne(top x / a) in the low bits, half to even.  x * top is exact for 16-bit x and
+// the quotient, corrected once by its remainder, is within one unit of 2^-24: a
+// quotient half way between codes comes out exactly (it is representable and
+// the remainder is exact), and any other is further from half way than that, both
+// sides of the comparison being 19-bit integers in one unit.
 template <int BITS>
 __device__ inline uint32_t code_of(float x, float topf, float a, float inv) {
     const float y = x * topf;
     const float q0 = y * inv;
     const float q = fmaf(fmaf(-q0, a, y), inv, q0);
+    // 1.5 * 2^23 rounds at the last bit
     return __float_as_uint(q + (12582912.0f + (BITS == 8 ? 128.0f : 8.0f)));
+}
+
+__device__ inline uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(b, a, 0x0c0c0400) | __builtin_amdgcn_perm(d, c, 0x0c0c0400) << 16;
 }
 
 // HBM-bound: reads 2 T H D elements, writes half (8 bits) or a quarter of that
@@ -234,87 +226,95 @@ __device__ inline uint32_t code_of(float x, float topf, float a, float inv) {
 template <int BITS, int D, int DT, bool VEC>
 __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatch b, KvRows kr,
                                                                KvRows vr, int sets) {
-    constexpr int ROW = D * BITS / 8, NP = ROW / 16;
-    using L = Lanes<NP>;
-    constexpr int E = BITS == 8 ? 16 : 32;  // elements in a piece
-    __shared__ __align__(16) uint8_t lds[kWaves][4 * kTilePitch];
+    using R = Run<BITS, D>;
+    __shared__ __align__(16) uint8_t lds[kWaves][R::LDS];
+    __shared__ int mags[kWaves][R::TW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Unit u = unit_of<L::TW>(c, b, static_cast<int64_t>(blockIdx.x) * kWaves + wave, sets);
+    const Unit u = unit_of<R::TW>(c, b, sets);
     if (!u.any || !u.q.ok) return;  // wave-uniform; the waves share nothing
-    const int t = lane / L::LP, lc = lane % L::LP;
-    const int j = u.first + t;
-    const int page = group_page(c, b, u, j);
-    const bool live = j >= u.lo && j < u.q.n && page >= 0;
+    const Groups<R::TW> gr(c, b, u);
+    const uint32_t live = gr.live & gr.held();
+    if (!live) return;
+    const int col = lane % R::CL, sub = lane / R::CL;
     const KvRows src = u.value ? vr : kr;
-    const int64_t at = (u.q.row + (j - (u.q.n - u.q.q))) * src.tok + u.head * src.head;
-
-    float x[L::IT][E];
+    const int64_t row0 = u.q.row + (u.first - (u.q.n - u.q.q));
+    float x[R::NI][8];
 #pragma unroll
-    for (int i = 0; i < L::IT; i++) {
-        const int e = (lc + i * L::LP) * 16;
+    for (int i = 0; i < R::NI; i++) {
+        const int t = i * R::RI + sub;
 #pragma unroll
-        for (int w = 0; w < E; w++) x[i][w] = 0.0f;
-        if (live) {
-            load16<DT, VEC>(src.p, at + e, x[i]);
-            if constexpr (BITS == 4) load16<DT, VEC>(src.p, at + D / 2 + e, x[i] + 16);
-        }
+        for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
+        if (live >> t & 1)
+            load8<DT, VEC>(src.p, (row0 + t) * src.tok + u.head * src.head + col * 8, x[i]);
     }
-    // |x| as an integer: infinities and NaN are the largest
-    int mag = 0;
-#pragma unroll
-    for (int i = 0; i < L::IT; i++)
-#pragma unroll
-        for (int w = 0; w < E; w++) mag = max(mag, __float_as_int(x[i][w]) & 0x7fffffff);
-#pragma unroll
-    for (int o = 1; o < L::LP; o <<= 1) mag = max(mag, __shfl_xor(mag, o));
     constexpr float top = BITS == 8 ? 127.0f : 7.0f;
-    const float amax = __int_as_float(mag);
-    const bool finite = mag < 0x7f800000, held = finite && amax >= kFloor;
-    // top * x must not overflow: very large rows are scaled by 2^-64 first
-    const float f = amax > 0x1p100f ? 0x1p-64f : 1.0f;
-    const float a = held ? amax * f : 1.0f, inv = 1.0f / a, topf = held ? top * f : 0.0f;
-    const float scale = held ? amax / top : finite ? 0.0f : __uint_as_float(0x7fc00000u);
-
-    uint8_t* const blk = kv_block(c, max(page, 0), u.head);
-    uint8_t* const codes = blk + (u.value ? c.codes : 0);
-    const int in_page = (1 << c.shift) - 1, slot = j & in_page;
-    if (live && lc == 0)
-        reinterpret_cast<float*>(blk + 2 * c.codes)[(u.value << c.shift) + slot] = scale;
-    // Values: after the transpose a lane holds one byte column of 16 tokens, of
-    // which it may write those that are new.
-    const Column o = column_of<L::LP>(lane, live && lc == 0);
-    const int opage = __shfl(page, o.group * 16 * L::LP);
-    uint8_t* const ocodes = kv_block(c, max(opage, 0), u.head) + c.codes +
-                            ((u.first + o.group * 16) & in_page) * ROW;
 #pragma unroll
-    for (int i = 0; i < L::IT; i++) {
-        u32x4 w;
+    for (int i = 0; i < R::NI; i++) {
+        // |x| as an integer: infinities and NaN are the largest
+        int mag = 0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            uint32_t d[4];
+        for (int e = 0; e < 8; e++) mag = max(mag, __float_as_int(x[i][e]) & 0x7fffffff);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                d[e] = code_of<BITS>(x[i][4 * k + e], topf, a, inv);
-                if constexpr (BITS == 4)
-                    d[e] = (d[e] & 15u) | code_of<4>(x[i][16 + 4 * k + e], topf, a, inv) << 4;
-            }
-            const uint32_t p01 = __builtin_amdgcn_perm(d[1], d[0], 0x0c0c0400);
-            const uint32_t p23 = __builtin_amdgcn_perm(d[3], d[2], 0x0c0c0400);
-            w[k] = finite ? p01 | p23 << 16 : BITS == 8 ? 0x80808080u : 0x88888888u;
-        }
-        if (!u.value) {
-            if (live)
-                *reinterpret_cast<u32x4*>(codes + key_at<ROW>(slot, lc + i * L::LP)) = w;
-            continue;
-        }
-        w = transpose16(lds[wave], lane, (t >> 4) * L::LP + lc, t & 15, lane >> 4, lane & 15, w);
-        uint8_t* const dst = ocodes + ((o.piece + i * L::LP) * 16 + (lane & 15)) * 16;
-        if (o.mask == 0xffff) {
-            *reinterpret_cast<u32x4*>(dst) = w;
+        for (int o = 1; o < R::CL; o <<= 1) mag = max(mag, __shfl_xor(mag, o));
+        const float amax = __int_as_float(mag);
+        const bool finite = mag < 0x7f800000, held = finite && amax >= kFloor;
+        // top * x must not overflow: very large rows are scaled by 2^-64 first
+        const float f = amax > 0x1p100f ? 0x1p-64f : 1.0f;
+        const float a = held ? amax * f : 1.0f, topf = held ? top * f : 0.0f;
+        const float inv = __builtin_amdgcn_rcpf(a);
+        uint32_t d[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) d[e] = code_of<BITS>(x[i][e], topf, a, inv);
+        u32x2 w = {bytes4(d[0], d[1], d[2], d[3]), bytes4(d[4], d[5], d[6], d[7])};
+        if (!finite) w = BITS == 8 ? u32x2{0x80808080u, 0x80808080u} : u32x2{0x08080808u, 0x08080808u};
+        const int t = i * R::RI + sub;
+        uint8_t* const at = lds[wave] + (t >> 4) * R::NP * kTilePitch + (t & 15) * 16;
+        if constexpr (BITS == 8) {
+            *reinterpret_cast<u32x2*>(at + (col >> 1) * kTilePitch + (col & 1) * 8) = w;
         } else {
+            // the lane D/16 on holds the elements of the high nibbles
+            const uint32_t m = 0x0f0f0f0fu;
+            const uint32_t h0 = __shfl_xor(static_cast<int>(w[0]), R::CL / 2) & m;
+            const uint32_t h1 = __shfl_xor(static_cast<int>(w[1]), R::CL / 2) & m;
+            if (col < R::CL / 2)
+                *reinterpret_cast<u32x2*>(at + (col >> 1) * kTilePitch + (col & 1) * 8) =
+                    u32x2{(w[0] & m) | h0 << 4, (w[1] & m) | h1 << 4};
+        }
+        if (col == 0) mags[wave][t] = mag;
+    }
+    wave_lds_fence();
+    if (lane < R::TW && (live >> lane & 1)) {
+        const float amax = __int_as_float(mags[wave][lane]);
+        const float scale = !(amax < INFINITY) ? nan32() : amax >= kFloor ? amax / top : 0.0f;
+        const int g = lane >> 4;
+        float* const sc = reinterpret_cast<float*>((R::TW == 32 && g ? gr.block[R::TW / 16 - 1] : gr.block[0]) +
+                                                   2 * c.codes);
+        sc[(u.value << c.shift) + (R::TW == 32 && g ? gr.slot[R::TW / 16 - 1] : gr.slot[0]) +
+           (lane & 15)] = scale;
+    }
 #pragma unroll
-            for (int r = 0; r < 16; r++)
-                if (o.mask >> r & 1) dst[r] = static_cast<uint8_t>(w[r >> 2] >> (8 * (r & 3)));
+    for (int i = 0; i < R::OUT; i++) {
+        const int k = lane + 64 * i, g = R::TW == 32 ? k / R::ROW : 0, in = k - g * R::ROW;
+        uint8_t* const blk = R::TW == 32 && g ? gr.block[R::TW / 16 - 1] : gr.block[0];
+        const int slot = R::TW == 32 && g ? gr.slot[R::TW / 16 - 1] : gr.slot[0];
+        const uint32_t mine = live >> (g * 16) & 0xffff;
+        if (!u.value) {
+            const int t = in / (R::NP * 4) * 4 + (in & 3), piece = in % (R::NP * 4) >> 2;
+            const u32x4 w = *reinterpret_cast<const u32x4*>(
+                lds[wave] + (g * R::NP + piece) * kTilePitch + t * 16);
+            if (mine >> t & 1) *reinterpret_cast<u32x4*>(blk + slot * R::ROW + in * 16) = w;
+        } else {
+            uint8_t* const tile = lds[wave] + (k >> 4) * kTilePitch;
+            transpose16(tile, lane);
+            const u32x4 w = *reinterpret_cast<const u32x4*>(tile + (k & 15) * 16);
+            uint8_t* const dst = blk + c.codes + slot * R::ROW + in * 16;
+            if (mine == 0xffff) {
+                *reinterpret_cast<u32x4*>(dst) = w;
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (mine >> r & 1) dst[r] = static_cast<uint8_t>(w[r >> 2] >> (8 * (r & 3)));
+            }
         }
     }
 }
@@ -323,74 +323,88 @@ __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatc
 template <int BITS, int D, int DT, bool VEC>
 __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvCache c, KvBatch b, void* ko,
                                                               void* vo, int sets) {
-    constexpr int ROW = D * BITS / 8, NP = ROW / 16;
-    using L = Lanes<NP>;
-    constexpr int E = BITS == 8 ? 16 : 32;
-    __shared__ __align__(16) uint8_t lds[kWaves][4 * kTilePitch];
+    using R = Run<BITS, D>;
+    __shared__ __align__(16) uint8_t lds[kWaves][R::LDS];
+    __shared__ float scales[kWaves][R::TW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Unit u = unit_of<L::TW>(c, b, static_cast<int64_t>(blockIdx.x) * kWaves + wave, sets);
+    const Unit u = unit_of<R::TW>(c, b, sets);
     void* const out = u.value ? vo : ko;
     if (!u.any || !out) return;  // wave-uniform; the waves share nothing
-    const int t = lane / L::LP, lc = lane % L::LP;
-    int j = u.first + t, row = j - (u.q.n - u.q.q);
-    bool live = j >= u.lo && j < u.q.n;
-    int page = -1;
-    if (u.q.ok) {
-        page = group_page(c, b, u, j);
-    } else {  // no positions to go by: the run's share of the rows becomes NaN
-        row = j;
-        live = row < u.q.q;
+    const Groups<R::TW> gr(c, b, u);
+    int64_t row0 = u.q.row + (u.first - (u.q.n - u.q.q));
+    uint32_t live = gr.live;
+    if (!u.q.ok) {  // no positions to go by: the run's share of the rows becomes NaN
+        row0 = u.q.row + u.first;
+        live = 0;
+        for (int t = 0; t < R::TW; t++)
+            if (u.first + t < u.q.q) live |= 1u << t;
     }
-    const int in_page = (1 << c.shift) - 1, slot = j & in_page;
-    const uint8_t* const blk = kv_block(c, max(page, 0), u.head);
-    const uint8_t* const codes = blk + (u.value ? c.codes : 0);
-    float scale = __uint_as_float(0x7fc00000u);
-    if (live && page >= 0)
-        scale = reinterpret_cast<const float*>(blk + 2 * c.codes)[(u.value << c.shift) + slot];
-    const Column o = column_of<L::LP>(lane, live && lc == 0);
-    const int opage = __shfl(page, o.group * 16 * L::LP);
-    const uint8_t* const ocodes = kv_block(c, max(opage, 0), u.head) + c.codes +
-                                  ((u.first + o.group * 16) & in_page) * ROW;
-    const int64_t at = ((u.q.row + row) * c.H + u.head) * D;
+    if (lane < R::TW) {
+        const int g = lane >> 4;
+        const uint8_t* const blk = R::TW == 32 && g ? gr.block[R::TW / 16 - 1] : gr.block[0];
+        const int slot = (R::TW == 32 && g ? gr.slot[R::TW / 16 - 1] : gr.slot[0]) + (lane & 15);
+        float s = nan32();
+        if (blk && (live >> lane & 1))
+            s = reinterpret_cast<const float*>(blk + 2 * c.codes)[(u.value << c.shift) + slot];
+        scales[wave][lane] = s;
+    }
+    u32x4 w[R::OUT];
 #pragma unroll
-    for (int i = 0; i < L::IT; i++) {
-        u32x4 w = {0, 0, 0, 0};
-        if (u.value) {
-            if (o.mask && opage >= 0)
-                w = *reinterpret_cast<const u32x4*>(
-                    ocodes + ((o.piece + i * L::LP) * 16 + (lane & 15)) * 16);
-            w = transpose16(lds[wave], lane, lane >> 4, lane & 15, (t >> 4) * L::LP + lc, t & 15, w);
-        } else if (live && page >= 0) {
-            w = *reinterpret_cast<const u32x4*>(codes + key_at<ROW>(slot, lc + i * L::LP));
-        }
-        float x[E];
+    for (int i = 0; i < R::OUT; i++) {
+        const int k = lane + 64 * i, g = R::TW == 32 ? k / R::ROW : 0, in = k - g * R::ROW;
+        const uint8_t* const blk = R::TW == 32 && g ? gr.block[R::TW / 16 - 1] : gr.block[0];
+        const int slot = R::TW == 32 && g ? gr.slot[R::TW / 16 - 1] : gr.slot[0];
+        w[i] = u32x4{0, 0, 0, 0};
+        if (blk)
+            w[i] = *reinterpret_cast<const u32x4*>(blk + (u.value ? c.codes : 0) + slot * R::ROW +
+                                                   in * 16);
+    }
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const uint32_t by = w[e >> 2] >> (8 * (e & 3));
-            if constexpr (BITS == 8) {
-                x[e] = (static_cast<float>(by & 255u) - 128.0f) * scale;
-            } else {
-                x[e] = (static_cast<float>(by & 15u) - 8.0f) * scale;
-                x[16 + e] = (static_cast<float>(by >> 4 & 15u) - 8.0f) * scale;
-            }
+    for (int i = 0; i < R::OUT; i++) {
+        const int k = lane + 64 * i, g = R::TW == 32 ? k / R::ROW : 0, in = k - g * R::ROW;
+        if (!u.value) {
+            const int t = in / (R::NP * 4) * 4 + (in & 3), piece = in % (R::NP * 4) >> 2;
+            *reinterpret_cast<u32x4*>(lds[wave] + (g * R::NP + piece) * kTilePitch + t * 16) = w[i];
+        } else {
+            uint8_t* const tile = lds[wave] + (k >> 4) * kTilePitch;
+            *reinterpret_cast<u32x4*>(tile + (k & 15) * 16) = w[i];
+            wave_lds_fence();
+            transpose16(tile, lane);
         }
-        if (live) {
-            const int e = (lc + i * L::LP) * 16;
-            store16<DT, VEC>(out, at + e, x);
-            if constexpr (BITS == 4) store16<DT, VEC>(out, at + D / 2 + e, x + 16);
+    }
+    wave_lds_fence();
+    const int col = lane % R::CL, sub = lane / R::CL;
+    constexpr int HALF = BITS == 8 ? R::CL : R::CL / 2;  // lanes of the low nibbles
+    const int byte = col % HALF;
+#pragma unroll
+    for (int i = 0; i < R::NI; i++) {
+        const int t = i * R::RI + sub;
+        u32x2 v = *reinterpret_cast<const u32x2*>(lds[wave] +
+                                                  ((t >> 4) * R::NP + (byte >> 1)) * kTilePitch +
+                                                  (t & 15) * 16 + (byte & 1) * 8);
+        if (BITS == 4 && col >= HALF) v >>= 4;
+        const float scale = scales[wave][t];
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t by = v[e >> 2] >> (8 * (e & 3)) & (BITS == 8 ? 255u : 15u);
+            x[e] = (static_cast<float>(by) - (BITS == 8 ? 128.0f : 8.0f)) * scale;
         }
+        if (live >> t & 1)
+            store8<DT, VEC>(out, ((row0 + t) * c.H + u.head) * D + col * 8, x);
     }
 }
 
-// The launch's units: per sequence the token runs of max_q tokens (one more
-// than they fill, for a run that starts inside a group), every head, keys and
-// values.  False where they do not fit a launch.
+// The launch's units: per sequence the runs of max_q tokens (one more than they
+// fill, for a run that starts inside a group), every head, keys and values.
+// False where they do not fit a launch.
 bool units(const KvBatch& b, const KvCache& c, int TW, int* sets, unsigned* blocks) {
     const int64_t s = (static_cast<int64_t>(b.max_q) + 15 + TW - 1) / TW;
+    if (s * b.n_seq >= int64_t(1) << 31) return false;
     const int64_t n = (s * b.n_seq * c.H * 2 + kWaves - 1) / kWaves;
     *sets = static_cast<int>(s);
     *blocks = static_cast<unsigned>(n);
-    return n < (int64_t(1) << 31) / (64 * kWaves) * 2;
+    return n < int64_t(1) << 23;
 }
 
 // f<BITS, D, DT, VEC> for the run-time values.
@@ -415,18 +429,13 @@ hipError_t pick(int bits, int D, int dt, bool vec, A&&... a) {
 #undef JHQ_KV_V
 }
 
-template <int BITS, int D>
-constexpr int run_tokens() {
-    return Lanes<D * BITS / 128>::TW;
-}
-
 template <int BITS, int D, int DT, bool VEC>
 struct Write {
     static hipError_t run(const KvCache& c, const KvBatch& b, const KvRows& k, const KvRows& v,
                           hipStream_t s) {
         int sets;
         unsigned blocks;
-        if (!units(b, c, run_tokens<BITS, D>(), &sets, &blocks)) return hipErrorInvalidValue;
+        if (!units(b, c, Run<BITS, D>::TW, &sets, &blocks)) return hipErrorInvalidValue;
         kv_write_kernel<BITS, D, DT, VEC><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
         return hipGetLastError();
     }
@@ -437,7 +446,7 @@ struct Read {
     static hipError_t run(const KvCache& c, const KvBatch& b, void* k, void* v, hipStream_t s) {
         int sets;
         unsigned blocks;
-        if (!units(b, c, run_tokens<BITS, D>(), &sets, &blocks)) return hipErrorInvalidValue;
+        if (!units(b, c, Run<BITS, D>::TW, &sets, &blocks)) return hipErrorInvalidValue;
         kv_read_kernel<BITS, D, DT, VEC><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
         return hipGetLastError();
     }
