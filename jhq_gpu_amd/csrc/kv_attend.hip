@@ -972,18 +972,21 @@ void kv_many_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
     }
 }
 
-// Adds the parts of rows, a thread 4 elements of every fourth part of a row; latency
-// bounds it.  NT > 0: parts of kv_stream_kernel, rows in the order (sequence, head,
-// row); 0: of kv_many_kernel, (sequence, new token, query head).
-template <int D>
-constexpr int kJoinRows = 256 / D;  // rows of a workgroup
+// Adds the parts of rows; latency bounds it.  NT > 0: parts of kv_stream_kernel, rows
+// in the order (sequence, head, row), often many: a thread has 4 elements of every
+// fourth part of a row.  NT = 0: parts of kv_many_kernel, (sequence, new token, query
+// head), few parts and more rows: a thread has all of its elements' parts.
+template <int NT>
+constexpr int kJoinSplit = NT ? 4 : 1;
+template <int D, int NT>
+constexpr int kJoinRows = 1024 / D / kJoinSplit<NT>;  // rows of a workgroup
 
 template <int D, int NT>
 __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
-    constexpr int T = D / 4, R = kJoinRows<D>;
-    __shared__ __align__(16) float acc[R][4][D];
-    __shared__ float ml[R][4][2];
-    const int t = threadIdx.x % T, y = threadIdx.x / T % 4, r = threadIdx.x / (4 * T);
+    constexpr int T = D / 4, R = kJoinRows<D, NT>, Y = kJoinSplit<NT>;
+    __shared__ __align__(16) float acc[R][Y][D];
+    __shared__ float ml[R][Y][2];
+    const int t = threadIdx.x % T, y = threadIdx.x / T % Y, r = threadIdx.x / (Y * T);
     const int x = blockIdx.x * R + r, per = b.max_q * a.heads;
     const int seq = x / per, in = x % per;
     int n = 0;            // parts
@@ -1022,7 +1025,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAt
     float m = kNone, l = 0.0f;
     f4 o = {0, 0, 0, 0};
 #pragma unroll 4
-    for (int k = y; k < n; k += 4) {
+    for (int k = y; k < n; k += Y) {
         const int64_t at = slot + k * next + (k ? jump : 0);
         const float2 st = *reinterpret_cast<const float2*>(stats + at * 2);
         const f4 v = *reinterpret_cast<const f4*>(a.work + at * D + t * 4);
@@ -1043,9 +1046,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAt
     l = 0.0f;
     o = f4{0, 0, 0, 0};
 #pragma unroll
-    for (int z = 0; z < 4; z++) m = fmaxf(m, ml[r][z][0]);
+    for (int z = 0; z < Y; z++) m = fmaxf(m, ml[r][z][0]);
 #pragma unroll
-    for (int z = 0; z < 4; z++) {
+    for (int z = 0; z < Y; z++) {
         const float f = __builtin_amdgcn_exp2f(ml[r][z][0] - m);
         l = fmaf(ml[r][z][1], f, l);
         o += *reinterpret_cast<const f4*>(acc[r][z] + t * 4) * f;
@@ -1097,7 +1100,7 @@ Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
                                                                       p.tile / G + 2 + kStep)
                                     : b.max_kv;
         // no split where the tiles fill the chip (two on each of 256 CUs)
-        const int64_t parts = std::max<int64_t>(1, 512 / tiles);
+        const int64_t parts = std::max<int64_t>(1, (512 + tiles - 1) / tiles);
         int64_t chunk = std::max<int64_t>(512, (seen + parts - 1) / parts);
         chunk = (chunk + kStep - 1) / kStep * kStep;
         p.nsplit = static_cast<int>(std::max<int64_t>(1, (seen + chunk - 1) / chunk));
@@ -1118,8 +1121,8 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const C
     const int64_t out = static_cast<int64_t>(b.n_seq) * b.max_q * a.heads;
     const int64_t blocks = ch.path == Path::kStream ? (1 << p.log_workers) / 4
                                                     : static_cast<int64_t>(c.H) * b.n_seq * p.tiles * p.nsplit;
-    const int64_t joins = ch.path == Path::kStream || p.nsplit > 1
-                              ? (out + kJoinRows<D> - 1) / kJoinRows<D> : 0;
+    const int jrows = ch.path == Path::kMany ? kJoinRows<D, 0> : kJoinRows<D, 1>;
+    const int64_t joins = ch.path == Path::kStream || p.nsplit > 1 ? (out + jrows - 1) / jrows : 0;
     if (blocks >= 1 << 23 || joins >= 1 << 23) return hipErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(blocks)), jgrid(static_cast<unsigned>(joins));
     switch (ch.path) {
@@ -1138,11 +1141,11 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const C
                 kv_stream_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
             break;
         case Path::kMany:
-            if (ch.waves == 8)
-                kv_many_kernel<BITS, D, D == 256 ? 1 : 2, 8><<<grid, 512, 0, s>>>(c, b, a, p);
-            else if (ch.nc == 1)
+            if (ch.nc == 1 && ch.waves == 4)
                 kv_many_kernel<BITS, D, 1, 4><<<grid, 256, 0, s>>>(c, b, a, p);
-            else if constexpr (D < 256)
+            else if constexpr (D == 256)
+                kv_many_kernel<BITS, D, 1, 8><<<grid, 512, 0, s>>>(c, b, a, p);
+            else
                 kv_many_kernel<BITS, D, 2, 4><<<grid, 256, 0, s>>>(c, b, a, p);
             break;
     }

@@ -20,17 +20,22 @@ __all__ = ["KVCache", "KVBatch"]
 JHQ_BF16, JHQ_F16 = 3, 4
 
 
+_DTYPES = {}  # torch type -> element type, filled when torch is first needed
+
+
 def _torch():
     import torch
+    if not _DTYPES:
+        _DTYPES.update({torch.float32: _jg.JHQ_F32, torch.bfloat16: JHQ_BF16,
+                        torch.float16: JHQ_F16})
     return torch
 
 
 def _dtype(t, what):
-    torch = _torch()
-    try:
-        return {torch.float32: _jg.JHQ_F32, torch.bfloat16: JHQ_BF16, torch.float16: JHQ_F16}[t]
-    except KeyError:
-        raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t}") from None
+    dt = _DTYPES.get(t)
+    if dt is None:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t}")
+    return dt
 
 
 class KVBatch:
@@ -62,6 +67,7 @@ class KVBatch:
             raise ValueError(f"max_kv = {max_kv} tokens do not fit {int(pages.shape[1])} pages of "
                              f"{page_size}")
         self.pages, self.kv_len, self.cu_q = pages, kv_len, cu_q
+        self._index = device.index
         self.n_tokens, self.max_q, self.max_kv = int(n_tokens), int(max_q), int(max_kv)
         self._c = _jg._KvBatch(n, int(pages.shape[1]), pages.data_ptr(), kv_len.data_ptr(),
                                cu_q.data_ptr(), self.n_tokens, self.max_q, self.max_kv)
@@ -87,29 +93,43 @@ class KVCache:
         self.device = self.data.device
         self.num_pages, self.page_size = int(num_pages), int(page_size)
         self.kv_heads, self.head_dim, self.bits = int(kv_heads), int(head_dim), int(bits)
+        self._ptr = self.data.data_ptr()
+        self._scale = 1.0 / math.sqrt(self.head_dim)
+        self._index = self.device.index
+        # plain numbers: a torch.cuda.Stream object costs two microseconds a call
+        self._current, self._device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
         self._write, self._read, self._attend = L.jhq_k_kv_write, L.jhq_k_kv_read, L.jhq_k_kv_attend
 
     def batch(self, pages, kv_len, cu_q, n_tokens, max_q, max_kv):
         """The sequences of a call (KVBatch)."""
         return KVBatch(self.device, self.page_size, pages, kv_len, cu_q, n_tokens, max_q, max_kv)
 
-    def _stream(self, stream):
+    def _call(self, entry, stream, batch, *args):
+        if batch._index != self._index:
+            raise ValueError(f"the batch is on cuda:{batch._index}, the cache on {self.device}")
+        if self._device() != self._index:  # kernels are launched on the current device
+            with _torch().cuda.device(self._index):
+                return self._call(entry, stream, batch, *args)
         if stream is None:
-            return _torch().cuda.current_stream(self.device).cuda_stream
-        return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+            s = self._current(self._index)
+        else:
+            s = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+        rc = entry(self._ref, self._ptr, batch._ref, *args, s)
+        if rc:
+            _jg._check(rc)
 
     def _rows(self, t, what, heads, batch):
         """Element type and strides of a [n_tokens, heads, head_dim] tensor."""
-        if t.dim() != 3 or t.shape[0] != batch.n_tokens or t.shape[1] != heads \
-                or t.shape[2] != self.head_dim:
+        if t.shape != (batch.n_tokens, heads, self.head_dim):
             raise ValueError(f"{what} must be [{batch.n_tokens}, {heads}, {self.head_dim}], got "
                              f"{tuple(t.shape)}")
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise ValueError(f"{what} is on {t.device}, the cache on {self.device}")
-        st = t.stride()
-        if st[2] != 1:
+        tok, head, el = t.stride()
+        if el != 1:
             raise ValueError(f"{what}: the elements of a row must be contiguous")
-        return _dtype(t.dtype, what), st[0], st[1]
+        dt = _DTYPES.get(t.dtype)
+        return _dtype(t.dtype, what) if dt is None else dt, tok, head
 
     def write(self, k, v, batch, stream=None):
         """Quantises the batch's new tokens into the cache: k, v [n_tokens,
@@ -119,18 +139,17 @@ class KVCache:
         dv, vt, vh = self._rows(v, "v", self.kv_heads, batch)
         if dt != dv:
             raise ValueError(f"k is {k.dtype}, v is {v.dtype}")
-        _jg._check(self._write(self._ref, self.data.data_ptr(), batch._ref, k.data_ptr(), kt, kh,
-                               v.data_ptr(), vt, vh, dt, self._stream(stream)))
+        self._call(self._write, stream, batch, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, dt)
 
     def read(self, batch, dtype=None, k_out=None, v_out=None, stream=None):
         """The batch's new tokens as the cache holds them: k, v [n_tokens,
         kv_heads, head_dim] in `dtype` (default float32), or into k_out and
         v_out (contiguous, one type).  Rows that no sequence's tokens stand
         behind keep what they had (zero in new tensors)."""
-        torch = _torch()
         if (k_out is None) != (v_out is None):
             raise ValueError("k_out and v_out go together")
         if k_out is None:
+            torch = _torch()
             shape = (batch.n_tokens, self.kv_heads, self.head_dim)
             dtype = torch.float32 if dtype is None else dtype
             _dtype(dtype, "dtype")
@@ -144,8 +163,7 @@ class KVCache:
             raise ValueError(f"k_out is {k_out.dtype}, v_out is {v_out.dtype}")
         if not (k_out.is_contiguous() and v_out.is_contiguous()):
             raise ValueError("k_out and v_out must be contiguous")
-        _jg._check(self._read(self._ref, self.data.data_ptr(), batch._ref, k_out.data_ptr(),
-                              v_out.data_ptr(), dt, self._stream(stream)))
+        self._call(self._read, stream, batch, k_out.data_ptr(), v_out.data_ptr(), dt)
         return k_out, v_out
 
     def work_bytes(self, batch, q_heads, window=0):
@@ -165,12 +183,12 @@ class KVCache:
         work: a uint8 tensor of work_bytes() bytes, this call's alone until it has
         run; without it the call takes one from torch's allocator.  Rows outside
         cu_q keep what they had (zero where out is None)."""
-        torch = _torch()
-        heads = int(q.shape[1]) if q.dim() == 3 else 0
+        heads = q.shape[1] if q.dim() == 3 else 0
         dt, qt, qh = self._rows(q, "q", heads, batch)
         if dt == _jg.JHQ_F32:
             raise ValueError("q must be bfloat16 or float16")
         if out is None:
+            torch = _torch()
             with torch.cuda.stream(_as_stream(stream, self.device)):
                 out = torch.zeros((batch.n_tokens, heads, self.head_dim), dtype=q.dtype,
                                   device=self.device)
@@ -179,6 +197,7 @@ class KVCache:
                 raise ValueError("out must be contiguous and of q's type")
         lp = None
         if lse is not None:
+            torch = _torch()
             if lse.dtype != torch.float32 or tuple(lse.shape) != (batch.n_tokens, heads) \
                     or not lse.is_contiguous() or lse.device != self.device:
                 raise ValueError(f"lse must be a contiguous float32 [{batch.n_tokens}, {heads}] "
@@ -187,16 +206,16 @@ class KVCache:
         if work is None:
             n = self.work_bytes(batch, heads, window) if heads else 0
             if n:
+                torch = _torch()
                 with torch.cuda.stream(_as_stream(stream, self.device)):
                     work = torch.empty(n, dtype=torch.uint8, device=self.device)
-        elif work.dtype != torch.uint8 or not work.is_contiguous() or work.device != self.device:
+        elif work.element_size() != 1 or not work.is_contiguous() \
+                or work.get_device() != self._index:
             raise ValueError(f"work must be a contiguous uint8 tensor on {self.device}")
         wp, wn = (work.data_ptr(), work.numel()) if work is not None else (None, 0)
-        _jg._check(self._attend(self._ref, self.data.data_ptr(), batch._ref, q.data_ptr(), qt, qh,
-                                heads, dt,
-                                1.0 / math.sqrt(self.head_dim) if scale is None else float(scale),
-                                1 if causal else 0, int(window), out.data_ptr(), lp, wp, wn,
-                                self._stream(stream)))
+        self._call(self._attend, stream, batch, q.data_ptr(), qt, qh, heads, dt,
+                   self._scale if scale is None else float(scale), 1 if causal else 0, window,
+                   out.data_ptr(), lp, wp, wn)
         return out
 
 
