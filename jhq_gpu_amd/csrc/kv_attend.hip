@@ -138,6 +138,7 @@ struct Share {
     int lo, hi;      // tokens [lo, hi), lo a multiple of kStep
     int full_lo, full_hi;  // tokens that every row sees
     bool any;
+    bool alone;      // no other part of these rows
 };
 
 // Positions seen by new token i: [first, last).
@@ -178,6 +179,7 @@ __device__ inline Share share_of(const KvCache& c, const KvBatch& b, const KvAtt
     r.any = mine >= 0;
     if (!r.any) return r;
     span_of(r, a);
+    r.alone = p.nsplit == 1 || r.hi - r.lo <= p.chunk;
     r.lo += r.split * p.chunk;
     if (p.nsplit > 1) r.hi = min(r.hi, r.lo + p.chunk);
     return r;
@@ -842,7 +844,7 @@ void kv_many_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
         if (w.split == 0) fail_rows<D>(w, a, threadIdx.x, 64 * W);
         return;
     }
-    if (p.nsplit > 1 && w.lo >= w.hi) return;  // the join knows which parts there are
+    if (w.split && w.lo >= w.hi) return;  // the join knows which parts there are
 
     Where<BITS, D> where(c, b, w, lane);
     if (w.lo < w.hi) where.look(w.lo);
@@ -954,7 +956,7 @@ void kv_many_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
         __syncthreads();
     }
     rows.join();
-    if (p.nsplit == 1) return finish<BITS, D, NC>(w, a, r0, lane, rows);
+    if (w.alone) return finish<BITS, D, NC>(w, a, r0, lane, rows);
 #pragma unroll
     for (int k = 0; k < NC; k++) {
         const int row = r0 + k * 16 + r;
@@ -1013,8 +1015,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAt
                 const int last = min((tile + 1) * p.tile, s.q * a.G) - 1;
                 const int from = see_lo(s, a, tile * p.tile / a.G) / kStep * kStep;
                 const int hi = see_hi(s, a, last / a.G);
-                n = max(1, (hi - from + p.chunk - 1) / p.chunk);
-                if (hi <= from) n = -1;  // sees nothing: no part
+                // a tile of one part has been written already
+                n = hi - from > p.chunk ? (hi - from + p.chunk - 1) / p.chunk : 0;
                 row = slot = (s.row + i) * a.heads + h;
                 next = p.rows;
             }
