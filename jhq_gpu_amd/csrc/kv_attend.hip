@@ -4,8 +4,8 @@
 // ck_j> and o_i = sum_j w_ij vs_j cv_j / sum_j w_ij, w_ij = exp(s_ij).  Both
 // products run on the matrix cores (f32_16x16x32_f16) on the codes themselves:
 // a code is exact in float16, queries are exact there too once the largest is
-// scaled to 2^14 (only what is 2^-28 of it becomes subnormal), and sums are
-// float32.  The scales go where they cost one operation per score:
+// scaled to 2^14 (only what is 2^-28 of it becomes subnormal; rows much smaller than
+// their neighbours have a scale of their own), and sums are float32.  The scales go where they cost one operation per score:
 //   a_ij  = S_ij * (scale log2e ks_j) + log2 vs_j
 //   p'_ij = 2^(a_ij - m_i)            = w_ij vs_j 2^-m_i
 //   l_i   = sum_j p'_ij / vs_j          o_i = sum_j p'_ij cv_j / l_i
@@ -42,7 +42,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int kStep = 64;          // tokens of a step
 constexpr int kLeast = 2;          // steps of a streaming wave at least
 constexpr int kShortSpan = 1024;   // tokens that one workgroup takes alone
-constexpr float kNone = -1e30f;    // running maximum before the first token
+constexpr float kNone = -FLT_MAX;  // running maximum before the first token
 constexpr float kSlack = 8.0f;     // how far a score may pass it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -201,6 +201,8 @@ struct Rows {
     f4 o[NC][M::DT];
     float m[NC], l[NC];
     int hi[NC], lo[NC];  // the row's tokens
+    float part[NC];      // what the row's scores are multiplied by where some are uneven
+    bool uneven;
 
     // Row 16 k + lane % 16 of the wave's, which start at r0 (the share's last row
     // stands in for rows past it).
@@ -243,13 +245,14 @@ struct Rows {
         return value16(a, v[i >> 1] >> (16 * (i & 1)) & 0xffff);
     }
 
-    // The largest finite magnitude of the wave's query elements: magnitudes of
-    // either type are in the order of their bits.
-    __device__ float largest(const KvAttend& a) const {
+    // The largest finite magnitude of each row's query elements (own, by the lane), and
+    // of the wave's: magnitudes of either type are in the order of their bits.
+    __device__ float largest(const KvAttend& a, float (&own)[NC]) const {
         const uint32_t inf = a.dtype == JHQ_BF16 ? 0x7f80 : 0x7c00;
-        us2 two = {0, 0};
+        int big = 0;
 #pragma unroll
-        for (int k = 0; k < NC; k++)
+        for (int k = 0; k < NC; k++) {
+            us2 two = {0, 0};
 #pragma unroll
             for (int s = 0; s < M::KS; s++) {
                 const u4 v = __builtin_bit_cast(u4, q[k][s]);
@@ -257,37 +260,53 @@ struct Rows {
                 for (int i = 0; i < 4; i++)
                     two = __builtin_elementwise_max(two, __builtin_bit_cast(us2, v[i] & 0x7fff7fffu));
             }
-        uint32_t big = max(two[0], two[1]);
-        if (__any(big >= inf)) {
-            big = 0;
-#pragma unroll
-            for (int k = 0; k < NC; k++)
+            uint32_t row = max(two[0], two[1]);
+            if (__any(row >= inf)) {
+                row = 0;
 #pragma unroll
                 for (int s = 0; s < M::KS; s++) {
                     const u4 v = __builtin_bit_cast(u4, q[k][s]);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const uint32_t x = v[i] & 0x7fff, y = v[i] >> 16 & 0x7fff;
-                        big = max(big, max(x < inf ? x : 0, y < inf ? y : 0));
+                        row = max(row, max(x < inf ? x : 0, y < inf ? y : 0));
                     }
                 }
+            }
+            int r = static_cast<int>(row);
+            r = max(r, __shfl_xor(r, 16));
+            r = max(r, __shfl_xor(r, 32));
+            own[k] = value16(a, r);
+            big = max(big, r);
         }
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), o)));
+        for (int o = 1; o < 16; o <<= 1) big = max(big, __shfl_xor(big, o));
         return value16(a, big);
     }
 
-    // Turns the queries to operands, scaled by the power of two that takes big to
-    // 2^13 .. 2^14; returns its inverse, which S has to be multiplied by.
-    __device__ float scale(const KvAttend& a, float big) {
+    // The power of two that takes x to 2^13 .. 2^14.
+    __device__ static int exponent(float x) {
         int e = 0;
-        if (big > 0.0f) {
-            frexpf(big, &e);
+        if (x > 0.0f) {
+            frexpf(x, &e);
             e = max(-126, min(126, 14 - e));
         }
-        const float f = ldexpf(1.0f, e);
+        return e;
+    }
+
+    // Turns the queries to operands, scaled by the power of two that takes big, the
+    // largest of the workgroup's, to 2^13 .. 2^14; returns its inverse, which S has to be
+    // multiplied by.  A row that is smaller than big by more than 2^-16, of which that
+    // would leave too little, is scaled by its own, and its scores by the quotient.
+    __device__ float scale(const KvAttend& a, float big, const float (&own)[NC]) {
+        const int e = exponent(big);
+        bool any = false;
 #pragma unroll
-        for (int k = 0; k < NC; k++)
+        for (int k = 0; k < NC; k++) {
+            const int ek = own[k] > 0.0f && own[k] < big * 0x1p-16f ? exponent(own[k]) : e;
+            any |= ek != e;
+            part[k] = ldexpf(1.0f, e - ek);
+            const float f = ldexpf(1.0f, ek);
 #pragma unroll
             for (int s = 0; s < M::KS; s++) {
                 const u4 v = __builtin_bit_cast(u4, q[k][s]);
@@ -295,6 +314,8 @@ struct Rows {
                 for (int i = 0; i < 8; i++)
                     q[k][s][i] = static_cast<_Float16>(element(a, v, place<BITS>(i)) * f);
             }
+        }
+        uneven = __any(any);
         return ldexpf(1.0f, -e);
     }
 
@@ -306,6 +327,12 @@ struct Rows {
         const f4* const kk = reinterpret_cast<const f4*>(sc + at);
         const f4* const lv = reinterpret_cast<const f4*>(sc + 64 + at);
         const f4* const iv = reinterpret_cast<const f4*>(sc + 128 + at);
+        if (uneven) {
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) s[k][t] *= part[k];
+        }
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const f4 x = kk[t], y = lv[t];
@@ -625,6 +652,8 @@ struct Stream {
                     rows.add_values(t, vr[t][2 * hf], vr[t][2 * hf + 1], pr);
             }
             if (next < w.hi) load_values();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
         rows.join();
     }
@@ -633,7 +662,7 @@ struct Stream {
 // Few rows (16 NT at most) over short contexts: one workgroup has all tokens of a
 // sequence's head, its W waves take every W-th step, and what they have is joined
 // in LDS, so that one launch does it.
-template <int D, int NT>
+template <int D>
 constexpr int kShortWaves = D == 256 ? 4 : 8;
 
 template <int BITS, int D, int NT, int W>
@@ -654,7 +683,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv_short_kernel(KvCache c, KvBa
     const int j = w.lo + wave * kStep;
     rows.start(w, a, w.r0, lane);
     st.open(j, W * kStep);
-    const float f = rows.scale(a, rows.largest(a)) * (a.scale * kLog2e);
+    float own[NT];
+    const float big = rows.largest(a, own);
+    const float f = rows.scale(a, big, own) * (a.scale * kLog2e);
     st.run(rows, j, W * kStep, f, sc[wave]);
 #pragma unroll
     for (int k = 0; k < NT; k++) {
@@ -802,7 +833,9 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
             Stream<BITS, D, NT> st(c, b, w, lane);
             rows.start(w, a, 0, lane);
             st.open(w.lo, kStep);
-            const float f = rows.scale(a, rows.largest(a)) * (a.scale * kLog2e);
+            float own[NT];
+            const float big = rows.largest(a, own);
+            const float f = rows.scale(a, big, own) * (a.scale * kLog2e);
             st.run(rows, w.lo, kStep, f, sc[wave]);
             if (from == 0 && to == n)
                 finish<BITS, D, NT>(w, a, 0, lane, rows);
@@ -884,12 +917,13 @@ void kv_many_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
         if (j + kStep < w.hi) where.look(j + kStep);
     };
     if (w.lo < w.hi) fetch(w.lo);
-    float big = rows.largest(a);
+    float own[NC];
+    float big = rows.largest(a, own);
     if (lane == 0) bigs[wave] = big;
     __syncthreads();
 #pragma unroll
     for (int x = 0; x < W; x++) big = fmaxf(big, bigs[x]);
-    const float f = rows.scale(a, big) * (a.scale * kLog2e);
+    const float f = rows.scale(a, big, own) * (a.scale * kLog2e);
     auto stage = [&](int buf) {
         if (has_keys) {
 #pragma unroll
@@ -1070,6 +1104,11 @@ struct Choice {
     int64_t work;  // bytes
 };
 
+// Rows up to which a wave reads the cache for itself.  Two column tiles of 256-wide
+// heads do not fit its registers: 32 sequences of 8000 tokens, 32 rows, 162 us so and
+// 111 us through LDS.
+constexpr int few_rows(int D) { return D == 256 ? 16 : 32; }
+
 Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
     Choice r;
     Plan& p = r.p;
@@ -1078,7 +1117,7 @@ Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
                                 : b.max_kv;
     // the streaming kernel numbers steps with an int
     const bool counted = static_cast<int64_t>(b.n_seq) * c.H * (span / kStep + 2) < INT32_MAX / 2;
-    r.path = rows > 32 ? Path::kMany
+    r.path = rows > few_rows(D) ? Path::kMany
              : span <= kShortSpan ? Path::kShort : counted ? Path::kStream : Path::kMany;
     r.nc = r.path == Path::kMany ? (rows <= 64 ? 1 : 2) : (rows <= 16 ? 1 : 2);
     r.waves = r.path == Path::kMany && D == 256 && r.nc == 2 ? 8 : 4;
@@ -1130,16 +1169,16 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const C
     switch (ch.path) {
         case Path::kShort:
             if (ch.nc == 1)
-                kv_short_kernel<BITS, D, 1, kShortWaves<D, 1>>
-                    <<<grid, 64 * kShortWaves<D, 1>, 0, s>>>(c, b, a, p);
-            else
-                kv_short_kernel<BITS, D, 2, kShortWaves<D, 2>>
-                    <<<grid, 64 * kShortWaves<D, 2>, 0, s>>>(c, b, a, p);
+                kv_short_kernel<BITS, D, 1, kShortWaves<D>>
+                    <<<grid, 64 * kShortWaves<D>, 0, s>>>(c, b, a, p);
+            else if constexpr (few_rows(D) > 16)
+                kv_short_kernel<BITS, D, 2, kShortWaves<D>>
+                    <<<grid, 64 * kShortWaves<D>, 0, s>>>(c, b, a, p);
             break;
         case Path::kStream:
             if (ch.nc == 1)
                 kv_stream_kernel<BITS, D, 1><<<grid, 256, 0, s>>>(c, b, a, p);
-            else
+            else if constexpr (few_rows(D) > 16)
                 kv_stream_kernel<BITS, D, 2><<<grid, 256, 0, s>>>(c, b, a, p);
             break;
         case Path::kMany:
@@ -1157,7 +1196,7 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const C
         kv_join_kernel<D, 0><<<jgrid, 256, 0, s>>>(c, b, a, p);
     else if (ch.nc == 1)
         kv_join_kernel<D, 1><<<jgrid, 256, 0, s>>>(c, b, a, p);
-    else
+    else if constexpr (few_rows(D) > 16)
         kv_join_kernel<D, 2><<<jgrid, 256, 0, s>>>(c, b, a, p);
     return hipGetLastError();
 }

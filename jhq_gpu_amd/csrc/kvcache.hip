@@ -540,6 +540,16 @@ int check_cache(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch*
     return JHQ_OK;
 }
 
+// f's result; an exception (no memory for a message) does not leave a C entry point.
+template <class T, class F>
+T entry(T failed, F f) noexcept {
+    try {
+        return f();
+    } catch (...) {
+        return failed;
+    }
+}
+
 bool idle(const jhq_kv_batch* b) { return b->n_seq == 0 || b->n_tokens == 0 || b->max_q == 0; }
 
 int check_heads(const jhq_kv_params* p, int q_heads, int window) {
@@ -549,11 +559,7 @@ int check_heads(const jhq_kv_params* p, int q_heads, int window) {
     return JHQ_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-int64_t jhq_kv_bytes(const jhq_kv_params* p) {
+int64_t do_bytes(const jhq_kv_params* p) {
     if (check_params(p) != JHQ_OK) return 0;
     // at most 2^31 pages x 2^10 heads x 2^10 tokens x 520 bytes: past 2^60
     const __int128 n = static_cast<__int128>(p->num_pages) * p->kv_heads * block_bytes(*p);
@@ -564,9 +570,9 @@ int64_t jhq_kv_bytes(const jhq_kv_params* p) {
     return static_cast<int64_t>(n);
 }
 
-int jhq_k_kv_write(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, const void* d_k,
-                   int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok, int64_t v_head,
-                   int dtype, void* stream) {
+int do_write(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, const void* d_k,
+             int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok, int64_t v_head,
+             int dtype, void* stream) {
     const int rc = check_cache(p, d_cache, b);
     if (rc != JHQ_OK) return rc;
     if (dtype != JHQ_F32 && dtype != JHQ_BF16 && dtype != JHQ_F16)
@@ -579,8 +585,8 @@ int jhq_k_kv_write(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b,
                                               static_cast<hipStream_t>(stream)));
 }
 
-int jhq_k_kv_read(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b, void* d_k,
-                  void* d_v, int dtype, void* stream) {
+int do_read(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b, void* d_k,
+                 void* d_v, int dtype, void* stream) {
     const int rc = check_cache(p, d_cache, b);
     if (rc != JHQ_OK) return rc;
     if (dtype != JHQ_F32 && dtype != JHQ_BF16 && dtype != JHQ_F16)
@@ -591,7 +597,7 @@ int jhq_k_kv_read(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batc
                                             static_cast<hipStream_t>(stream)));
 }
 
-int64_t jhq_kv_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_heads, int window) {
+int64_t do_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_heads, int window) {
     if (check_params(p) != JHQ_OK || check_batch(b) != JHQ_OK ||
         check_heads(p, q_heads, window) != JHQ_OK)
         return -1;
@@ -600,10 +606,10 @@ int64_t jhq_kv_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_h
                                q_heads / p->kv_heads, window);
 }
 
-int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
-                    const void* d_q, int64_t q_tok, int64_t q_head, int q_heads, int dtype,
-                    float scale, int causal, int window, void* d_out, float* d_lse, void* d_work,
-                    int64_t work_bytes, void* stream) {
+int do_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
+              const void* d_q, int64_t q_tok, int64_t q_head, int q_heads, int dtype,
+              float scale, int causal, int window, void* d_out, float* d_lse, void* d_work,
+              int64_t work_bytes, void* stream) {
     int rc = check_cache(p, d_cache, b);
     if (rc == JHQ_OK) rc = check_heads(p, q_heads, window);
     if (rc != JHQ_OK) return rc;
@@ -613,7 +619,7 @@ int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_ba
     if (!std::isfinite(scale)) return bad("scale must be finite");
     if (idle(b)) return JHQ_OK;
     if (!d_q || !d_out) return bad("null queries or output");
-    const int64_t need = jhq_kv_work_bytes(p, b, q_heads, window);
+    const int64_t need = do_work_bytes(p, b, q_heads, window);
     if (need < 0) return JHQ_EINVAL;
     if (need > 0 && !d_work) return bad("null workspace");
     if (work_bytes < need)
@@ -626,6 +632,41 @@ int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_ba
                              causal, window, d_out, q16, out8, d_lse, static_cast<float*>(d_work)};
     return launched("kv_attend", jhq::kv_attend(cache_of(*p, d_cache), batch_of(*b), p->bits,
                                                 p->head_dim, a, static_cast<hipStream_t>(stream)));
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t jhq_kv_bytes(const jhq_kv_params* p) {
+    return entry(int64_t(0), [&] { return do_bytes(p); });
+}
+
+int64_t jhq_kv_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_heads, int window) {
+    return entry(int64_t(-1), [&] { return do_work_bytes(p, b, q_heads, window); });
+}
+
+int jhq_k_kv_write(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, const void* d_k,
+                   int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok, int64_t v_head,
+                   int dtype, void* stream) {
+    return entry(static_cast<int>(JHQ_ENOMEM), [&] {
+        return do_write(p, d_cache, b, d_k, k_tok, k_head, d_v, v_tok, v_head, dtype, stream);
+    });
+}
+
+int jhq_k_kv_read(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b, void* d_k,
+                  void* d_v, int dtype, void* stream) {
+    return entry(static_cast<int>(JHQ_ENOMEM), [&] { return do_read(p, d_cache, b, d_k, d_v, dtype, stream); });
+}
+
+int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
+                    const void* d_q, int64_t q_tok, int64_t q_head, int q_heads, int dtype,
+                    float scale, int causal, int window, void* d_out, float* d_lse, void* d_work,
+                    int64_t work_bytes, void* stream) {
+    return entry(static_cast<int>(JHQ_ENOMEM), [&] {
+        return do_attend(p, d_cache, b, d_q, q_tok, q_head, q_heads, dtype, scale, causal, window,
+                         d_out, d_lse, d_work, work_bytes, stream);
+    });
 }
 
 }  // extern "C"

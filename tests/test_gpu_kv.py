@@ -387,6 +387,33 @@ def test_values_of_very_different_sizes(gpu, new):
     assert torch.equal(out, small)  # powers of two in q and scale cancel
 
 
+@pytest.mark.parametrize("new,D,bits", [([2], 128, 8), ([9], 64, 4), ([100], 128, 8), ([70], 256, 4)])
+def test_queries_of_very_different_sizes(gpu, new, D, bits):
+    """Rows 2^-50 to 2^90 apart in one tile: none costs another its precision."""
+    import torch
+    w = World(gpu, [300], 1, D, bits, 16, "bf16", seed=11)
+    w.fill()
+    T, Hq = new[0], 4
+    q = torch.randn(T, Hq, D, generator=torch.Generator().manual_seed(6)) * 1.5
+    size = torch.tensor([1.0, 2.0 ** 90, 2.0 ** -50, 2.0 ** -14]).repeat(T)[torch.randperm(4 * T)]
+    size = size.view(T, Hq, 1)
+    _check(w, new, Hq, q=(q * size).bfloat16())  # bounds are each row's own
+
+
+@pytest.mark.parametrize("new", [1, 5, 80])
+def test_very_negative_scores(gpu, new):
+    """Scores of -1e36 are scores: a row whose tokens are all alike gets their value."""
+    import torch
+    D, n = 64, 90
+    w = World(gpu, [n], 1, D, 8, 16, "bf16")
+    w.k = torch.full((n, 1, D), -1e18).bfloat16()
+    w.v = torch.linspace(-1, 1, D).expand(n, 1, D).bfloat16()
+    w.fill()
+    out = w.cache.attend(torch.full((new, 2, D), 1e18, device=gpu).bfloat16(), w.batch([new]))
+    want = torch.tensor(w.held()[1][0, 0]).bfloat16()
+    assert torch.equal(out.cpu(), want.expand(new, 2, D))
+
+
 def test_strided_queries_outputs_and_streams(gpu):
     """Queries inside a fused projection and on no 16-byte boundary, own output,
     workspace and stream."""
