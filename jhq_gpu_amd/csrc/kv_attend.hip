@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 namespace jhq {
 namespace {
@@ -201,8 +202,8 @@ struct Rows {
     f4 o[NC][M::DT];
     float m[NC], l[NC];
     int hi[NC], lo[NC];  // the row's tokens
-    float part[NC];      // what the row's scores are multiplied by where some are uneven
-    bool uneven;
+    float part[NC];      // what the row's scores are multiplied by where rows are uneven
+    bool uneven;         // some part of the wave's is not 1
 
     // Row 16 k + lane % 16 of the wave's, which start at r0 (the share's last row
     // stands in for rows past it).
@@ -322,7 +323,7 @@ struct Rows {
     // Scores of half a step (its tiles 2 hf, 2 hf + 1) to weights.  s[k][t][i]: token
     // j0 + 16 g + 8 hf + 4 t + i.  sc: the step's kk, lv and iv (64 floats each).
     __device__ void weigh(f4 (&s)[NC][2], const float* sc, int lane, int j0, int hf, bool masked,
-                          h8 (&p)[NC]) {
+                          bool uneven, h8 (&p)[NC]) {
         const int at = (lane >> 4) * 16 + hf * 8;
         const f4* const kk = reinterpret_cast<const f4*>(sc + at);
         const f4* const lv = reinterpret_cast<const f4*>(sc + 64 + at);
@@ -646,7 +647,7 @@ struct Stream {
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
                 h8 pr[NT];
-                rows.weigh(s[hf], sc, lane, j, hf, masked, pr);
+                rows.weigh(s[hf], sc, lane, j, hf, masked, rows.uneven, pr);
 #pragma unroll
                 for (int t = 0; t < M::ET; t++)
                     rows.add_values(t, vr[t][2 * hf], vr[t][2 * hf + 1], pr);
@@ -961,34 +962,45 @@ void kv_many_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
     };
     int buf = 0;
     if (w.lo < w.hi) stage(0);
-    __syncthreads();
-    for (int j = w.lo; j < w.hi; j += kStep, buf ^= 1) {
-        if (j + kStep < w.hi) fetch(j + kStep);
-        const bool masked = j < w.full_lo || j + kStep > w.full_hi;
+    const bool uneven = __syncthreads_or(rows.uneven);
+    auto steps = [&](auto uneven) {
+        for (int j = w.lo; j < w.hi; j += kStep, buf ^= 1) {
+            if (j + kStep < w.hi) fetch(j + kStep);
+            const bool masked = j < w.full_lo || j + kStep > w.full_hi;
 #pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-            f4 s[NC][2];
+            for (int hf = 0; hf < 2; hf++) {
+                f4 s[NC][2];
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int q = 0; q < M::KS; q++) {
-                    const h8 x = kf[buf][((hf * 2 + t) * M::KS + q) * 64 + lane];
+                    for (int q = 0; q < M::KS; q++) {
+                        const h8 x = kf[buf][((hf * 2 + t) * M::KS + q) * 64 + lane];
 #pragma unroll
-                    for (int k = 0; k < NC; k++)
-                        s[k][t] = mfma(x, rows.q[k][q], q ? s[k][t] : f4{0, 0, 0, 0});
+                        for (int k = 0; k < NC; k++)
+                            s[k][t] = mfma(x, rows.q[k][q], q ? s[k][t] : f4{0, 0, 0, 0});
+                    }
+                h8 pr[NC];
+                rows.weigh(s, sc[buf], lane, j, hf, masked, uneven, pr);
+#pragma unroll
+                for (int t = 0; t < M::DT; t++) {
+                    const h8 v = vf[buf][(hf * M::DT + t) * 64 + lane];
+#pragma unroll
+                    for (int k = 0; k < NC; k++) rows.o[k][t] = mfma(v, pr[k], rows.o[k][t]);
                 }
-            h8 pr[NC];
-            rows.weigh(s, sc[buf], lane, j, hf, masked, pr);
-#pragma unroll
-            for (int t = 0; t < M::DT; t++) {
-                const h8 v = vf[buf][(hf * M::DT + t) * 64 + lane];
-#pragma unroll
-                for (int k = 0; k < NC; k++) rows.o[k][t] = mfma(v, pr[k], rows.o[k][t]);
             }
+            if (j + kStep < w.hi) stage(buf ^ 1);
+            __syncthreads();
         }
-        if (j + kStep < w.hi) stage(buf ^ 1);
-        __syncthreads();
-    }
+    };
+    // A loop of its own for the rare tile, as a branch in it costs the others 3% (4096
+    // tokens over 16096: 1053 and 1024 us); but two loops cost 64-wide heads the third
+    // wave of a SIMD (753 and 776 us).
+    if constexpr (D == 64)
+        steps(uneven);
+    else if (uneven)
+        steps(std::true_type());
+    else
+        steps(std::false_type());
     rows.join();
     if (w.alone) return finish<BITS, D, NC>(w, a, r0, lane, rows);
 #pragma unroll
