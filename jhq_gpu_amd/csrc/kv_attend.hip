@@ -93,13 +93,17 @@ __device__ inline void half4(uint32_t a, uint32_t b, h8& lo, h8& hi) {
     const h2 hib = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
     const h2 sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
     const uint32_t w[4] = {a, a >> 8, b, b >> 8};
+    // 1024 twice, in a register: with two constants in it, "and, or" is not one
+    // instruction
+    uint32_t k = 0x64006400u;
+    asm("" : "+v"(k));
     h2 l[4], h[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        l[i] = __builtin_bit_cast(h2, (w[i] & 0x000f000fu) | 0x64006400u) + lob;
+        l[i] = __builtin_bit_cast(h2, (w[i] & 0x000f000fu) | k) + lob;
         // 1024 + 16 n
-        h[i] = __builtin_elementwise_fma(
-            __builtin_bit_cast(h2, (w[i] & 0x00f000f0u) | 0x64006400u), sixteenth, hib);
+        h[i] = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w[i] & 0x00f000f0u) | k), sixteenth,
+                                         hib);
     }
     lo = __builtin_bit_cast(h8, l);
     hi = __builtin_bit_cast(h8, h);
