@@ -5,7 +5,8 @@
 // products run on the matrix cores (f32_16x16x32_f16) on the codes themselves:
 // a code is exact in float16, queries are exact there too once the largest is
 // scaled to 2^14 (only what is 2^-28 of it becomes subnormal; rows much smaller than
-// their neighbours have a scale of their own), and sums are float32.  The scales go where they cost one operation per score:
+// their neighbours have a scale of their own), and sums are float32.  The scales go
+// where they cost one operation per score:
 //   a_ij  = S_ij * (scale log2e ks_j) + log2 vs_j
 //   p'_ij = 2^(a_ij - m_i)            = w_ij vs_j 2^-m_i
 //   l_i   = sum_j p'_ij / vs_j          o_i = sum_j p'_ij cv_j / l_i
@@ -41,8 +42,12 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = 64;          // tokens of a step
-constexpr int kLeast = 2;          // steps of a streaming wave at least
-constexpr int kShortSpan = 1024;   // tokens that one workgroup takes alone
+// Steps of a streaming wave at least: 8 sequences of 2000 tokens 13.7 us with two, 14.9 with
+// one, 17.0 with four.
+constexpr int kLeast = 2;
+// Tokens that one workgroup takes alone: one sequence of 1000 tokens 9.7 us so and 11.8
+// streaming, of 2000 13.9 and 11.8; 64 of 1000 27.1 and 29.6.
+constexpr int kShortSpan = 1024;
 constexpr float kNone = -FLT_MAX;  // running maximum before the first token
 constexpr float kSlack = 8.0f;     // how far a score may pass it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -125,7 +130,7 @@ __device__ inline float value16(const KvAttend& a, uint32_t h) {
                : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
 }
 
-// How the work is cut; made on the host by plan_of.
+// How the work is cut; made on the host by choose().
 struct Plan {
     int tile;     // rows of a tile
     int tiles;    // tiles of a sequence with max_q new tokens
@@ -666,7 +671,9 @@ struct Stream {
 
 // Few rows (16 NT at most) over short contexts: one workgroup has all tokens of a
 // sequence's head, its W waves take every W-th step, and what they have is joined
-// in LDS, so that one launch does it.
+// in LDS, so that one launch does it.  Latency bounds it (a chain of four loads:
+// lengths, page, codes, and the queries beside them): 777 tokens, 2 x 8 rows of
+// 128, 9.4 us.  Eight waves fit their registers; of 256-wide heads only four.
 template <int D>
 constexpr int kShortWaves = D == 256 ? 4 : 8;
 
@@ -730,6 +737,10 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv_short_kernel(KvCache c, KvBa
 // a part (two at most for a wave: slot 0 where the head began before it, 1 where it
 // goes on after it), and kv_join_kernel adds the parts.  The wave that begins a
 // head notes which waves have parts of it.
+// 64 sequences of 300 to 9000 tokens, 8 heads of 128, 8 bits: 560 MB in 105 us, 5.3 TB/s
+// (reading alone reaches 6.2), the parts' sum in 5 more; cut into equal chunks of each
+// sequence instead, 149 us.  Four of 130 k tokens, 64 heads on 8 of 128, 4 bits: 425 MB in 83 us, 5.1
+// TB/s; there the vector units are busy half of the time.
 
 // Steps of sequence s (a head of it); 0 where it has no new token.
 __device__ inline int steps_of(const KvSeq& s, const KvAttend& a, int* lo, int* hi) {
@@ -803,7 +814,9 @@ __device__ inline int2* joins_of(const KvAttend& a, const Plan& p) {
 }
 
 // Streaming waves on a SIMD: two hide each other's latencies as long as a wave's
-// sums, operands and loads in flight fit half of its registers.
+// sums, operands and loads in flight fit half of its registers.  Four contexts of
+// 130 k in 4 bits: one 123 us, two 90, four, which spill, 145; 32 sequences of 8000, 64-wide
+// heads: 67, 49, 57; 256-wide ones: one 105, two, which spill, 169.
 template <int D, int NT>
 constexpr int kStreamWaves = D * NT >= 256 ? 1 : 2;
 
@@ -861,10 +874,18 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
     }
 }
 
-// Many rows: 16 NC of them a wave, W waves.  What bounds it are the matrix cores
-// and the exponentials.  A step's keys and values are turned to float16 once for the
-// workgroup, in LDS in the order in which the operands are read (16 bytes a lane,
-// consecutive), while the next step's bytes are on their way into registers.
+// Many rows: 16 NC of them a wave, W waves.  A step's keys and values are turned to
+// float16 once for the workgroup, in LDS in the order in which the operands are read
+// (16 bytes a lane, consecutive), while the next step's bytes are on their way into
+// registers.
+// What bounds it are the vector and the matrix instructions of a SIMD's two waves,
+// which overlap little: 8192 tokens over 36193, 32 heads of 128 on 8, 8 bits, 4.73 ms,
+// 911 TFLOP/s (a large float16 product reaches 1343), the matrix cores 38% busy, the
+// vector units 54%, LDS 35%.  At 4096 tokens over 16096 (922 TFLOP/s) a copy of it without
+// the exponentials reaches 1237, without turning codes to float16 1066, without either 1483.
+// Two column tiles a wave: with one a step in LDS serves half as many rows (614
+// TFLOP/s), with three and four the registers spill (564, 614).  256-wide heads: LDS
+// holds one workgroup, so it has eight waves of one tile (835; four waves of two 604).
 template <int BITS, int D, int NC, int W>
 __global__ __launch_bounds__(64 * W, W == 8 || D < 256 ? 2 : 1)
 void kv_many_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
@@ -1110,7 +1131,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAt
 }
 
 // What a call runs: 16 or 32 rows from registers (short or streaming), or tiles of 64 or
-// 128 rows through LDS.
+// 128 rows through LDS.  At 32 rows the former takes 71 us and the latter 76 for 64
+// sequences of 8000 tokens on 2 heads of 128 in 8 bits, 61 and 70 in 4, 37 and 54 with heads
+// of 64.
 enum class Path { kShort, kStream, kMany };
 struct Choice {
     Path path;
@@ -1156,7 +1179,10 @@ Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
         const int64_t seen = window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) +
                                                                       p.tile / G + 2 + kStep)
                                     : b.max_kv;
-        // no split where the tiles fill the chip (two on each of 256 CUs)
+        // Parts only as far as the tiles do not fill the chip with two on each of 256 CUs:
+        // 16 sequences of 8000 tokens, 64 rows on each of 8 heads: parts up to 256 workgroups
+        // 115 us, 512 81, 1024 89, 2048 104; a prompt of 2999 tokens, where 768 tiles need
+        // none: 120, and 152 with parts up to 1024.
         const int64_t parts = std::max<int64_t>(1, (512 + tiles - 1) / tiles);
         int64_t chunk = std::max<int64_t>(512, (seen + parts - 1) / parts);
         chunk = (chunk + kStep - 1) / kStep * kStep;
