@@ -879,8 +879,8 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
 // (16 bytes a lane, consecutive), while the next step's bytes are on their way into
 // registers.
 // What bounds it are the vector and the matrix instructions of a SIMD's two waves,
-// which overlap little: 8192 tokens over 36193, 32 heads of 128 on 8, 8 bits, 4.73 ms,
-// 911 TFLOP/s (a large float16 product reaches 1343), the matrix cores 38% busy, the
+// which overlap little: 8192 tokens over 36193, 32 heads of 128 on 8, 8 bits, 4.67 ms,
+// 923 TFLOP/s (a large float16 product reaches 1343), the matrix cores 38% busy, the
 // vector units 54%, LDS 35%.  At 4096 tokens over 16096 (922 TFLOP/s) a copy of it without
 // the exponentials reaches 1237, without turning codes to float16 1066, without either 1483.
 // Two column tiles a wave: with one a step in LDS serves half as many rows (614

@@ -222,7 +222,7 @@ __device__ inline uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d
 }
 
 // HBM-bound: reads 2 T H D elements, writes half (8 bits) or a quarter of that
-// in 16-bit types.  19192 tokens, 8 heads of 128, 8 bits: 119 MB in 25.6 us, 4.7 TB/s (a
+// in 16-bit types.  19192 tokens, 8 heads of 128, 8 bits: 119 MB in 25.0 us, 4.8 TB/s (a
 // large copy moves 4.8).
 template <int BITS, int D, int DT, bool VEC>
 __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatch b, KvRows kr,
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatc
 }
 
 // HBM-bound: the reverse of kv_write_kernel, out rows contiguous.  316386 tokens, 8 heads
-// of 64, 4 bits to float16: 761 MB in 163 us, 4.7 TB/s; elements one by one, as the codes
+// of 64, 4 bits to float16: 830 MB in 163 us, 5.1 TB/s; elements one by one, as the codes
 // lie, took 268 with the write before it, which is now 181 with it.
 template <int BITS, int D, int DT, bool VEC>
 __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvCache c, KvBatch b, void* ko,
