@@ -431,7 +431,10 @@ int64_t jhq_kv_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_h
  * window).  Query head h reads key/value head h / (q_heads / kv_heads):
  *   out = sum_j w_j v_j,  w = softmax_j(scale * <q, k_j>),
  *   lse = ln sum_j exp(scale * <q, k_j>)
- * a row that sees nothing gives 0 and -inf.  d_q as d_k above, dtype JHQ_BF16
+ * a row that sees nothing gives 0 and -inf.  Weights are held together with
+ * their values' scales in float32's range: a value row below 2^-100 of another
+ * that a query sees counts too little in the sum of the softmax, and so does a
+ * row of zeros beside values above 2^24.  d_q as d_k above, dtype JHQ_BF16
  * or JHQ_F16; d_out [n_tokens][q_heads][head_dim] contiguous in the same type;
  * d_lse [n_tokens][q_heads] float32 or NULL.  d_work: work_bytes >=
  * jhq_kv_work_bytes() bytes, 16-byte aligned, this call's alone until its

@@ -12,7 +12,10 @@
 //   l_i   = sum_j p'_ij / vs_j          o_i = sum_j p'_ij cv_j / l_i
 // m_i is a running maximum of a_ij, so p' is rounded to float16 relative to the
 // row's largest weighted scale whatever the sizes of the values.  A value scale
-// of 0 (all codes 0) counts as 2^-80, below any scale the cache holds.  m_i moves
+// of 0 (all codes 0) counts as 2^-80, below any scale the cache holds.  The price is
+// range: p' / vs is lost where p' is below 2^-126, so a weight w_max 2^-24 is in l_i as
+// long as scales differ by less than 2^102 (l_i without the scale would take a second
+// exponential, and the one is a quarter of the time with many rows).  m_i moves
 // only when some a_ij passes it by more than 8 (p' <= 2^8): then, and not at
 // every step, sums and accumulators are rescaled.
 //

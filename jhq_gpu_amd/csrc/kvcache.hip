@@ -504,12 +504,16 @@ int check_params(const jhq_kv_params* p) {
     return JHQ_OK;
 }
 
+// Positions, a window before one, and the steps a kernel goes past the end stay
+// within int.  A window as long as the longest sequence is none, so longer ones are cut.
+constexpr int kMaxTokens = 1 << 30;
+
 int check_batch(const jhq_kv_batch* b) {
     if (!b) return bad("null batch");
     if (b->n_seq < 0 || b->max_pages < 0 || b->n_tokens < 0 || b->max_q < 0 || b->max_kv < 0)
         return bad("negative size in the batch");
-    // positions, and the tile a kernel may step past the end, stay within int
-    if (b->max_kv > (1 << 30) || b->max_q > (1 << 30)) return bad("max_q and max_kv are at most 2^30");
+    if (b->max_kv > kMaxTokens || b->max_q > kMaxTokens)
+        return bad("max_q and max_kv are at most 2^30");
     if (b->n_seq > 0 && (!b->d_kv_len || !b->d_cu_q || (b->max_pages > 0 && !b->d_pages)))
         return bad("null array in the batch");
     return JHQ_OK;
@@ -632,7 +636,7 @@ int do_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b
     const int q16 = jhq::aligned16(d_q) && q_tok % 8 == 0 && q_head % 8 == 0;
     const int out8 = (reinterpret_cast<uintptr_t>(d_out) & 7) == 0;
     const jhq::KvAttend a = {{d_q, q_tok, q_head}, q_heads, q_heads / p->kv_heads, dtype, scale,
-                             causal, window, d_out, q16, out8, d_lse, static_cast<float*>(d_work)};
+                             causal, std::min(window, kMaxTokens), d_out, q16, out8, d_lse, static_cast<float*>(d_work)};
     return launched("kv_attend", jhq::kv_attend(cache_of(*p, d_cache), batch_of(*b), p->bits,
                                                 p->head_dim, a, static_cast<hipStream_t>(stream)));
 }

@@ -89,6 +89,8 @@ class KVCache:
         if n == 0:
             _jg._check(_jg.JHQ_EINVAL)
         torch = _torch()
+        if torch.device(device).type != "cuda":
+            raise ValueError(f"the cache must be on a GPU, not on {device}")
         self.data = torch.empty(n, dtype=torch.uint8, device=device)
         self.device = self.data.device
         self.num_pages, self.page_size = int(num_pages), int(page_size)

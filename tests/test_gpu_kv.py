@@ -280,6 +280,22 @@ def test_windows(gpu, window, new):
     _check(w, new, 8, window=window)
 
 
+@pytest.mark.parametrize("new", [6, 40, 200])
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31 - 1])
+def test_windows_longer_than_any_sequence(gpu, window, new):
+    """Such a window hides nothing, also where new tokens stand far before position 0
+    (more of them than tokens)."""
+    import torch
+    w = World(gpu, [3], 2, 64, 8, 16, "bf16", seed=6)
+    w.fill()
+    q = torch.randn(new, 4, 64, generator=torch.Generator().manual_seed(3)).bfloat16().to(gpu)
+    b = w.cache.batch(w.i32(w.table), w.i32([3]), w.i32([0, new]), new, new, 3)
+    lse = [torch.zeros(new, 4, device=gpu) for _ in range(2)]
+    out = w.cache.attend(q, b, window=window, lse=lse[0])
+    assert torch.equal(out, w.cache.attend(q, b, lse=lse[1])) and torch.equal(*lse)
+    assert torch.isfinite(lse[0][-3:]).all() and torch.isneginf(lse[0][:-3]).all()
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1], [120, 40, 9], [400, 40, 70]])
 def test_everything_visible(gpu, new):
     lens = [400, 40, 131]

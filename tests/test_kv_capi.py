@@ -130,3 +130,9 @@ def test_write_and_read_refuse():
     assert L.jhq_k_kv_write(P, None, B, FAKE, 1, 1, FAKE, 1, 1, 3, None) == jg.JHQ_EINVAL
     assert L.jhq_k_kv_write(None, FAKE, B, FAKE, 1, 1, FAKE, 1, 1, 3, None) == jg.JHQ_EINVAL
     assert L.jhq_k_kv_write(P, FAKE, None, FAKE, 1, 1, FAKE, 1, 1, 3, None) == jg.JHQ_EINVAL
+
+
+@pytest.mark.parametrize("device", ["cpu", "meta"])
+def test_a_cache_is_on_a_gpu(device):
+    with pytest.raises(ValueError, match="GPU"):
+        jg.KVCache(4, 16, 2, 64, device=device)
