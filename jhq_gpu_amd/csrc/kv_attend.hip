@@ -137,6 +137,7 @@ __device__ inline float value16(const KvAttend& a, uint32_t h) {
 struct Plan {
     int tile;     // rows of a tile
     int tiles;    // tiles of a sequence with max_q new tokens
+    int64_t real; // tiles of all sequences at most
     int log_workers;  // of the streaming kernel, a power of two
     int nsplit;   // parts that a tile's tokens may be cut into (many rows)
     int chunk;    // tokens of a part, a multiple of kStep
@@ -171,20 +172,85 @@ __device__ inline void span_of(Share& r, const KvAttend& a) {
     r.full_hi = see_hi(r.s, a, i0);
 }
 
+// The sum over a full wave, uniform: along rows of 16 lanes, then from row to row.
+__device__ inline int wave_sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // row_shr:2
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // row_shr:4
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // row_shr:8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+    return __builtin_amdgcn_readlane(x, 63);
+}
+
+// The lane's sequence of 64, no new token past the last.
+__device__ inline KvSeq lane_seq(const KvCache& c, const KvBatch& b, int s) {
+    if (s < b.n_seq) return kv_seq(b, s, c.shift);
+    return {0, 0, 0, true};
+}
+
+// The i-th tile of those that the sequences have, in the order of their numbers from each
+// sequence's end, then of the sequences; false past the last.  Tile numbers below t have
+// sum_s min(tiles_s, t) tiles, which is searched for i.
+__device__ inline bool tile_at(const KvCache& c, const KvBatch& b, const KvAttend& a, const Plan& p,
+                               int i, int* seq, int* tile) {
+    const int lane = threadIdx.x & 63;
+    auto tiles_of = [&](int s) { return (lane_seq(c, b, s).q * a.G + p.tile - 1) / p.tile; };
+    const int first = tiles_of(lane);
+    auto below = [&](int t) {
+        int n = min(first, t);
+        for (int s = lane + 64; s < b.n_seq; s += 64) n += min(tiles_of(s), t);
+        return wave_sum(n);
+    };
+    if (i >= below(p.tiles)) return false;
+    int lo = 0, hi = p.tiles - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (below(mid) <= i)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    int r = i - below(lo);
+    for (int x = 0; x < b.n_seq; x += 64) {
+        const uint64_t has = __ballot((x ? tiles_of(x + lane) : first) > lo);
+        const int n = __builtin_popcountll(has);
+        if (r < n) {
+            const int before = __builtin_amdgcn_mbcnt_hi(
+                static_cast<uint32_t>(has >> 32),
+                __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(has), 0));
+            *seq = x + __builtin_ctzll(__ballot((has >> lane & 1) && before == r));
+            *tile = lo;
+            return true;
+        }
+        r -= n;
+    }
+    return false;
+}
+
 // A workgroup's tile of rows and part of their tokens.
 __device__ inline Share share_of(const KvCache& c, const KvBatch& b, const KvAttend& a,
                                  const Plan& p) {
     Share r;
     // Heads vary fastest (workgroups go round the 8 XCDs, whose L2 caches then
     // hold few heads each), then sequences, then tiles from the last, which sees
-    // most, then parts.
-    uint32_t w = blockIdx.x;
-    r.head = w % c.H;
-    w /= c.H;
-    r.seq = w % b.n_seq;
-    w /= b.n_seq;
-    const int tile = w % p.tiles;
-    r.split = w / p.tiles;
+    // most, then parts.  Of several sequences only the tiles that they have are
+    // counted, so that the XCDs get equally many whatever the lengths.  12 chunks of 1 to
+    // 1500 tokens, window 1024, 8 heads on 4 of 256: 118 us, and 163 counting as many for
+    // each sequence, where two heads' sequences of one parity shared an XCD; 10 of 100 to
+    // 700, 12 heads of 64, whose keys then lay in one XCD's L2: 87 and 84.
+    const uint32_t w = blockIdx.x / c.H, real = static_cast<uint32_t>(p.real);
+    r.head = blockIdx.x % c.H;
+    r.split = w / real;
+    int tile = w % real;
+    r.seq = 0;
+    r.any = false;
+    if (p.tiles == 1) {
+        r.seq = tile;
+        tile = 0;
+    } else if (b.n_seq > 1 && !tile_at(c, b, a, p, tile, &r.seq, &tile)) {
+        return r;
+    }
     r.s = kv_seq(b, r.seq, c.shift);
     const int rows = r.s.q * a.G, mine = (rows + p.tile - 1) / p.tile - 1 - tile;
     r.r0 = mine * p.tile;
@@ -753,18 +819,6 @@ __device__ inline int steps_of(const KvSeq& s, const KvAttend& a, int* lo, int* 
     return s.q == 0 ? 0 : max(1, (*hi - *lo + kStep - 1) / kStep);
 }
 
-__device__ inline int wave_sum(int x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-    return x;
-}
-
-// The lane's sequence of 64, no new token past the last.
-__device__ inline KvSeq lane_seq(const KvCache& c, const KvBatch& b, int s) {
-    if (s < b.n_seq) return kv_seq(b, s, c.shift);
-    return {0, 0, 0, true};
-}
-
 // A wave's first step: where it lies, and how many there are.
 struct Cut {
     int per, at, end;  // steps of a wave; this wave's
@@ -780,7 +834,7 @@ __device__ inline Cut cut_of(const KvCache& c, const KvBatch& b, const KvAttend&
     int sum = n0;
     for (int s = lane + 64; s < b.n_seq; s += 64) sum += steps_of(lane_seq(c, b, s), a, &lo, &hi);
     Cut r;
-    const int total = __builtin_amdgcn_readfirstlane(wave_sum(sum)) * c.H;
+    const int total = wave_sum(sum) * c.H;
     r.per = max(kLeast, (total + (1 << p.log_workers) - 1) >> p.log_workers);
     r.at = min(static_cast<int64_t>(worker) * r.per, static_cast<int64_t>(total));
     r.end = min(r.at + r.per, total);
@@ -1166,6 +1220,10 @@ Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
     if (r.waves == 8) r.nc = 1;
     p.tile = r.path == Path::kMany ? r.nc * 16 * r.waves : r.nc * 16;
     p.tiles = static_cast<int>((rows + p.tile - 1) / p.tile);
+    // sequences whose rows overlap, which cu_q in order cannot say, may have more: the
+    // tiles past these are not run
+    p.real = std::min<int64_t>(static_cast<int64_t>(b.n_seq) * p.tiles,
+                               b.n_tokens * G / p.tile + b.n_seq);
     p.rows = b.n_tokens * c.H * G;
     p.nsplit = 1;
     p.chunk = 0;
@@ -1177,8 +1235,7 @@ Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
                  static_cast<int64_t>(b.n_seq) * c.H * 8;
     } else if (r.path == Path::kMany) {
         // workgroups without a split: no more tiles than the rows fill
-        const int64_t tiles = std::min<int64_t>(static_cast<int64_t>(b.n_seq) * p.tiles,
-                                                b.n_tokens * G / p.tile + b.n_seq) * c.H;
+        const int64_t tiles = p.real * c.H;
         const int64_t seen = window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) +
                                                                       p.tile / G + 2 + kStep)
                                     : b.max_kv;
@@ -1206,7 +1263,7 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const C
     if (static_cast<int64_t>(b.max_q) * a.G > 1 << 30) return hipErrorInvalidValue;
     const int64_t out = static_cast<int64_t>(b.n_seq) * b.max_q * a.heads;
     const int64_t blocks = ch.path == Path::kStream ? (1 << p.log_workers) / 4
-                                                    : static_cast<int64_t>(c.H) * b.n_seq * p.tiles * p.nsplit;
+                                                    : c.H * p.real * p.nsplit;
     const int jrows = ch.path == Path::kMany ? kJoinRows<D, 0> : kJoinRows<D, 1>;
     const int64_t joins = ch.path == Path::kStream || p.nsplit > 1 ? (out + jrows - 1) / jrows : 0;
     if (blocks >= 1 << 23 || joins >= 1 << 23) return hipErrorInvalidValue;

@@ -271,6 +271,20 @@ def test_chunks(gpu, bits, D, H, page, G):
     _check(w, new, H * G)
 
 
+@pytest.mark.parametrize("n_seq", [3, 64, 65, 150])
+def test_chunks_of_many_ragged_sequences(gpu, n_seq):
+    """Sequences with no tile beside ones with several, fewer and more of them than a
+    wave has lanes."""
+    rng = np.random.default_rng(n_seq)
+    new = [int(x) for x in rng.choice([0, 0, 1, 31, 33, 63, 64, 65, 129, 200], n_seq)]
+    new[0], new[-1] = 0, 130
+    lens = [q + int(x) for q, x in zip(new, rng.choice([0, 1, 50, 130], n_seq))]
+    w = World(gpu, lens, 2, 64, 8, 16, "f16", seed=n_seq)
+    w.fill()
+    _check(w, new, 4)
+    _check(w, new, 4, window=40)
+
+
 @pytest.mark.parametrize("window", [1, 15, 64, 100, 5000])
 @pytest.mark.parametrize("new", [[1, 1, 1], [200, 40, 3], [20, 20, 2]])
 def test_windows(gpu, window, new):
