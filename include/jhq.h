@@ -431,7 +431,8 @@ int64_t jhq_kv_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_h
  * window).  Query head h reads key/value head h / (q_heads / kv_heads):
  *   out = sum_j w_j v_j,  w = softmax_j(scale * <q, k_j>),
  *   lse = ln sum_j exp(scale * <q, k_j>)
- * a row that sees nothing gives 0 and -inf.  Weights are held together with
+ * a row that sees nothing gives 0 and -inf, and one whose every score is -inf (an
+ * infinite query element, scores past float32's range) NaN, as 0 / 0 is.  Weights are held together with
  * their values' scales in float32's range: a value row below 2^-100 of another
  * that a query sees counts too little in the sum of the softmax, and so does a
  * row of zeros beside values above 2^24.  d_q as d_k above, dtype JHQ_BF16

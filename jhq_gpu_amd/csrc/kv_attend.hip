@@ -162,6 +162,9 @@ __device__ inline int see_hi(const KvSeq& s, const KvAttend& a, int i) {
 __device__ inline int see_lo(const KvSeq& s, const KvAttend& a, int i) {
     return a.window ? max(0, s.n - s.q + i + 1 - a.window) : 0;
 }
+__device__ inline bool sees_any(const KvSeq& s, const KvAttend& a, int i) {
+    return see_hi(s, a, i) > see_lo(s, a, i);
+}
 
 // The tokens that rows [r0, r0 + rn) of a share's sequence attend to.
 __device__ inline void span_of(Share& r, const KvAttend& a) {
@@ -552,8 +555,14 @@ __device__ inline void store4(const KvAttend& a, int64_t i, f4 x) {
     }
 }
 
-__device__ inline float lse_of(float m, float l) {
-    return l == 0.0f ? -INFINITY : kLn2 * (m + log2f(l));
+// What a row's sums of values are multiplied by, and its log-sum-exp.  A sum of 0 is that
+// of a row that sees nothing, or of one whose every score is -inf (an infinite query
+// element, scores past float32's range): that one's softmax is 0 / 0.
+__device__ inline float inverse_of(float l, bool sees) {
+    return l == 0.0f ? (sees ? nan32() : 0.0f) : 1.0f / l;
+}
+__device__ inline float lse_of(float m, float l, bool sees) {
+    return l == 0.0f ? (sees ? nan32() : -INFINITY) : kLn2 * (m + log2f(l));
 }
 
 // A share whose sequence is not in order: its rows become NaN.
@@ -579,10 +588,11 @@ __device__ void finish(const Share& w, const KvAttend& a, int r0, int lane,
         if (row >= w.r0 + w.rn) continue;
         int64_t q;
         const int64_t o = row_of(w, a, row, &q);
-        const float f = r.l[k] == 0.0f ? 0.0f : 1.0f / r.l[k];
+        const bool sees = r.hi[k] > r.lo[k];
+        const float f = inverse_of(r.l[k], sees);
 #pragma unroll
         for (int t = 0; t < D / 16; t++) store4(a, o * D + t * 16 + g * 4, r.o[k][t] * f);
-        if (a.lse && g == 0) a.lse[o] = lse_of(r.m[k], r.l[k]);
+        if (a.lse && g == 0) a.lse[o] = lse_of(r.m[k], r.l[k], sees);
     }
 }
 
@@ -793,8 +803,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv_short_kernel(KvCache c, KvBa
         }
         int64_t q;
         const int64_t at = row_of(w, a, w.r0 + row, &q);
-        store4(a, at * D + e, o * (l == 0.0f ? 0.0f : 1.0f / l));
-        if (a.lse && e == 0) a.lse[at] = lse_of(m, l);
+        const bool sees = sees_any(w.s, a, (w.r0 + row) / a.G);
+        store4(a, at * D + e, o * inverse_of(l, sees));
+        if (a.lse && e == 0) a.lse[at] = lse_of(m, l, sees);
     }
 }
 
@@ -1123,8 +1134,10 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAt
     int64_t row = 0;      // of the output
     int64_t slot = 0, next = 0;  // the first part's row, and from one to the next
     int64_t jump = 0;     // added from the second on
+    bool sees = false;
     if (seq < b.n_seq) {
         const KvSeq s = kv_seq(b, seq, c.shift);
+        sees = sees_any(s, a, NT > 0 ? in % (b.max_q * a.G) / a.G : in / a.heads);
         if constexpr (NT > 0) {
             const int rows = b.max_q * a.G, head = in / rows, k = in % rows, i = k / a.G;
             if (i < s.q && s.ok) {
@@ -1183,8 +1196,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAt
         l = fmaf(ml[r][z][1], f, l);
         o += *reinterpret_cast<const f4*>(acc[r][z] + t * 4) * f;
     }
-    store4(a, row * D + t * 4, o * (l == 0.0f ? 0.0f : 1.0f / l));
-    if (a.lse && t == 0) a.lse[row] = lse_of(m, l);
+    store4(a, row * D + t * 4, o * inverse_of(l, sees));
+    if (a.lse && t == 0) a.lse[row] = lse_of(m, l, sees);
 }
 
 // What a call runs: 16 or 32 rows from registers (short or streaming), or tiles of 64 or
