@@ -432,10 +432,13 @@ int64_t jhq_kv_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_h
  *   out = sum_j w_j v_j,  w = softmax_j(scale * <q, k_j>),
  *   lse = ln sum_j exp(scale * <q, k_j>)
  * a row that sees nothing gives 0 and -inf, and one whose every score is -inf (an
- * infinite query element, scores past float32's range) NaN, as 0 / 0 is.  Weights are held together with
- * their values' scales in float32's range: a value row below 2^-100 of another
- * that a query sees counts too little in the sum of the softmax, and so does a
- * row of zeros beside values above 2^24.  d_q as d_k above, dtype JHQ_BF16
+ * infinite query element, scores past float32's range) NaN, as 0 / 0 is.
+ * For the sum of values, a weight times its value's scale is rounded to float16
+ * relative to the row's largest: 11 bits from 2^-23 of it on, fewer below, and
+ * nothing below 2^-34.  The sum of the softmax has weights unrounded, held
+ * together with their values' scales in float32's range: a value row below
+ * 2^-110 of another that a query sees counts too little in it, and so does a row
+ * of zeros beside values above 2^32.  d_q as d_k above, dtype JHQ_BF16
  * or JHQ_F16; d_out [n_tokens][q_heads][head_dim] contiguous in the same type;
  * d_lse [n_tokens][q_heads] float32 or NULL.  d_work: work_bytes >=
  * jhq_kv_work_bytes() bytes, 16-byte aligned, this call's alone until its

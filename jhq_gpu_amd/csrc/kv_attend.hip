@@ -10,14 +10,16 @@
 //   a_ij  = S_ij * (scale log2e ks_j) + log2 vs_j
 //   p'_ij = 2^(a_ij - m_i)            = w_ij vs_j 2^-m_i
 //   l_i   = sum_j p'_ij / vs_j          o_i = sum_j p'_ij cv_j / l_i
-// m_i is a running maximum of a_ij, so p' is rounded to float16 relative to the
-// row's largest weighted scale whatever the sizes of the values.  A value scale
-// of 0 (all codes 0) counts as 2^-80, below any scale the cache holds.  The price is
+// m_i is a running maximum of a_ij less 9, so p' is rounded to float16 relative to the
+// row's largest weighted scale whatever the sizes of the values, and in the upper part
+// of float16's range: the largest p' is 2^9 to 2^15, one of 2^-23 of it still has 11
+// bits, and only what is below 2^-34 of it is lost from o_i (of 2^20 tokens 2^-14).  A
+// value scale of 0 (all codes 0) counts as 2^-80, below any scale the cache holds.  The price is
 // range: p' / vs is lost where p' is below 2^-126, so a weight w_max 2^-24 is in l_i as
-// long as scales differ by less than 2^102 (l_i without the scale would take a second
+// long as scales differ by less than 2^111 (l_i without the scale would take a second
 // exponential, and the one is a quarter of the time with many rows).  m_i moves
-// only when some a_ij passes it by more than 8 (p' <= 2^8): then, and not at
-// every step, sums and accumulators are rescaled.
+// only when some a_ij passes the maximum that it stands for by more than 6 (p' <=
+// 2^15): then, and not at every step, sums and accumulators are rescaled.
 //
 // Layout.  Scores are computed transposed, S^T = K Q^T: a lane of the result
 // holds one query row (column lane % 16) and 4 tokens, so a row's statistics
@@ -52,7 +54,11 @@ constexpr int kLeast = 2;
 // streaming, of 2000 13.9 and 11.8; 64 of 1000 27.1 and 29.6.
 constexpr int kShortSpan = 1024;
 constexpr float kNone = -FLT_MAX;  // running maximum before the first token
-constexpr float kSlack = 8.0f;     // how far a score may pass it
+// log2 of the largest weight where the maximum has just moved, and how far a score may pass
+// that maximum before it moves again.  11 and 4 hold weights down to 2^-36 and move it more
+// often (the 4-bit passages of 64-wide heads 86.8 us with 0 and 8, 87.3 with 9 and 6, 87.8 with
+// 11 and 4).
+constexpr float kHead = 9.0f, kSlack = 6.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // The wave's number in its workgroup, as a value the compiler knows to be uniform.
@@ -443,12 +449,12 @@ struct Rows {
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) top[k] = fmaxf(top[k], s[k][t][i]);
-            over |= top[k] > m[k] + kSlack;
+            over |= top[k] > m[k] + (kHead + kSlack);
         }
         if (__any(over)) {
 #pragma unroll
             for (int k = 0; k < NC; k++) {
-                float n = fmaxf(m[k], top[k]);
+                float n = fmaxf(m[k], top[k] - kHead);
                 n = fmaxf(n, __shfl_xor(n, 16));
                 n = fmaxf(n, __shfl_xor(n, 32));
                 const float f = __builtin_amdgcn_exp2f(m[k] - n);

@@ -1,9 +1,11 @@
 """The quantised key/value cache on the device at the edges of its ranges: scores
-that are not finite."""
+that are not finite, weights far below the largest."""
 import numpy as np
 import pytest
 
 import kv_ref as ref
+
+import jhq_gpu_amd as jg
 
 from test_gpu_kv import World, _np
 
@@ -39,3 +41,41 @@ def test_rows_whose_every_score_is_minus_infinity(gpu, n, new, D, kind):
     others[hit] = False
     assert (np.abs(out - o) <= tol)[others].all()
     assert (np.abs(lse - l) <= ltol)[others].all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n,new,H,G", [(900, 1, 1, 1), (1 << 20, 1, 1, 1), (131073, 40, 1, 1),
+                                       (131073, 1024, 4, 16)])  # the last: no parts
+@pytest.mark.parametrize("low", [25.1, 24.2, 28.3])
+def test_many_small_weights_beside_a_large_one(gpu, bits, n, new, H, G, low):
+    """One token of weight 1, all others 2^-low: together they are up to some percent of the
+    output, and all of it in the element that the one token's value does not have.
+
+    Bound: weights are rounded to 2^-11 of themselves or to 2^-34 of the largest, the result
+    to 2^-11, logits (of magnitude low ln 2) are off by (D + 8) 2^-24 of it, and of the
+    sums of weights and values, which are kept in 4 and in 2 places a row, an addition is off by
+    2^-24 at most."""
+    import torch
+    D, page = 64, 1024
+    c = jg.KVCache(-(-n // page), page, H, D, bits=bits, device=gpu)
+    k = torch.zeros(n, H, D, dtype=torch.float16, device=gpu)
+    v = torch.zeros_like(k)
+    k[..., 1], v[..., 0] = 1, 1
+    hot = n // 3
+    k[hot, :, 0], k[hot, :, 1], v[hot, :, 0], v[hot, :, 1] = 1, 0, 0, 1
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=gpu)  # noqa: E731
+    pages = torch.arange(c.num_pages, dtype=torch.int32, device=gpu)[None]
+    c.write(k, v, c.batch(pages, i32([n]), i32([0, n]), n, n, n))
+    q = torch.zeros(new, H * G, D, dtype=torch.float16, device=gpu)
+    q[..., 0] = 1
+    scale = low * np.log(2)
+    out = _np(c.attend(q, c.batch(pages, i32([n]), i32([0, new]), new, new, n), scale=scale))
+    w = 2.0 ** -low
+    small = (np.arange(n - new, n)[:, None]) * w  # all that are seen but one
+    want = np.concatenate([small / (1 + small), 1 / (1 + small)], 1)
+    rel = (2.0 ** -11 + max(2.0 ** -11, 2.0 ** -34 / w) + 2 * scale * (D + 8) * 2.0 ** -24
+           + (n / 4 + n / 2) * 2.0 ** -24)
+    want = np.repeat(want[:, None], H * G, 1)
+    err = np.abs(out[..., :2] - want)
+    assert (err <= rel * want + 2.0 ** -25).all(), (err / want).max() / rel  # float16's smallest
+    assert not out[..., 2:].any()
