@@ -1121,10 +1121,12 @@ void kv_many_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
     }
 }
 
-// Adds the parts of rows; latency bounds it.  NT > 0: parts of kv_stream_kernel, rows
-// in the order (sequence, head, row), often many: a thread has 4 elements of every
-// fourth part of a row.  NT = 0: parts of kv_many_kernel, (sequence, new token, query
-// head), few parts and more rows: a thread has all of its elements' parts.
+// Adds the parts of rows; latency bounds it.  Workgroups go over the call's rows (new token,
+// query head), whose sequence a search of cu_q finds: a grid over sequences of max_q tokens
+// each has workgroups without a row wherever lengths differ (2048 tokens beside 63 single ones,
+// 8000 each, 32 heads on 8 of 128: 895 us a call so and 662 over rows).  NT > 0: parts of kv_stream_kernel,
+// often many: a thread has 4 elements of every fourth part of a row.  NT = 0: parts of
+// kv_many_kernel, few parts and more rows: a thread has all of its elements' parts.
 template <int NT>
 constexpr int kJoinSplit = NT ? 4 : 1;
 template <int D, int NT>
@@ -1133,42 +1135,48 @@ constexpr int kJoinRows = 1024 / D / kJoinSplit<NT>;  // rows of a workgroup
 template <int D, int NT>
 __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
     constexpr int T = D / 4, R = kJoinRows<D, NT>, Y = kJoinSplit<NT>;
+    constexpr int WR = 64 > Y * T ? 64 / (Y * T) : 1;  // rows of a wave
     __shared__ __align__(16) float acc[R][Y][D];
     __shared__ float ml[R][Y][2];
     const int t = threadIdx.x % T, y = threadIdx.x / T % Y, r = threadIdx.x / (Y * T);
-    const int x = blockIdx.x * R + r, per = b.max_q * a.heads;
-    const int seq = x / per, in = x % per;
+    const int x = blockIdx.x * R + r;
+    const int tok = x / a.heads, h = x - tok * a.heads;
+    const int first = __builtin_amdgcn_readfirstlane(x);
+    int seq = 0;
+#pragma unroll
+    for (int k = 0; k < WR; k++) {
+        // a wave's rows are mostly one token's
+        const int mine = (first + k) / a.heads;
+        if (k && mine == (first + k - 1) / a.heads) continue;
+        const int s = last_at_most(b.n_seq, mine, [&](int i) { return b.cu_q[i]; });
+        if (mine <= tok) seq = s;
+    }
     int n = 0;            // parts
     int64_t row = 0;      // of the output
     int64_t slot = 0, next = 0;  // the first part's row, and from one to the next
     int64_t jump = 0;     // added from the second on
     bool sees = false;
-    if (seq < b.n_seq) {
-        const KvSeq s = kv_seq(b, seq, c.shift);
-        sees = sees_any(s, a, NT > 0 ? in % (b.max_q * a.G) / a.G : in / a.heads);
+    const KvSeq s = kv_seq(b, seq, c.shift);
+    const int i = static_cast<int>(tok - s.row);
+    if (s.ok && i >= 0 && i < s.q) {
+        sees = sees_any(s, a, i);
+        row = static_cast<int64_t>(tok) * a.heads + h;
         if constexpr (NT > 0) {
-            const int rows = b.max_q * a.G, head = in / rows, k = in % rows, i = k / a.G;
-            if (i < s.q && s.ok) {
-                const int2 j = joins_of<D, NT>(a, p)[seq * c.H + head];
-                n = j.y ? j.y + 1 : 0;  // one wave had it all and has written it
-                row = (s.row + i) * a.heads + head * a.G + (k - i * a.G);
-                slot = static_cast<int64_t>(2 * j.x + 1) * (NT * 16) + k;
-                next = 2 * NT * 16;
-                jump = -NT * 16;
-            }
+            const int2 j = joins_of<D, NT>(a, p)[seq * c.H + h / a.G];
+            n = j.y ? j.y + 1 : 0;  // one wave had it all and has written it
+            slot = static_cast<int64_t>(2 * j.x + 1) * (NT * 16) + i * a.G + h % a.G;
+            next = 2 * NT * 16;
+            jump = -NT * 16;
         } else {
-            const int i = in / a.heads, h = in % a.heads;
-            if (i < s.q && s.ok) {
-                // as in share_of
-                const int tile = (i * a.G + h % a.G) / p.tile;
-                const int last = min((tile + 1) * p.tile, s.q * a.G) - 1;
-                const int from = see_lo(s, a, tile * p.tile / a.G) / kStep * kStep;
-                const int hi = see_hi(s, a, last / a.G);
-                // a tile of one part has been written already
-                n = hi - from > p.chunk ? (hi - from + p.chunk - 1) / p.chunk : 0;
-                row = slot = (s.row + i) * a.heads + h;
-                next = p.rows;
-            }
+            // as in share_of
+            const int tile = (i * a.G + h % a.G) / p.tile;
+            const int last = min((tile + 1) * p.tile, s.q * a.G) - 1;
+            const int from = see_lo(s, a, tile * p.tile / a.G) / kStep * kStep;
+            const int hi = see_hi(s, a, last / a.G);
+            // a tile of one part has been written already
+            n = hi - from > p.chunk ? (hi - from + p.chunk - 1) / p.chunk : 0;
+            slot = row;
+            next = p.rows;
         }
     }
     const float* const stats = a.work + (NT > 0 ? (int64_t(2) << p.log_workers) * (NT * 16) * D
@@ -1294,7 +1302,7 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const C
     const Plan& p = ch.p;
     // rows and positions are ints in the kernels, and a launch has 2^32 threads
     if (static_cast<int64_t>(b.max_q) * a.G > 1 << 30) return hipErrorInvalidValue;
-    const int64_t out = static_cast<int64_t>(b.n_seq) * b.max_q * a.heads;
+    const int64_t out = p.rows;
     const int64_t blocks = ch.path == Path::kStream ? (1 << p.log_workers) / 4
                                                     : c.H * p.real * p.nsplit;
     const int jrows = ch.path == Path::kMany ? kJoinRows<D, 0> : kJoinRows<D, 1>;

@@ -59,6 +59,22 @@ __device__ inline KvSeq kv_seq(const KvBatch& b, int s, int shift) {
     return r;
 }
 
+// The last s in [0, n) with key(s) <= x, for ascending keys of which the first is; the wave's
+// lanes ask for one x together and look at 64 keys at once.
+template <class F>
+__device__ inline int last_at_most(int n, int64_t x, F key) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = 0, len = n;
+    while (len > 1) {
+        const uint32_t step = (len + 63) / 64, i = lane * step;
+        const uint64_t le = __ballot(i < len && key(static_cast<int>(lo + i)) <= x) | 1;
+        const uint32_t at = (63 - __builtin_clzll(le)) * step;
+        lo += at;
+        len = min(step, len - at);
+    }
+    return static_cast<int>(lo);
+}
+
 // Page of token j of sequence s, or -1 where the table names none.
 __device__ inline int kv_page(const KvBatch& b, const KvCache& c, int s, int j) {
     const int p = b.pages[static_cast<int64_t>(s) * b.max_pages + (j >> c.shift)];

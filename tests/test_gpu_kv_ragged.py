@@ -1,0 +1,62 @@
+"""The quantised key/value cache on the device with batches whose sequences differ much:
+bounds far above most lengths, a long chunk beside single tokens, many idle slots."""
+import numpy as np
+import pytest
+
+import kv_ref as ref
+
+import jhq_gpu_amd as jg
+from test_gpu_kv import World, _check, _np
+
+pytestmark = pytest.mark.gpu
+
+
+def test_attend_within_wide_bounds(gpu):
+    """128 sequences with 512 new tokens in all, whose bounds allow 8192 each over 16384 (as a
+    captured call's do): the call is sized by its rows, and its results are those of tight
+    bounds within both runs' roundings."""
+    import torch
+    rng = np.random.default_rng(4)
+    new = [int(x) for x in rng.integers(0, 8, 128)]
+    new[5], new[77] = 0, 40
+    while sum(new) > 512:
+        new[int(rng.integers(128))] = 0
+    lens = [q + int(x) for q, x in zip(new, rng.integers(0, 60, 128))]
+    w = World(gpu, lens, 8, 128, 8, 64, "bf16", seed=4)
+    w.fill()
+    table = np.full((128, 16384 // 64), -1, np.int32)
+    table[:, :w.table.shape[1]] = w.table
+    b = w.cache.batch(w.i32(table), w.i32(lens), w.i32(np.concatenate([[0], np.cumsum(new)])), 512,
+                      8192, 16384)
+    q = torch.randn(512, 64, 128, generator=torch.Generator().manual_seed(1)).bfloat16()
+    lse = torch.full((512, 64), 7.0, device=gpu)
+    out = _np(w.cache.attend(q.to(gpu), b, lse=lse))
+    lse = lse.cpu().numpy()
+    k, v = w.held()
+    at = 0
+    for s, (a, n) in enumerate(zip(new, lens)):
+        sl = slice(w.at[s], w.at[s] + n)
+        o, l, tol, ltol = ref.attend(_np(q[at:at + a]).astype(np.float64), k[sl], v[sl], 128 ** -0.5,
+                                     unit=ref.UNIT["bf16"])
+        assert (np.abs(out[at:at + a] - o) <= tol).all(), s
+        assert (np.abs(lse[at:at + a] - l) <= ltol).all(), s
+        at += a
+    assert not out[at:].any() and (lse[at:] == 7.0).all()  # rows of no sequence
+
+
+@pytest.mark.parametrize("n_seq", [3, 71, 4200])
+@pytest.mark.parametrize("D,bits,G", [(64, 8, 3), (128, 4, 4), (256, 8, 2)])
+@pytest.mark.parametrize("chunk", [1, 9, 150])
+def test_one_chunk_beside_single_tokens(gpu, n_seq, D, bits, G, chunk):
+    """A chunk over a longer context beside single tokens and idle slots, more of them than
+    the waves of a search look at in one round, in two and in three; at the lowest count the
+    chunk's tokens are split into parts."""
+    rng = np.random.default_rng(n_seq + chunk)
+    new = [int(x) for x in rng.random(n_seq) < 60 / n_seq]
+    lens = [q and int(x) for q, x in zip(new, rng.integers(1, 40, n_seq))]
+    for at, n in ((n_seq // 2, 2300), (n_seq - 1, 1100)):
+        new[at], lens[at] = chunk, n
+    new[0] = lens[0] = 0
+    w = World(gpu, lens, 1, D, bits, 16, "f16", seed=n_seq)
+    w.fill()
+    _check(w, new, G)
