@@ -155,6 +155,11 @@ struct Unit {
     bool any;
 };
 
+// The sequences' runs are numbered one after the other: sets of them each or, where sets is 0
+// (lengths differ), from cu_q / TW + 2 seq on, which leaves floor(q / TW) + 2 at least for q new
+// tokens that may begin and end inside a group, and is found by a search.  A prompt of 32768 tokens
+// beside 511 single ones, 8 heads of 128, 8 bits: written in 2624 us with sets, 46 so; 64 prompts
+// of 100 to 500: 24.5, 21.9.
 template <int TW>
 __device__ inline Unit unit_of(const KvCache& c, const KvBatch& b, int sets) {
     Unit r;
@@ -163,14 +168,25 @@ __device__ inline Unit unit_of(const KvCache& c, const KvBatch& b, int sets) {
     u >>= 1;
     r.head = u % c.H;
     u /= c.H;
-    const int set = u % sets;
-    r.seq = u / sets;
-    r.any = r.seq < b.n_seq;
-    if (!r.any) return r;
+    int set;
+    if (sets) {
+        set = u % sets;
+        r.seq = u / sets;
+        r.any = r.seq < b.n_seq;
+        if (!r.any) return r;
+    } else {
+        auto begin = [&](int s) { return b.cu_q[s] / TW + int64_t(2) * s; };
+        r.seq = last_at_most(b.n_seq, u, begin);
+        set = static_cast<int>(u - begin(r.seq));
+        r.any = set >= 0;
+        if (!r.any) return r;
+    }
     r.q = kv_seq(b, r.seq, c.shift);
+    r.any = r.q.q > 0;
+    if (!r.any) return r;
     r.lo = max(r.q.n - r.q.q, 0);
     r.first = r.lo / kKvGroup * kKvGroup + set * TW;
-    r.any = r.q.q > 0 && (r.first < r.q.n || !r.q.ok);
+    r.any = r.first < r.q.n || !r.q.ok;
     return r;
 }
 
@@ -398,14 +414,17 @@ __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvCache c, KvBatch
     }
 }
 
-// The launch's units: per sequence the runs of max_q tokens (one more than they
-// fill, for a run that starts inside a group), every head, keys and values.
-// False where they do not fit a launch.
+// The launch's units: every head, keys and values, of each sequence's runs of max_q tokens
+// (one more than they fill, for a run that starts inside a group), or of the runs that n_tokens
+// tokens can have in n_seq sequences (sets 0) where those are fewer.  False where they do not
+// fit a launch.
 bool units(const KvBatch& b, const KvCache& c, int TW, int* sets, unsigned* blocks) {
-    const int64_t s = (static_cast<int64_t>(b.max_q) + 15 + TW - 1) / TW;
-    if (s * b.n_seq >= int64_t(1) << 31) return false;
-    const int64_t n = (s * b.n_seq * c.H * 2 + kWaves - 1) / kWaves;
-    *sets = static_cast<int>(s);
+    const int64_t each = (static_cast<int64_t>(b.max_q) + 15 + TW - 1) / TW;
+    const int64_t all = b.n_tokens / TW + int64_t(2) * b.n_seq;
+    *sets = each * b.n_seq <= all ? static_cast<int>(each) : 0;
+    const int64_t runs = std::min(each * b.n_seq, all);
+    if (runs >= int64_t(1) << 31) return false;
+    const int64_t n = (runs * c.H * 2 + kWaves - 1) / kWaves;
     *blocks = static_cast<unsigned>(n);
     return n < int64_t(1) << 23;
 }

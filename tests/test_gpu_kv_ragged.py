@@ -60,3 +60,46 @@ def test_one_chunk_beside_single_tokens(gpu, n_seq, D, bits, G, chunk):
     w = World(gpu, lens, 1, D, bits, 16, "f16", seed=n_seq)
     w.fill()
     _check(w, new, G)
+
+
+@pytest.mark.parametrize("bits,D,page", [(8, 128, 64), (4, 64, 16), (4, 128, 32)])
+@pytest.mark.parametrize("n_seq,chunk", [(3, 700), (130, 3000), (1024, 32768), (4200, 500)])
+def test_one_prompt_beside_single_tokens_in_and_back(gpu, bits, D, page, n_seq, chunk):
+    """A prompt beside single tokens and idle slots, written in two steps (the first ends inside
+    a group) and read back: equal to the definition's bit for bit, whatever the lengths."""
+    import torch
+    H = 8 if n_seq == 1024 else 2
+    rng = np.random.default_rng(n_seq)
+    lens = [int(x) for x in rng.choice([0, 1, 1, 1, 17], n_seq)]
+    lens[n_seq // 3], lens[0], lens[-1] = chunk, 0, 33
+    w = World(gpu, lens, H, D, bits, page, "bf16", seed=n_seq)
+    k, v = w.k.to(gpu), w.v.to(gpu)
+    first = [n - 1 if n > 1 else 0 for n in lens]
+    for new, have in ((first, first), ([n - f for n, f in zip(lens, first)], lens)):
+        r = torch.from_numpy(w.rows(new, have)).to(gpu)
+        w.cache.write(k[r], v[r], w.batch(new, have))
+    got = w.cache.read(w.batch(lens))
+    for a, x in zip(got, (w.k, w.v)):
+        assert np.array_equal(_np(a), ref.value32(_np(x), bits))
+    # the last 20 tokens at most of each alone, into rows that begin past the first
+    tail = [min(n, 20) for n in lens]
+    cu = np.concatenate([[0], np.cumsum(tail)]) + 5
+    b = w.cache.batch(w.i32(w.table), w.i32(lens), w.i32(cu), int(cu[-1]) + 3, chunk, chunk)
+    a, _ = w.cache.read(b)
+    assert np.array_equal(_np(a)[5:-3], ref.value32(_np(w.k), bits)[w.rows(tail)])
+    assert not a[:5].any() and not a[-3:].any()
+
+
+def test_wide_bounds_in_and_back(gpu):
+    """256 sequences whose bounds allow 131072 new tokens each, with some 640 in all."""
+    rng = np.random.default_rng(1)
+    lens = [int(x) for x in rng.integers(0, 6, 256)]
+    w = World(gpu, lens, 8, 128, 8, 64, "bf16", seed=2)
+    table = np.full((256, 131072 // 64), -1, np.int32)
+    table[:, :w.table.shape[1]] = w.table
+    b = w.cache.batch(w.i32(table), w.i32(lens), w.i32(np.concatenate([[0], np.cumsum(lens)])),
+                      sum(lens), 131072, 131072)
+    w.cache.write(w.k.to(gpu), w.v.to(gpu), b)
+    k, v = w.cache.read(b)
+    assert np.array_equal(_np(k), ref.value32(_np(w.k), 8))
+    assert np.array_equal(_np(v), ref.value32(_np(w.v), 8))
