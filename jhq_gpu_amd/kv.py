@@ -12,6 +12,7 @@ device tensors, calls only enqueue work, on the current stream or the given one.
 """
 import ctypes
 import math
+import operator
 
 import jhq_gpu_amd as _jg
 
@@ -36,6 +37,15 @@ def _dtype(t, what):
     if dt is None:
         raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t}")
     return dt
+
+
+def _window(window):
+    """A window as the C entry points take it: an int, where one past 2^30, which hides
+    nothing, is cut to it (ctypes would take it modulo 2^32)."""
+    window = operator.index(window)
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    return min(window, 1 << 30)
 
 
 class KVBatch:
@@ -170,7 +180,7 @@ class KVCache:
 
     def work_bytes(self, batch, q_heads, window=0):
         """Bytes of workspace that attend needs for this batch."""
-        n = int(_jg.lib().jhq_kv_work_bytes(self._ref, batch._ref, int(q_heads), int(window)))
+        n = int(_jg.lib().jhq_kv_work_bytes(self._ref, batch._ref, int(q_heads), _window(window)))
         if n < 0:
             _jg._check(_jg.JHQ_EINVAL)
         return n
@@ -185,6 +195,7 @@ class KVCache:
         work: a uint8 tensor of work_bytes() bytes, this call's alone until it has
         run; without it the call takes one from torch's allocator.  Rows outside
         cu_q keep what they had (zero where out is None)."""
+        window = _window(window)
         heads = q.shape[1] if q.dim() == 3 else 0
         dt, qt, qh = self._rows(q, "q", heads, batch)
         if dt == _jg.JHQ_F32:

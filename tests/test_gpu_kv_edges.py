@@ -79,3 +79,21 @@ def test_many_small_weights_beside_a_large_one(gpu, bits, n, new, H, G, low):
     err = np.abs(out[..., :2] - want)
     assert (err <= rel * want + 2.0 ** -25).all(), (err / want).max() / rel  # float16's smallest
     assert not out[..., 2:].any()
+
+
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 32, 2 ** 32 + 16, 2 ** 70, np.int64(2 ** 32 + 16)])
+def test_windows_past_32_bits(gpu, new, window):
+    """They hide nothing, whatever their lower bits say; negative ones are refused likewise."""
+    import torch
+    w = World(gpu, [300], 2, 64, 8, 16, "bf16", seed=6)
+    w.fill()
+    q = torch.randn(new, 4, 64, generator=torch.Generator().manual_seed(3)).bfloat16().to(gpu)
+    b = w.batch([new])
+    assert torch.equal(w.cache.attend(q, b, window=window), w.cache.attend(q, b))
+    assert w.cache.work_bytes(b, 4, window) == w.cache.work_bytes(b, 4, 1 << 30)
+    for bad in (-window, 16 - 2 ** 32):
+        with pytest.raises(ValueError, match="window"):
+            w.cache.attend(q, b, window=bad)
+        with pytest.raises(ValueError, match="window"):
+            w.cache.work_bytes(b, 4, bad)
