@@ -39,6 +39,14 @@ def _dtype(t, what):
     return dt
 
 
+def _int32(v, what):
+    """v as an int, refused where ctypes would cut it to its lower 32 bits."""
+    v = int(v)
+    if not -1 << 31 <= v < 1 << 31:
+        raise ValueError(f"{what} is out of range: {v}")
+    return v
+
+
 def _window(window):
     """A window as the C entry points take it: an int, where one past 2^30, which hides
     nothing, is cut to it (ctypes would take it modulo 2^32)."""
@@ -91,6 +99,10 @@ class KVCache:
     (a uint8 tensor); its contents before the first write do not matter."""
 
     def __init__(self, num_pages, page_size, kv_heads, head_dim, bits=8, device="cuda"):
+        # what is wrong within 32 bits the library refuses
+        for name, v in (("num_pages", num_pages), ("page_size", page_size), ("kv_heads", kv_heads),
+                        ("head_dim", head_dim), ("bits", bits)):
+            _int32(v, name)
         self._c = _jg._KvParams(int(bits), int(kv_heads), int(head_dim), int(page_size),
                                 int(num_pages))
         self._ref = ctypes.byref(self._c)
@@ -180,7 +192,7 @@ class KVCache:
 
     def work_bytes(self, batch, q_heads, window=0):
         """Bytes of workspace that attend needs for this batch."""
-        n = int(_jg.lib().jhq_kv_work_bytes(self._ref, batch._ref, int(q_heads), _window(window)))
+        n = int(_jg.lib().jhq_kv_work_bytes(self._ref, batch._ref, _int32(q_heads, "q_heads"), _window(window)))
         if n < 0:
             _jg._check(_jg.JHQ_EINVAL)
         return n
