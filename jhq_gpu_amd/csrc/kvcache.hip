@@ -155,12 +155,12 @@ struct Unit {
     bool any;
 };
 
-// The sequences' runs are numbered one after the other: sets of them each or, where sets is 0
-// (lengths differ), from cu_q / TW + 2 seq on, which leaves floor(q / TW) + 2 at least for q new
+// The sequences' runs are numbered one after the other: sets of them each or, where lengths
+// differ (SEARCH), from cu_q / TW + 2 seq on, which leaves floor(q / TW) + 2 at least for q new
 // tokens that may begin and end inside a group, and is found by a search.  A prompt of 32768 tokens
 // beside 511 single ones, 8 heads of 128, 8 bits: written in 2624 us with sets, 46 so; 64 prompts
 // of 100 to 500: 24.5, 21.9.
-template <int TW>
+template <int TW, bool SEARCH>
 __device__ inline Unit unit_of(const KvCache& c, const KvBatch& b, int sets) {
     Unit r;
     uint32_t u = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -169,7 +169,7 @@ __device__ inline Unit unit_of(const KvCache& c, const KvBatch& b, int sets) {
     r.head = u % c.H;
     u /= c.H;
     int set;
-    if (sets) {
+    if constexpr (!SEARCH) {
         set = u % sets;
         r.seq = u / sets;
         r.any = r.seq < b.n_seq;
@@ -240,14 +240,14 @@ __device__ inline uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d
 // HBM-bound: reads 2 T H D elements, writes half (8 bits) or a quarter of that
 // in 16-bit types.  19192 tokens, 8 heads of 128, 8 bits: 119 MB in 25.0 us, 4.8 TB/s (a
 // large copy moves 4.8).
-template <int BITS, int D, int DT, bool VEC>
+template <int BITS, int D, int DT, bool VEC, bool SEARCH>
 __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatch b, KvRows kr,
                                                                KvRows vr, int sets) {
     using R = Run<BITS, D>;
     __shared__ __align__(16) uint8_t lds[kWaves][R::LDS];
     __shared__ int mags[kWaves][R::TW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Unit u = unit_of<R::TW>(c, b, sets);
+    const Unit u = unit_of<R::TW, SEARCH>(c, b, sets);
     if (!u.any || !u.q.ok) return;  // wave-uniform; the waves share nothing
     const Groups<R::TW> gr(c, b, u);
     const uint32_t live = gr.live & gr.held();
@@ -339,14 +339,14 @@ __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatc
 // HBM-bound: the reverse of kv_write_kernel, out rows contiguous.  316386 tokens, 8 heads
 // of 64, 4 bits to float16: 830 MB in 163 us, 5.1 TB/s; elements one by one, as the codes
 // lie, took 268 with the write before it, which is now 181 with it.
-template <int BITS, int D, int DT, bool VEC>
+template <int BITS, int D, int DT, bool VEC, bool SEARCH>
 __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvCache c, KvBatch b, void* ko,
                                                               void* vo, int sets) {
     using R = Run<BITS, D>;
     __shared__ __align__(16) uint8_t lds[kWaves][R::LDS];
     __shared__ float scales[kWaves][R::TW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Unit u = unit_of<R::TW>(c, b, sets);
+    const Unit u = unit_of<R::TW, SEARCH>(c, b, sets);
     void* const out = u.value ? vo : ko;
     if (!u.any || !out) return;  // wave-uniform; the waves share nothing
     const Groups<R::TW> gr(c, b, u);
@@ -416,13 +416,15 @@ __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvCache c, KvBatch
 
 // The launch's units: every head, keys and values, of each sequence's runs of max_q tokens
 // (one more than they fill, for a run that starts inside a group), or of the runs that n_tokens
-// tokens can have in n_seq sequences (sets 0) where those are fewer.  False where they do not
-// fit a launch.
+// tokens can have in n_seq sequences (sets 0) where those are fewer by a third: 5509 tokens of 3
+// sequences in and out, a head of 256, 561 and 350 runs: 15.0 us without a search, 13.8 with; 303 of
+// 3, 8 heads of 256, 33 and 24 runs: 12.1, 12.7.  False where they do not fit a launch.
 bool units(const KvBatch& b, const KvCache& c, int TW, int* sets, unsigned* blocks) {
     const int64_t each = (static_cast<int64_t>(b.max_q) + 15 + TW - 1) / TW;
     const int64_t all = b.n_tokens / TW + int64_t(2) * b.n_seq;
-    *sets = each * b.n_seq <= all ? static_cast<int>(each) : 0;
-    const int64_t runs = std::min(each * b.n_seq, all);
+    const bool search = 2 * each * b.n_seq > 3 * all;
+    const int64_t runs = search ? all : each * b.n_seq;
+    *sets = search ? 0 : static_cast<int>(each);
     if (runs >= int64_t(1) << 31) return false;
     const int64_t n = (runs * c.H * 2 + kWaves - 1) / kWaves;
     *blocks = static_cast<unsigned>(n);
@@ -458,7 +460,10 @@ struct Write {
         int sets;
         unsigned blocks;
         if (!units(b, c, Run<BITS, D>::TW, &sets, &blocks)) return hipErrorInvalidValue;
-        kv_write_kernel<BITS, D, DT, VEC><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
+        if (sets)
+            kv_write_kernel<BITS, D, DT, VEC, false><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
+        else
+            kv_write_kernel<BITS, D, DT, VEC, true><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
         return hipGetLastError();
     }
 };
@@ -469,7 +474,10 @@ struct Read {
         int sets;
         unsigned blocks;
         if (!units(b, c, Run<BITS, D>::TW, &sets, &blocks)) return hipErrorInvalidValue;
-        kv_read_kernel<BITS, D, DT, VEC><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
+        if (sets)
+            kv_read_kernel<BITS, D, DT, VEC, false><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
+        else
+            kv_read_kernel<BITS, D, DT, VEC, true><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
         return hipGetLastError();
     }
 };
