@@ -1274,15 +1274,19 @@ Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
         // none: 120, and 152 with parts up to 1024.
         const int64_t parts = std::max<int64_t>(1, (512 + tiles - 1) / tiles);
         int64_t chunk = std::max<int64_t>(512, (seen + parts - 1) / parts);
-        // Long contexts beyond that where the last round of tiles leaves a tenth of the places
-        // empty: a part of 4096 tokens or more outweighs its place in the join.
-        // 2 x 2500 tokens over 32500, 16 heads on 4 of 128: 2065 us without, 1511 with; 2 x 1683
-        // over 94506, 16 heads of 64, 4 bits: 5750, 4061; 8 x 100 to 1000 over 12000: 400, 358;
-        // 256-wide heads 565, 578.  Where tiles end in whole rounds it costs: 4096 over
-        // 16096, 1021 without and 1115 with; 6000 on themselves 361, 413.
-        const int64_t places = D == 256 ? 256 : 512;
-        const int64_t last = (tiles + places - 1) / places * places;
-        if (10 * tiles < 9 * last) {
+        // Long contexts beyond that where the last round of workgroups leaves a tenth of the places
+        // empty: a part of 4096 tokens or more outweighs its place in the join.  2500 tokens
+        // over 32500, 32 heads on 8 of 128: 2027 us without, 1467 with; on 8 of 256 3683, 3237; 16
+        // heads of 64, 4 bits, 561, 490; 64 x 10 to 100 over 9000 of the latter 570, 482.  Where
+        // rounds are whole it costs: 2 x 1000 over 21000, 8 heads on 2 of 256, 450 without and 526
+        // with; 4096 over 16096, 32 on 8 of 128, 1021, 1115.  Tiles are counted as the bounds allow:
+        // where ragged lengths have fewer, it can be wrong (100 x 1 to 40 over 6000, 32 on 8 of
+        // 128: 551, 579).
+        const bool three = D == 64 && c.codes >> c.shift == 32;  // workgroups of a CU: 4 bits
+        const int64_t places = D == 256 ? 256 : three ? 768 : 512;
+        const int64_t groups = tiles * ((seen + chunk - 1) / chunk);
+        const int64_t last = (groups + places - 1) / places * places;
+        if (10 * groups < 9 * last) {
             const int64_t finer = (4 * places + tiles - 1) / tiles;
             chunk = std::min(chunk, std::max<int64_t>(4096, (seen + finer - 1) / finer));
         }
