@@ -59,6 +59,7 @@ constexpr float kNone = -FLT_MAX;  // running maximum before the first token
 // often (the 4-bit passages of 64-wide heads 86.8 us with 0 and 8, 87.3 with 9 and 6, 87.8 with
 // 11 and 4).
 constexpr float kHead = 9.0f, kSlack = 6.0f;
+constexpr float kHeadPart = 0x1p-9f;  // 2^-kHead
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // The wave's number in its workgroup, as a value the compiler knows to be uniform.
@@ -568,7 +569,9 @@ __device__ inline float inverse_of(float l, bool sees) {
     return l == 0.0f ? (sees ? nan32() : 0.0f) : 1.0f / l;
 }
 __device__ inline float lse_of(float m, float l, bool sees) {
-    return l == 0.0f ? (sees ? nan32() : -INFINITY) : kLn2 * (m + log2f(l));
+    // both terms without kHead, which would only add to their roundings
+    const float x = (m + kHead) + log2f(l * kHeadPart);
+    return l == 0.0f ? (sees ? nan32() : -INFINITY) : kLn2 * x;
 }
 
 // A share whose sequence is not in order: its rows become NaN.

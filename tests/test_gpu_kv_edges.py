@@ -97,3 +97,21 @@ def test_windows_past_32_bits(gpu, new, window):
             w.cache.attend(q, b, window=bad)
         with pytest.raises(ValueError, match="window"):
             w.cache.work_bytes(b, 4, bad)
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_log_sum_exp_of_single_tokens(gpu, D):
+    """Rows that see one token: the log-sum-exp is the score, within kv_ref's bound for small
+    ones."""
+    import torch
+    w = World(gpu, [1] * 300, 2, D, 8, 16, "bf16", seed=D)
+    w.fill()
+    q = (torch.randn(300, 16, D, generator=torch.Generator().manual_seed(5)) * 1.5).bfloat16()
+    lse = torch.zeros(300, 16, device=gpu)
+    w.cache.attend(q.to(gpu), w.batch([1] * 300), scale=0.05 * D ** -0.5, lse=lse)
+    lse = lse.cpu().numpy()
+    k, v = w.held()
+    qq = _np(q).astype(np.float64)
+    for s in range(300):
+        _, want, _, tol = ref.attend(qq[s:s + 1], k[s:s + 1], v[s:s + 1], 0.05 * D ** -0.5)
+        assert (np.abs(lse[s] - want[0]) <= tol[0]).all(), s
