@@ -103,39 +103,3 @@ def test_wide_bounds_in_and_back(gpu):
     k, v = w.cache.read(b)
     assert np.array_equal(_np(k), ref.value32(_np(w.k), 8))
     assert np.array_equal(_np(v), ref.value32(_np(w.v), 8))
-
-
-@pytest.mark.parametrize("D,bits,H,G,new,n,window,causal", [
-    (128, 8, 4, 16, 600, 20000, 0, True),     # parts of 4096 tokens, five of them
-    (128, 8, 4, 16, 600, 20000, 0, False),
-    (128, 4, 4, 16, 600, 20000, 9000, True),
-    (256, 8, 2, 8, 700, 21000, 0, True),
-    (64, 4, 4, 16, 900, 13000, 0, True),
-])
-def test_every_step_counts_once_in_many_parts(gpu, D, bits, H, G, new, n, window, causal):
-    """With scale 0 all weights are alike: each step of 64 tokens has a value of its own, so that
-    a step or a part that is left out or counted twice shows in its element.  Sizes at which many
-    rows are cut into parts because the last round of workgroups would be part empty.
-
-    Bound: weights 1 are exact, their sums of at most 2^20 too; one division and the rounding of the
-    result, and half a unit of the log-sum-exp's float32."""
-    import torch
-    c = jg.KVCache(-(-n // 64), 64, H, D, bits=bits, device=gpu)
-    step = np.arange(n) // 64 % D
-    v = np.zeros((n, D), np.float32)
-    v[np.arange(n), step] = 1
-    vt = torch.from_numpy(v).half().to(gpu)[:, None].expand(n, H, D)
-    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=gpu)  # noqa: E731
-    pages = torch.randperm(c.num_pages, generator=torch.Generator().manual_seed(1)).int()[None]
-    pages = pages.to(gpu)
-    c.write(torch.ones_like(vt), vt, c.batch(pages, i32([n]), i32([0, n]), n, n, n))
-    q = torch.randn(new, H * G, D, generator=torch.Generator().manual_seed(2)).half().to(gpu)
-    lse = torch.zeros(new, H * G, device=gpu)
-    out = _np(c.attend(q, c.batch(pages, i32([n]), i32([0, new]), new, new, n), scale=0.0,
-                       causal=causal, window=window, lse=lse))
-    hi = np.arange(n - new, n) + 1 if causal else np.full(new, n)
-    lo = np.maximum(0, hi - window) if window else np.zeros_like(hi)
-    upto = np.concatenate([np.zeros((1, D)), np.cumsum(v, 0, dtype=np.float64)])
-    want = ((upto[hi] - upto[lo]) / (hi - lo)[:, None])[:, None]
-    assert (np.abs(out - want) <= want * (2.0 ** -11 + 2.0 ** -20) + 2.0 ** -25).all()
-    assert (np.abs(lse.cpu().numpy() - np.log(hi - lo)[:, None]) <= 1e-5).all()
