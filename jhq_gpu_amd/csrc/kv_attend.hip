@@ -50,6 +50,12 @@ constexpr int kStep = 64;          // tokens of a step
 // Steps of a streaming wave at least: 8 sequences of 2000 tokens 13.7 us with two, 14.9 with
 // one, 17.0 with four.
 constexpr int kLeast = 2;
+// Sequences up to which tiles are numbered by their place from the end, which takes a sum over
+// all sequences for every bit of their number: a lane holds one.  Tiles of more are numbered one
+// sequence after the other, in one pass.  New tokens over 300 more, 32 heads on 8 of 128: 1024 of 1 to
+// 58 791 us sorted and 600 not, 512 of 1 to 117 608 and 491, 128 of 1 to 468 482 and 460; 12 of 64:
+// 128 of 234 136, 141; 64 of 468 150, 163.  12 windowed chunks on heads of 256: 115, 160.
+constexpr int kSorted = 64;
 // Tokens that one workgroup takes alone: one sequence of 1000 tokens 9.7 us so and 11.8
 // streaming, of 2000 13.9 and 11.8; 64 of 1000 27.1 and 29.6.
 constexpr int kShortSpan = 1024;
@@ -199,17 +205,52 @@ __device__ inline KvSeq lane_seq(const KvCache& c, const KvBatch& b, int s) {
     return {0, 0, 0, true};
 }
 
+// Tiles of sequence s, none past the last.
+__device__ inline int tiles_of(const KvCache& c, const KvBatch& b, const KvAttend& a, const Plan& p,
+                               int s) {
+    return (lane_seq(c, b, s).q * a.G + p.tile - 1) / p.tile;
+}
+
+// The i-th tile of those that the sequences have, one sequence after the other; false past the
+// last.
+__device__ inline bool tile_in_order(const KvCache& c, const KvBatch& b, const KvAttend& a,
+                                     const Plan& p, int i, int* seq, int* tile) {
+    const int lane = threadIdx.x & 63;
+    for (int x = 0; x < b.n_seq; x += 256) {
+        int n[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) n[u] = tiles_of(c, b, a, p, x + u * 64 + lane);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int sum = wave_sum(n[u]);
+            if (i < sum) {
+                int in = n[u];  // inclusive sum
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int y = __shfl_up(in, o);
+                    if (lane >= o) in += y;
+                }
+                const int k = __builtin_ctzll(__ballot(in > i));
+                *seq = x + u * 64 + k;
+                *tile = i - __builtin_amdgcn_readlane(in - n[u], k);
+                return true;
+            }
+            i -= sum;
+        }
+    }
+    return false;
+}
+
 // The i-th tile of those that the sequences have, in the order of their numbers from each
 // sequence's end, then of the sequences; false past the last.  Tile numbers below t have
 // sum_s min(tiles_s, t) tiles, which is searched for i.
 __device__ inline bool tile_at(const KvCache& c, const KvBatch& b, const KvAttend& a, const Plan& p,
                                int i, int* seq, int* tile) {
     const int lane = threadIdx.x & 63;
-    auto tiles_of = [&](int s) { return (lane_seq(c, b, s).q * a.G + p.tile - 1) / p.tile; };
-    const int first = tiles_of(lane);
+    const int first = tiles_of(c, b, a, p, lane);
     auto below = [&](int t) {
         int n = min(first, t);
-        for (int s = lane + 64; s < b.n_seq; s += 64) n += min(tiles_of(s), t);
+        for (int s = lane + 64; s < b.n_seq; s += 64) n += min(tiles_of(c, b, a, p, s), t);
         return wave_sum(n);
     };
     if (i >= below(p.tiles)) return false;
@@ -223,7 +264,7 @@ __device__ inline bool tile_at(const KvCache& c, const KvBatch& b, const KvAtten
     }
     int r = i - below(lo);
     for (int x = 0; x < b.n_seq; x += 64) {
-        const uint64_t has = __ballot((x ? tiles_of(x + lane) : first) > lo);
+        const uint64_t has = __ballot((x ? tiles_of(c, b, a, p, x + lane) : first) > lo);
         const int n = __builtin_popcountll(has);
         if (r < n) {
             const int before = __builtin_amdgcn_mbcnt_hi(
@@ -244,11 +285,11 @@ __device__ inline Share share_of(const KvCache& c, const KvBatch& b, const KvAtt
     Share r;
     // Heads vary fastest (workgroups go round the 8 XCDs, whose L2 caches then
     // hold few heads each), then sequences, then tiles from the last, which sees
-    // most, then parts.  Of several sequences only the tiles that they have are
-    // counted, so that the XCDs get equally many whatever the lengths.  12 chunks of 1 to
-    // 1500 tokens, window 1024, 8 heads on 4 of 256: 118 us, and 163 counting as many for
-    // each sequence, where two heads' sequences of one parity shared an XCD; 10 of 100 to
-    // 700, 12 heads of 64, whose keys then lay in one XCD's L2: 87 and 84.
+    // most (of many sequences: sequence by sequence), then parts.  Of several only the tiles
+    // that they have are counted, so that the XCDs get equally many whatever the lengths.
+    // 12 chunks of 1 to 1500 tokens, window 1024, 8 heads on 4 of 256: 118 us, and 163
+    // counting as many for each sequence, where two heads' sequences of one parity shared an
+    // XCD; 10 of 100 to 700, 12 heads of 64, whose keys then lay in one XCD's L2: 87 and 84.
     const uint32_t w = blockIdx.x / c.H, real = static_cast<uint32_t>(p.real);
     r.head = blockIdx.x % c.H;
     r.split = w / real;
@@ -258,6 +299,8 @@ __device__ inline Share share_of(const KvCache& c, const KvBatch& b, const KvAtt
     if (p.tiles == 1) {
         r.seq = tile;
         tile = 0;
+    } else if (b.n_seq > kSorted) {
+        if (!tile_in_order(c, b, a, p, tile, &r.seq, &tile)) return r;
     } else if (b.n_seq > 1 && !tile_at(c, b, a, p, tile, &r.seq, &tile)) {
         return r;
     }
