@@ -806,7 +806,9 @@ struct Stream {
 // sequence's head, its W waves take every W-th step, and what they have is joined
 // in LDS, so that one launch does it.  Latency bounds it (a chain of four loads:
 // lengths, page, codes, and the queries beside them): 777 tokens, 2 x 8 rows of
-// 128, 9.4 us.  Eight waves fit their registers; of 256-wide heads only four.
+// 128, 9.4 us.  Eight waves, of 256-wide heads four, whose registers would not suffice for more;
+// 32 rows of 128 in 8 bits spill seven of them and are faster all the same (64 x 1 over 1000, 2 heads:
+// 16.8 us, and 18.3 with four waves).
 template <int D>
 constexpr int kShortWaves = D == 256 ? 4 : 8;
 
@@ -1001,9 +1003,9 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
 // (16 bytes a lane, consecutive), while the next step's bytes are on their way into
 // registers.
 // What bounds it are the vector and the matrix instructions of a SIMD's two waves,
-// which overlap little: 8192 tokens over 36193, 32 heads of 128 on 8, 8 bits, 4.67 ms,
-// 923 TFLOP/s (a large float16 product reaches 1343), the matrix cores 38% busy, the
-// vector units 54%, LDS 35%.  At 4096 tokens over 16096 (922 TFLOP/s) a copy of it without
+// which overlap little: 8192 tokens over 36193, 32 heads of 128 on 8, 8 bits, 4.7 to
+// 5.0 ms on different cards, 923 to 861 TFLOP/s (a large float16 product reaches 1343), the
+// matrix cores 37% busy, the vector units 54%, LDS 35%.  At 4096 tokens over 16096 (922 TFLOP/s) a copy of it without
 // the exponentials reaches 1237, without turning codes to float16 1066, without either 1483.
 // Two column tiles a wave: with one a step in LDS serves half as many rows (614
 // TFLOP/s), with three and four the registers spill (564, 614).  256-wide heads: LDS

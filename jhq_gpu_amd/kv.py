@@ -4,6 +4,8 @@ of include/jhq.h; no counterpart in the reference).
 A cache is a buffer of pages; which pages hold which sequence is the caller's
 page table, and a ``KVBatch`` says what one call works on.  Everything is torch
 device tensors, calls only enqueue work, on the current stream or the given one.
+It is a store for serving: no gradient passes through write, read or attend, and
+what they return never requires one, whatever the inputs do.
 
     cache = KVCache(num_pages=4096, page_size=64, kv_heads=8, head_dim=128, bits=8)
     batch = cache.batch(pages, kv_len, cu_q, n_tokens, max_q, max_kv)
