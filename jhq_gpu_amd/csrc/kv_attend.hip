@@ -155,6 +155,7 @@ struct Plan {
     int nsplit;   // parts that a tile's tokens may be cut into (many rows)
     int chunk;    // tokens of a part, a multiple of kStep
     int64_t rows; // of the partial results: n_tokens * query heads
+    int per;      // tokens that the join takes for a sequence, 0: it goes over rows
 };
 
 // Rows of one head of one sequence, and tokens that they attend to.
@@ -1169,10 +1170,11 @@ void kv_many_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
     }
 }
 
-// Adds the parts of rows; latency bounds it.  Workgroups go over the call's rows (new token,
-// query head), whose sequence a search of cu_q finds: a grid over sequences of max_q tokens
-// each has workgroups without a row wherever lengths differ (2048 tokens beside 63 single ones,
-// 8000 each, 32 heads on 8 of 128: 895 us a call so and 662 over rows).  NT > 0: parts of kv_stream_kernel,
+// Adds the parts of rows; latency bounds it.  Workgroups go over sequences of max_q tokens each
+// or, where those are many more than the call's rows (new token, query head), over the rows, whose
+// sequence a search of cu_q finds: 2048 tokens beside 63 single ones, 8000 each, 32 heads on 8
+// of 128, 895 us a call in the first way and 662 in the second; 64 single tokens in the first
+// lines of arrays of 65536, 109 and 701.  NT > 0: parts of kv_stream_kernel,
 // often many: a thread has 4 elements of every fourth part of a row.  NT = 0: parts of
 // kv_many_kernel, few parts and more rows: a thread has all of its elements' parts.
 template <int NT>
@@ -1189,26 +1191,32 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAt
     const int t = threadIdx.x % T, y = threadIdx.x / T % Y, r = threadIdx.x / (Y * T);
     const int x = blockIdx.x * R + r;
     const int tok = x / a.heads, h = x - tok * a.heads;
-    const int first = __builtin_amdgcn_readfirstlane(x);
-    int seq = 0;
+    int seq = 0, i = 0;
+    if (p.per) {
+        seq = tok / p.per;
+        i = tok - seq * p.per;
+    } else {
+        const int first = __builtin_amdgcn_readfirstlane(x);
 #pragma unroll
-    for (int k = 0; k < WR; k++) {
-        // a wave's rows are mostly one token's
-        const int mine = (first + k) / a.heads;
-        if (k && mine == (first + k - 1) / a.heads) continue;
-        const int s = last_at_most(b.n_seq, mine, [&](int i) { return b.cu_q[i]; });
-        if (mine <= tok) seq = s;
+        for (int k = 0; k < WR; k++) {
+            // a wave's rows are mostly one token's
+            const int mine = (first + k) / a.heads;
+            if (k && mine == (first + k - 1) / a.heads) continue;
+            const int s = last_at_most(b.n_seq, mine, [&](int j) { return b.cu_q[j]; });
+            if (mine <= tok) seq = s;
+        }
     }
     int n = 0;            // parts
     int64_t row = 0;      // of the output
     int64_t slot = 0, next = 0;  // the first part's row, and from one to the next
     int64_t jump = 0;     // added from the second on
     bool sees = false;
-    const KvSeq s = kv_seq(b, seq, c.shift);
-    const int i = static_cast<int>(tok - s.row);
+    KvSeq s = {0, 0, 0, false};
+    if (seq < b.n_seq) s = kv_seq(b, seq, c.shift);
+    if (!p.per) i = static_cast<int>(tok - s.row);
     if (s.ok && i >= 0 && i < s.q) {
         sees = sees_any(s, a, i);
-        row = static_cast<int64_t>(tok) * a.heads + h;
+        row = (s.row + i) * a.heads + h;
         if constexpr (NT > 0) {
             const int2 j = joins_of<D, NT>(a, p)[seq * c.H + h / a.G];
             n = j.y ? j.y + 1 : 0;  // one wave had it all and has written it
@@ -1302,6 +1310,8 @@ Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
     p.real = std::min<int64_t>(static_cast<int64_t>(b.n_seq) * p.tiles,
                                b.n_tokens * G / p.tile + b.n_seq);
     p.rows = b.n_tokens * c.H * G;
+    const int64_t all = static_cast<int64_t>(b.n_seq) * b.max_q;
+    p.per = 2 * all > 3 * b.n_tokens ? 0 : b.max_q;
     p.nsplit = 1;
     p.chunk = 0;
     p.log_workers = 0;
@@ -1354,7 +1364,7 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const C
     const Plan& p = ch.p;
     // rows and positions are ints in the kernels, and a launch has 2^32 threads
     if (static_cast<int64_t>(b.max_q) * a.G > 1 << 30) return hipErrorInvalidValue;
-    const int64_t out = p.rows;
+    const int64_t out = p.per ? static_cast<int64_t>(b.n_seq) * p.per * a.heads : p.rows;
     const int64_t blocks = ch.path == Path::kStream ? (1 << p.log_workers) / 4
                                                     : c.H * p.real * p.nsplit;
     const int jrows = ch.path == Path::kMany ? kJoinRows<D, 0> : kJoinRows<D, 1>;

@@ -103,3 +103,28 @@ def test_wide_bounds_in_and_back(gpu):
     k, v = w.cache.read(b)
     assert np.array_equal(_np(k), ref.value32(_np(w.k), 8))
     assert np.array_equal(_np(v), ref.value32(_np(w.v), 8))
+
+
+def test_few_sequences_in_long_arrays(gpu):
+    """Single tokens whose rows are the first of arrays of 2^18: the call is sized by the
+    sequences, and the other rows keep what they had."""
+    import torch
+    w = World(gpu, [1200] * 6, 2, 256, 8, 64, "bf16", seed=3)
+    w.fill()
+    q = torch.randn(6, 32, 256, generator=torch.Generator().manual_seed(1)).bfloat16().to(gpu)
+    want = w.cache.attend(q, w.batch([1] * 6))
+    T = 1 << 18
+    long = torch.zeros(T, 32, 256, dtype=torch.bfloat16, device=gpu)
+    long[3:9] = q
+    cu = w.i32(np.arange(7) + 3)
+    b = w.cache.batch(w.i32(w.table), w.i32(w.lens), cu, T, 1, 1200)
+    out = torch.full_like(long, 5.0)
+    w.cache.attend(long, b, out=out)
+    assert torch.equal(out[3:9], want)
+    assert (out[:3] == 5).all() and (out[9:] == 5).all()
+    k = torch.ones(T, 2, 256, dtype=torch.bfloat16, device=gpu)
+    w.cache.write(k, k, b)
+    got = torch.zeros_like(k), torch.zeros_like(k)
+    w.cache.read(b, k_out=got[0], v_out=got[1])
+    for x in got:
+        assert (x[3:9] == 1).all() and not x[:3].any() and not x[9:].any()
