@@ -385,12 +385,14 @@ typedef struct {
  * arrays (cu_q[0] >= 0, ascending, cu_q[n_seq] <= n_tokens).  A sequence may
  * have no new token, or no token at all.  The arrays are device memory, read
  * when the kernels run; max_q and max_kv, the host's bounds on the new tokens
- * and tokens of one sequence, size the launch.
+ * and tokens of one sequence (2^30 at most each, and max_q * q_heads / kv_heads
+ * too), choose and size the launches.
  * What a bound, the page table or cu_q contradicts is not touched: a token
  * whose page is none of the buffer's is not written, reads back as NaN and
  * counts as NaN where it is attended to; a sequence with more tokens than
  * max_kv or its pages, or more new ones than max_q, is not written and its
- * rows (the first max_q of them) read back and come out as NaN. */
+ * rows (the first max_q of them) read back and come out as NaN; where cu_q does
+ * not ascend, any of the sequences may be left out. */
 typedef struct {
     int            n_seq;     /* sequences                                     */
     int            max_pages; /* entries of a row of pages                     */

@@ -1282,7 +1282,7 @@ struct Choice {
     int nc;     // column tiles of a wave
     int waves;  // of a workgroup of many rows
     Plan p;
-    int64_t work;  // bytes
+    int64_t work;  // bytes, -1: more than 2^50
 };
 
 // Rows up to which a wave reads the cache for itself.  Two column tiles of 256-wide
@@ -1352,7 +1352,8 @@ Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
         p.nsplit = static_cast<int>(std::max<int64_t>(1, (seen + chunk - 1) / chunk));
         if (p.nsplit > 1) {
             p.chunk = static_cast<int>(chunk);
-            r.work = p.nsplit * p.rows * (D + 2) * 4;
+            const __int128 work = static_cast<__int128>(p.nsplit) * p.rows * (D + 2) * 4;
+            r.work = work > int64_t(1) << 50 ? -1 : static_cast<int64_t>(work);
         }
     }
     return r;
@@ -1362,8 +1363,7 @@ template <int BITS, int D>
 hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const Choice& ch,
                   hipStream_t s) {
     const Plan& p = ch.p;
-    // rows and positions are ints in the kernels, and a launch has 2^32 threads
-    if (static_cast<int64_t>(b.max_q) * a.G > 1 << 30) return hipErrorInvalidValue;
+    // a launch has 2^32 threads
     const int64_t out = p.per ? static_cast<int64_t>(b.n_seq) * p.per * a.heads : p.rows;
     const int64_t blocks = ch.path == Path::kStream ? (1 << p.log_workers) / 4
                                                     : c.H * p.real * p.nsplit;

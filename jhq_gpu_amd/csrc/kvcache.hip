@@ -563,8 +563,10 @@ jhq::KvCache cache_of(const jhq_kv_params& p, const void* base) {
     return c;
 }
 
+// cu_q names no row past 2^31 - 1.
 jhq::KvBatch batch_of(const jhq_kv_batch& b) {
-    return {b.d_pages, b.d_kv_len, b.d_cu_q, b.n_tokens, b.n_seq, b.max_pages, b.max_q, b.max_kv};
+    const int64_t rows = std::min<int64_t>(b.n_tokens, INT32_MAX);
+    return {b.d_pages, b.d_kv_len, b.d_cu_q, rows, b.n_seq, b.max_pages, b.max_q, b.max_kv};
 }
 
 int check_cache(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b) {
@@ -638,8 +640,15 @@ int64_t do_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_heads
         check_heads(p, q_heads, window) != JHQ_OK)
         return -1;
     if (idle(b)) return 0;
-    return jhq::kv_attend_work(cache_of(*p, nullptr), batch_of(*b), p->head_dim,
-                               q_heads / p->kv_heads, window);
+    // rows and positions are ints in the kernels
+    if (static_cast<int64_t>(b->max_q) * (q_heads / p->kv_heads) > 1 << 30) {
+        bad("max_q * q_heads / kv_heads must be at most 2^30");
+        return -1;
+    }
+    const int64_t n = jhq::kv_attend_work(cache_of(*p, nullptr), batch_of(*b), p->head_dim,
+                                          q_heads / p->kv_heads, window);
+    if (n < 0) bad("the workspace would have more than 2^50 bytes");
+    return n;
 }
 
 int do_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
