@@ -1006,8 +1006,9 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
 // What bounds it are the vector and the matrix instructions of a SIMD's two waves,
 // which overlap little: 8192 tokens over 36193, 32 heads of 128 on 8, 8 bits, 4.7 to
 // 5.0 ms on different cards, 923 to 861 TFLOP/s (a large float16 product reaches 1343), the
-// matrix cores 37% busy, the vector units 54%, LDS 35%.  At 4096 tokens over 16096 (922 TFLOP/s) a copy of it without
-// the exponentials reaches 1237, without turning codes to float16 1066, without either 1483.
+// matrix cores 37% busy, the vector units 54%, LDS 35%.  At 4096 tokens over 16096 (922
+// TFLOP/s) a copy of it without the exponentials reaches 1237, without turning codes to
+// float16 1066, without either 1483.
 // Two column tiles a wave: with one a step in LDS serves half as many rows (614
 // TFLOP/s), with three and four the registers spill (564, 614).  256-wide heads: LDS
 // holds one workgroup, so it has eight waves of one tile (835; four waves of two 604).
