@@ -414,6 +414,38 @@ int jhq_k_kv_write(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b,
                    int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok, int64_t v_head,
                    int dtype, void* stream);
 
+/* ---- rotary positions ----
+ *
+ * The first rot_dim elements of a head stand in pairs: pair i is (i, i + rot_dim / 2) or,
+ * interleaved, (2i, 2i + 1).  At position p it becomes amplitude * (x0 cos a - x1 sin a, x1 cos a +
+ * x0 sin a), a = 2 pi (p * d_turns[i] 2^-64 mod 1): frequencies are given as 2^-64ths of a turn a
+ * position, so that the product is exact modulo a turn, however far the position.  The elements from
+ * rot_dim on stay as they are.  Computed in float32, rounded once. */
+typedef struct {
+    int             head_dim;    /* even, 2 .. 1024                             */
+    int             rot_dim;     /* elements in pairs: even, 2 .. head_dim      */
+    int             interleaved; /* 0: halves; 1: pairs side by side            */
+    float           amplitude;
+    const uint64_t* d_turns;     /* [rot_dim / 2], device memory                */
+} jhq_rotary;
+
+/* Turns rows: d_x, element (t, h, e) at t * x_tok + h * x_head + e, dtype JHQ_F32, JHQ_BF16 or
+ * JHQ_F16; d_out likewise, in the same type.  d_out may be d_x with the same strides, and must
+ * not share memory with it otherwise.  Positions: d_pos [n_tokens], of pos_bytes = 4 or 8 bytes, signed;
+ * or, where d_pos is NULL, those of the batch's new tokens (kv_len - q + i, from kv_len, cu_q
+ * and n_seq alone; n_tokens is the batch's; rows that no sequence has are left alone).  inverse 1
+ * turns by -a: the gradient with respect to x of what inverse 0 computes. */
+int jhq_k_rotary(const jhq_rotary* r, const void* d_x, int64_t x_tok, int64_t x_head,
+                 int64_t n_tokens, int heads, int dtype, const void* d_pos, int pos_bytes,
+                 const jhq_kv_batch* b, int inverse, void* d_out, int64_t out_tok, int64_t out_head,
+                 void* stream);
+
+/* jhq_k_kv_write with keys turned to their tokens' positions on the way (r->head_dim is the
+ * cache's): quantised from float32, not rounded to dtype between. */
+int jhq_k_kv_write_rotary(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, const void* d_k,
+                          int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok,
+                          int64_t v_head, int dtype, const jhq_rotary* r, void* stream);
+
 /* Reads the new tokens' keys and values back: code * scale in float32, rounded
  * once to dtype; d_k, d_v [n_tokens][kv_heads][head_dim] contiguous (NULL: not
  * wanted).  A batch whose new tokens are all tokens (cu_q the running sum of

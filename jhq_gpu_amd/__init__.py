@@ -20,7 +20,7 @@ __all__ = [
     "Params", "JHQGpuIndex", "JHQError", "JHQDeviceError", "JHQNotBuiltError",
     "lib", "lib_path", "k_rotate", "k_primary_encode", "k_residual_encode", "k_assign",
     "k_assign_noalloc", "k_build_lut", "k_scan_topck", "k_refine", "k_final_topk",
-    "STEP_NAMES", "KVCache", "KVBatch",
+    "STEP_NAMES", "KVCache", "KVBatch", "Rotary",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -89,10 +89,18 @@ class _KvBatch(ctypes.Structure):
     ]
 
 
+class _Rotary(ctypes.Structure):
+    _fields_ = [
+        ("head_dim", ctypes.c_int), ("rot_dim", ctypes.c_int), ("interleaved", ctypes.c_int),
+        ("amplitude", ctypes.c_float), ("d_turns", ctypes.c_void_p),
+    ]
+
+
 _VP = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _KVP, _KVB = ctypes.POINTER(_KvParams), ctypes.POINTER(_KvBatch)
+_ROP = ctypes.POINTER(_Rotary)
 
 _SIGS = {
     "jhq_params_default": (None, [ctypes.POINTER(_Params)]),
@@ -141,6 +149,8 @@ _SIGS = {
     "jhq_kv_bytes": (_I64, [_KVP]),
     "jhq_kv_work_bytes": (_I64, [_KVP, _KVB, _I, _I]),
     "jhq_k_kv_write": (_I, [_KVP, _VP, _KVB, _VP, _I64, _I64, _VP, _I64, _I64, _I, _VP]),
+    "jhq_k_kv_write_rotary": (_I, [_KVP, _VP, _KVB, _VP, _I64, _I64, _VP, _I64, _I64, _I, _ROP, _VP]),
+    "jhq_k_rotary": (_I, [_ROP, _VP, _I64, _I64, _I64, _I, _I, _VP, _I, _KVB, _I, _VP, _I64, _I64, _VP]),
     "jhq_k_kv_read": (_I, [_KVP, _VP, _KVB, _VP, _VP, _I, _VP]),
     "jhq_k_kv_attend": (_I, [_KVP, _VP, _KVB, _VP, _I64, _I64, _I, _I, ctypes.c_float, _I, _I, _VP,
                              _VP, _VP, _I64, _VP]),
@@ -507,3 +517,4 @@ def k_final_topk(comp, topck_pos, list_ids, final_dists, final_ids, stream=None)
 
 
 from .kv import KVBatch, KVCache  # noqa: E402  (after the names it uses)
+from .rotary import Rotary  # noqa: E402

@@ -91,9 +91,11 @@ struct KvRows {
     int64_t tok, head;  // strides in elements
 };
 
-// bits, D, dtype as checked by the entry points.
+struct Rotary;
+
+// bits, D, dtype as checked by the entry points.  r: what keys are turned by, or null.
 hipError_t kv_write(const KvCache& c, const KvBatch& b, int bits, int D, const KvRows& k,
-                    const KvRows& v, int dtype, hipStream_t s);
+                    const KvRows& v, int dtype, const Rotary* r, hipStream_t s);
 hipError_t kv_read(const KvCache& c, const KvBatch& b, int bits, int D, void* k, void* v, int dtype,
                    hipStream_t s);
 

@@ -10,6 +10,7 @@
 // pass through LDS, [piece][token][16 bytes]; values, which the cache holds
 // token-minor, have their 16 x 16 byte tiles turned there.
 #include "kvcache.h"
+#include "rotary.h"
 
 #include <hip/hip_runtime.h>
 
@@ -75,6 +76,14 @@ __device__ inline void load8(const void* base, int64_t i, float* x) {
             x[j] = DT == JHQ_BF16 ? __uint_as_float(static_cast<uint32_t>(h[j]) << 16)
                                   : static_cast<float>(__builtin_bit_cast(_Float16, h[j]));
     }
+}
+
+template <int DT>
+__device__ inline float load1(const void* base, int64_t i) {
+    if constexpr (DT == JHQ_F32) return static_cast<const float*>(base)[i];
+    const uint16_t h = static_cast<const uint16_t*>(base)[i];
+    return DT == JHQ_BF16 ? __uint_as_float(static_cast<uint32_t>(h) << 16)
+                          : static_cast<float>(__builtin_bit_cast(_Float16, h));
 }
 
 template <int DT>
@@ -237,13 +246,54 @@ __device__ inline uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d
     return __builtin_amdgcn_perm(b, a, 0x0c0c0400) | __builtin_amdgcn_perm(d, c, 0x0c0c0400) << 16;
 }
 
+// A lane's 8 elements from element 8 col of the row at `row` turned to position pos, as rotary.hip
+// turns them; f: their frequencies.  In halves the pairs' other elements are another lane's: they are
+// read once more, from the cache.
+template <int DT, bool VEC>
+__device__ inline void turn8(const Rotary& r, const void* base, int64_t row, int col, int64_t pos,
+                             const uint64_t* f, float* x) {
+    const int el = col * 8, half = r.rot / 2;
+    if (el >= r.rot) return;
+    if (r.interleaved) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            if (el + e >= r.rot) break;
+            float c, s;
+            turn_of(f[e], pos, c, s);
+            c *= r.amp, s *= r.sign;
+            const float x0 = x[e], x1 = x[e + 1];
+            x[e] = fmaf(x0, c, -(x1 * s));
+            x[e + 1] = fmaf(x1, c, x0 * s);
+        }
+        return;
+    }
+    float y[8];
+    if (half % 8 == 0) {
+        load8<DT, VEC>(base, row + (el < half ? el + half : el - half), y);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (el + e < r.rot)
+                y[e] = load1<DT>(base, row + (el + e < half ? el + e + half : el + e - half));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        if (el + e >= r.rot) break;
+        float c, s;
+        turn_of(f[e], pos, c, s);
+        c *= r.amp, s *= r.sign;
+        x[e] = fmaf(x[e], c, el + e < half ? -(y[e] * s) : y[e] * s);
+    }
+}
+
 // HBM-bound: reads 2 T H D elements, writes half (8 bits) or a quarter of that
 // in 16-bit types.  A large copy moves 4.8 TB/s; 19192 tokens, 8 heads of 128, 8 bits: 119 MB in
 // 31.6 us, 3.8 TB/s, from float32 198 MB in 41.0, 4.8; 4 bits, 8 heads of 64, 16384 tokens 3.1 TB/s and
 // 65536 4.1; 64 single tokens 5.1 us.
-template <int BITS, int D, int DT, bool VEC, bool SEARCH>
+// ROT: keys are turned to their positions first, in float32, and not rounded before they are held.
+template <int BITS, int D, int DT, bool VEC, bool SEARCH, bool ROT>
 __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatch b, KvRows kr,
-                                                               KvRows vr, int sets) {
+                                                               KvRows vr, int sets, Rotary rot) {
     using R = Run<BITS, D>;
     __shared__ __align__(16) uint8_t lds[kWaves][R::LDS];
     __shared__ int mags[kWaves][R::TW];
@@ -264,6 +314,24 @@ __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatc
         for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
         if (live >> t & 1)
             load8<DT, VEC>(src.p, (row0 + t) * src.tok + u.head * src.head + col * 8, x[i]);
+    }
+    if constexpr (ROT) {
+        if (!u.value) {
+            uint64_t f[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int el = col * 8 + e, half = rot.rot / 2;
+                f[e] = el >= rot.rot ? 0
+                                     : rot.turns[rot.interleaved ? el >> 1 : el < half ? el : el - half];
+            }
+#pragma unroll
+            for (int i = 0; i < R::NI; i++) {
+                const int t = i * R::RI + sub;
+                if (live >> t & 1)
+                    turn8<DT, VEC>(rot, src.p, (row0 + t) * src.tok + u.head * src.head, col, u.first + t,
+                                   f, x[i]);
+            }
+        }
     }
     constexpr float top = BITS == 8 ? 127.0f : 7.0f;
 #pragma unroll
@@ -458,15 +526,19 @@ hipError_t pick(int bits, int D, int dt, bool vec, A&&... a) {
 template <int BITS, int D, int DT, bool VEC>
 struct Write {
     static hipError_t run(const KvCache& c, const KvBatch& b, const KvRows& k, const KvRows& v,
-                          hipStream_t s) {
+                          const Rotary* r, hipStream_t s) {
         int sets;
         unsigned blocks;
         if (!units(b, c, Run<BITS, D>::TW, &sets, &blocks)) return hipErrorInvalidValue;
-        if (sets)
-            kv_write_kernel<BITS, D, DT, VEC, false><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
-        else
-            kv_write_kernel<BITS, D, DT, VEC, true><<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets);
-        return hipGetLastError();
+        auto go = [&](auto kernel) {
+            kernel<<<blocks, 64 * kWaves, 0, s>>>(c, b, k, v, sets, r ? *r : Rotary{});
+            return hipGetLastError();
+        };
+        if (r)
+            return sets ? go(kv_write_kernel<BITS, D, DT, VEC, false, true>)
+                        : go(kv_write_kernel<BITS, D, DT, VEC, true, true>);
+        return sets ? go(kv_write_kernel<BITS, D, DT, VEC, false, false>)
+                    : go(kv_write_kernel<BITS, D, DT, VEC, true, false>);
     }
 };
 
@@ -489,12 +561,12 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 }  // namespace
 
 hipError_t kv_write(const KvCache& c, const KvBatch& b, int bits, int D, const KvRows& k,
-                    const KvRows& v, int dtype, hipStream_t s) {
+                    const KvRows& v, int dtype, const Rotary* r, hipStream_t s) {
     // 16-byte loads where every row starts on 16 bytes
     const int e = dtype == JHQ_F32 ? 4 : 8;
     const bool vec = aligned16(k.p) && aligned16(v.p) && k.tok % e == 0 && k.head % e == 0 &&
                      v.tok % e == 0 && v.head % e == 0;
-    return pick<Write>(bits, D, dtype, vec, c, b, k, v, s);
+    return pick<Write>(bits, D, dtype, vec, c, b, k, v, r, s);
 }
 
 hipError_t kv_read(const KvCache& c, const KvBatch& b, int bits, int D, void* k, void* v, int dtype,
@@ -610,16 +682,23 @@ int64_t do_bytes(const jhq_kv_params* p) {
 
 int do_write(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, const void* d_k,
              int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok, int64_t v_head,
-             int dtype, void* stream) {
+             int dtype, const jhq_rotary* r, void* stream) {
     const int rc = check_cache(p, d_cache, b);
     if (rc != JHQ_OK) return rc;
+    jhq::Rotary rot = {};
+    if (r) {
+        const std::string wrong = jhq::rotary_wrong(r);
+        if (!wrong.empty()) return bad(wrong);
+        if (r->head_dim != p->head_dim) return bad("rotary: head_dim is another than the cache's");
+        rot = jhq::rotary_of(*r, false);
+    }
     if (dtype != JHQ_F32 && dtype != JHQ_BF16 && dtype != JHQ_F16)
         return bad("keys and values must be JHQ_F32, JHQ_BF16 or JHQ_F16");
     if (idle(b)) return JHQ_OK;
     if (!d_k || !d_v) return bad("null keys or values");
     return launched("kv_write", jhq::kv_write(cache_of(*p, d_cache), batch_of(*b), p->bits,
                                               p->head_dim, {d_k, k_tok, k_head},
-                                              {d_v, v_tok, v_head}, dtype,
+                                              {d_v, v_tok, v_head}, dtype, r ? &rot : nullptr,
                                               static_cast<hipStream_t>(stream)));
 }
 
@@ -695,7 +774,16 @@ int jhq_k_kv_write(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b,
                    int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok, int64_t v_head,
                    int dtype, void* stream) {
     return entry(static_cast<int>(JHQ_ENOMEM), [&] {
-        return do_write(p, d_cache, b, d_k, k_tok, k_head, d_v, v_tok, v_head, dtype, stream);
+        return do_write(p, d_cache, b, d_k, k_tok, k_head, d_v, v_tok, v_head, dtype, nullptr, stream);
+    });
+}
+
+int jhq_k_kv_write_rotary(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, const void* d_k,
+                          int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok,
+                          int64_t v_head, int dtype, const jhq_rotary* r, void* stream) {
+    return entry(static_cast<int>(JHQ_ENOMEM), [&] {
+        if (!r) return bad("null rotary parameters");
+        return do_write(p, d_cache, b, d_k, k_tok, k_head, d_v, v_tok, v_head, dtype, r, stream);
     });
 }
 

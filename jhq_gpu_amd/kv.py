@@ -125,6 +125,7 @@ class KVCache:
         # plain numbers: a torch.cuda.Stream object costs two microseconds a call
         self._current, self._device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
         self._write, self._read, self._attend = L.jhq_k_kv_write, L.jhq_k_kv_read, L.jhq_k_kv_attend
+        self._write_rotary = L.jhq_k_kv_write_rotary
 
     def batch(self, pages, kv_len, cu_q, n_tokens, max_q, max_kv):
         """The sequences of a call (KVBatch)."""
@@ -157,15 +158,22 @@ class KVCache:
         dt = _DTYPES.get(t.dtype)
         return _dtype(t.dtype, what) if dt is None else dt, tok, head
 
-    def write(self, k, v, batch, stream=None):
+    def write(self, k, v, batch, stream=None, rotary=None):
         """Quantises the batch's new tokens into the cache: k, v [n_tokens,
         kv_heads, head_dim], float32, bfloat16 or float16, any strides between
-        rows."""
+        rows.  rotary: a Rotary that turns the keys to their tokens' positions on the
+        way, in float32."""
         dt, kt, kh = self._rows(k, "k", self.kv_heads, batch)
         dv, vt, vh = self._rows(v, "v", self.kv_heads, batch)
         if dt != dv:
             raise ValueError(f"k is {k.dtype}, v is {v.dtype}")
-        self._call(self._write, stream, batch, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, dt)
+        if rotary is None:
+            self._call(self._write, stream, batch, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, dt)
+            return
+        if rotary._index != self._index:
+            raise ValueError(f"the rotary is on {rotary.device}, the cache on {self.device}")
+        self._call(self._write_rotary, stream, batch, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, dt,
+                   rotary._ref)
 
     def read(self, batch, dtype=None, k_out=None, v_out=None, stream=None):
         """The batch's new tokens as the cache holds them: k, v [n_tokens,
