@@ -454,6 +454,20 @@ int jhq_k_kv_write_rotary(const jhq_kv_params* p, void* d_cache, const jhq_kv_ba
 int jhq_k_kv_read(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b, void* d_k,
                   void* d_v, int dtype, void* stream);
 
+/* Copies whole pages of every head: page d_src[i] to page d_dst[i], i < n.  No page may be
+ * written twice or read and written in one call (its contents would be either's); pairs that name a
+ * page that the cache does not have, or one page twice, are left out. */
+int jhq_k_kv_copy_pages(const jhq_kv_params* p, void* d_cache, const int32_t* d_src,
+                        const int32_t* d_dst, int64_t n, void* stream);
+
+/* Copies tokens as they are held, codes and scales: the batch's new token in row t becomes the
+ * token at slot d_slots[t] = page * page_size + place of the cache d_from, which may be d_cache
+ * or another of the same bits, kv_heads and head_dim (d_slots [n_tokens], device memory).  A slot
+ * that d_from does not have makes a token that reads back and counts as NaN.  Tokens that
+ * the call writes must not be among those that it reads. */
+int jhq_k_kv_copy(const jhq_kv_params* from, const void* d_from, const int64_t* d_slots,
+                  const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, void* stream);
+
 /* Device memory that jhq_k_kv_attend needs for this batch (0: none; -1 and a
  * message where an argument is not valid). */
 int64_t jhq_kv_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_heads, int window);

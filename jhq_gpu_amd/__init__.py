@@ -20,7 +20,7 @@ __all__ = [
     "Params", "JHQGpuIndex", "JHQError", "JHQDeviceError", "JHQNotBuiltError",
     "lib", "lib_path", "k_rotate", "k_primary_encode", "k_residual_encode", "k_assign",
     "k_assign_noalloc", "k_build_lut", "k_scan_topck", "k_refine", "k_final_topk",
-    "STEP_NAMES", "KVCache", "KVBatch", "Rotary",
+    "STEP_NAMES", "KVCache", "KVBatch", "KVPages", "Rotary",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -151,6 +151,8 @@ _SIGS = {
     "jhq_k_kv_write": (_I, [_KVP, _VP, _KVB, _VP, _I64, _I64, _VP, _I64, _I64, _I, _VP]),
     "jhq_k_kv_write_rotary": (_I, [_KVP, _VP, _KVB, _VP, _I64, _I64, _VP, _I64, _I64, _I, _ROP, _VP]),
     "jhq_k_rotary": (_I, [_ROP, _VP, _I64, _I64, _I64, _I, _I, _VP, _I, _KVB, _I, _VP, _I64, _I64, _VP]),
+    "jhq_k_kv_copy_pages": (_I, [_KVP, _VP, _VP, _VP, _I64, _VP]),
+    "jhq_k_kv_copy": (_I, [_KVP, _VP, _VP, _KVP, _VP, _KVB, _VP]),
     "jhq_k_kv_read": (_I, [_KVP, _VP, _KVB, _VP, _VP, _I, _VP]),
     "jhq_k_kv_attend": (_I, [_KVP, _VP, _KVB, _VP, _I64, _I64, _I, _I, ctypes.c_float, _I, _I, _VP,
                              _VP, _VP, _I64, _VP]),
@@ -517,4 +519,5 @@ def k_final_topk(comp, topck_pos, list_ids, final_dists, final_ids, stream=None)
 
 
 from .kv import KVBatch, KVCache  # noqa: E402  (after the names it uses)
+from .pages import KVPages  # noqa: E402
 from .rotary import Rotary  # noqa: E402

@@ -99,6 +99,12 @@ hipError_t kv_write(const KvCache& c, const KvBatch& b, int bits, int D, const K
 hipError_t kv_read(const KvCache& c, const KvBatch& b, int bits, int D, void* k, void* v, int dtype,
                    hipStream_t s);
 
+// slots: of each of the batch's rows, in f.
+hipError_t kv_copy(const KvCache& f, const KvCache& c, const KvBatch& b, int bits, int D,
+                   const int64_t* slots, hipStream_t s);
+hipError_t kv_copy_pages(const KvCache& c, const int32_t* src, const int32_t* dst, int64_t n,
+                         hipStream_t s);
+
 struct KvAttend {
     KvRows q;
     int heads, G;    // query heads; of them per key/value head

@@ -484,6 +484,145 @@ __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvCache c, KvBatch
     }
 }
 
+// Whole pages, 16 bytes a lane and kCopyDeep of them in flight; HBM-bound.  A pair that names a page
+// that the cache does not have is left out.
+constexpr int kCopyDeep = 4;
+constexpr int kCopyRun = 256 * 16 * kCopyDeep;  // bytes of a workgroup
+
+__global__ __launch_bounds__(256) void kv_copy_pages_kernel(KvCache c, const int32_t* src,
+                                                            const int32_t* dst, int per) {
+    const uint32_t pair = blockIdx.x / per, part = blockIdx.x % per;
+    const int from = src[pair], to = dst[pair];
+    if (from < 0 || from >= c.num_pages || to < 0 || to >= c.num_pages || from == to) return;
+    const int64_t bytes = c.block * c.H, at = static_cast<int64_t>(part) * kCopyRun + threadIdx.x * 16;
+    const uint8_t* const a = c.base + from * bytes;
+    uint8_t* const b = c.base + to * bytes;
+    u32x4 v[kCopyDeep];
+#pragma unroll
+    for (int i = 0; i < kCopyDeep; i++)
+        if (at + i * 4096 < bytes) v[i] = *reinterpret_cast<const u32x4*>(a + at + i * 4096);
+#pragma unroll
+    for (int i = 0; i < kCopyDeep; i++)
+        if (at + i * 4096 < bytes) *reinterpret_cast<u32x4*>(b + at + i * 4096) = v[i];
+}
+
+// Tokens as they are held, from any slots (page * page_size + place) of cache f to the batch's new
+// tokens; HBM-bound.  Keys move 16 bytes a lane, a piece of a token, to where they lie in order.
+// Values stand token by token within a group of 16: a lane makes the 16 bytes of an element from
+// its 16 bytes in each of the groups that the tokens come from, which the wave takes one after the
+// other, the next on its way while it picks tokens out of one.  A slot that the cache does not have
+// counts as a row that is not finite.
+template <int BITS, int D, bool SEARCH>
+__global__ __launch_bounds__(64 * kWaves) void kv_copy_kernel(KvCache f, KvCache c, KvBatch b,
+                                                              const int64_t* slots, int sets) {
+    using R = Run<BITS, D>;
+    constexpr uint32_t zero = BITS == 8 ? 0x80808080u : 0x88888888u;  // codes 0
+    const int lane = threadIdx.x & 63;
+    const Unit u = unit_of<R::TW, SEARCH>(c, b, sets);
+    if (!u.any || !u.q.ok) return;  // wave-uniform; the waves share nothing
+    const Groups<R::TW> gr(c, b, u);
+    const uint32_t live = gr.live & gr.held();
+    if (!live) return;
+    const int64_t row0 = u.q.row + (u.first - (u.q.n - u.q.q));
+    // the run's slots, one a lane; -1: none
+    int64_t slot = -1;
+    if (lane < R::TW && (live >> lane & 1)) slot = slots[row0 + lane];
+    if (slot < 0 || slot >> f.shift >= f.num_pages) slot = -1;
+    const int in_page = (1 << f.shift) - 1;
+    const int page = slot < 0 ? -1 : static_cast<int>(slot >> f.shift);
+    const int place = static_cast<int>(slot) & in_page;
+    if (lane < R::TW && (live >> lane & 1)) {
+        float s = nan32();
+        if (page >= 0)
+            s = reinterpret_cast<const float*>(kv_block(f, page, u.head) +
+                                               2 * f.codes)[(u.value << f.shift) + place];
+        const int g = lane >> 4;
+        uint8_t* const blk = R::TW == 32 && g ? gr.block[R::TW / 16 - 1] : gr.block[0];
+        const int to = (R::TW == 32 && g ? gr.slot[R::TW / 16 - 1] : gr.slot[0]) + (lane & 15);
+        reinterpret_cast<float*>(blk + 2 * c.codes)[(u.value << c.shift) + to] = s;
+    }
+    if (!u.value) {
+        u32x4 w[R::OUT];
+#pragma unroll
+        for (int i = 0; i < R::OUT; i++) {
+            const int k = lane + 64 * i, g = R::TW == 32 ? k / R::ROW : 0, in = k - g * R::ROW;
+            const int t = in / (R::NP * 4) * 4 + (in & 3), piece = in % (R::NP * 4) >> 2;
+            const int pg = __shfl(page, g * 16 + t), pl = __shfl(place, g * 16 + t);
+            w[i] = u32x4{zero, zero, zero, zero};
+            if (pg >= 0)
+                w[i] = *reinterpret_cast<const u32x4*>(kv_block(f, pg, u.head) +
+                                                       (pl & ~3) * R::ROW + piece * 64 + (pl & 3) * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < R::OUT; i++) {
+            const int k = lane + 64 * i, g = R::TW == 32 ? k / R::ROW : 0, in = k - g * R::ROW;
+            const int t = in / (R::NP * 4) * 4 + (in & 3);
+            uint8_t* const blk = R::TW == 32 && g ? gr.block[R::TW / 16 - 1] : gr.block[0];
+            const int to = R::TW == 32 && g ? gr.slot[R::TW / 16 - 1] : gr.slot[0];
+            if (live >> (g * 16 + t) & 1) *reinterpret_cast<u32x4*>(blk + to * R::ROW + in * 16) = w[i];
+        }
+        return;
+    }
+    // byte columns of a lane, of each of the run's groups
+    constexpr int COLS = (R::ROW + 63) / 64;
+#pragma unroll
+    for (int g = 0; g < R::TW / 16; g++) {
+        const uint32_t mine = live >> (g * 16) & 0xffff;
+        if (!mine) continue;
+        // tokens whose group is another than the token's before
+        const int group = place & ~15, l0 = g * 16 + (lane & 15);
+        const int pg = __shfl(page, l0), gp = __shfl(group, l0);
+        const int pg0 = __shfl(page, max(l0 - 1, 0)), gp0 = __shfl(group, max(l0 - 1, 0));
+        const uint32_t first = (__ballot(pg != pg0 || gp != gp0) & 0xffff) | 1;
+        u32x4 next[COLS], cur[COLS], out[COLS];
+        auto load = [&](uint32_t from) {  // the group of the next first token in `from`
+            const int t = g * 16 + __builtin_ctz(from);
+            const int p = __builtin_amdgcn_readlane(page, t), at = __builtin_amdgcn_readlane(group, t);
+#pragma unroll
+            for (int i = 0; i < COLS; i++) {
+                next[i] = u32x4{zero, zero, zero, zero};
+                if (p >= 0 && lane + 64 * i < R::ROW)
+                    next[i] = *reinterpret_cast<const u32x4*>(kv_block(f, p, u.head) + f.codes +
+                                                              at * R::ROW + (lane + 64 * i) * 16);
+            }
+        };
+        load(first);
+#pragma unroll
+        for (int i = 0; i < COLS; i++) out[i] = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            if (first >> r & 1) {
+#pragma unroll
+                for (int i = 0; i < COLS; i++) cur[i] = next[i];
+                if (first >> r >> 1) load(first >> r >> 1 << r << 1);
+            }
+            const uint32_t x = __builtin_amdgcn_readlane(place, g * 16 + r) & 15;
+            // byte x of 16 to byte r % 4 of a word: 0x0c makes a zero
+            const uint32_t keep = 0x0c0c0c0cu & ~(0xffu << (8 * (r & 3)));
+            const uint32_t lo = keep | (x < 8 ? x : 0x0c) << (8 * (r & 3));
+            const uint32_t hi = keep | (x < 8 ? 0x0c : x - 8) << (8 * (r & 3));
+#pragma unroll
+            for (int i = 0; i < COLS; i++)
+                out[i][r >> 2] |= __builtin_amdgcn_perm(cur[i][1], cur[i][0], lo) |
+                                  __builtin_amdgcn_perm(cur[i][3], cur[i][2], hi);
+        }
+        uint8_t* const blk = R::TW == 32 && g ? gr.block[R::TW / 16 - 1] : gr.block[0];
+        const int to = R::TW == 32 && g ? gr.slot[R::TW / 16 - 1] : gr.slot[0];
+#pragma unroll
+        for (int i = 0; i < COLS; i++) {
+            if (lane + 64 * i >= R::ROW) continue;
+            uint8_t* const dst = blk + c.codes + to * R::ROW + (lane + 64 * i) * 16;
+            if (mine == 0xffff) {
+                *reinterpret_cast<u32x4*>(dst) = out[i];
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (mine >> r & 1) dst[r] = static_cast<uint8_t>(out[i][r >> 2] >> (8 * (r & 3)));
+            }
+        }
+    }
+}
+
 // The launch's units: every head, keys and values, of each sequence's runs of max_q tokens
 // (one more than they fill, for a run that starts inside a group), or of the runs that n_tokens
 // tokens can have in n_seq sequences (sets 0) where those are fewer by a third: 5509 tokens of 3
@@ -556,6 +695,19 @@ struct Read {
     }
 };
 
+template <int BITS, int D>
+hipError_t copy_run(const KvCache& f, const KvCache& c, const KvBatch& b, const int64_t* slots,
+                    hipStream_t s) {
+    int sets;
+    unsigned blocks;
+    if (!units(b, c, Run<BITS, D>::TW, &sets, &blocks)) return hipErrorInvalidValue;
+    if (sets)
+        kv_copy_kernel<BITS, D, false><<<blocks, 64 * kWaves, 0, s>>>(f, c, b, slots, sets);
+    else
+        kv_copy_kernel<BITS, D, true><<<blocks, 64 * kWaves, 0, s>>>(f, c, b, slots, sets);
+    return hipGetLastError();
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
@@ -572,6 +724,26 @@ hipError_t kv_write(const KvCache& c, const KvBatch& b, int bits, int D, const K
 hipError_t kv_read(const KvCache& c, const KvBatch& b, int bits, int D, void* k, void* v, int dtype,
                    hipStream_t s) {
     return pick<Read>(bits, D, dtype, aligned16(k) && aligned16(v), c, b, k, v, s);
+}
+
+hipError_t kv_copy(const KvCache& f, const KvCache& c, const KvBatch& b, int bits, int D,
+                   const int64_t* slots, hipStream_t s) {
+    if (bits == 8)
+        return D == 64    ? copy_run<8, 64>(f, c, b, slots, s)
+               : D == 128 ? copy_run<8, 128>(f, c, b, slots, s)
+                          : copy_run<8, 256>(f, c, b, slots, s);
+    return D == 64    ? copy_run<4, 64>(f, c, b, slots, s)
+           : D == 128 ? copy_run<4, 128>(f, c, b, slots, s)
+                      : copy_run<4, 256>(f, c, b, slots, s);
+}
+
+hipError_t kv_copy_pages(const KvCache& c, const int32_t* src, const int32_t* dst, int64_t n,
+                         hipStream_t s) {
+    const int64_t per = (c.block * c.H + kCopyRun - 1) / kCopyRun;
+    if (n >= 1 << 23 || n * per >= 1 << 23) return hipErrorInvalidValue;
+    kv_copy_pages_kernel<<<static_cast<unsigned>(n * per), 256, 0, s>>>(c, src, dst,
+                                                                       static_cast<int>(per));
+    return hipGetLastError();
 }
 
 }  // namespace jhq
@@ -714,6 +886,35 @@ int do_read(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b, 
                                             static_cast<hipStream_t>(stream)));
 }
 
+int do_copy_pages(const jhq_kv_params* p, void* d_cache, const int32_t* d_src, const int32_t* d_dst,
+                  int64_t n, void* stream) {
+    const int rc = check_params(p);
+    if (rc != JHQ_OK) return rc;
+    if (!d_cache) return bad("null cache");
+    if (!jhq::aligned16(d_cache)) return bad("the cache must be 16-byte aligned");
+    if (n < 0) return bad("negative number of pages");
+    if (n == 0) return JHQ_OK;
+    if (!d_src || !d_dst) return bad("null pages");
+    return launched("kv_copy_pages", jhq::kv_copy_pages(cache_of(*p, d_cache), d_src, d_dst, n,
+                                                        static_cast<hipStream_t>(stream)));
+}
+
+int do_copy(const jhq_kv_params* from, const void* d_from, const int64_t* d_slots,
+            const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, void* stream) {
+    int rc = check_cache(p, d_cache, b);
+    if (rc == JHQ_OK) rc = check_params(from);
+    if (rc != JHQ_OK) return rc;
+    if (!d_from) return bad("null source cache");
+    if (!jhq::aligned16(d_from)) return bad("the source cache must be 16-byte aligned");
+    if (from->bits != p->bits || from->kv_heads != p->kv_heads || from->head_dim != p->head_dim)
+        return bad("the source cache has other bits, heads or elements");
+    if (idle(b)) return JHQ_OK;
+    if (!d_slots) return bad("null slots");
+    return launched("kv_copy", jhq::kv_copy(cache_of(*from, d_from), cache_of(*p, d_cache), batch_of(*b),
+                                            p->bits, p->head_dim, d_slots,
+                                            static_cast<hipStream_t>(stream)));
+}
+
 int64_t do_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_heads, int window) {
     if (check_params(p) != JHQ_OK || check_batch(b) != JHQ_OK ||
         check_heads(p, q_heads, window) != JHQ_OK)
@@ -790,6 +991,18 @@ int jhq_k_kv_write_rotary(const jhq_kv_params* p, void* d_cache, const jhq_kv_ba
 int jhq_k_kv_read(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b, void* d_k,
                   void* d_v, int dtype, void* stream) {
     return entry(static_cast<int>(JHQ_ENOMEM), [&] { return do_read(p, d_cache, b, d_k, d_v, dtype, stream); });
+}
+
+int jhq_k_kv_copy_pages(const jhq_kv_params* p, void* d_cache, const int32_t* d_src,
+                        const int32_t* d_dst, int64_t n, void* stream) {
+    return entry(static_cast<int>(JHQ_ENOMEM),
+                 [&] { return do_copy_pages(p, d_cache, d_src, d_dst, n, stream); });
+}
+
+int jhq_k_kv_copy(const jhq_kv_params* from, const void* d_from, const int64_t* d_slots,
+                  const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, void* stream) {
+    return entry(static_cast<int>(JHQ_ENOMEM),
+                 [&] { return do_copy(from, d_from, d_slots, p, d_cache, b, stream); });
 }
 
 int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,

@@ -134,14 +134,17 @@ class KVCache:
     def _call(self, entry, stream, batch, *args):
         if batch._index != self._index:
             raise ValueError(f"the batch is on cuda:{batch._index}, the cache on {self.device}")
+        self._enqueue(entry, stream, self._ref, self._ptr, batch._ref, *args)
+
+    def _enqueue(self, entry, stream, *args):
         if self._device() != self._index:  # kernels are launched on the current device
             with _torch().cuda.device(self._index):
-                return self._call(entry, stream, batch, *args)
+                return self._enqueue(entry, stream, *args)
         if stream is None:
             s = self._current(self._index)
         else:
             s = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
-        rc = entry(self._ref, self._ptr, batch._ref, *args, s)
+        rc = entry(*args, s)
         if rc:
             _jg._check(rc)
 
@@ -199,6 +202,37 @@ class KVCache:
             raise ValueError("k_out and v_out must be contiguous")
         self._call(self._read, stream, batch, k_out.data_ptr(), v_out.data_ptr(), dt)
         return k_out, v_out
+
+    def copy_pages(self, src, dst, stream=None):
+        """Copies whole pages: src, dst int32 device tensors [n].  No page may be written twice or
+        both read and written in one call; pairs that name a page that the cache does
+        not have are left out."""
+        torch = _torch()
+        for name, t in (("src", src), ("dst", dst)):
+            if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous 1-d int32 tensor")
+            if t.get_device() != self._index:
+                raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
+        if src.shape != dst.shape:
+            raise ValueError(f"src has {src.shape[0]} pages, dst {dst.shape[0]}")
+        self._enqueue(_jg.lib().jhq_k_kv_copy_pages, stream, self._ref, self._ptr, src.data_ptr(),
+                      dst.data_ptr(), src.shape[0])
+
+    def copy(self, slots, batch, source=None, stream=None):
+        """Copies tokens as they are held: the batch's new token in row t becomes the token at
+        slot slots[t] = page * page_size + place of `source`, a cache of the same bits,
+        kv_heads and head_dim (default: this one).  slots: an int64 device tensor
+        [n_tokens]; a slot that source does not have makes a token that reads back and counts
+        as NaN.  Tokens that the call writes must not be among those that it reads."""
+        source = self if source is None else source
+        if slots.dtype != _torch().int64 or slots.shape != (batch.n_tokens,) or not slots.is_contiguous():
+            raise ValueError(f"slots must be a contiguous int64 [{batch.n_tokens}] tensor")
+        for name, i in (("slots are", slots.get_device()), ("the batch is", batch._index),
+                        ("the source is", source._index)):
+            if i != self._index:
+                raise ValueError(f"{name} on cuda:{i}, the cache on {self.device}")
+        self._enqueue(_jg.lib().jhq_k_kv_copy, stream, source._ref, source._ptr, slots.data_ptr(),
+                      self._ref, self._ptr, batch._ref)
 
     def work_bytes(self, batch, q_heads, window=0):
         """Bytes of workspace that attend needs for this batch."""
