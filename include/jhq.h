@@ -496,6 +496,23 @@ int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_ba
                     float scale, int causal, int window, void* d_out, float* d_lse, void* d_work,
                     int64_t work_bytes, void* stream);
 
+/* jhq_k_kv_attend of sequences in groups that share a prefix, whose tokens are read once for a
+ * group.  prefix is a batch of the groups: group g's rows are cu_q[g] .. cu_q[g + 1] of the
+ * call (its sequences' new tokens, one sequence after the other; n_tokens is the batch's),
+ * kv_len[g] the tokens of its prefix (0: none) and pages[g] their pages; max_q bounds a group's
+ * rows, max_kv a prefix.  The sequences in b are as without a prefix: their first kv_len[g] tokens
+ * are those of the prefix, and all of their new tokens stand behind them.  What the call computes is
+ * jhq_k_kv_attend of b; sizes choose whether a prefix is read once or by every sequence.
+ * Rows that no group has are those of sequences without one.  Where the host's
+ * bounds, a sequence or its length contradict a group, its rows may come out as NaN.  There is no
+ * window here: behind one, sequences share little. */
+int64_t jhq_kv_shared_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, const jhq_kv_batch* prefix,
+                                 int q_heads);
+int jhq_k_kv_attend_shared(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
+                           const jhq_kv_batch* prefix, const void* d_q, int64_t q_tok, int64_t q_head,
+                           int q_heads, int dtype, float scale, int causal, void* d_out, float* d_lse,
+                           void* d_work, int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

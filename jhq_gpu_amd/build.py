@@ -35,8 +35,8 @@ def _run(cmd):
 
 def build_engine(verbose=False):
     """Compile kernels.hip, jhq_capi.hip, gemm_chain.hip, insert.hip, kmeans.hip,
-    noalloc.hip, assign_mfma.hip, kvcache.hip, kv_attend.hip, rotary.hip and
-    host_train.cpp into libjhq_amd.so."""
+    noalloc.hip, assign_mfma.hip, kvcache.hip, kv_attend.hip, kv_shared.hip,
+    rotary.hip and host_train.cpp into libjhq_amd.so."""
     os.makedirs(BUILD, exist_ok=True)
     jobs = [
         ([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, "kernels.hip"),
@@ -57,6 +57,8 @@ def build_engine(verbose=False):
                                 "-o", os.path.join(BUILD, "kvcache.o")]),
         ([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, "kv_attend.hip"),
                                 "-o", os.path.join(BUILD, "kv_attend.o")]),
+        ([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, "kv_shared.hip"),
+                                "-o", os.path.join(BUILD, "kv_shared.o")]),
         ([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, "rotary.hip"),
                                 "-o", os.path.join(BUILD, "rotary.o")]),
         (["g++"] + CXX_FLAGS + ["-c", os.path.join(CSRC, "host_train.cpp"),
@@ -80,7 +82,8 @@ def build_engine(verbose=False):
           os.path.join(BUILD, "gemm_chain.o"),
           os.path.join(BUILD, "insert.o"), os.path.join(BUILD, "kmeans.o"), os.path.join(BUILD, "noalloc.o"),
           os.path.join(BUILD, "assign_mfma.o"), os.path.join(BUILD, "kvcache.o"),
-          os.path.join(BUILD, "kv_attend.o"), os.path.join(BUILD, "rotary.o"),
+          os.path.join(BUILD, "kv_attend.o"), os.path.join(BUILD, "kv_shared.o"),
+          os.path.join(BUILD, "rotary.o"),
           os.path.join(BUILD, "host_train.o")])
     os.replace(tmp, LIB)
     return LIB

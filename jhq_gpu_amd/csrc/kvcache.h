@@ -36,12 +36,22 @@ struct KvBatch {
     int n_seq, max_pages, max_q, max_kv;
 };
 
+// A batch whose sequences' leading tokens other rows read for them: the sequences with rows
+// lead_cu[g] .. lead_cu[g + 1] leave out their first lead_len[g].  And that batch of
+// leading tokens, every row of which sees all of its sequence's.
+struct KvOwn : KvBatch {
+    const int32_t *lead_cu, *lead_len;
+    int n_lead;
+};
+struct KvLead : KvBatch {};
+
 // A sequence's extent as the kernels use it: first row, new tokens, tokens.
 struct KvSeq {
     int64_t row;  // of its first new token
     int q, n;
     bool ok;      // false: the bounds contradict what the arrays say of it (then
                   // q is within max_q and n is 0)
+    int from;     // first token that the pass reads
 };
 
 #ifdef __HIPCC__
@@ -56,6 +66,29 @@ __device__ inline KvSeq kv_seq(const KvBatch& b, int s, int shift) {
            r.n <= (static_cast<int64_t>(b.max_pages) << shift);
     if (r.q > b.max_q) r.q = b.max_q;
     if (!r.ok) r.n = 0;
+    r.from = 0;
+    return r;
+}
+
+// As above, with what the group of its rows leaves out.  Lanes may ask for different sequences.
+__device__ inline KvSeq kv_seq(const KvOwn& b, int s, int shift) {
+    KvSeq r = kv_seq(static_cast<const KvBatch&>(b), s, shift);
+    if (r.q == 0) return r;
+    int g = 0;
+    for (int len = b.n_lead; len > 1;) {
+        const int half = len >> 1;
+        if (b.lead_cu[g + half] <= r.row) {
+            g += half;
+            len -= half;
+        } else {
+            len = half;
+        }
+    }
+    if (r.row < b.lead_cu[g] || r.row >= b.lead_cu[g + 1]) return r;
+    r.from = max(b.lead_len[g], 0);
+    // the group's rows are whole sequences, whose new tokens stand behind the prefix
+    if (r.from && (r.row + r.q > b.lead_cu[g + 1] || r.n - r.q < r.from)) r.ok = false;
+    if (!r.ok) r.n = r.from = 0;
     return r;
 }
 
@@ -119,5 +152,8 @@ struct KvAttend {
 int64_t kv_attend_work(const KvCache& c, const KvBatch& b, int D, int G, int window);
 hipError_t kv_attend(const KvCache& c, const KvBatch& b, int bits, int D, const KvAttend& a,
                      hipStream_t s);
+int64_t kv_shared_work(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G);
+hipError_t kv_attend_shared(const KvCache& c, const KvBatch& lead, const KvBatch& b, int bits, int D,
+                            const KvAttend& a, hipStream_t s);
 
 }  // namespace jhq

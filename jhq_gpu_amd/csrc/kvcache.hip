@@ -915,25 +915,41 @@ int do_copy(const jhq_kv_params* from, const void* d_from, const int64_t* d_slot
                                             static_cast<hipStream_t>(stream)));
 }
 
-int64_t do_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_heads, int window) {
+// What attention needs; lead: the sequences' prefixes, or null.  -1 and a message where an argument is
+// not valid.
+int64_t do_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, const jhq_kv_batch* lead,
+                      int q_heads, int window) {
     if (check_params(p) != JHQ_OK || check_batch(b) != JHQ_OK ||
         check_heads(p, q_heads, window) != JHQ_OK)
         return -1;
+    if (lead) {
+        if (check_batch(lead) != JHQ_OK) return -1;
+        if (lead->n_tokens != b->n_tokens) {
+            bad("the prefix has another number of rows than the batch");
+            return -1;
+        }
+        if (window) {
+            bad("a window and a prefix do not go together");
+            return -1;
+        }
+    }
     if (idle(b)) return 0;
     // rows and positions are ints in the kernels
-    if (static_cast<int64_t>(b->max_q) * (q_heads / p->kv_heads) > 1 << 30) {
+    const int G = q_heads / p->kv_heads;
+    if (static_cast<int64_t>(b->max_q) * G > 1 << 30 || (lead && static_cast<int64_t>(lead->max_q) * G > 1 << 30)) {
         bad("max_q * q_heads / kv_heads must be at most 2^30");
         return -1;
     }
-    const int64_t n = jhq::kv_attend_work(cache_of(*p, nullptr), batch_of(*b), p->head_dim,
-                                          q_heads / p->kv_heads, window);
+    const jhq::KvCache c = cache_of(*p, nullptr);
+    const int64_t n = lead ? jhq::kv_shared_work(c, batch_of(*lead), batch_of(*b), p->head_dim, G)
+                           : jhq::kv_attend_work(c, batch_of(*b), p->head_dim, G, window);
     if (n < 0) bad("the workspace would have more than 2^50 bytes");
     return n;
 }
 
 int do_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
-              const void* d_q, int64_t q_tok, int64_t q_head, int q_heads, int dtype,
-              float scale, int causal, int window, void* d_out, float* d_lse, void* d_work,
+              const jhq_kv_batch* lead, const void* d_q, int64_t q_tok, int64_t q_head, int q_heads,
+              int dtype, float scale, int causal, int window, void* d_out, float* d_lse, void* d_work,
               int64_t work_bytes, void* stream) {
     int rc = check_cache(p, d_cache, b);
     if (rc == JHQ_OK) rc = check_heads(p, q_heads, window);
@@ -942,10 +958,10 @@ int do_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b
     if (causal != 0 && causal != 1) return bad("causal must be 0 or 1");
     if (window && !causal) return bad("a window needs causal = 1");
     if (!std::isfinite(scale)) return bad("scale must be finite");
+    const int64_t need = lead || !idle(b) ? do_work_bytes(p, b, lead, q_heads, window) : 0;
+    if (need < 0) return JHQ_EINVAL;
     if (idle(b)) return JHQ_OK;
     if (!d_q || !d_out) return bad("null queries or output");
-    const int64_t need = do_work_bytes(p, b, q_heads, window);
-    if (need < 0) return JHQ_EINVAL;
     if (need > 0 && !d_work) return bad("null workspace");
     if (work_bytes < need)
         return bad("the workspace has " + std::to_string(work_bytes) + " bytes, " +
@@ -955,8 +971,11 @@ int do_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b
     const int out8 = (reinterpret_cast<uintptr_t>(d_out) & 7) == 0;
     const jhq::KvAttend a = {{d_q, q_tok, q_head}, q_heads, q_heads / p->kv_heads, dtype, scale,
                              causal, std::min(window, kMaxTokens), d_out, q16, out8, d_lse, static_cast<float*>(d_work)};
-    return launched("kv_attend", jhq::kv_attend(cache_of(*p, d_cache), batch_of(*b), p->bits,
-                                                p->head_dim, a, static_cast<hipStream_t>(stream)));
+    const jhq::KvCache c = cache_of(*p, d_cache);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return launched("kv_attend",
+                    lead ? jhq::kv_attend_shared(c, batch_of(*lead), batch_of(*b), p->bits, p->head_dim, a, s)
+                         : jhq::kv_attend(c, batch_of(*b), p->bits, p->head_dim, a, s));
 }
 
 }  // namespace
@@ -968,7 +987,16 @@ int64_t jhq_kv_bytes(const jhq_kv_params* p) {
 }
 
 int64_t jhq_kv_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_heads, int window) {
-    return entry(int64_t(-1), [&] { return do_work_bytes(p, b, q_heads, window); });
+    return entry(int64_t(-1), [&] { return do_work_bytes(p, b, nullptr, q_heads, window); });
+}
+
+int64_t jhq_kv_shared_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, const jhq_kv_batch* prefix,
+                                 int q_heads) {
+    return entry(int64_t(-1), [&]() -> int64_t {
+        if (prefix) return do_work_bytes(p, b, prefix, q_heads, 0);
+        bad("null prefix");
+        return -1;
+    });
 }
 
 int jhq_k_kv_write(const jhq_kv_params* p, void* d_cache, const jhq_kv_batch* b, const void* d_k,
@@ -1010,8 +1038,19 @@ int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_ba
                     float scale, int causal, int window, void* d_out, float* d_lse, void* d_work,
                     int64_t work_bytes, void* stream) {
     return entry(static_cast<int>(JHQ_ENOMEM), [&] {
-        return do_attend(p, d_cache, b, d_q, q_tok, q_head, q_heads, dtype, scale, causal, window,
+        return do_attend(p, d_cache, b, nullptr, d_q, q_tok, q_head, q_heads, dtype, scale, causal, window,
                          d_out, d_lse, d_work, work_bytes, stream);
+    });
+}
+
+int jhq_k_kv_attend_shared(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
+                           const jhq_kv_batch* prefix, const void* d_q, int64_t q_tok, int64_t q_head,
+                           int q_heads, int dtype, float scale, int causal, void* d_out, float* d_lse,
+                           void* d_work, int64_t work_bytes, void* stream) {
+    return entry(static_cast<int>(JHQ_ENOMEM), [&] {
+        if (!prefix) return bad("null prefix");
+        return do_attend(p, d_cache, b, prefix, d_q, q_tok, q_head, q_heads, dtype, scale, causal, 0, d_out,
+                         d_lse, d_work, work_bytes, stream);
     });
 }
 

@@ -125,7 +125,7 @@ class KVCache:
         # plain numbers: a torch.cuda.Stream object costs two microseconds a call
         self._current, self._device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
         self._write, self._read, self._attend = L.jhq_k_kv_write, L.jhq_k_kv_read, L.jhq_k_kv_attend
-        self._write_rotary = L.jhq_k_kv_write_rotary
+        self._write_rotary, self._attend_shared = L.jhq_k_kv_write_rotary, L.jhq_k_kv_attend_shared
 
     def batch(self, pages, kv_len, cu_q, n_tokens, max_q, max_kv):
         """The sequences of a call (KVBatch)."""
@@ -234,15 +234,25 @@ class KVCache:
         self._enqueue(_jg.lib().jhq_k_kv_copy, stream, source._ref, source._ptr, slots.data_ptr(),
                       self._ref, self._ptr, batch._ref)
 
-    def work_bytes(self, batch, q_heads, window=0):
+    def work_bytes(self, batch, q_heads, window=0, prefix=None):
         """Bytes of workspace that attend needs for this batch."""
-        n = int(_jg.lib().jhq_kv_work_bytes(self._ref, batch._ref, _int32(q_heads, "q_heads"), _window(window)))
+        if prefix is not None:
+            self._no_window(window)
+            n = int(_jg.lib().jhq_kv_shared_work_bytes(self._ref, batch._ref, prefix._ref,
+                                                       _int32(q_heads, "q_heads")))
+        else:
+            n = int(_jg.lib().jhq_kv_work_bytes(self._ref, batch._ref, _int32(q_heads, "q_heads"), _window(window)))
         if n < 0:
             _jg._check(_jg.JHQ_EINVAL)
         return n
 
+    @staticmethod
+    def _no_window(window):
+        if window:
+            raise ValueError("a window and a prefix do not go together")
+
     def attend(self, q, batch, scale=None, causal=True, window=0, out=None, lse=None, work=None,
-               stream=None):
+               stream=None, prefix=None):
         """Attention of the batch's new tokens, which the cache already holds, to
         their sequences; q [n_tokens, q_heads, head_dim] bfloat16 or float16,
         any strides between rows; returns out, the same shape and type,
@@ -250,8 +260,21 @@ class KVCache:
         [n_tokens, q_heads] tensor that gets the logarithms of the softmax sums.
         work: a uint8 tensor of work_bytes() bytes, this call's alone until it has
         run; without it the call takes one from torch's allocator.  Rows outside
-        cu_q keep what they had (zero where out is None)."""
+        cu_q keep what they had (zero where out is None).
+
+        prefix: a KVBatch that says which neighbouring sequences of the batch begin with the
+        same tokens, so that these are read once for all of them; what comes out is the
+        same.  Its sequences are the groups: rows cu_q[g] .. of the call are the new
+        tokens of group g's sequences, kv_len[g] the tokens that they share (0: none), all before
+        their new ones, pages[g] the pages of these (KVPages.prefix finds them).  No window then.
+        Sequences that contradict their group may come out as NaN."""
         window = _window(window)
+        if prefix is not None:
+            self._no_window(window)
+            if prefix._index != self._index:
+                raise ValueError(f"the prefix is on cuda:{prefix._index}, the cache on {self.device}")
+            if prefix.n_tokens != batch.n_tokens:
+                raise ValueError(f"the prefix has {prefix.n_tokens} rows, the batch {batch.n_tokens}")
         heads = q.shape[1] if q.dim() == 3 else 0
         dt, qt, qh = self._rows(q, "q", heads, batch)
         if dt == _jg.JHQ_F32:
@@ -273,7 +296,7 @@ class KVCache:
                                  f"tensor on {self.device}")
             lp = lse.data_ptr()
         if work is None:
-            n = self.work_bytes(batch, heads, window) if heads else 0
+            n = self.work_bytes(batch, heads, window, prefix) if heads else 0
             if n:
                 torch = _torch()
                 with torch.cuda.stream(_as_stream(stream, self.device)):
@@ -282,9 +305,13 @@ class KVCache:
                 or work.get_device() != self._index:
             raise ValueError(f"work must be a contiguous uint8 tensor on {self.device}")
         wp, wn = (work.data_ptr(), work.numel()) if work is not None else (None, 0)
-        self._call(self._attend, stream, batch, q.data_ptr(), qt, qh, heads, dt,
-                   self._scale if scale is None else float(scale), 1 if causal else 0, window,
-                   out.data_ptr(), lp, wp, wn)
+        scale, causal = self._scale if scale is None else float(scale), 1 if causal else 0
+        if prefix is None:
+            self._call(self._attend, stream, batch, q.data_ptr(), qt, qh, heads, dt, scale, causal, window,
+                       out.data_ptr(), lp, wp, wn)
+        else:
+            self._call(self._attend_shared, stream, batch, prefix._ref, q.data_ptr(), qt, qh, heads, dt,
+                       scale, causal, out.data_ptr(), lp, wp, wn)
         return out
 
 
