@@ -683,23 +683,6 @@ __device__ void keep(float* work, int64_t slot, int64_t slots, int rows, int lan
     }
 }
 
-// A wave's rows as the one part of theirs, by their places in the output: sums, then maxima and sums.
-template <int BITS, int D, int NC>
-__device__ void keep_rows(const Share& w, const KvAttend& a, float* work, int64_t all, int r0, int lane,
-                          const Rows<BITS, D, NC>& r) {
-    const int g = lane >> 4;
-#pragma unroll
-    for (int k = 0; k < NC; k++) {
-        const int row = r0 + k * 16 + (lane & 15);
-        if (row >= w.r0 + w.rn) continue;
-        int64_t q;
-        const int64_t o = row_of(w, a, row, &q);
-#pragma unroll
-        for (int t = 0; t < D / 16; t++) *reinterpret_cast<f4*>(work + o * D + t * 16 + g * 4) = r.o[k][t];
-        if (g == 0) *reinterpret_cast<float2*>(work + all * D + o * 2) = make_float2(r.m[k], r.l[k]);
-    }
-}
-
 // Where the bytes of a share's steps lie.  A lane's keys belong to token group
 // (lane % 16) / 4 of the step, its values and its token's scales to group lane / 16;
 // pages of a step or more are looked up once, for the whole wave.
@@ -842,8 +825,9 @@ struct Stream {
 template <int D>
 constexpr int kShortWaves = D == 256 ? 4 : 8;
 
-template <int BITS, int D, int NT, int W, class B = KvBatch>
-__global__ __launch_bounds__(64 * W, W / 4) void kv_short_kernel(KvCache c, B b, KvAttend a, Plan p) {
+template <int BITS, int D, int NT, int W>
+__global__ __launch_bounds__(64 * W, W / 4) void kv_short_kernel(KvCache c, KvBatch b, KvAttend a,
+                                                                 Plan p) {
     using M = Dim<BITS, D>;
     constexpr int R = NT * 16, P = D + 4;
     __shared__ __align__(16) float sc[W][192];
@@ -853,10 +837,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv_short_kernel(KvCache c, B b,
     const int g = lane >> 4, r = lane & 15;
     const Share w = share_of(c, b, a, p, blockIdx.x);
     if (!w.any) return;
-    if (!w.s.ok) {
-        if constexpr (!kParts<B>) fail_rows<D>(w, a, threadIdx.x, blockDim.x);
-        return;
-    }
+    if (!w.s.ok) return fail_rows<D>(w, a, threadIdx.x, blockDim.x);
     Rows<BITS, D, NT> rows;
     Stream<BITS, D, NT> st(c, b, w, lane);
     const int j = w.lo + wave * kStep;
@@ -891,11 +872,6 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv_short_kernel(KvCache c, B b,
         }
         int64_t q;
         const int64_t at = row_of(w, a, w.r0 + row, &q);
-        if constexpr (kParts<B>) {
-            *reinterpret_cast<f4*>(a.work + at * D + e) = o;
-            if (e == 0) *reinterpret_cast<float2*>(a.work + p.rows * D + at * 2) = make_float2(m, l);
-            continue;
-        }
         const bool sees = sees_any(w.s, a, (w.r0 + row) / a.G);
         store4(a, at * D + e, o * inverse_of(l, sees));
         if (a.lse && e == 0) a.lse[at] = lse_of(m, l, sees);
@@ -923,31 +899,33 @@ __device__ inline int steps_of(const KvSeq& s, const KvAttend& a, int* lo, int* 
     return s.q == 0 ? 0 : max(1, (*hi - *lo + kStep - 1) / kStep);
 }
 
-// A wave's first step: where it lies, and how many there are.
+// A worker's first step: where it lies, and how many there are.
 struct Cut {
-    int per, at, end;  // steps of a wave; this wave's
+    int per, at, end;  // steps of a worker; this one's
     int seq, first;    // the sequence of `at`, and the number of its first step
     KvSeq s;
 };
 
-template <class B>
-__device__ inline Cut cut_of(const KvCache& c, const B& b, const KvAttend& a, const Plan& p,
-                             int worker, int lane) {
-    int lo, hi;
-    const KvSeq s0 = lane_seq(c, b, lane);
-    const int n0 = steps_of(s0, a, &lo, &hi);
-    int sum = n0;
-    for (int s = lane + 64; s < b.n_seq; s += 64) sum += steps_of(lane_seq(c, b, s), a, &lo, &hi);
+// Steps of all sequences, of which a head of s has steps(s).
+template <class B, class F>
+__device__ inline int all_steps(const KvCache& c, const B& b, int lane, F steps) {
+    int sum = steps(lane_seq(c, b, lane));
+    for (int s = lane + 64; s < b.n_seq; s += 64) sum += steps(lane_seq(c, b, s));
+    return wave_sum(sum) * c.H;
+}
+
+// The cut of worker's steps where each has `per` of `total`.
+template <class B, class F>
+__device__ inline Cut cut_at(const KvCache& c, const B& b, int total, int per, int worker, int lane, F steps) {
     Cut r;
-    const int total = wave_sum(sum) * c.H;
-    r.per = max(kLeast, (total + (1 << p.log_workers) - 1) >> p.log_workers);
+    r.per = per;
     r.at = min(static_cast<int64_t>(worker) * r.per, static_cast<int64_t>(total));
     r.end = min(r.at + r.per, total);
     if (r.at >= r.end) return r;
     int base = 0;
     for (int x = 0;; x += 64) {
-        const KvSeq s = x ? lane_seq(c, b, x + lane) : s0;
-        const int n = x ? steps_of(s, a, &lo, &hi) : n0;
+        const KvSeq s = lane_seq(c, b, x + lane);
+        const int n = steps(s);
         int in = n;  // inclusive sum
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -976,13 +954,6 @@ __device__ inline int2* joins_of(const KvAttend& a, const Plan& p) {
     return reinterpret_cast<int2*>(a.work + (int64_t(2) << p.log_workers) * (NT * 16) * (D + 2));
 }
 
-// Behind those: rows that one wave has had all of, where they are a part (kParts).
-template <int D, int NT>
-__host__ __device__ inline float* whole_of(const KvCache& c, const KvBatch& b, float* work, const Plan& p) {
-    return work + (int64_t(2) << p.log_workers) * (NT * 16) * (D + 2) +
-           (static_cast<int64_t>(b.n_seq) * c.H + 1) / 2 * 4;
-}
-
 // Streaming waves on a SIMD: two hide each other's latencies as long as a wave's
 // sums, operands and loads in flight fit half of its registers.  Four contexts of
 // 130 k in 4 bits: one 123 us, two 90, four, which spill, 145; 32 sequences of 8000, 64-wide
@@ -990,11 +961,18 @@ __host__ __device__ inline float* whole_of(const KvCache& c, const KvBatch& b, f
 template <int D, int NT>
 constexpr int kStreamWaves = D * NT >= 256 ? 1 : 2;
 
-// The steps of one of the streaming waves; sc: 192 floats of LDS, the wave's.
-template <int BITS, int D, int NT, class B>
-__device__ inline void stream_steps(const KvCache& c, const B& b, const KvAttend& a, const Plan& p,
-                                    int worker, int lane, float* sc) {
-    const Cut cut = cut_of(c, b, a, p, worker, lane);
+template <int BITS, int D, int NT>
+__global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
+    __shared__ __align__(16) float sc[4][192];
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const int worker = blockIdx.x * 4 + wave;
+    auto steps = [&](const KvSeq& s) {
+        int lo, hi;
+        return steps_of(s, a, &lo, &hi);
+    };
+    const int total = all_steps(c, b, lane, steps);
+    const Cut cut = cut_at(c, b, total, max(kLeast, (total + (1 << p.log_workers) - 1) >> p.log_workers),
+                           worker, lane, steps);
     if (cut.at >= cut.end) return;
     int at = cut.at;
     Share w;
@@ -1011,7 +989,7 @@ __device__ inline void stream_steps(const KvCache& c, const B& b, const KvAttend
             joins_of<D, NT>(a, p)[w.seq * c.H + w.head] = int2{worker, (at + n - 1) / cut.per - worker};
         w.rn = w.s.q * a.G;
         if (!w.s.ok) {
-            if constexpr (!kParts<B>) fail_rows<D>(w, a, lane, 64);
+            fail_rows<D>(w, a, lane, 64);
         } else {
             span_of(w, a);
             w.lo = lo + from * kStep;
@@ -1023,13 +1001,10 @@ __device__ inline void stream_steps(const KvCache& c, const B& b, const KvAttend
             float own[NT];
             const float big = rows.largest(a, own);
             const float f = rows.scale(a, big, own) * (a.scale * kLog2e);
-            st.run(rows, w.lo, kStep, f, sc);
-            if (from == 0 && to == n) {
-                if constexpr (kParts<B>)
-                    keep_rows<BITS, D, NT>(w, a, whole_of<D, NT>(c, b, a.work, p), p.rows, 0, lane, rows);
-                else
-                    finish<BITS, D, NT>(w, a, 0, lane, rows);
-            } else
+            st.run(rows, w.lo, kStep, f, sc[wave]);
+            if (from == 0 && to == n)
+                finish<BITS, D, NT>(w, a, 0, lane, rows);
+            else
                 keep<D, NT>(a.work, 2 * worker + (from == 0), 2 << p.log_workers, w.rn, lane,
                             rows.o, rows.m, rows.l);
         }
@@ -1044,13 +1019,6 @@ __device__ inline void stream_steps(const KvCache& c, const B& b, const KvAttend
             } while (n == 0);
         }
     }
-}
-
-template <int BITS, int D, int NT, class B = KvBatch>
-__global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(KvCache c, B b, KvAttend a, Plan p) {
-    __shared__ __align__(16) float sc[4][192];
-    const int wave = wave_id();
-    stream_steps<BITS, D, NT>(c, b, a, p, blockIdx.x * 4 + wave, threadIdx.x & 63, sc[wave]);
 }
 
 // Many rows: 16 NC of them a wave, W waves.  A step's keys and values are turned to
@@ -1073,16 +1041,17 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
     __shared__ __align__(16) float sc[2][192];                      \
     __shared__ float bigs[W]
 
-template <int BITS, int D, int NC, int W, class B>
+// A workgroup's share, x: the block of a launch or what share_of() and keep() else are overloaded for.
+template <int BITS, int D, int NC, int W, class B, class X>
 __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a, const Plan& p,
-                                 uint32_t block, h8 (&kf)[2][4 * Dim<BITS, D>::KS * 64],
+                                 const X& x, h8 (&kf)[2][4 * Dim<BITS, D>::KS * 64],
                                  h8 (&vf)[2][2 * Dim<BITS, D>::DT * 64], float (&sc)[2][192],
                                  float (&bigs)[W]) {
     using M = Dim<BITS, D>;
     using K = typename KeyReg<M::LB>::type;
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int g = lane >> 4, r = lane & 15;
-    const Share w = share_of(c, b, a, p, block);
+    const Share w = share_of(c, b, a, p, x);
     if (!w.any) return;
     if (!w.s.ok) {
         if constexpr (!kParts<B>)
@@ -1213,6 +1182,10 @@ __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a
     else
         steps(std::false_type());
     rows.join();
+    if constexpr (!std::is_same<X, uint32_t>::value) {
+        x.keep(w, a, r0, lane, rows);
+        return;
+    }
     if (!kParts<B> && w.alone) return finish<BITS, D, NC>(w, a, r0, lane, rows);
 #pragma unroll
     for (int k = 0; k < NC; k++) {
@@ -1235,7 +1208,7 @@ template <int BITS, int D, int NC, int W, class B = KvBatch>
 __global__ __launch_bounds__(64 * W, W == 8 || D < 256 ? 2 : 1)
 void kv_many_kernel(KvCache c, B b, KvAttend a, Plan p) {
     JHQ_MANY_LDS(BITS, D, W);
-    many_rows<BITS, D, NC, W>(c, b, a, p, blockIdx.x, kf, vf, sc, bigs);
+    many_rows<BITS, D, NC, W>(c, b, a, p, static_cast<uint32_t>(blockIdx.x), kf, vf, sc, bigs);
 }
 
 // What a call runs: 16 or 32 rows from registers (short or streaming), or tiles of 64 or
@@ -1256,7 +1229,7 @@ struct Choice {
 // 111 us through LDS.
 constexpr int few_rows(int D) { return D == 256 ? 16 : 32; }
 
-// parts: rows' sums are kept, those of one part too.
+// parts: rows in parts even where a tile's tokens are one, and many rows whatever their number.
 inline Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window, bool parts = false) {
     Choice r;
     Plan& p = r.p;
@@ -1265,7 +1238,7 @@ inline Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int windo
                                 : b.max_kv;
     // the streaming kernel numbers steps with an int
     const bool counted = static_cast<int64_t>(b.n_seq) * c.H * (span / kStep + 2) < INT32_MAX / 2;
-    r.path = rows > few_rows(D) ? Path::kMany
+    r.path = parts || rows > few_rows(D) ? Path::kMany
              : span <= kShortSpan ? Path::kShort : counted ? Path::kStream : Path::kMany;
     r.nc = r.path == Path::kMany ? (rows <= 64 ? 1 : 2) : (rows <= 16 ? 1 : 2);
     r.waves = r.path == Path::kMany && D == 256 && r.nc == 2 ? 8 : 4;
@@ -1286,8 +1259,7 @@ inline Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int windo
     if (r.path == Path::kStream) {
         p.log_workers = D * r.nc >= 256 ? 10 : 11;  // kStreamWaves on each of 1024 SIMDs
         r.work = (int64_t(2) << p.log_workers) * p.tile * (D + 2) * 4 +
-                 (parts ? (static_cast<int64_t>(b.n_seq) * c.H + 1) / 2 * 16
-                        : static_cast<int64_t>(b.n_seq) * c.H * 8);
+                 static_cast<int64_t>(b.n_seq) * c.H * 8;
     } else if (r.path == Path::kMany) {
         // workgroups without a split: no more tiles than the rows fill
         const int64_t tiles = p.real * c.H;

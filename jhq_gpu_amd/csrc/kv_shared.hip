@@ -11,12 +11,224 @@
 namespace jhq {
 namespace {
 
-// A pass's parts, as the join finds them.
-struct Source {
-    Plan p;
-    Path path;
-    const float* work;
+// What a pass keeps of its rows.  A worker has steps of 64 tokens of consecutive tiles (rows of one head of a
+// sequence, tile of them at most).  A tile's steps are numbered from its `start` on: what comes before stands
+// for what beginning a tile costs, so that workers that begin several end with the others (64 single
+// tokens behind 16003: 72.3 us without, 66.8 with).  A tile of whose steps a worker has all is kept by
+// its rows' places in the output (`whole`); of the two that it may begin or end in the middle of, in slot
+// 2 worker (begun before it) and 2 worker + 1 (goes on after it).  Sums of values first, then maxima and
+// sums.  joins: the worker that begins a tile, and how many more have parts of it.
+struct Kept {
+    float* slots;
+    int64_t n;     // of them
+    int tile, start;
+    int2* joins;
+    float* whole;
+    int64_t rows;  // new tokens x query heads
 };
+
+__host__ __device__ inline int64_t even4(int64_t floats) { return (floats + 3) / 4 * 4; }
+
+// Its floats, laid out from base on.
+inline int64_t lay_out(Kept& k, float* base, int D, int64_t slots, int tile, int64_t joins, int64_t rows) {
+    k.n = slots;
+    k.tile = tile;
+    k.rows = rows;
+    k.slots = base;
+    const int64_t j = slots * tile * (D + 2);
+    k.joins = reinterpret_cast<int2*>(base + j);
+    const int64_t w = j + even4(2 * joins);
+    k.whole = base + w;
+    return w + even4(rows * (D + 2));
+}
+
+// The number of a sequence's first tile: a sequence of q rows has q / tile + 1 at most.
+__device__ inline int64_t first_tile(const Kept& k, const KvSeq& s, int seq, int G) {
+    return s.row * G / k.tile + seq;
+}
+
+// Keeps a wave's rows from r0 on; slot -1: all of their tokens.
+template <int BITS, int D, int NC>
+__device__ inline void keep_part(const Kept& k, int64_t slot, const Share& w, const KvAttend& a, int r0,
+                                 int lane, const Rows<BITS, D, NC>& r) {
+    const int g = lane >> 4;
+    float* const base = slot < 0 ? k.whole : k.slots;
+    float* const ml = base + (slot < 0 ? k.rows : k.n * k.tile) * D;
+#pragma unroll
+    for (int x = 0; x < NC; x++) {
+        const int row = r0 + x * 16 + (lane & 15);
+        if (row >= w.r0 + w.rn) continue;
+        int64_t q;
+        const int64_t at = slot < 0 ? row_of(w, a, row, &q) : slot * k.tile + (row - w.r0);
+#pragma unroll
+        for (int t = 0; t < D / 16; t++)
+            *reinterpret_cast<f4*>(base + at * D + t * 16 + g * 4) = r.o[x][t];
+        if (g == 0) *reinterpret_cast<float2*>(ml + at * 2) = make_float2(r.m[x], r.l[x]);
+    }
+}
+
+// Tokens that a sequence's rows see in a pass, and their steps.
+__device__ inline int extent(const KvOwn&, const KvSeq& s, const KvAttend& a, int* lo, int* hi) {
+    return steps_of(s, a, lo, hi);
+}
+__device__ inline int extent(const KvLead&, const KvSeq& s, const KvAttend&, int* lo, int* hi) {
+    *lo = 0;
+    *hi = s.q ? s.n : 0;
+    return (*hi + kStep - 1) / kStep;
+}
+
+// Numbers of the steps of a head of a sequence.
+template <class B>
+__device__ inline int tile_steps(const B& b, const KvSeq& s, const KvAttend& a, const Kept& k) {
+    int lo, hi;
+    const int n = extent(b, s, a, &lo, &hi);
+    return n ? (n + k.start) * ((s.q * a.G + k.tile - 1) / k.tile) : 0;
+}
+
+// A worker's way through its steps: f(w, slot) for each tile that it has steps of, in the order of
+// sequences, heads, tiles.
+template <class B, class F>
+__device__ inline void each_tile(const KvCache& c, const B& b, const KvAttend& a, const Kept& k, int total,
+                                 int workers, int least, int worker, int lane, bool first_lane, F f) {
+    auto steps = [&](const KvSeq& s) { return tile_steps(b, s, a, k); };
+    const Cut cut = cut_at(c, b, total, max(least, (total + workers - 1) / workers), worker, lane, steps);
+    int at = cut.at;
+    if (at >= cut.end) return;
+    Share w;
+    w.seq = cut.seq;
+    w.s = cut.s;
+    w.split = 0;
+    w.any = true;
+    w.alone = false;
+    int lo, hi, n = extent(b, w.s, a, &lo, &hi) + k.start;
+    int tiles = (w.s.q * a.G + k.tile - 1) / k.tile;
+    w.head = (at - cut.first) / (n * tiles);
+    int tile = (at - cut.first) % (n * tiles) / n, from = (at - cut.first) % n;
+    while (true) {
+        const int to = min(n, from + (cut.end - at));
+        const bool begins = from <= k.start;
+        if (to > k.start) {
+            if (begins && first_lane)
+                k.joins[(first_tile(k, w.s, w.seq, a.G) + tile) * c.H + w.head] =
+                    int2{worker, (at + n - from - 1) / cut.per - worker};
+            if (w.s.ok) {
+                w.r0 = tile * k.tile;
+                w.rn = min(k.tile, w.s.q * a.G - w.r0);
+                span_of(w, a);
+                w.lo = lo + (max(from, k.start) - k.start) * kStep;
+                w.hi = min(hi, lo + (to - k.start) * kStep);
+                f(w, begins && to == n ? int64_t(-1) : static_cast<int64_t>(2 * worker + begins));
+            }
+        }
+        at += to - from;
+        if (at >= cut.end) return;
+        from = 0;
+        if (++tile < tiles) continue;
+        tile = 0;
+        if (++w.head < c.H) continue;
+        w.head = 0;
+        do {
+            w.s = kv_seq(b, ++w.seq, c.shift);
+            n = extent(b, w.s, a, &lo, &hi);
+            tiles = n ? (w.s.q * a.G + k.tile - 1) / k.tile : 0;
+            n += k.start;
+        } while (tiles == 0);
+    }
+}
+
+// One wave's steps of few rows (16 NT at most), straight from the cache into registers; sc: 192
+// floats of LDS, the wave's.
+template <int BITS, int D, int NT, class B>
+__device__ inline void few_steps(const KvCache& c, const B& b, const KvAttend& a, const Kept& k, int total,
+                                 int workers, int worker, int lane, float* sc) {
+    each_tile(c, b, a, k, total, workers, kLeast, worker, lane, lane == 0, [&](const Share& w, int64_t slot) {
+        Rows<BITS, D, NT> rows;
+        Stream<BITS, D, NT> st(c, b, w, lane);
+        rows.start(w, a, 0, lane);
+        st.open(w.lo, kStep);
+        float own[NT];
+        const float big = rows.largest(a, own);
+        const float f = rows.scale(a, big, own) * (a.scale * kLog2e);
+        st.run(rows, w.lo, kStep, f, sc);
+        keep_part<BITS, D, NT>(k, slot, w, a, 0, lane, rows);
+    });
+}
+
+// A tile of one of the workgroups that have many rows, for many_rows().
+struct Piece {
+    const Share& w;
+    const Kept& k;
+    int64_t slot;
+    template <int BITS, int D, int NC>
+    __device__ void keep(const Share& s, const KvAttend& a, int r0, int lane,
+                         const Rows<BITS, D, NC>& r) const {
+        keep_part<BITS, D, NC>(k, slot, s, a, r0, lane, r);
+    }
+};
+template <class B>
+__device__ inline Share share_of(const KvCache&, const B&, const KvAttend&, const Plan&, const Piece& x) {
+    return x.w;
+}
+
+// How a launch's workgroups are dealt out: to the prefixes and to what stands behind, so that both end
+// together.  The cost of a step of each is that of a workgroup (of four waves' steps behind).
+struct Deal {
+    int places;
+    float lead, own;
+};
+
+__device__ inline int dealt(const Deal& d, int lead, int own) {
+    if (lead == 0 || own == 0) return lead ? d.places : 0;
+    const float x = lead * d.lead, y = own * d.own;
+    return min(d.places - 1, max(1, static_cast<int>(d.places * x / (x + y) + 0.5f)));
+}
+
+// Prefixes and what stands behind them in one launch: the former, many rows, are bound by vector and matrix
+// instructions, the latter by reading the cache.  LEAD: 0 few rows before, else tiles of 64 LEAD.
+template <int BITS, int D, int LEAD>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2)
+void kv_both_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a, KvAttend la, Kept ok, Kept lk, Deal d) {
+    constexpr int NC = LEAD ? LEAD : 1;
+    __shared__ __align__(16) float few[4][192];
+    const int lane = threadIdx.x & 63, wave = wave_id(), block = blockIdx.x;
+    const int lt = all_steps(c, lead, lane, [&](const KvSeq& s) { return tile_steps(lead, s, la, lk); });
+    const int ot = all_steps(c, b, lane, [&](const KvSeq& s) { return tile_steps(b, s, a, ok); });
+    const int n = dealt(d, lt, ot);
+    if (block >= n) {
+        few_steps<BITS, D, 1>(c, b, a, ok, ot, (d.places - n) * 4, (block - n) * 4 + wave, lane, few[wave]);
+        return;
+    }
+    if constexpr (LEAD == 0) {
+        few_steps<BITS, D, 1>(c, lead, la, lk, lt, n * 4, block * 4 + wave, lane, few[wave]);
+    } else {
+        JHQ_MANY_LDS(BITS, D, 4);
+        each_tile(c, lead, la, lk, lt, n, 1, block, lane, threadIdx.x == 0, [&](const Share& w, int64_t slot) {
+            many_rows<BITS, D, NC, 4>(c, lead, la, Plan{}, Piece{w, lk, slot}, kf, vf, sc, bigs);
+        });
+    }
+}
+
+// Prefixes alone.
+template <int BITS, int D, int NC, int W>
+__global__ __launch_bounds__(64 * W, W == 8 || D < 256 ? 2 : 1)
+void kv_lead_kernel(KvCache c, KvLead lead, KvAttend la, Kept lk) {
+    JHQ_MANY_LDS(BITS, D, W);
+    const int lane = threadIdx.x & 63;
+    const int lt = all_steps(c, lead, lane, [&](const KvSeq& s) { return tile_steps(lead, s, la, lk); });
+    each_tile(c, lead, la, lk, lt, gridDim.x, 1, blockIdx.x, lane, threadIdx.x == 0,
+              [&](const Share& w, int64_t slot) {
+                  many_rows<BITS, D, NC, W>(c, lead, la, Plan{}, Piece{w, lk, slot}, kf, vf, sc, bigs);
+              });
+}
+
+// What stands behind alone, 17 to 32 rows.
+template <int BITS, int D>
+__global__ __launch_bounds__(256, (kStreamWaves<D, 2>)) void kv_own_kernel(KvCache c, KvOwn b, KvAttend a, Kept ok) {
+    __shared__ __align__(16) float few[4][192];
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const int ot = all_steps(c, b, lane, [&](const KvSeq& s) { return tile_steps(b, s, a, ok); });
+    few_steps<BITS, D, 2>(c, b, a, ok, ot, gridDim.x * 4, blockIdx.x * 4 + wave, lane, few[wave]);
+}
 
 // The parts of a row: their number, the first one's place and the way to the others, sums of values
 // and (maximum, sum).
@@ -27,38 +239,33 @@ struct Parts {
     __device__ int64_t at(int k) const { return first + k * next + (k ? jump : 0); }
 };
 
-template <int D, class B>
-__device__ inline Parts parts_of(const Source& x, const KvCache& c, const B& b, const KvAttend& a,
-                                 const KvSeq& s, int seq, int i, int h) {
-    const Plan& p = x.p;
-    const int64_t row = (s.row + i) * a.heads + h;
-    if (x.path == Path::kShort) return {1, row, 0, 0, x.work, x.work + p.rows * D};
-    if (x.path == Path::kStream) {
-        const int64_t slots = (int64_t(2) << p.log_workers) * p.tile;
-        const float* const behind = x.work + slots * (D + 2);
-        const int2 j = reinterpret_cast<const int2*>(behind)[seq * c.H + h / a.G];
-        if (j.y == 0) {
-            const float* const whole = behind + (static_cast<int64_t>(b.n_seq) * c.H + 1) / 2 * 4;
-            return {1, row, 0, 0, whole, whole + p.rows * D};
-        }
-        return {j.y + 1, static_cast<int64_t>(2 * j.x + 1) * p.tile + i * a.G + h % a.G,
-                2 * static_cast<int64_t>(p.tile), -static_cast<int64_t>(p.tile), x.work,
-                x.work + slots * D};
-    }
-    // as in share_of
+// Of row x (token i, query head h) of sequence seq.
+__device__ inline Parts parts_of(const Kept& k, const KvSeq& s, int seq, int i, int h, int H, const KvAttend& a,
+                                 int D) {
+    const int x = i * a.G + h % a.G;
+    const int2 j = k.joins[(first_tile(k, s, seq, a.G) + x / k.tile) * H + h / a.G];
+    // one worker has had it all
+    if (j.y == 0) return {1, (s.row + i) * a.heads + h, 0, 0, k.whole, k.whole + k.rows * D};
+    return {j.y + 1, static_cast<int64_t>(2 * j.x + 1) * k.tile + x % k.tile, 2 * static_cast<int64_t>(k.tile),
+            -static_cast<int64_t>(k.tile), k.slots, k.slots + k.n * k.tile * D};
+}
+
+// Of kv_many_kernel, whose plan is p; as in share_of.
+__device__ inline Parts parts_of(const Plan& p, const float* work, const KvSeq& s, int i, int h, const KvAttend& a,
+                                 int D) {
     const int tile = (i * a.G + h % a.G) / p.tile;
     const int last = min((tile + 1) * p.tile, s.q * a.G) - 1;
     const int from = see_lo(s, a, tile * p.tile / a.G) / kStep * kStep;
     const int hi = see_hi(s, a, last / a.G);
     const int n = p.nsplit > 1 && hi - from > p.chunk ? (hi - from + p.chunk - 1) / p.chunk : 1;
-    return {n, row, p.rows, 0, x.work, x.work + p.nsplit * p.rows * D};
+    return {n, (s.row + i) * a.heads + h, p.rows, 0, work, work + p.nsplit * p.rows * D};
 }
 
 // Joins what the passes have of a row; latency and reading the parts bound it.  A thread has 4
 // elements of every Y-th part.
 template <int D, int Y>
 __global__ __launch_bounds__(256) void kv_shared_join_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a,
-                                                             Source ls, Source os) {
+                                                             Kept lk, Kept ok, Plan p, int many) {
     constexpr int T = D / 4, R = 256 / (T * Y);
     constexpr int WR = 64 > Y * T ? 64 / (Y * T) : 1;  // rows of a wave
     __shared__ __align__(16) float acc[R][Y][D];
@@ -79,21 +286,20 @@ __global__ __launch_bounds__(256) void kv_shared_join_kernel(KvCache c, KvOwn b,
     }
     const KvSeq s = kv_seq(b, seq, c.shift);
     const int64_t i = tok - s.row;
-    const bool has = x < os.p.rows && i >= 0 && i < s.q;
-    bool ok = s.ok, sees = false;
+    const bool has = x < lk.rows && i >= 0 && i < s.q;
+    bool good = s.ok, sees = false;
     Parts A = {}, O = {};
-    if (has && ok) {
+    if (has && good) {
         sees = sees_any(s, a, static_cast<int>(i));
-        O = parts_of<D>(os, c, b, a, s, seq, static_cast<int>(i), h);
+        O = many ? parts_of(p, a.work, s, static_cast<int>(i), h, a, D)
+                 : parts_of(ok, s, seq, static_cast<int>(i), h, c.H, a, D);
         const KvSeq w = kv_seq(lead, grp, c.shift);
         const int64_t li = tok - w.row;
         if (tok >= lead.cu_q[grp] && tok < lead.cu_q[grp + 1]) {
-            ok = w.ok && li < w.q;
-            if (ok) {
-                KvAttend la = a;
-                la.causal = 0;
-                sees |= w.n > 0;
-                A = parts_of<D>(ls, c, lead, la, w, grp, static_cast<int>(li), h);
+            good = w.ok && li < w.q;
+            if (good && w.n > 0) {
+                sees = true;
+                A = parts_of(lk, w, grp, static_cast<int>(li), h, c.H, a, D);
             }
         }
     }
@@ -134,69 +340,73 @@ __global__ __launch_bounds__(256) void kv_shared_join_kernel(KvCache c, KvOwn b,
     if (!has) return;
     const int64_t row = static_cast<int64_t>(tok) * a.heads + h;
     const float bad = nan32();
-    store4(a, row * D + t * 4, ok ? o * inverse_of(l, sees) : f4{bad, bad, bad, bad});
-    if (a.lse && t == 0) a.lse[row] = ok ? lse_of(m, l, sees) : bad;
+    store4(a, row * D + t * 4, good ? o * inverse_of(l, sees) : f4{bad, bad, bad, bad});
+    if (a.lse && t == 0) a.lse[row] = good ? lse_of(m, l, sees) : bad;
 }
 
 // What a call runs.
 struct Both {
-    bool shared;  // false: attention as without a prefix
-    Choice lead, own;
-    int64_t work;  // bytes, -1: more than 2^50
+    bool shared;    // false: attention as without a prefix
+    bool one;       // both passes in one launch
+    int lead;       // column tiles of a wave over the prefix, 0: few rows
+    int waves;      // of its workgroups
+    bool many;      // kv_many_kernel behind the prefix
+    Choice own;     // which it is chosen by, or attention's as without a prefix
+    int few;        // else rows of a tile there
+    int places;     // workgroups of a launch
+    Kept lk, ok;
+    int64_t work;   // bytes, -1: more than 2^50
 };
 
-Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G) {
-    Both r;
-    r.shared = lead.n_seq > 0 && lead.max_kv > 0 && static_cast<int64_t>(b.max_q) * G < 128;
+Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G, float* work) {
+    Both r = {};
+    const int64_t rows = static_cast<int64_t>(b.max_q) * G, before = static_cast<int64_t>(lead.max_q) * G;
+    const int64_t all = b.n_tokens * c.H * G;
+    r.one = rows <= 16;
+    r.many = rows > few_rows(D);
+    r.lead = r.one && before <= 16 ? 0 : before <= 64 ? 1 : 2;
+    r.waves = !r.one && D == 256 && r.lead == 2 ? 8 : 4;
+    r.places = D == 256 ? 256 : 512;
+    const int tile = r.lead ? 64 * r.lead : 16;
+    if (r.waves == 8) r.lead = 1;
+    // steps are numbered with an int
+    const int64_t tiles = b.n_tokens * G / tile + lead.n_seq;
+    const __int128 steps = static_cast<__int128>(tiles) * c.H * (lead.max_kv / kStep + 8) +
+                           static_cast<__int128>(b.n_seq) * c.H * (b.max_kv / kStep + 8);
+    r.shared = lead.n_seq > 0 && lead.max_kv > 0 && rows < 128 && steps < INT32_MAX / 2;
     if (!r.shared) {
         r.own = choose(c, b, D, G, 0);
         r.work = r.own.work;
         return r;
     }
-    r.lead = choose(c, lead, D, G, 0, true);
-    if (r.lead.work > 0) r.lead.work = (r.lead.work + 15) & ~int64_t(15);  // the other pass's lies behind
-    r.own = choose(c, b, D, G, 0, true);
-    r.work = r.lead.work < 0 || r.own.work < 0 ? -1 : r.lead.work + r.own.work;
-    return r;
-}
-
-template <int BITS, int D, class B>
-hipError_t pass(const KvCache& c, const B& b, const KvAttend& a, const Choice& ch, hipStream_t s) {
-    const Plan& p = ch.p;
-    const int64_t blocks = ch.path == Path::kStream ? (1 << p.log_workers) / 4 : c.H * p.real * p.nsplit;
-    if (blocks >= 1 << 23) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(blocks));
-    switch (ch.path) {
-        case Path::kShort:
-            if (ch.nc == 1)
-                kv_short_kernel<BITS, D, 1, kShortWaves<D>, B><<<grid, 64 * kShortWaves<D>, 0, s>>>(c, b, a, p);
-            else if constexpr (few_rows(D) > 16)
-                kv_short_kernel<BITS, D, 2, kShortWaves<D>, B><<<grid, 64 * kShortWaves<D>, 0, s>>>(c, b, a, p);
-            break;
-        case Path::kStream:
-            if (ch.nc == 1)
-                kv_stream_kernel<BITS, D, 1, B><<<grid, 256, 0, s>>>(c, b, a, p);
-            else if constexpr (few_rows(D) > 16)
-                kv_stream_kernel<BITS, D, 2, B><<<grid, 256, 0, s>>>(c, b, a, p);
-            break;
-        case Path::kMany:
-            if (ch.nc == 1 && ch.waves == 4)
-                kv_many_kernel<BITS, D, 1, 4, B><<<grid, 256, 0, s>>>(c, b, a, p);
-            else if constexpr (D == 256)
-                kv_many_kernel<BITS, D, 1, 8, B><<<grid, 512, 0, s>>>(c, b, a, p);
-            else
-                kv_many_kernel<BITS, D, 2, 4, B><<<grid, 256, 0, s>>>(c, b, a, p);
-            break;
+    if (all > int64_t(1) << 40) {
+        r.work = -1;
+        return r;
     }
-    return hipGetLastError();
+    const int64_t workers = r.places * (r.lead ? 1 : 4);
+    int64_t floats = lay_out(r.lk, work, D, 2 * workers, tile, tiles * c.H, all);
+    r.lk.start = 3;
+    r.ok.start = 1;
+    if (r.many) {
+        r.own = choose(c, b, D, G, 0, true);
+        r.work = r.own.work < 0 || floats > int64_t(1) << 48 ? -1 : floats * 4 + r.own.work;
+        r.ok.slots = work + floats;
+        return r;
+    }
+    r.few = r.one ? 16 : 32;
+    r.work = (floats + lay_out(r.ok, work + floats, D, 2 * r.places * 4, r.few,
+                               static_cast<int64_t>(b.n_seq) * c.H + all / r.few, all)) * 4;
+    if (r.work > int64_t(1) << 50) r.work = -1;
+    return r;
 }
 
 template <int BITS, int D>
 hipError_t launch(const KvCache& c, const KvBatch& lead, const KvBatch& b, const KvAttend& a,
                   const Both& ch, hipStream_t s) {
     constexpr int Y = 4;
-    const int64_t joins = (ch.own.p.rows + 256 / (D / 4 * Y) - 1) / (256 / (D / 4 * Y));
-    if (joins >= 1 << 23) return hipErrorInvalidValue;
+    const int64_t joins = (ch.lk.rows + 256 / (D / 4 * Y) - 1) / (256 / (D / 4 * Y));
+    const int64_t blocks = ch.many ? c.H * ch.own.p.real * ch.own.p.nsplit : 1;
+    if (joins >= 1 << 23 || blocks >= 1 << 23) return hipErrorInvalidValue;
     KvLead lb;
     static_cast<KvBatch&>(lb) = lead;
     KvOwn ob;
@@ -206,24 +416,53 @@ hipError_t launch(const KvCache& c, const KvBatch& lead, const KvBatch& b, const
     ob.n_lead = lead.n_seq;
     KvAttend la = a, oa = a;
     la.causal = 0;
-    oa.work = a.work + ch.lead.work / 4;
-    hipError_t e = pass<BITS, D>(c, lb, la, ch.lead, s);
-    if (e == hipSuccess) e = pass<BITS, D>(c, ob, oa, ch.own, s);
+    if (ch.many) oa.work = ch.ok.slots;
+    if (ch.one) {
+        const Deal d = {ch.places, 1.0f, 0.3f};
+        auto go = [&](auto kernel) { kernel<<<ch.places, 256, 0, s>>>(c, ob, lb, a, la, ch.ok, ch.lk, d); };
+        if (ch.lead == 0)
+            go(kv_both_kernel<BITS, D, 0>);
+        else if (ch.lead == 1)
+            go(kv_both_kernel<BITS, D, 1>);
+        else
+            go(kv_both_kernel<BITS, D, 2>);
+    } else {
+        auto go = [&](auto kernel) { kernel<<<ch.places, 64 * ch.waves, 0, s>>>(c, lb, la, ch.lk); };
+        if (ch.lead == 1 && ch.waves == 4)
+            go(kv_lead_kernel<BITS, D, 1, 4>);
+        else if constexpr (D == 256)
+            go(kv_lead_kernel<BITS, D, 1, 8>);
+        else
+            go(kv_lead_kernel<BITS, D, 2, 4>);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        const dim3 grid(static_cast<unsigned>(blocks));
+        if (!ch.many) {
+            if constexpr (few_rows(D) > 16) kv_own_kernel<BITS, D><<<ch.places, 256, 0, s>>>(c, ob, a, ch.ok);
+        } else if (ch.own.nc == 1 && ch.own.waves == 4) {
+            kv_many_kernel<BITS, D, 1, 4, KvOwn><<<grid, 256, 0, s>>>(c, ob, oa, ch.own.p);
+        } else if constexpr (D == 256) {
+            kv_many_kernel<BITS, D, 1, 8, KvOwn><<<grid, 512, 0, s>>>(c, ob, oa, ch.own.p);
+        } else {
+            kv_many_kernel<BITS, D, 2, 4, KvOwn><<<grid, 256, 0, s>>>(c, ob, oa, ch.own.p);
+        }
+    }
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    kv_shared_join_kernel<D, Y><<<static_cast<unsigned>(joins), 256, 0, s>>>(
-        c, ob, lb, a, {ch.lead.p, ch.lead.path, la.work}, {ch.own.p, ch.own.path, oa.work});
+    kv_shared_join_kernel<D, Y><<<static_cast<unsigned>(joins), 256, 0, s>>>(c, ob, lb, oa, ch.lk, ch.ok,
+                                                                           ch.own.p, ch.many);
     return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t kv_shared_work(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G) {
-    return choose_both(c, lead, b, D, G).work;
+    return choose_both(c, lead, b, D, G, nullptr).work;
 }
 
 hipError_t kv_attend_shared(const KvCache& c, const KvBatch& lead, const KvBatch& b, int bits, int D,
                             const KvAttend& a, hipStream_t s) {
-    const Both p = choose_both(c, lead, b, D, a.G);
+    const Both p = choose_both(c, lead, b, D, a.G, a.work);
     if (!p.shared) return kv_attend(c, b, bits, D, a, s);
     if (bits == 8)
         return D == 64    ? launch<8, 64>(c, lead, b, a, p, s)
