@@ -502,14 +502,15 @@ int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_ba
  * kv_len[g] the tokens of its prefix (0: none) and pages[g] their pages; max_q bounds a group's
  * rows, max_kv a prefix.  The sequences in b are as without a prefix: their first kv_len[g] tokens
  * are those of the prefix, and all of their new tokens stand behind them.  What the call computes is
- * jhq_k_kv_attend of b; sizes choose whether a prefix is read once or by every sequence.
+ * jhq_k_kv_attend of b: the bounds choose whether prefixes are read once or by every
+ * sequence, or once = 1 has them read once.
  * Rows that no group has are those of sequences without one.  Where the host's
  * bounds, a sequence or its length contradict a group, its rows may come out as NaN.  There is no
  * window here: behind one, sequences share little. */
 int64_t jhq_kv_shared_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, const jhq_kv_batch* prefix,
-                                 int q_heads);
+                                 int once, int q_heads);
 int jhq_k_kv_attend_shared(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
-                           const jhq_kv_batch* prefix, const void* d_q, int64_t q_tok, int64_t q_head,
+                           const jhq_kv_batch* prefix, int once, const void* d_q, int64_t q_tok, int64_t q_head,
                            int q_heads, int dtype, float scale, int causal, void* d_out, float* d_lse,
                            void* d_work, int64_t work_bytes, void* stream);
 

@@ -148,8 +148,8 @@ _SIGS = {
     "jhq_k_final_topk": (_I, [_VP] * 5 + [_I, _I, _I, _VP]),
     "jhq_kv_bytes": (_I64, [_KVP]),
     "jhq_kv_work_bytes": (_I64, [_KVP, _KVB, _I, _I]),
-    "jhq_kv_shared_work_bytes": (_I64, [_KVP, _KVB, _KVB, _I]),
-    "jhq_k_kv_attend_shared": (_I, [_KVP, _VP, _KVB, _KVB, _VP, _I64, _I64, _I, _I, ctypes.c_float, _I, _VP,
+    "jhq_kv_shared_work_bytes": (_I64, [_KVP, _KVB, _KVB, _I, _I]),
+    "jhq_k_kv_attend_shared": (_I, [_KVP, _VP, _KVB, _KVB, _I, _VP, _I64, _I64, _I, _I, ctypes.c_float, _I, _VP,
                                     _VP, _VP, _I64, _VP]),
     "jhq_k_kv_write": (_I, [_KVP, _VP, _KVB, _VP, _I64, _I64, _VP, _I64, _I64, _I, _VP]),
     "jhq_k_kv_write_rotary": (_I, [_KVP, _VP, _KVB, _VP, _I64, _I64, _VP, _I64, _I64, _I, _ROP, _VP]),

@@ -954,6 +954,11 @@ __device__ inline int2* joins_of(const KvAttend& a, const Plan& p) {
     return reinterpret_cast<int2*>(a.work + (int64_t(2) << p.log_workers) * (NT * 16) * (D + 2));
 }
 
+// Rows up to which a wave reads the cache for itself.  Two column tiles of 256-wide
+// heads do not fit its registers: 32 sequences of 8000 tokens, 32 rows, 162 us so and
+// 111 us through LDS.
+constexpr int few_rows(int D) { return D == 256 ? 16 : 32; }
+
 // Streaming waves on a SIMD: two hide each other's latencies as long as a wave's
 // sums, operands and loads in flight fit half of its registers.  Four contexts of
 // 130 k in 4 bits: one 123 us, two 90, four, which spill, 145; 32 sequences of 8000, 64-wide
@@ -1041,6 +1046,10 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
     __shared__ __align__(16) float sc[2][192];                      \
     __shared__ float bigs[W]
 
+// Steps that many_rows has on their way.
+template <class X, int BITS, int D, int NC, int W>
+constexpr int ahead_of = 1;
+
 // A workgroup's share, x: the block of a launch or what share_of() and keep() else are overloaded for.
 template <int BITS, int D, int NC, int W, class B, class X>
 __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a, const Plan& p,
@@ -1070,14 +1079,28 @@ __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a
     constexpr int VT = (M::ET + 3) / 4;
     const int part = wave & 3;
     const bool has_keys = W == 4 || wave < 4, has_values = W == 4 || wave >= 4;
-    K kr[M::NU];
-    u4 vr[VT];
-    float ks = 0, vs = 0;
-    bool dead = true, lost = true;
-    auto fetch = [&](int j) {
+    // Steps on their way into registers.
+    constexpr int S = ahead_of<X, BITS, D, NC, W>;
+    typedef std::integral_constant<int, 0> Zero;
+    typedef std::integral_constant<int, S - 1> Last;
+    K krs[S][M::NU];
+    u4 vrs[S][VT];
+    float kss[S], vss[S];
+    bool deads[S], losts[S];
+#pragma unroll
+    for (int z = 0; z < S; z++) kss[z] = vss[z] = 0, deads[z] = losts[z] = true;
+    auto fetch = [&](int j, auto slot) {
+        constexpr int z = decltype(slot)::value;
+        K(&kr)[M::NU] = krs[z];
+        u4(&vr)[VT] = vrs[z];
+        float &ks = kss[z], &vs = vss[z];
+        bool &dead = deads[z], &lost = losts[z];
         const uint8_t *k, *v;
         const float* s;
         where.find(j, k, v, s);
+        const bool none = where.pv < 0;
+        // before the codes: waiting for a page then is not waiting for them
+        if (S > 1 && j + kStep < w.hi) where.look(j + kStep);
         if (has_keys) {
 #pragma unroll
             for (int u = 0; u < M::NU; u++)
@@ -1093,11 +1116,12 @@ __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a
             ks = s[0];
             vs = s[1 << c.shift];
             dead = j + lane >= w.s.n;
-            lost = where.pv < 0;
+            lost = none;
         }
-        if (j + kStep < w.hi) where.look(j + kStep);
+        if (S == 1 && j + kStep < w.hi) where.look(j + kStep);
     };
-    if (w.lo < w.hi) fetch(w.lo);
+    if (w.lo < w.hi) fetch(w.lo, Zero());
+    if (S > 1 && w.lo + kStep < w.hi) fetch(w.lo + kStep, Last());
     float own[NC];
     float big = rows.largest(a, own);
     if (lane == 0) bigs[wave] = big;
@@ -1105,7 +1129,12 @@ __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a
 #pragma unroll
     for (int x = 0; x < W; x++) big = fmaxf(big, bigs[x]);
     const float f = rows.scale(a, big, own) * (a.scale * kLog2e);
-    auto stage = [&](int buf) {
+    auto stage = [&](int buf, auto slot) {
+        constexpr int z = decltype(slot)::value;
+        K(&kr)[M::NU] = krs[z];
+        u4(&vr)[VT] = vrs[z];
+        const float ks = kss[z], vs = vss[z];
+        const bool dead = deads[z], lost = losts[z];
         if (has_keys) {
 #pragma unroll
             for (int o = 0; o < M::LB / 8; o++) {
@@ -1141,11 +1170,9 @@ __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a
         if (wave == W - 4) token_terms(ks, vs, f, dead, lost, sc[buf] + lane);
     };
     int buf = 0;
-    if (w.lo < w.hi) stage(0);
+    if (w.lo < w.hi) stage(0, Zero());
     const bool uneven = __syncthreads_or(rows.uneven);
-    auto steps = [&](auto uneven) {
-        for (int j = w.lo; j < w.hi; j += kStep, buf ^= 1) {
-            if (j + kStep < w.hi) fetch(j + kStep);
+    auto step = [&](int j, int buf, auto uneven) {
             const bool masked = j < w.full_lo || j + kStep > w.full_hi;
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
@@ -1168,14 +1195,33 @@ __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a
                     for (int k = 0; k < NC; k++) rows.o[k][t] = mfma(v, pr[k], rows.o[k][t]);
                 }
             }
-            if (j + kStep < w.hi) stage(buf ^ 1);
+    };
+    // In parts, tiles may have few rows: waves without one only bring the others their operands.
+    const bool rows_here = std::is_same<X, uint32_t>::value || r0 < w.r0 + w.rn;
+    auto steps = [&](auto uneven) {
+        for (int j = w.lo; j < w.hi; j += kStep, buf ^= 1) {
+            if (j + kStep < w.hi) fetch(j + kStep, Zero());
+            if (rows_here) step(j, buf, uneven);
+            if (j + kStep < w.hi) stage(buf ^ 1, Zero());
             __syncthreads();
         }
+    };
+    auto two = [&](int j, auto p) {  // a step whose buffer and slot are p
+        constexpr int z = decltype(p)::value;
+        if (j + 2 * kStep < w.hi) fetch(j + 2 * kStep, p);
+        if (rows_here) step(j, z, uneven);
+        if (j + kStep < w.hi) stage(z ^ 1, std::integral_constant<int, S - 1 - z>());
+        __syncthreads();
     };
     // A loop of its own for the rare tile, as a branch in it costs the others 3% (4096
     // tokens over 16096: 1053 and 1024 us); but two loops cost 64-wide heads the third
     // wave of a SIMD (753 and 776 us).
-    if constexpr (D == 64)
+    if constexpr (S > 1) {
+        for (int j = w.lo; j < w.hi; j += 2 * kStep) {
+            two(j, Zero());
+            if (j + kStep < w.hi) two(j + kStep, Last());
+        }
+    } else if constexpr (D == 64 || !std::is_same<X, uint32_t>::value)
         steps(uneven);
     else if (uneven)
         steps(std::true_type());
@@ -1204,99 +1250,11 @@ __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a
     }
 }
 
-template <int BITS, int D, int NC, int W, class B = KvBatch>
+template <int BITS, int D, int NC, int W>
 __global__ __launch_bounds__(64 * W, W == 8 || D < 256 ? 2 : 1)
-void kv_many_kernel(KvCache c, B b, KvAttend a, Plan p) {
+void kv_many_kernel(KvCache c, KvBatch b, KvAttend a, Plan p) {
     JHQ_MANY_LDS(BITS, D, W);
     many_rows<BITS, D, NC, W>(c, b, a, p, static_cast<uint32_t>(blockIdx.x), kf, vf, sc, bigs);
-}
-
-// What a call runs: 16 or 32 rows from registers (short or streaming), or tiles of 64 or
-// 128 rows through LDS.  At 32 rows the former takes 71 us and the latter 76 for 64
-// sequences of 8000 tokens on 2 heads of 128 in 8 bits, 61 and 70 in 4, 37 and 54 with heads
-// of 64.
-enum class Path { kShort, kStream, kMany };
-struct Choice {
-    Path path;
-    int nc;     // column tiles of a wave
-    int waves;  // of a workgroup of many rows
-    Plan p;
-    int64_t work;  // bytes, -1: more than 2^50
-};
-
-// Rows up to which a wave reads the cache for itself.  Two column tiles of 256-wide
-// heads do not fit its registers: 32 sequences of 8000 tokens, 32 rows, 162 us so and
-// 111 us through LDS.
-constexpr int few_rows(int D) { return D == 256 ? 16 : 32; }
-
-// parts: rows in parts even where a tile's tokens are one, and many rows whatever their number.
-inline Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window, bool parts = false) {
-    Choice r;
-    Plan& p = r.p;
-    const int64_t rows = static_cast<int64_t>(b.max_q) * G;
-    const int64_t span = window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) + b.max_q + kStep)
-                                : b.max_kv;
-    // the streaming kernel numbers steps with an int
-    const bool counted = static_cast<int64_t>(b.n_seq) * c.H * (span / kStep + 2) < INT32_MAX / 2;
-    r.path = parts || rows > few_rows(D) ? Path::kMany
-             : span <= kShortSpan ? Path::kShort : counted ? Path::kStream : Path::kMany;
-    r.nc = r.path == Path::kMany ? (rows <= 64 ? 1 : 2) : (rows <= 16 ? 1 : 2);
-    r.waves = r.path == Path::kMany && D == 256 && r.nc == 2 ? 8 : 4;
-    if (r.waves == 8) r.nc = 1;
-    p.tile = r.path == Path::kMany ? r.nc * 16 * r.waves : r.nc * 16;
-    p.tiles = static_cast<int>((rows + p.tile - 1) / p.tile);
-    // sequences whose rows overlap, which cu_q in order cannot say, may have more: the
-    // tiles past these are not run
-    p.real = std::min<int64_t>(static_cast<int64_t>(b.n_seq) * p.tiles,
-                               b.n_tokens * G / p.tile + b.n_seq);
-    p.rows = b.n_tokens * c.H * G;
-    const int64_t all = static_cast<int64_t>(b.n_seq) * b.max_q;
-    p.per = 2 * all > 3 * b.n_tokens ? 0 : b.max_q;
-    p.nsplit = 1;
-    p.chunk = 0;
-    p.log_workers = 0;
-    r.work = 0;
-    if (r.path == Path::kStream) {
-        p.log_workers = D * r.nc >= 256 ? 10 : 11;  // kStreamWaves on each of 1024 SIMDs
-        r.work = (int64_t(2) << p.log_workers) * p.tile * (D + 2) * 4 +
-                 static_cast<int64_t>(b.n_seq) * c.H * 8;
-    } else if (r.path == Path::kMany) {
-        // workgroups without a split: no more tiles than the rows fill
-        const int64_t tiles = p.real * c.H;
-        const int64_t seen = window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) +
-                                                                      p.tile / G + 2 + kStep)
-                                    : b.max_kv;
-        // Parts only as far as the tiles do not fill the chip with two on each of 256 CUs:
-        // 16 sequences of 8000 tokens, 64 rows on each of 8 heads: parts up to 256 workgroups
-        // 115 us, 512 81, 1024 89, 2048 104; a prompt of 2999 tokens, where 768 tiles need
-        // none: 120, and 152 with parts up to 1024.
-        const int64_t parts = std::max<int64_t>(1, (512 + tiles - 1) / tiles);
-        int64_t chunk = std::max<int64_t>(512, (seen + parts - 1) / parts);
-        // Long contexts beyond that where the last round of workgroups leaves a tenth of the places
-        // empty: a part of 4096 tokens or more outweighs its place in the join.  2500 tokens
-        // over 32500, 32 heads on 8 of 128: 2027 us without, 1467 with; on 8 of 256 3683, 3237; 16
-        // heads of 64, 4 bits, 561, 490; 64 x 10 to 100 over 9000 of the latter 570, 482.  Where
-        // rounds are whole it costs: 2 x 1000 over 21000, 8 heads on 2 of 256, 450 without and 526
-        // with; 4096 over 16096, 32 on 8 of 128, 1021, 1115.  Tiles are counted as the bounds allow:
-        // where ragged lengths have fewer, it can be wrong (100 x 1 to 40 over 6000, 32 on 8 of
-        // 128: 551, 579).
-        const bool three = D == 64 && c.codes >> c.shift == 32;  // workgroups of a CU: 4 bits
-        const int64_t places = D == 256 ? 256 : three ? 768 : 512;
-        const int64_t groups = tiles * ((seen + chunk - 1) / chunk);
-        const int64_t last = (groups + places - 1) / places * places;
-        if (10 * groups < 9 * last) {
-            const int64_t finer = (4 * places + tiles - 1) / tiles;
-            chunk = std::min(chunk, std::max<int64_t>(4096, (seen + finer - 1) / finer));
-        }
-        chunk = (chunk + kStep - 1) / kStep * kStep;
-        p.nsplit = static_cast<int>(std::max<int64_t>(1, (seen + chunk - 1) / chunk));
-        if (p.nsplit > 1) p.chunk = static_cast<int>(chunk);
-    }
-    if (p.nsplit > 1 || parts) {
-        const __int128 work = r.work + static_cast<__int128>(p.nsplit) * p.rows * (D + 2) * 4;
-        r.work = work > int64_t(1) << 50 ? -1 : static_cast<int64_t>(work);
-    }
-    return r;
 }
 
 }  // namespace

@@ -107,6 +107,88 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvCache c, KvBatch b, KvAt
     if (a.lse && t == 0) a.lse[row] = lse_of(m, l, sees);
 }
 
+// What a call runs: 16 or 32 rows from registers (short or streaming), or tiles of 64 or
+// 128 rows through LDS.  At 32 rows the former takes 71 us and the latter 76 for 64
+// sequences of 8000 tokens on 2 heads of 128 in 8 bits, 61 and 70 in 4, 37 and 54 with heads
+// of 64.
+enum class Path { kShort, kStream, kMany };
+struct Choice {
+    Path path;
+    int nc;     // column tiles of a wave
+    int waves;  // of a workgroup of many rows
+    Plan p;
+    int64_t work;  // bytes, -1: more than 2^50
+};
+
+Choice choose(const KvCache& c, const KvBatch& b, int D, int G, int window) {
+    Choice r;
+    Plan& p = r.p;
+    const int64_t rows = static_cast<int64_t>(b.max_q) * G;
+    const int64_t span = window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) + b.max_q + kStep)
+                                : b.max_kv;
+    // the streaming kernel numbers steps with an int
+    const bool counted = static_cast<int64_t>(b.n_seq) * c.H * (span / kStep + 2) < INT32_MAX / 2;
+    r.path = rows > few_rows(D) ? Path::kMany
+             : span <= kShortSpan ? Path::kShort : counted ? Path::kStream : Path::kMany;
+    r.nc = r.path == Path::kMany ? (rows <= 64 ? 1 : 2) : (rows <= 16 ? 1 : 2);
+    r.waves = r.path == Path::kMany && D == 256 && r.nc == 2 ? 8 : 4;
+    if (r.waves == 8) r.nc = 1;
+    p.tile = r.path == Path::kMany ? r.nc * 16 * r.waves : r.nc * 16;
+    p.tiles = static_cast<int>((rows + p.tile - 1) / p.tile);
+    // sequences whose rows overlap, which cu_q in order cannot say, may have more: the
+    // tiles past these are not run
+    p.real = std::min<int64_t>(static_cast<int64_t>(b.n_seq) * p.tiles,
+                               b.n_tokens * G / p.tile + b.n_seq);
+    p.rows = b.n_tokens * c.H * G;
+    const int64_t all = static_cast<int64_t>(b.n_seq) * b.max_q;
+    p.per = 2 * all > 3 * b.n_tokens ? 0 : b.max_q;
+    p.nsplit = 1;
+    p.chunk = 0;
+    p.log_workers = 0;
+    r.work = 0;
+    if (r.path == Path::kStream) {
+        p.log_workers = D * r.nc >= 256 ? 10 : 11;  // kStreamWaves on each of 1024 SIMDs
+        r.work = (int64_t(2) << p.log_workers) * p.tile * (D + 2) * 4 +
+                 static_cast<int64_t>(b.n_seq) * c.H * 8;
+    } else if (r.path == Path::kMany) {
+        // workgroups without a split: no more tiles than the rows fill
+        const int64_t tiles = p.real * c.H;
+        const int64_t seen = window ? std::min<int64_t>(b.max_kv, static_cast<int64_t>(window) +
+                                                                      p.tile / G + 2 + kStep)
+                                    : b.max_kv;
+        // Parts only as far as the tiles do not fill the chip with two on each of 256 CUs:
+        // 16 sequences of 8000 tokens, 64 rows on each of 8 heads: parts up to 256 workgroups
+        // 115 us, 512 81, 1024 89, 2048 104; a prompt of 2999 tokens, where 768 tiles need
+        // none: 120, and 152 with parts up to 1024.
+        const int64_t parts = std::max<int64_t>(1, (512 + tiles - 1) / tiles);
+        int64_t chunk = std::max<int64_t>(512, (seen + parts - 1) / parts);
+        // Long contexts beyond that where the last round of workgroups leaves a tenth of the places
+        // empty: a part of 4096 tokens or more outweighs its place in the join.  2500 tokens
+        // over 32500, 32 heads on 8 of 128: 2027 us without, 1467 with; on 8 of 256 3683, 3237; 16
+        // heads of 64, 4 bits, 561, 490; 64 x 10 to 100 over 9000 of the latter 570, 482.  Where
+        // rounds are whole it costs: 2 x 1000 over 21000, 8 heads on 2 of 256, 450 without and 526
+        // with; 4096 over 16096, 32 on 8 of 128, 1021, 1115.  Tiles are counted as the bounds allow:
+        // where ragged lengths have fewer, it can be wrong (100 x 1 to 40 over 6000, 32 on 8 of
+        // 128: 551, 579).
+        const bool three = D == 64 && c.codes >> c.shift == 32;  // workgroups of a CU: 4 bits
+        const int64_t places = D == 256 ? 256 : three ? 768 : 512;
+        const int64_t groups = tiles * ((seen + chunk - 1) / chunk);
+        const int64_t last = (groups + places - 1) / places * places;
+        if (10 * groups < 9 * last) {
+            const int64_t finer = (4 * places + tiles - 1) / tiles;
+            chunk = std::min(chunk, std::max<int64_t>(4096, (seen + finer - 1) / finer));
+        }
+        chunk = (chunk + kStep - 1) / kStep * kStep;
+        p.nsplit = static_cast<int>(std::max<int64_t>(1, (seen + chunk - 1) / chunk));
+        if (p.nsplit > 1) {
+            p.chunk = static_cast<int>(chunk);
+            const __int128 work = static_cast<__int128>(p.nsplit) * p.rows * (D + 2) * 4;
+            r.work = work > int64_t(1) << 50 ? -1 : static_cast<int64_t>(work);
+        }
+    }
+    return r;
+}
+
 template <int BITS, int D>
 hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, const Choice& ch,
                   hipStream_t s) {

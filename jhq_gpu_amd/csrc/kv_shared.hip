@@ -8,6 +8,8 @@
 // attention over all tokens:  m = max m_p, l = sum 2^(m_p - m) l_p, o = sum 2^(m_p - m) o_p / l.
 #include "kv_attend.h"
 
+#include <cmath>
+
 namespace jhq {
 namespace {
 
@@ -116,7 +118,7 @@ __device__ inline void each_tile(const KvCache& c, const B& b, const KvAttend& a
                 w.rn = min(k.tile, w.s.q * a.G - w.r0);
                 span_of(w, a);
                 w.lo = lo + (max(from, k.start) - k.start) * kStep;
-                w.hi = min(hi, lo + (to - k.start) * kStep);
+                w.hi = min(w.hi, lo + (to - k.start) * kStep);
                 f(w, begins && to == n ? int64_t(-1) : static_cast<int64_t>(2 * worker + begins));
             }
         }
@@ -165,6 +167,9 @@ struct Piece {
         keep_part<BITS, D, NC>(k, slot, s, a, r0, lane, r);
     }
 };
+template <int BITS, int D, int NC, int W>
+constexpr int ahead_of<Piece, BITS, D, NC, W> = D == 256 ? (NC == 1 && W == 4 ? 2 : 1)
+                                                : 2;
 template <class B>
 __device__ inline Share share_of(const KvCache&, const B&, const KvAttend&, const Plan&, const Piece& x) {
     return x.w;
@@ -183,10 +188,14 @@ __device__ inline int dealt(const Deal& d, int lead, int own) {
     return min(d.places - 1, max(1, static_cast<int>(d.places * x / (x + y) + 0.5f)));
 }
 
+// Workgroups of a CU.
+template <int D, int LEAD>
+constexpr int kBothWaves = D == 256 ? 1 : D == 64 && LEAD < 2 ? 3 : 2;
+
 // Prefixes and what stands behind them in one launch: the former, many rows, are bound by vector and matrix
 // instructions, the latter by reading the cache.  LEAD: 0 few rows before, else tiles of 64 LEAD.
 template <int BITS, int D, int LEAD>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2)
+__global__ __launch_bounds__(256, (kBothWaves<D, LEAD>))
 void kv_both_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a, KvAttend la, Kept ok, Kept lk, Deal d) {
     constexpr int NC = LEAD ? LEAD : 1;
     __shared__ __align__(16) float few[4][192];
@@ -208,26 +217,24 @@ void kv_both_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a, KvAttend la, Ke
     }
 }
 
-// Prefixes alone.
+// More rows behind the prefixes too: tiles of 16 NC W rows on both sides.
 template <int BITS, int D, int NC, int W>
 __global__ __launch_bounds__(64 * W, W == 8 || D < 256 ? 2 : 1)
-void kv_lead_kernel(KvCache c, KvLead lead, KvAttend la, Kept lk) {
+void kv_tiles_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a, KvAttend la, Kept ok, Kept lk, Deal d) {
     JHQ_MANY_LDS(BITS, D, W);
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, block = blockIdx.x;
     const int lt = all_steps(c, lead, lane, [&](const KvSeq& s) { return tile_steps(lead, s, la, lk); });
-    each_tile(c, lead, la, lk, lt, gridDim.x, 1, blockIdx.x, lane, threadIdx.x == 0,
-              [&](const Share& w, int64_t slot) {
-                  many_rows<BITS, D, NC, W>(c, lead, la, Plan{}, Piece{w, lk, slot}, kf, vf, sc, bigs);
-              });
-}
-
-// What stands behind alone, 17 to 32 rows.
-template <int BITS, int D>
-__global__ __launch_bounds__(256, (kStreamWaves<D, 2>)) void kv_own_kernel(KvCache c, KvOwn b, KvAttend a, Kept ok) {
-    __shared__ __align__(16) float few[4][192];
-    const int lane = threadIdx.x & 63, wave = wave_id();
     const int ot = all_steps(c, b, lane, [&](const KvSeq& s) { return tile_steps(b, s, a, ok); });
-    few_steps<BITS, D, 2>(c, b, a, ok, ot, gridDim.x * 4, blockIdx.x * 4 + wave, lane, few[wave]);
+    const int n = dealt(d, lt, ot);
+    if (block < n)
+        each_tile(c, lead, la, lk, lt, n, 1, block, lane, threadIdx.x == 0, [&](const Share& w, int64_t slot) {
+            many_rows<BITS, D, NC, W>(c, lead, la, Plan{}, Piece{w, lk, slot}, kf, vf, sc, bigs);
+        });
+    else
+        each_tile(c, b, a, ok, ot, d.places - n, 1, block - n, lane, threadIdx.x == 0,
+                  [&](const Share& w, int64_t slot) {
+                      many_rows<BITS, D, NC, W>(c, b, a, Plan{}, Piece{w, ok, slot}, kf, vf, sc, bigs);
+                  });
 }
 
 // The parts of a row: their number, the first one's place and the way to the others, sums of values
@@ -250,22 +257,11 @@ __device__ inline Parts parts_of(const Kept& k, const KvSeq& s, int seq, int i, 
             -static_cast<int64_t>(k.tile), k.slots, k.slots + k.n * k.tile * D};
 }
 
-// Of kv_many_kernel, whose plan is p; as in share_of.
-__device__ inline Parts parts_of(const Plan& p, const float* work, const KvSeq& s, int i, int h, const KvAttend& a,
-                                 int D) {
-    const int tile = (i * a.G + h % a.G) / p.tile;
-    const int last = min((tile + 1) * p.tile, s.q * a.G) - 1;
-    const int from = see_lo(s, a, tile * p.tile / a.G) / kStep * kStep;
-    const int hi = see_hi(s, a, last / a.G);
-    const int n = p.nsplit > 1 && hi - from > p.chunk ? (hi - from + p.chunk - 1) / p.chunk : 1;
-    return {n, (s.row + i) * a.heads + h, p.rows, 0, work, work + p.nsplit * p.rows * D};
-}
-
 // Joins what the passes have of a row; latency and reading the parts bound it.  A thread has 4
 // elements of every Y-th part.
 template <int D, int Y>
 __global__ __launch_bounds__(256) void kv_shared_join_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a,
-                                                             Kept lk, Kept ok, Plan p, int many) {
+                                                             Kept lk, Kept ok) {
     constexpr int T = D / 4, R = 256 / (T * Y);
     constexpr int WR = 64 > Y * T ? 64 / (Y * T) : 1;  // rows of a wave
     __shared__ __align__(16) float acc[R][Y][D];
@@ -291,8 +287,7 @@ __global__ __launch_bounds__(256) void kv_shared_join_kernel(KvCache c, KvOwn b,
     Parts A = {}, O = {};
     if (has && good) {
         sees = sees_any(s, a, static_cast<int>(i));
-        O = many ? parts_of(p, a.work, s, static_cast<int>(i), h, a, D)
-                 : parts_of(ok, s, seq, static_cast<int>(i), h, c.H, a, D);
+        O = parts_of(ok, s, seq, static_cast<int>(i), h, c.H, a, D);
         const KvSeq w = kv_seq(lead, grp, c.shift);
         const int64_t li = tok - w.row;
         if (tok >= lead.cu_q[grp] && tok < lead.cu_q[grp + 1]) {
@@ -347,56 +342,64 @@ __global__ __launch_bounds__(256) void kv_shared_join_kernel(KvCache c, KvOwn b,
 // What a call runs.
 struct Both {
     bool shared;    // false: attention as without a prefix
-    bool one;       // both passes in one launch
-    int lead;       // column tiles of a wave over the prefix, 0: few rows
-    int waves;      // of its workgroups
-    bool many;      // kv_many_kernel behind the prefix
-    Choice own;     // which it is chosen by, or attention's as without a prefix
-    int few;        // else rows of a tile there
-    int places;     // workgroups of a launch
+    bool few;       // 16 rows at most behind the prefix
+    int lead;       // column tiles of a wave over the prefix, 0: few rows there too
+    int waves;      // of a workgroup
+    int places;     // workgroups of the launch
     Kept lk, ok;
     int64_t work;   // bytes, -1: more than 2^50
 };
 
-Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G, float* work) {
+// Whether a prefix is read once, by estimates of both ways from the call's bounds (the longest prefix
+// stands for all): reading the cache at 5 TB/s or, over more rows than a wave takes for itself,
+// steps of tiles, whichever is longer; and for the passes' parts 9 us, 150 ns a sequence and, at 128
+// elements, 1.7 ns a row.  Measured, attention of every sequence and with the prefix read once, us (32 heads on
+// 8 of 128, 8 bits, up to 200 tokens of their own): single tokens, 64 behind 900 28.6 and 28.4, behind
+// 4000 65.5 and 37.0; 8 behind 4000 23.5 and 22.0, behind 16000 49.4 and 30.9; 3 behind 16000 25.8
+// and 28.9; chunks of up to 16, 12 behind 2000 31.5 and 43.6, behind 8000 89.6 and 68.2; of up to 80,
+// 32 behind 8000 543 and 501, behind 2000 178 and 256.
+bool worth(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G) {
+    const double step = (D == 64 ? 3.0 : D == 128 ? 5.0 : 15.0) * c.H * (lead.max_kv / kStep + 1);  // ns
+    const double read = (2.0 * (c.codes >> c.shift) + 8) * c.H * lead.max_kv / 5000;
+    const double rows = static_cast<double>(b.max_q) * G, before = static_cast<double>(lead.max_q) * G;
+    const double all = static_cast<double>(b.n_tokens) * G;
+    auto tiles = [&](double each, int n, double most) {
+        return each <= few_rows(D) ? 0.0 : std::min(n * std::ceil(each / most), all / most + n);
+    };
+    const double every = std::max(b.n_seq * read, tiles(rows, b.n_seq, rows <= 64 ? 64 : 128) * step);
+    const double once = std::max(lead.n_seq * read, tiles(before, lead.n_seq, before <= 64 ? 64 : 128) * step);
+    return every > once + 9000 + 150.0 * b.n_seq + 1.7 * D / 128 * all * c.H;
+}
+
+Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G, bool once, float* work) {
     Both r = {};
     const int64_t rows = static_cast<int64_t>(b.max_q) * G, before = static_cast<int64_t>(lead.max_q) * G;
     const int64_t all = b.n_tokens * c.H * G;
-    r.one = rows <= 16;
-    r.many = rows > few_rows(D);
-    r.lead = r.one && before <= 16 ? 0 : before <= 64 ? 1 : 2;
-    r.waves = !r.one && D == 256 && r.lead == 2 ? 8 : 4;
-    r.places = D == 256 ? 256 : 512;
-    const int tile = r.lead ? 64 * r.lead : 16;
+    r.few = rows <= 16;
+    r.lead = std::max(rows, before) <= 16 ? 0 : std::max(rows, before) <= 64 ? 1 : 2;
+    r.waves = !r.few && D == 256 && r.lead == 2 ? 8 : 4;
+    r.places = D == 256 ? 256 : r.few && D == 64 && r.lead < 2 ? 768 : 512;
+    const int tile = r.lead ? 64 * r.lead : 16, own = r.few ? 16 : tile;
     if (r.waves == 8) r.lead = 1;
     // steps are numbered with an int
-    const int64_t tiles = b.n_tokens * G / tile + lead.n_seq;
-    const __int128 steps = static_cast<__int128>(tiles) * c.H * (lead.max_kv / kStep + 8) +
-                           static_cast<__int128>(b.n_seq) * c.H * (b.max_kv / kStep + 8);
-    r.shared = lead.n_seq > 0 && lead.max_kv > 0 && rows < 128 && steps < INT32_MAX / 2;
+    const int64_t tiles = b.n_tokens * G / tile + lead.n_seq, own_tiles = b.n_tokens * G / own + b.n_seq;
+    const __int128 steps = (static_cast<__int128>(tiles) * (lead.max_kv / kStep + 8) +
+                            static_cast<__int128>(own_tiles) * (b.max_kv / kStep + 8)) * c.H;
+    r.shared = lead.n_seq > 0 && lead.max_kv > 0 && steps < INT32_MAX / 2 &&
+               (once || worth(c, lead, b, D, G));
     if (!r.shared) {
-        r.own = choose(c, b, D, G, 0);
-        r.work = r.own.work;
+        r.work = kv_attend_work(c, b, D, G, 0);
         return r;
     }
     if (all > int64_t(1) << 40) {
         r.work = -1;
         return r;
     }
-    const int64_t workers = r.places * (r.lead ? 1 : 4);
-    int64_t floats = lay_out(r.lk, work, D, 2 * workers, tile, tiles * c.H, all);
-    r.lk.start = 3;
-    r.ok.start = 1;
-    if (r.many) {
-        r.own = choose(c, b, D, G, 0, true);
-        r.work = r.own.work < 0 || floats > int64_t(1) << 48 ? -1 : floats * 4 + r.own.work;
-        r.ok.slots = work + floats;
-        return r;
-    }
-    r.few = r.one ? 16 : 32;
-    r.work = (floats + lay_out(r.ok, work + floats, D, 2 * r.places * 4, r.few,
-                               static_cast<int64_t>(b.n_seq) * c.H + all / r.few, all)) * 4;
+    const int64_t floats = lay_out(r.lk, work, D, 2 * r.places * (r.lead ? 1 : 4), tile, tiles * c.H, all);
+    r.work = (floats + lay_out(r.ok, work + floats, D, 2 * r.places * (r.few ? 4 : 1), own, own_tiles * c.H, all)) * 4;
     if (r.work > int64_t(1) << 50) r.work = -1;
+    r.lk.start = 3;
+    r.ok.start = r.few ? 1 : 3;
     return r;
 }
 
@@ -405,8 +408,7 @@ hipError_t launch(const KvCache& c, const KvBatch& lead, const KvBatch& b, const
                   const Both& ch, hipStream_t s) {
     constexpr int Y = 4;
     const int64_t joins = (ch.lk.rows + 256 / (D / 4 * Y) - 1) / (256 / (D / 4 * Y));
-    const int64_t blocks = ch.many ? c.H * ch.own.p.real * ch.own.p.nsplit : 1;
-    if (joins >= 1 << 23 || blocks >= 1 << 23) return hipErrorInvalidValue;
+    if (joins >= 1 << 23) return hipErrorInvalidValue;
     KvLead lb;
     static_cast<KvBatch&>(lb) = lead;
     KvOwn ob;
@@ -414,55 +416,39 @@ hipError_t launch(const KvCache& c, const KvBatch& lead, const KvBatch& b, const
     ob.lead_cu = lead.cu_q;
     ob.lead_len = lead.kv_len;
     ob.n_lead = lead.n_seq;
-    KvAttend la = a, oa = a;
+    KvAttend la = a;
     la.causal = 0;
-    if (ch.many) oa.work = ch.ok.slots;
-    if (ch.one) {
-        const Deal d = {ch.places, 1.0f, 0.3f};
-        auto go = [&](auto kernel) { kernel<<<ch.places, 256, 0, s>>>(c, ob, lb, a, la, ch.ok, ch.lk, d); };
-        if (ch.lead == 0)
-            go(kv_both_kernel<BITS, D, 0>);
-        else if (ch.lead == 1)
-            go(kv_both_kernel<BITS, D, 1>);
-        else
-            go(kv_both_kernel<BITS, D, 2>);
-    } else {
-        auto go = [&](auto kernel) { kernel<<<ch.places, 64 * ch.waves, 0, s>>>(c, lb, la, ch.lk); };
-        if (ch.lead == 1 && ch.waves == 4)
-            go(kv_lead_kernel<BITS, D, 1, 4>);
-        else if constexpr (D == 256)
-            go(kv_lead_kernel<BITS, D, 1, 8>);
-        else
-            go(kv_lead_kernel<BITS, D, 2, 4>);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-        const dim3 grid(static_cast<unsigned>(blocks));
-        if (!ch.many) {
-            if constexpr (few_rows(D) > 16) kv_own_kernel<BITS, D><<<ch.places, 256, 0, s>>>(c, ob, a, ch.ok);
-        } else if (ch.own.nc == 1 && ch.own.waves == 4) {
-            kv_many_kernel<BITS, D, 1, 4, KvOwn><<<grid, 256, 0, s>>>(c, ob, oa, ch.own.p);
-        } else if constexpr (D == 256) {
-            kv_many_kernel<BITS, D, 1, 8, KvOwn><<<grid, 512, 0, s>>>(c, ob, oa, ch.own.p);
-        } else {
-            kv_many_kernel<BITS, D, 2, 4, KvOwn><<<grid, 256, 0, s>>>(c, ob, oa, ch.own.p);
-        }
-    }
+    const Deal d = {ch.places, 1.0f, !ch.few || ch.lead == 0 ? 1.0f : ch.lead == 1 ? 0.4f : 0.3f};
+    auto go = [&](auto kernel) {
+        kernel<<<ch.places, 64 * ch.waves, 0, s>>>(c, ob, lb, a, la, ch.ok, ch.lk, d);
+    };
+    if (ch.few && ch.lead == 0)
+        go(kv_both_kernel<BITS, D, 0>);
+    else if (ch.few && ch.lead == 1)
+        go(kv_both_kernel<BITS, D, 1>);
+    else if (ch.few)
+        go(kv_both_kernel<BITS, D, 2>);
+    else if (ch.lead == 1 && ch.waves == 4)
+        go(kv_tiles_kernel<BITS, D, 1, 4>);
+    else if constexpr (D == 256)
+        go(kv_tiles_kernel<BITS, D, 1, 8>);
+    else
+        go(kv_tiles_kernel<BITS, D, 2, 4>);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    kv_shared_join_kernel<D, Y><<<static_cast<unsigned>(joins), 256, 0, s>>>(c, ob, lb, oa, ch.lk, ch.ok,
-                                                                           ch.own.p, ch.many);
+    kv_shared_join_kernel<D, Y><<<static_cast<unsigned>(joins), 256, 0, s>>>(c, ob, lb, a, ch.lk, ch.ok);
     return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t kv_shared_work(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G) {
-    return choose_both(c, lead, b, D, G, nullptr).work;
+int64_t kv_shared_work(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G, bool once) {
+    return choose_both(c, lead, b, D, G, once, nullptr).work;
 }
 
 hipError_t kv_attend_shared(const KvCache& c, const KvBatch& lead, const KvBatch& b, int bits, int D,
-                            const KvAttend& a, hipStream_t s) {
-    const Both p = choose_both(c, lead, b, D, a.G, a.work);
+                            const KvAttend& a, bool once, hipStream_t s) {
+    const Both p = choose_both(c, lead, b, D, a.G, once, a.work);
     if (!p.shared) return kv_attend(c, b, bits, D, a, s);
     if (bits == 8)
         return D == 64    ? launch<8, 64>(c, lead, b, a, p, s)

@@ -152,8 +152,9 @@ struct KvAttend {
 int64_t kv_attend_work(const KvCache& c, const KvBatch& b, int D, int G, int window);
 hipError_t kv_attend(const KvCache& c, const KvBatch& b, int bits, int D, const KvAttend& a,
                      hipStream_t s);
-int64_t kv_shared_work(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G);
+// once: the prefix is read once whatever that costs, else where it pays.
+int64_t kv_shared_work(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G, bool once);
 hipError_t kv_attend_shared(const KvCache& c, const KvBatch& lead, const KvBatch& b, int bits, int D,
-                            const KvAttend& a, hipStream_t s);
+                            const KvAttend& a, bool once, hipStream_t s);
 
 }  // namespace jhq

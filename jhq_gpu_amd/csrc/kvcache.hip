@@ -917,7 +917,7 @@ int do_copy(const jhq_kv_params* from, const void* d_from, const int64_t* d_slot
 
 // What attention needs; lead: the sequences' prefixes, or null.  -1 and a message where an argument is
 // not valid.
-int64_t do_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, const jhq_kv_batch* lead,
+int64_t do_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, const jhq_kv_batch* lead, int once,
                       int q_heads, int window) {
     if (check_params(p) != JHQ_OK || check_batch(b) != JHQ_OK ||
         check_heads(p, q_heads, window) != JHQ_OK)
@@ -928,8 +928,8 @@ int64_t do_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, const jhq_k
             bad("the prefix has another number of rows than the batch");
             return -1;
         }
-        if (window) {
-            bad("a window and a prefix do not go together");
+        if (once != 0 && once != 1) {
+            bad("once must be 0 or 1");
             return -1;
         }
     }
@@ -941,14 +941,14 @@ int64_t do_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, const jhq_k
         return -1;
     }
     const jhq::KvCache c = cache_of(*p, nullptr);
-    const int64_t n = lead ? jhq::kv_shared_work(c, batch_of(*lead), batch_of(*b), p->head_dim, G)
+    const int64_t n = lead ? jhq::kv_shared_work(c, batch_of(*lead), batch_of(*b), p->head_dim, G, once)
                            : jhq::kv_attend_work(c, batch_of(*b), p->head_dim, G, window);
     if (n < 0) bad("the workspace would have more than 2^50 bytes");
     return n;
 }
 
 int do_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
-              const jhq_kv_batch* lead, const void* d_q, int64_t q_tok, int64_t q_head, int q_heads,
+              const jhq_kv_batch* lead, int once, const void* d_q, int64_t q_tok, int64_t q_head, int q_heads,
               int dtype, float scale, int causal, int window, void* d_out, float* d_lse, void* d_work,
               int64_t work_bytes, void* stream) {
     int rc = check_cache(p, d_cache, b);
@@ -958,7 +958,7 @@ int do_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b
     if (causal != 0 && causal != 1) return bad("causal must be 0 or 1");
     if (window && !causal) return bad("a window needs causal = 1");
     if (!std::isfinite(scale)) return bad("scale must be finite");
-    const int64_t need = lead || !idle(b) ? do_work_bytes(p, b, lead, q_heads, window) : 0;
+    const int64_t need = lead || !idle(b) ? do_work_bytes(p, b, lead, once, q_heads, window) : 0;
     if (need < 0) return JHQ_EINVAL;
     if (idle(b)) return JHQ_OK;
     if (!d_q || !d_out) return bad("null queries or output");
@@ -974,7 +974,7 @@ int do_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b
     const jhq::KvCache c = cache_of(*p, d_cache);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return launched("kv_attend",
-                    lead ? jhq::kv_attend_shared(c, batch_of(*lead), batch_of(*b), p->bits, p->head_dim, a, s)
+                    lead ? jhq::kv_attend_shared(c, batch_of(*lead), batch_of(*b), p->bits, p->head_dim, a, once, s)
                          : jhq::kv_attend(c, batch_of(*b), p->bits, p->head_dim, a, s));
 }
 
@@ -987,13 +987,13 @@ int64_t jhq_kv_bytes(const jhq_kv_params* p) {
 }
 
 int64_t jhq_kv_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, int q_heads, int window) {
-    return entry(int64_t(-1), [&] { return do_work_bytes(p, b, nullptr, q_heads, window); });
+    return entry(int64_t(-1), [&] { return do_work_bytes(p, b, nullptr, 0, q_heads, window); });
 }
 
 int64_t jhq_kv_shared_work_bytes(const jhq_kv_params* p, const jhq_kv_batch* b, const jhq_kv_batch* prefix,
-                                 int q_heads) {
+                                 int once, int q_heads) {
     return entry(int64_t(-1), [&]() -> int64_t {
-        if (prefix) return do_work_bytes(p, b, prefix, q_heads, 0);
+        if (prefix) return do_work_bytes(p, b, prefix, once, q_heads, 0);
         bad("null prefix");
         return -1;
     });
@@ -1038,18 +1038,18 @@ int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_ba
                     float scale, int causal, int window, void* d_out, float* d_lse, void* d_work,
                     int64_t work_bytes, void* stream) {
     return entry(static_cast<int>(JHQ_ENOMEM), [&] {
-        return do_attend(p, d_cache, b, nullptr, d_q, q_tok, q_head, q_heads, dtype, scale, causal, window,
+        return do_attend(p, d_cache, b, nullptr, 0, d_q, q_tok, q_head, q_heads, dtype, scale, causal, window,
                          d_out, d_lse, d_work, work_bytes, stream);
     });
 }
 
 int jhq_k_kv_attend_shared(const jhq_kv_params* p, const void* d_cache, const jhq_kv_batch* b,
-                           const jhq_kv_batch* prefix, const void* d_q, int64_t q_tok, int64_t q_head,
+                           const jhq_kv_batch* prefix, int once, const void* d_q, int64_t q_tok, int64_t q_head,
                            int q_heads, int dtype, float scale, int causal, void* d_out, float* d_lse,
                            void* d_work, int64_t work_bytes, void* stream) {
     return entry(static_cast<int>(JHQ_ENOMEM), [&] {
         if (!prefix) return bad("null prefix");
-        return do_attend(p, d_cache, b, prefix, d_q, q_tok, q_head, q_heads, dtype, scale, causal, 0, d_out,
+        return do_attend(p, d_cache, b, prefix, once, d_q, q_tok, q_head, q_heads, dtype, scale, causal, 0, d_out,
                          d_lse, d_work, work_bytes, stream);
     });
 }

@@ -234,12 +234,12 @@ class KVCache:
         self._enqueue(_jg.lib().jhq_k_kv_copy, stream, source._ref, source._ptr, slots.data_ptr(),
                       self._ref, self._ptr, batch._ref)
 
-    def work_bytes(self, batch, q_heads, window=0, prefix=None):
-        """Bytes of workspace that attend needs for this batch."""
+    def work_bytes(self, batch, q_heads, window=0, prefix=None, once=False):
+        """Bytes of workspace that attend needs for this batch, prefix and once."""
         if prefix is not None:
             self._no_window(window)
             n = int(_jg.lib().jhq_kv_shared_work_bytes(self._ref, batch._ref, prefix._ref,
-                                                       _int32(q_heads, "q_heads")))
+                                                       1 if once else 0, _int32(q_heads, "q_heads")))
         else:
             n = int(_jg.lib().jhq_kv_work_bytes(self._ref, batch._ref, _int32(q_heads, "q_heads"), _window(window)))
         if n < 0:
@@ -252,7 +252,7 @@ class KVCache:
             raise ValueError("a window and a prefix do not go together")
 
     def attend(self, q, batch, scale=None, causal=True, window=0, out=None, lse=None, work=None,
-               stream=None, prefix=None):
+               stream=None, prefix=None, once=False):
         """Attention of the batch's new tokens, which the cache already holds, to
         their sequences; q [n_tokens, q_heads, head_dim] bfloat16 or float16,
         any strides between rows; returns out, the same shape and type,
@@ -267,7 +267,9 @@ class KVCache:
         same.  Its sequences are the groups: rows cu_q[g] .. of the call are the new
         tokens of group g's sequences, kv_len[g] the tokens that they share (0: none), all before
         their new ones, pages[g] the pages of these (KVPages.prefix finds them).  No window then.
-        Sequences that contradict their group may come out as NaN."""
+        Sequences that contradict their group may come out as NaN.  The bounds choose whether
+        prefixes are read once (from some 50 MB saved on, with single tokens); once=True has them
+        read once."""
         window = _window(window)
         if prefix is not None:
             self._no_window(window)
@@ -296,7 +298,7 @@ class KVCache:
                                  f"tensor on {self.device}")
             lp = lse.data_ptr()
         if work is None:
-            n = self.work_bytes(batch, heads, window, prefix) if heads else 0
+            n = self.work_bytes(batch, heads, window, prefix, once) if heads else 0
             if n:
                 torch = _torch()
                 with torch.cuda.stream(_as_stream(stream, self.device)):
@@ -310,7 +312,7 @@ class KVCache:
             self._call(self._attend, stream, batch, q.data_ptr(), qt, qh, heads, dt, scale, causal, window,
                        out.data_ptr(), lp, wp, wn)
         else:
-            self._call(self._attend_shared, stream, batch, prefix._ref, q.data_ptr(), qt, qh, heads, dt,
+            self._call(self._attend_shared, stream, batch, prefix._ref, 1 if once else 0, q.data_ptr(), qt, qh, heads, dt,
                        scale, causal, out.data_ptr(), lp, wp, wn)
         return out
 

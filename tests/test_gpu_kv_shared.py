@@ -78,7 +78,7 @@ class Shared:
                                 max(self.lens) if max_kv is None else max_kv)
 
     def prefix(self, n_tokens=None, first=0, max_q=None, max_kv=None, lens=None):
-        width = max(1, max(len(t) for t in self.leads))
+        width = max(1, max(len(t) for t in self.leads), -(-(max_kv or 0) // self.page))
         table = np.full((len(self.leads), width), -1, np.int32)
         for b, t in enumerate(self.leads):
             table[b, :len(t)] = t
@@ -116,10 +116,14 @@ class Shared:
         q = self.queries(Hq)
         b, p = self.batch(**kw), self.prefix()
         lse = torch.full(q.shape[:2], 7.0, device=self.gpu)
-        out = self.cache.attend(q.to(self.gpu), b, causal=causal, scale=scale, lse=lse, prefix=p)
+        out = self.cache.attend(q.to(self.gpu), b, causal=causal, scale=scale, lse=lse, prefix=p, once=True)
         assert out.dtype == q.dtype and out.shape == q.shape
-        assert torch.equal(out, self.cache.attend(q.to(self.gpu), b, causal=causal, scale=scale, prefix=p))
+        assert torch.equal(out, self.cache.attend(q.to(self.gpu), b, causal=causal, scale=scale, prefix=p,
+                                                  once=True))
         self.check(q, out, lse, causal, scale)
+        # as the bounds choose
+        self.check(q, self.cache.attend(q.to(self.gpu), b, causal=causal, scale=scale, prefix=p), None, causal,
+                   scale)
         return q, out
 
 
@@ -149,7 +153,6 @@ def test_groups(gpu, bits, D, H, page, groups, G):
 def test_bounds_choose_the_kernels(gpu, groups, bound):
     """The same batch under wide bounds, which choose the kernels for long contexts."""
     w = Shared(gpu, GROUPS[groups], 2, 64, 8, 16, "bf16", seed=3)
-    w.cache_pages = None
     q = w.queries(8)
     b = w.batch()
     width = -(-bound // 16)
@@ -162,7 +165,7 @@ def test_bounds_choose_the_kernels(gpu, groups, bound):
     ptable[:, :p.pages.shape[1]] = p.pages
     wp = w.cache.batch(ptable, p.kv_len, p.cu_q, p.n_tokens, p.max_q, bound)
     for x, y in ((wide, p), (b, wp), (wide, wp)):
-        w.check(q, w.cache.attend(q.to(gpu), x, prefix=y))
+        w.check(q, w.cache.attend(q.to(gpu), x, prefix=y, once=True))
 
 
 @pytest.mark.parametrize("groups", ["few_short", "many_long", "chunks", "wide_chunks"])
@@ -210,8 +213,11 @@ def test_no_prefix_at_all(gpu):
     q, out = w.attend(8)
     b = w.batch()
     assert torch.equal(out, w.cache.attend(q.to(gpu), b))  # nothing is shared: the same kernels
+    # no tokens in any: the prefixes' kernel has nothing to do
+    wide = w.prefix(max_kv=16)
+    w.check(q, w.cache.attend(q.to(gpu), b, prefix=wide, once=True))
     empty = w.cache.batch(w.i32(np.zeros((0, 1))), w.i32([]), w.i32([0]), b.n_tokens, 0, 0)
-    assert torch.equal(out, w.cache.attend(q.to(gpu), b, prefix=empty))
+    assert torch.equal(out, w.cache.attend(q.to(gpu), b, prefix=empty, once=True))
 
 
 def test_rows_of_no_group(gpu):
@@ -224,10 +230,10 @@ def test_rows_of_no_group(gpu):
     p = w.cache.batch(w.i32([w.leads[1]]), w.i32([90]), w.i32([4 + 3, 4 + 5]), T + 9, 2, 90)
     out = torch.full_like(q, 7.0).to(gpu)
     lse = torch.full((T + 9, 4), 7.0, device=gpu)
-    assert w.cache.attend(q.to(gpu), b, prefix=p, out=out, lse=lse) is out
+    assert w.cache.attend(q.to(gpu), b, prefix=p, out=out, lse=lse, once=True) is out
     assert (out[:4] == 7).all() and (out[T + 4:] == 7).all() and (lse[:4] == 7).all() and (lse[T + 4:] == 7).all()
     w.check(q[4:T + 4], out[4:T + 4], lse[4:T + 4])
-    fresh = w.cache.attend(q.to(gpu), b, prefix=p)
+    fresh = w.cache.attend(q.to(gpu), b, prefix=p, once=True)
     assert (fresh[:4] == 0).all() and torch.equal(fresh[4:T + 4], out[4:T + 4])
 
 
@@ -237,7 +243,7 @@ def test_rows_that_see_nothing(gpu):
     w = Shared(gpu, [(0, [(6, 2)]), (40, [(1, 3), (1, 1)])], 2, 64, 8, 16, "f16", seed=9)
     q = w.queries(4)
     lse = torch.zeros(8, 4, device=gpu)
-    out = w.cache.attend(q.to(gpu), w.batch(), prefix=w.prefix(), lse=lse)
+    out = w.cache.attend(q.to(gpu), w.batch(), prefix=w.prefix(), lse=lse, once=True)
     assert (out[:4] == 0).all() and torch.isneginf(lse[:4]).all()
     assert torch.isfinite(lse[4:]).all() and (out[4:] != 0).any()
     w.check(q, out, lse)
@@ -255,13 +261,13 @@ def test_not_finite(gpu):
     for table, n, kv in ((w.leads[0], 21, (ok, bad)), (w.tables[3], 72, (bad, ok))):
         w.cache.write(*kv, w.cache.batch(w.i32([table]), w.i32([n]), w.i32([0, 1]), 1, 1, n))
     q = w.queries(4)
-    out = w.cache.attend(q.to(gpu), w.batch(), prefix=w.prefix())
+    out = w.cache.attend(q.to(gpu), w.batch(), prefix=w.prefix(), once=True)
     assert torch.isnan(out[:2]).all() and torch.isnan(out[3:]).all()
     assert torch.isfinite(out[2]).all()
     w.check(q, out, skip=(0, 1, 3))
     q2 = q.clone()
     q2[2, 1, 3] = float("inf")
-    out2 = w.cache.attend(q2.to(gpu), w.batch(), prefix=w.prefix())
+    out2 = w.cache.attend(q2.to(gpu), w.batch(), prefix=w.prefix(), once=True)
     assert torch.isnan(out2[2, 1]).all() and torch.equal(out2[2, [0, 2, 3]], out[2, [0, 2, 3]])
 
 
@@ -275,7 +281,7 @@ def test_contradictions(gpu):
     b = w.batch()
 
     def call(p, b=b):
-        return w.cache.attend(q.to(gpu), b, prefix=p)
+        return w.cache.attend(q.to(gpu), b, prefix=p, once=True)
     good = call(w.prefix())
     w.check(q, good)
     far = w.prefix(lens=[73, 70], max_kv=80)  # the first sequences' new tokens begin at 72 and 71
@@ -309,32 +315,32 @@ def test_strides_streams_and_graphs(gpu):
     w = Shared(gpu, groups, 2, 128, 8, 16, "bf16", seed=12)
     q = w.queries(8).to(gpu)
     b, p = w.batch(), w.prefix()
-    want = w.cache.attend(q, b, prefix=p)
+    want = w.cache.attend(q, b, prefix=p, once=True)
     fused = torch.zeros(5, 12, 128, dtype=q.dtype, device=gpu)
     fused[:, 2:10] = q
     odd = torch.zeros(5 * (8 * 128 + 3) + 1, dtype=q.dtype, device=gpu)[1:].view(5, -1)[:, :1024].unflatten(1, (8, 128))
     odd.copy_(q)
     for x in (fused[:, 2:10], odd, q.transpose(0, 1).contiguous().transpose(0, 1)):
-        assert torch.equal(w.cache.attend(x, b, prefix=p), want)
+        assert torch.equal(w.cache.attend(x, b, prefix=p, once=True), want)
     buf = torch.zeros(q.numel() + 1, dtype=q.dtype, device=gpu)[1:].view_as(q)
-    assert torch.equal(w.cache.attend(q, b, prefix=p, out=buf), want)
+    assert torch.equal(w.cache.attend(q, b, prefix=p, once=True, out=buf), want)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
-    got = w.cache.attend(q, b, prefix=p, stream=s)
+    got = w.cache.attend(q, b, prefix=p, once=True, stream=s)
     torch.cuda.synchronize()
     assert torch.equal(got, want)
     out = torch.zeros_like(q)
-    work = torch.full((w.cache.work_bytes(b, 8, prefix=p),), 0xff, dtype=torch.uint8, device=gpu)
+    work = torch.full((w.cache.work_bytes(b, 8, prefix=p, once=True),), 0xff, dtype=torch.uint8, device=gpu)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        w.cache.attend(q, b, prefix=p, out=out, work=work)
+        w.cache.attend(q, b, prefix=p, once=True, out=out, work=work)
     full = (b.kv_len.clone(), p.kv_len.clone())
     for i in range(4):
         b.kv_len.copy_(full[0] - torch.tensor([i, 2 * i, 0, i, 0], dtype=torch.int32, device=gpu))
         p.kv_len.copy_(full[1] - 7 * i)  # less of it shared: the same attention
         graph.replay()
         work.fill_(0xff)
-        assert torch.equal(out, w.cache.attend(q, b, prefix=p, work=work))
+        assert torch.equal(out, w.cache.attend(q, b, prefix=p, once=True, work=work))
         keep = w.kv, w.lens
         w.lens = b.kv_len.tolist()
         w.kv = [[x[:n] for x in kv] for kv, n in zip(w.kv, w.lens)]
@@ -350,7 +356,27 @@ def test_refusals(gpu):
     for bad in (lambda: w.cache.attend(q, b, prefix=p, window=5), lambda: w.cache.work_bytes(b, 4, 5, prefix=p),
                 lambda: w.cache.attend(q, b, prefix=w.prefix(n_tokens=3)),
                 lambda: w.cache.work_bytes(b, 4, prefix=w.prefix(n_tokens=3)),
-                lambda: w.cache.attend(q, b, prefix=p, work=torch.empty(16, dtype=torch.uint8, device=gpu)),
+                lambda: w.cache.attend(q, b, prefix=p, once=True, work=torch.empty(16, dtype=torch.uint8, device=gpu)),
                 lambda: w.cache.attend(q[:, :3], b, prefix=p)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("new,P,seqs,G,pays", [(1, 16000, 24, 4, True), (1, 60000, 4, 8, True),
+                                               (9, 24000, 12, 4, True), (40, 9000, 12, 2, False)])
+def test_where_it_pays(gpu, new, P, seqs, G, pays):
+    """The bounds choose to read the prefix once, or by every sequence: the results of one way or the
+    other, and both within rounding of the same values."""
+    import torch
+    w = Shared(gpu, [(P, [(new, new + 11 * i) for i in range(seqs)])], 4, 128, 8, 64, "bf16", seed=seqs)
+    q = w.queries(4 * G).to(gpu)
+    b, p = w.batch(), w.prefix()
+    out = w.cache.attend(q, b, prefix=p)
+    once, alone = w.cache.attend(q, b, prefix=p, once=True), w.cache.attend(q, b)
+    assert torch.equal(out, once if pays else alone)
+    assert w.cache.work_bytes(b, 4 * G, prefix=p) == w.cache.work_bytes(
+        b, 4 * G, **(dict(prefix=p, once=True) if pays else {}))
+    rows = slice(sum(w.new[:-1]), None)  # the last sequence against float64
+    w.new, w.lens, w.kv = w.new[-1:], w.lens[-1:], w.kv[-1:]
+    w.check(q[rows].cpu(), once[rows])
+    w.check(q[rows].cpu(), alone[rows])

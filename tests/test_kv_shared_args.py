@@ -20,13 +20,13 @@ def _err():
     return jg.lib().jhq_last_error().decode()
 
 
-def _calls(b, p, heads=4, work=FAKE, work_bytes=1 << 60, **kw):
+def _calls(b, p, heads=4, once=0, work=FAKE, work_bytes=1 << 60, **kw):
     a = dict(cache=FAKE, q=FAKE, out=FAKE, dtype=3, causal=1)
     a.update(kw)
     L, P = jg.lib(), ctypes.byref(jg._KvParams(8, 2, 128, 64, 10))
     B, R = ctypes.byref(b), ctypes.byref(p) if p else None
-    n = L.jhq_kv_shared_work_bytes(P, B, R, heads)
-    rc = L.jhq_k_kv_attend_shared(P, a["cache"], B, R, a["q"], 512, 128, heads, a["dtype"], 0.1, a["causal"],
+    n = L.jhq_kv_shared_work_bytes(P, B, R, once, heads)
+    rc = L.jhq_k_kv_attend_shared(P, a["cache"], B, R, once, a["q"], 512, 128, heads, a["dtype"], 0.1, a["causal"],
                                   a["out"], None, work, work_bytes, None)
     return n, rc
 
@@ -44,11 +44,12 @@ def test_batches_are_refused(b, p, msg):
 
 
 @pytest.mark.parametrize("kw,msg", [
-    (dict(cache=None), "null cache"), (dict(q=None), "null queries"), (dict(out=None), "null"),
+    (dict(once=2), "once"), (dict(cache=None), "null cache"), (dict(q=None), "null queries"), (dict(out=None), "null"),
     (dict(dtype=0), "queries"), (dict(causal=2), "causal"), (dict(work=None), "null workspace"),
     (dict(work=FAKE + 4), "aligned"), (dict(work_bytes=0), "workspace"), (dict(heads=3), "multiple"),
 ])
 def test_arguments_are_refused(kw, msg):
+    kw = dict(dict(once=1), **kw)
     _, rc = _calls(_batch(), _batch(), **kw)
     assert rc == jg.JHQ_EINVAL and msg in _err()
 
@@ -68,8 +69,8 @@ def test_workspaces(n_tokens, max_q, rows):
         for n_lead in (0, 1, 1 << 20):
             b = _batch(n_tokens=n_tokens, max_q=max_q, max_kv=1 << 22)
             p = _batch(n_tokens=n_tokens, max_q=rows, max_kv=lead_kv, n_seq=n_lead)
-            n, _ = _calls(b, p, heads=4, cache=None)
-            assert -1 <= n <= 1 << 51
-            if n < 0:
-                n, _ = _calls(b, p, heads=4, cache=None)
-                assert n == -1 and (n_tokens > 1 << 30)
+            for once in (0, 1):
+                n, _ = _calls(b, p, once=once, cache=None)
+                assert -1 <= n <= 1 << 50
+                if n < 0:
+                    assert "2^50" in _err() or n_tokens > 1 << 30
