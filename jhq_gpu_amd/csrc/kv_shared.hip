@@ -366,9 +366,12 @@ bool worth(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G
     auto tiles = [&](double each, int n, double most) {
         return each <= few_rows(D) ? 0.0 : std::min(n * std::ceil(each / most), all / most + n);
     };
-    const double every = std::max(b.n_seq * read, tiles(rows, b.n_seq, rows <= 64 ? 64 : 128) * step);
-    const double once = std::max(lead.n_seq * read, tiles(before, lead.n_seq, before <= 64 ? 64 : 128) * step);
-    return every > once + 9000 + 150.0 * b.n_seq + 1.7 * D / 128 * all * c.H;
+    // sequences without new tokens cost nothing
+    const int n = static_cast<int>(std::min<int64_t>(b.n_seq, b.n_tokens));
+    const int groups = static_cast<int>(std::min<int64_t>(lead.n_seq, b.n_tokens));
+    const double every = std::max(n * read, tiles(rows, n, rows <= 64 ? 64 : 128) * step);
+    const double once = std::max(groups * read, tiles(before, groups, before <= 64 ? 64 : 128) * step);
+    return every > once + 9000 + 150.0 * n + 1.7 * D / 128 * all * c.H;
 }
 
 Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G, bool once, float* work) {

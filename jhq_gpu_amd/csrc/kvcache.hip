@@ -298,12 +298,21 @@ __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatc
     __shared__ __align__(16) uint8_t lds[kWaves][R::LDS];
     __shared__ int mags[kWaves][R::TW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane % R::CL, sub = lane / R::CL;
+    uint64_t freq[8];
+    if constexpr (ROT) {  // first, on their way while the rows are found
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int el = col * 8 + e, half = rot.rot / 2;
+            freq[e] = el >= rot.rot ? 0
+                                    : rot.turns[rot.interleaved ? el >> 1 : el < half ? el : el - half];
+        }
+    }
     const Unit u = unit_of<R::TW, SEARCH>(c, b, sets);
     if (!u.any || !u.q.ok) return;  // wave-uniform; the waves share nothing
     const Groups<R::TW> gr(c, b, u);
     const uint32_t live = gr.live & gr.held();
     if (!live) return;
-    const int col = lane % R::CL, sub = lane / R::CL;
     const KvRows src = u.value ? vr : kr;
     const int64_t row0 = u.q.row + (u.first - (u.q.n - u.q.q));
     float x[R::NI][8];
@@ -317,19 +326,12 @@ __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatc
     }
     if constexpr (ROT) {
         if (!u.value) {
-            uint64_t f[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int el = col * 8 + e, half = rot.rot / 2;
-                f[e] = el >= rot.rot ? 0
-                                     : rot.turns[rot.interleaved ? el >> 1 : el < half ? el : el - half];
-            }
 #pragma unroll
             for (int i = 0; i < R::NI; i++) {
                 const int t = i * R::RI + sub;
                 if (live >> t & 1)
                     turn8<DT, VEC>(rot, src.p, (row0 + t) * src.tok + u.head * src.head, col, u.first + t,
-                                   f, x[i]);
+                                   freq, x[i]);
             }
         }
     }
@@ -507,119 +509,163 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(KvCache c, const int
 }
 
 // Tokens as they are held, from any slots (page * page_size + place) of cache f to the batch's new
-// tokens; HBM-bound.  Keys move 16 bytes a lane, a piece of a token, to where they lie in order.
-// Values stand token by token within a group of 16: a lane makes the 16 bytes of an element from
-// its 16 bytes in each of the groups that the tokens come from, which the wave takes one after the
-// other, the next on its way while it picks tokens out of one.  A slot that the cache does not have
-// counts as a row that is not finite.
+// tokens; HBM-bound.  A wave has a run's keys or values in `per` heads: where its tokens lie is the
+// same for each.  Keys move 16 bytes a lane, a piece of a token, to where they lie in order.  Values stand
+// token by token within a group of 16: a lane makes the 16 bytes of an element from its 16 bytes in
+// each of the groups that the tokens come from, kMoveDeep of which are on their way at once (half of
+// the tokens at random: three on average).  A slot that the cache does not have counts as a row that
+// is not finite.
+constexpr int kMoveDeep = 4;
+constexpr int kMoveWaves = 16384;
+
 template <int BITS, int D, bool SEARCH>
 __global__ __launch_bounds__(64 * kWaves) void kv_copy_kernel(KvCache f, KvCache c, KvBatch b,
-                                                              const int64_t* slots, int sets) {
+                                                              const int64_t* slots, int sets, int per) {
     using R = Run<BITS, D>;
     constexpr uint32_t zero = BITS == 8 ? 0x80808080u : 0x88888888u;  // codes 0
+    constexpr int TW = R::TW, NG = TW / 16;
     const int lane = threadIdx.x & 63;
-    const Unit u = unit_of<R::TW, SEARCH>(c, b, sets);
+    KvCache parts = c;
+    parts.H = (c.H + per - 1) / per;
+    const Unit u = unit_of<TW, SEARCH>(parts, b, sets);
     if (!u.any || !u.q.ok) return;  // wave-uniform; the waves share nothing
-    const Groups<R::TW> gr(c, b, u);
-    const uint32_t live = gr.live & gr.held();
+    const int h0 = u.head * per, h1 = min(h0 + per, c.H);
+    // where the run's tokens go: blocks of head 0 (null: no such page), places in them
+    uint8_t* dst[NG];
+    int to[NG];
+    uint32_t live = 0;
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        const int j = u.first + g * 16;
+        const int page = j < u.q.n ? kv_page(b, c, u.seq, j) : -1;
+        dst[g] = page < 0 ? nullptr : kv_block(c, page, 0);
+        to[g] = j & ((1 << c.shift) - 1);
+        const int lo = min(max(u.lo - j, 0), 16), hi = min(max(u.q.n - j, 0), 16);
+        if (page >= 0 && lo < hi) live |= (((1u << hi) - 1) & ~((1u << lo) - 1)) << (g * 16);
+    }
     if (!live) return;
-    const int64_t row0 = u.q.row + (u.first - (u.q.n - u.q.q));
-    // the run's slots, one a lane; -1: none
+    // and come from: a token a lane, page -1: none
+    const bool mine = lane < TW && (live >> (lane & (TW - 1)) & 1);
     int64_t slot = -1;
-    if (lane < R::TW && (live >> lane & 1)) slot = slots[row0 + lane];
+    if (mine) slot = slots[u.q.row + (u.first - (u.q.n - u.q.q)) + lane];
     if (slot < 0 || slot >> f.shift >= f.num_pages) slot = -1;
-    const int in_page = (1 << f.shift) - 1;
     const int page = slot < 0 ? -1 : static_cast<int>(slot >> f.shift);
-    const int place = static_cast<int>(slot) & in_page;
-    if (lane < R::TW && (live >> lane & 1)) {
+    const int place = static_cast<int>(slot) & ((1 << f.shift) - 1);
+    auto block = [&](int g) { return NG == 2 && g ? dst[NG - 1] : dst[0]; };
+    auto place_of = [&](int g) { return NG == 2 && g ? to[NG - 1] : to[0]; };
+    auto scale = [&](int h) {
+        if (!mine) return;
         float s = nan32();
         if (page >= 0)
-            s = reinterpret_cast<const float*>(kv_block(f, page, u.head) +
-                                               2 * f.codes)[(u.value << f.shift) + place];
-        const int g = lane >> 4;
-        uint8_t* const blk = R::TW == 32 && g ? gr.block[R::TW / 16 - 1] : gr.block[0];
-        const int to = (R::TW == 32 && g ? gr.slot[R::TW / 16 - 1] : gr.slot[0]) + (lane & 15);
-        reinterpret_cast<float*>(blk + 2 * c.codes)[(u.value << c.shift) + to] = s;
-    }
+            s = reinterpret_cast<const float*>(kv_block(f, page, h) + 2 * f.codes)[(u.value << f.shift) + place];
+        reinterpret_cast<float*>(block(lane >> 4) + h * c.block + 2 * c.codes)[
+            (u.value << c.shift) + place_of(lane >> 4) + (lane & 15)] = s;
+    };
     if (!u.value) {
-        u32x4 w[R::OUT];
+        const uint8_t* from[R::OUT];
+        int64_t at[R::OUT];
+        bool has[R::OUT];
 #pragma unroll
         for (int i = 0; i < R::OUT; i++) {
-            const int k = lane + 64 * i, g = R::TW == 32 ? k / R::ROW : 0, in = k - g * R::ROW;
+            const int k = lane + 64 * i, g = TW == 32 ? k / R::ROW : 0, in = k - g * R::ROW;
             const int t = in / (R::NP * 4) * 4 + (in & 3), piece = in % (R::NP * 4) >> 2;
             const int pg = __shfl(page, g * 16 + t), pl = __shfl(place, g * 16 + t);
-            w[i] = u32x4{zero, zero, zero, zero};
-            if (pg >= 0)
-                w[i] = *reinterpret_cast<const u32x4*>(kv_block(f, pg, u.head) +
-                                                       (pl & ~3) * R::ROW + piece * 64 + (pl & 3) * 16);
+            from[i] = pg < 0 ? nullptr
+                             : kv_block(f, pg, 0) + (pl & ~3) * R::ROW + piece * 64 + (pl & 3) * 16;
+            has[i] = live >> (g * 16 + t) & 1;
+            at[i] = has[i] ? block(g) - c.base + place_of(g) * R::ROW + in * 16 : 0;
         }
+        for (int h = h0; h < h1; h++) {
+            u32x4 w[R::OUT];
 #pragma unroll
-        for (int i = 0; i < R::OUT; i++) {
-            const int k = lane + 64 * i, g = R::TW == 32 ? k / R::ROW : 0, in = k - g * R::ROW;
-            const int t = in / (R::NP * 4) * 4 + (in & 3);
-            uint8_t* const blk = R::TW == 32 && g ? gr.block[R::TW / 16 - 1] : gr.block[0];
-            const int to = R::TW == 32 && g ? gr.slot[R::TW / 16 - 1] : gr.slot[0];
-            if (live >> (g * 16 + t) & 1) *reinterpret_cast<u32x4*>(blk + to * R::ROW + in * 16) = w[i];
+            for (int i = 0; i < R::OUT; i++) {
+                w[i] = u32x4{zero, zero, zero, zero};
+                if (from[i]) w[i] = *reinterpret_cast<const u32x4*>(from[i] + h * f.block);
+            }
+            scale(h);
+#pragma unroll
+            for (int i = 0; i < R::OUT; i++)
+                if (has[i]) *reinterpret_cast<u32x4*>(c.base + at[i] + h * c.block) = w[i];
         }
         return;
     }
-    // byte columns of a lane, of each of the run's groups
-    constexpr int COLS = (R::ROW + 63) / 64;
+    // Byte columns of a lane; rows of fewer than 64 bytes: two heads at once.
+    constexpr int COLS = (R::ROW + 63) / 64, HP = R::ROW < 64 ? 64 / R::ROW : 1;
+    const int col = lane % (R::ROW < 64 ? R::ROW : 64), sub = lane / (R::ROW < 64 ? R::ROW : 64);
+    // the tokens whose group is another than the token's before
+    uint32_t first[NG];
+    const int group = place & ~15;
+    const int pg0 = __shfl(page, max(lane - 1, 0)), gp0 = __shfl(group, max(lane - 1, 0));
+    const uint64_t differ = __ballot(page != pg0 || group != gp0);
 #pragma unroll
-    for (int g = 0; g < R::TW / 16; g++) {
-        const uint32_t mine = live >> (g * 16) & 0xffff;
-        if (!mine) continue;
-        // tokens whose group is another than the token's before
-        const int group = place & ~15, l0 = g * 16 + (lane & 15);
-        const int pg = __shfl(page, l0), gp = __shfl(group, l0);
-        const int pg0 = __shfl(page, max(l0 - 1, 0)), gp0 = __shfl(group, max(l0 - 1, 0));
-        const uint32_t first = (__ballot(pg != pg0 || gp != gp0) & 0xffff) | 1;
-        u32x4 next[COLS], cur[COLS], out[COLS];
-        auto load = [&](uint32_t from) {  // the group of the next first token in `from`
-            const int t = g * 16 + __builtin_ctz(from);
-            const int p = __builtin_amdgcn_readlane(page, t), at = __builtin_amdgcn_readlane(group, t);
+    for (int g = 0; g < NG; g++) first[g] = (differ >> (g * 16) & 0xffff) | 1;
+    for (int hb = h0; hb < h1; hb += HP) {
+        const int h = min(hb + sub, h1 - 1);
+        const bool here = hb + sub < h1;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const uint32_t part = live >> (g * 16) & 0xffff;
+            if (!part) continue;
+            u32x4 out[COLS];
+#pragma unroll
+            for (int i = 0; i < COLS; i++) out[i] = u32x4{0, 0, 0, 0};
+            uint32_t left = first[g];
+            while (left) {
+                u32x4 v[kMoveDeep][COLS];
+                uint32_t tokens[kMoveDeep];
+#pragma unroll
+                for (int k = 0; k < kMoveDeep; k++) {
+                    tokens[k] = 0;
+                    if (!left) continue;
+                    const uint32_t low = left & -left;
+                    left ^= low;
+                    // from this first token to before the next
+                    tokens[k] = (left ? (left & -left) : 0x10000u) - low;
+                    const int t = g * 16 + __builtin_ctz(low);
+                    const int p = __builtin_amdgcn_readlane(page, t), at = __builtin_amdgcn_readlane(group, t);
+#pragma unroll
+                    for (int i = 0; i < COLS; i++) {
+                        v[k][i] = u32x4{zero, zero, zero, zero};
+                        if (p >= 0)
+                            v[k][i] = *reinterpret_cast<const u32x4*>(kv_block(f, p, h) + f.codes + at * R::ROW +
+                                                                      (col + 64 * i) * 16);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < kMoveDeep; k++) {
+                    if (!tokens[k]) continue;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        if (!(tokens[k] >> r & 1)) continue;
+                        const uint32_t x = __builtin_amdgcn_readlane(place, g * 16 + r) & 15;
+                        // byte x of 16 to byte r % 4 of a word: 0x0c makes a zero
+                        const uint32_t keep = 0x0c0c0c0cu & ~(0xffu << (8 * (r & 3)));
+                        const uint32_t lo = keep | (x < 8 ? x : 0x0c) << (8 * (r & 3));
+                        const uint32_t hi = keep | (x < 8 ? 0x0c : x - 8) << (8 * (r & 3));
+#pragma unroll
+                        for (int i = 0; i < COLS; i++)
+                            out[i][r >> 2] |= __builtin_amdgcn_perm(v[k][i][1], v[k][i][0], lo) |
+                                              __builtin_amdgcn_perm(v[k][i][3], v[k][i][2], hi);
+                    }
+                }
+            }
+            uint8_t* const into = block(g) + h * c.block + c.codes + place_of(g) * R::ROW;
 #pragma unroll
             for (int i = 0; i < COLS; i++) {
-                next[i] = u32x4{zero, zero, zero, zero};
-                if (p >= 0 && lane + 64 * i < R::ROW)
-                    next[i] = *reinterpret_cast<const u32x4*>(kv_block(f, p, u.head) + f.codes +
-                                                              at * R::ROW + (lane + 64 * i) * 16);
-            }
-        };
-        load(first);
+                uint8_t* const x = into + (col + 64 * i) * 16;
+                if (!here) continue;
+                if (part == 0xffff) {
+                    *reinterpret_cast<u32x4*>(x) = out[i];
+                } else {
 #pragma unroll
-        for (int i = 0; i < COLS; i++) out[i] = u32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            if (first >> r & 1) {
-#pragma unroll
-                for (int i = 0; i < COLS; i++) cur[i] = next[i];
-                if (first >> r >> 1) load(first >> r >> 1 << r << 1);
-            }
-            const uint32_t x = __builtin_amdgcn_readlane(place, g * 16 + r) & 15;
-            // byte x of 16 to byte r % 4 of a word: 0x0c makes a zero
-            const uint32_t keep = 0x0c0c0c0cu & ~(0xffu << (8 * (r & 3)));
-            const uint32_t lo = keep | (x < 8 ? x : 0x0c) << (8 * (r & 3));
-            const uint32_t hi = keep | (x < 8 ? 0x0c : x - 8) << (8 * (r & 3));
-#pragma unroll
-            for (int i = 0; i < COLS; i++)
-                out[i][r >> 2] |= __builtin_amdgcn_perm(cur[i][1], cur[i][0], lo) |
-                                  __builtin_amdgcn_perm(cur[i][3], cur[i][2], hi);
-        }
-        uint8_t* const blk = R::TW == 32 && g ? gr.block[R::TW / 16 - 1] : gr.block[0];
-        const int to = R::TW == 32 && g ? gr.slot[R::TW / 16 - 1] : gr.slot[0];
-#pragma unroll
-        for (int i = 0; i < COLS; i++) {
-            if (lane + 64 * i >= R::ROW) continue;
-            uint8_t* const dst = blk + c.codes + to * R::ROW + (lane + 64 * i) * 16;
-            if (mine == 0xffff) {
-                *reinterpret_cast<u32x4*>(dst) = out[i];
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if (mine >> r & 1) dst[r] = static_cast<uint8_t>(out[i][r >> 2] >> (8 * (r & 3)));
+                    for (int r = 0; r < 16; r++)
+                        if (part >> r & 1) x[r] = static_cast<uint8_t>(out[i][r >> 2] >> (8 * (r & 3)));
+                }
             }
         }
+#pragma unroll
+        for (int k = 0; k < HP; k++)
+            if (hb + k < h1) scale(hb + k);
     }
 }
 
@@ -698,13 +744,22 @@ struct Read {
 template <int BITS, int D>
 hipError_t copy_run(const KvCache& f, const KvCache& c, const KvBatch& b, const int64_t* slots,
                     hipStream_t s) {
+    constexpr int TW = Run<BITS, D>::TW, HP = Run<BITS, D>::ROW < 64 ? 64 / Run<BITS, D>::ROW : 1;
     int sets;
     unsigned blocks;
-    if (!units(b, c, Run<BITS, D>::TW, &sets, &blocks)) return hipErrorInvalidValue;
+    // a wave has as many heads as leave enough waves for the chip
+    KvCache parts = c;
+    parts.H = 1;
+    if (!units(b, parts, TW, &sets, &blocks)) return hipErrorInvalidValue;
+    const int64_t waves = static_cast<int64_t>(blocks) * kWaves;
+    const int64_t most = waves * c.H / kMoveWaves;
+    const int per = static_cast<int>(std::min<int64_t>(c.H, std::max<int64_t>(HP, most / HP * HP)));
+    parts.H = (c.H + per - 1) / per;
+    if (!units(b, parts, TW, &sets, &blocks)) return hipErrorInvalidValue;
     if (sets)
-        kv_copy_kernel<BITS, D, false><<<blocks, 64 * kWaves, 0, s>>>(f, c, b, slots, sets);
+        kv_copy_kernel<BITS, D, false><<<blocks, 64 * kWaves, 0, s>>>(f, c, b, slots, sets, per);
     else
-        kv_copy_kernel<BITS, D, true><<<blocks, 64 * kWaves, 0, s>>>(f, c, b, slots, sets);
+        kv_copy_kernel<BITS, D, true><<<blocks, 64 * kWaves, 0, s>>>(f, c, b, slots, sets, per);
     return hipGetLastError();
 }
 

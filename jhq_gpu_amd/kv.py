@@ -126,6 +126,7 @@ class KVCache:
         self._current, self._device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
         self._write, self._read, self._attend = L.jhq_k_kv_write, L.jhq_k_kv_read, L.jhq_k_kv_attend
         self._write_rotary, self._attend_shared = L.jhq_k_kv_write_rotary, L.jhq_k_kv_attend_shared
+        self._copy_pages, self._copy = L.jhq_k_kv_copy_pages, L.jhq_k_kv_copy
 
     def batch(self, pages, kv_len, cu_q, n_tokens, max_q, max_kv):
         """The sequences of a call (KVBatch)."""
@@ -207,15 +208,15 @@ class KVCache:
         """Copies whole pages: src, dst int32 device tensors [n].  No page may be written twice or
         both read and written in one call; pairs that name a page that the cache does
         not have are left out."""
-        torch = _torch()
+        int32 = _torch().int32
         for name, t in (("src", src), ("dst", dst)):
-            if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            if t.dtype != int32 or t.dim() != 1 or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous 1-d int32 tensor")
             if t.get_device() != self._index:
                 raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
         if src.shape != dst.shape:
             raise ValueError(f"src has {src.shape[0]} pages, dst {dst.shape[0]}")
-        self._enqueue(_jg.lib().jhq_k_kv_copy_pages, stream, self._ref, self._ptr, src.data_ptr(),
+        self._enqueue(self._copy_pages, stream, self._ref, self._ptr, src.data_ptr(),
                       dst.data_ptr(), src.shape[0])
 
     def copy(self, slots, batch, source=None, stream=None):
@@ -231,7 +232,7 @@ class KVCache:
                         ("the source is", source._index)):
             if i != self._index:
                 raise ValueError(f"{name} on cuda:{i}, the cache on {self.device}")
-        self._enqueue(_jg.lib().jhq_k_kv_copy, stream, source._ref, source._ptr, slots.data_ptr(),
+        self._enqueue(self._copy, stream, source._ref, source._ptr, slots.data_ptr(),
                       self._ref, self._ptr, batch._ref)
 
     def work_bytes(self, batch, q_heads, window=0, prefix=None, once=False):

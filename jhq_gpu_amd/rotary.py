@@ -5,15 +5,17 @@ the reference).
     q = rope.apply(q, batch)                 # the batch's new tokens, before attend
     cache.write(k, v, batch, rotary=rope)    # keys turn on their way into the cache
 """
+import ctypes
 import math
 import operator
-from fractions import Fraction
 
 import jhq_gpu_amd as _jg
 
 from . import kv as _kv
 
 __all__ = ["Rotary"]
+
+_DTYPES, _POSITIONS = {}, {}  # element types, and the bytes of positions' types; filled with the first Rotary
 
 _PER_TURN = 0x28BE60DB9391054A7F09D5F47D4D3770  # 2^128 / (2 pi)
 
@@ -121,9 +123,11 @@ class Rotary:
         self.device = self._turns.device
         self._index = self.device.index
         self._c = _jg._Rotary(head_dim, rot_dim, 1 if interleaved else 0, amp, self._turns.data_ptr())
-        import ctypes
         self._ref = ctypes.byref(self._c)
         self._entry = _jg.lib().jhq_k_rotary
+        self._current, self._device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+        _DTYPES.update(_kv._DTYPES)
+        _POSITIONS.update({torch.int32: 4, torch.int64: 8})
 
     def apply(self, x, positions, inverse=False, out=None, stream=None):
         """Turns x [n_tokens, heads, head_dim] (float32, bfloat16 or float16, any strides
@@ -132,60 +136,72 @@ class Rotary:
         had, zero where out is None).  Computed in float32 and rounded once.  out: a tensor
         of x's shape and type, x itself among them; it must not share memory with x
         otherwise.  inverse turns back: the gradient's pass."""
-        torch = _kv._torch()
-        n, heads = self._check(x, "x")
-        dt = _kv._dtype(x.dtype, "x")
-        batch = isinstance(positions, _kv.KVBatch)
-        if batch:
+        n, heads, xt, xh = self._rows(x, "x")
+        dt = _DTYPES.get(x.dtype)
+        if dt is None:
+            dt = _kv._dtype(x.dtype, "x")
+        if type(positions) is _kv.KVBatch:
             if positions._index != self._index:
                 raise ValueError(f"the batch is on cuda:{positions._index}, the rotary on {self.device}")
             if positions.n_tokens != n:
                 raise ValueError(f"the batch has {positions.n_tokens} rows, x {n}")
             pp, size, ref = None, 0, positions._ref
         else:
-            if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (n,) \
+            size, ref = _POSITIONS.get(positions.dtype), None
+            if size is None or positions.dim() != 1 or positions.shape[0] != n \
                     or not positions.is_contiguous():
                 raise ValueError(f"positions must be a contiguous int32 or int64 [{n}] tensor")
             if positions.get_device() != self._index:
                 raise ValueError(f"positions are on {positions.device}, the rotary on {self.device}")
-            pp, size, ref = positions.data_ptr(), positions.element_size(), None
+            pp = positions.data_ptr()
         if out is None:
-            new = torch.zeros if batch else torch.empty
+            torch = _kv._torch()
+            new = torch.empty if ref is None else torch.zeros
             with torch.cuda.stream(_kv._as_stream(stream, self.device)):
                 out = new((n, heads, self.head_dim), dtype=x.dtype, device=self.device)
-        elif out.dtype != x.dtype or self._check(out, "out") != (n, heads):
-            raise ValueError(f"out must be of x's shape and type, got {tuple(out.shape)} {out.dtype}")
-        elif any(s == 0 and d > 1 for s, d in zip(out.stride(), out.shape)):
-            raise ValueError("out must not have rows that share memory")
+            ot, oh = heads * self.head_dim, self.head_dim
+        elif out is x:
+            ot, oh = xt, xh
+        else:
+            on, oheads, ot, oh = self._rows(out, "out")
+            if on != n or oheads != heads or out.dtype != x.dtype:
+                raise ValueError(f"out must be of x's shape and type, got {tuple(out.shape)} {out.dtype}")
         if n == 0 or heads == 0:
             return out
-        if torch._C._cuda_getDevice() != self._index:  # kernels are launched on the current device
-            with torch.cuda.device(self._index):
+        if (ot == 0 and n > 1) or (oh == 0 and heads > 1):
+            raise ValueError("out must not have rows that share memory")
+        if self._device() != self._index:  # kernels are launched on the current device
+            with _kv._torch().cuda.device(self._index):
                 return self.apply(x, positions, inverse, out, stream)
         if stream is None:
-            s = torch._C._cuda_getCurrentRawStream(self._index)
+            s = self._current(self._index)
         else:
             s = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
-        rc = self._entry(self._ref, x.data_ptr(), x.stride(0), x.stride(1), n, heads, dt, pp, size, ref,
-                         1 if inverse else 0, out.data_ptr(), out.stride(0), out.stride(1), s)
+        rc = self._entry(self._ref, x.data_ptr(), xt, xh, n, heads, dt, pp, size, ref, 1 if inverse else 0,
+                         out.data_ptr(), ot, oh, s)
         if rc:
             _jg._check(rc)
         return out
 
-    def _check(self, x, what):
+    def _rows(self, x, what):
+        """Rows, heads and strides of a [n_tokens, heads, head_dim] tensor."""
         if x.dim() != 3 or x.shape[2] != self.head_dim:
             raise ValueError(f"{what} must be [n_tokens, heads, {self.head_dim}], got {tuple(x.shape)}")
         if x.get_device() != self._index:
             raise ValueError(f"{what} is on {x.device}, the rotary on {self.device}")
-        if x.stride(2) != 1:
+        n, heads, _ = x.shape
+        tok, head, el = x.stride()
+        if el != 1:
             raise ValueError(f"{what}: the elements of a row must be contiguous")
-        return x.shape[0], x.shape[1]
+        return n, heads, tok, head
 
 
 def turns(frequencies):
     """Radians a position as 2^-64ths of a turn modulo one turn, in int64."""
     out = []
     for x in frequencies:
-        n = round(Fraction(x) * _PER_TURN / (1 << 64)) % (1 << 64)
+        m, e = math.frexp(x)  # x = m 2^e, 53 bits of m
+        n, down = int(m * (1 << 53)) * _PER_TURN, 64 + 53 - e
+        n = (n + (1 << down - 1) >> down if down > 0 else n << -down) % (1 << 64)
         out.append(n - (1 << 64) if n >= 1 << 63 else n)
     return out
