@@ -20,33 +20,6 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import jhq_gpu_amd as jg  # noqa: E402
 
 
-class Pages:
-    """Page tables of some sequences over one pool of pages."""
-
-    def __init__(self, cache, n_seq, max_tokens):
-        self.cache = cache
-        self.max_pages = -(-max_tokens // cache.page_size)
-        self.free = list(range(cache.num_pages))[::-1]
-        self.table = np.zeros((n_seq, self.max_pages), np.int32)
-        self.held = [0] * n_seq
-        self.length = np.zeros(n_seq, np.int32)
-
-    def extend(self, new):
-        """Room for new[s] more tokens of each sequence; the batch that writes or
-        attends with them."""
-        self.length += np.asarray(new, np.int32)
-        for s, n in enumerate(self.length):
-            while self.held[s] * self.cache.page_size < n:
-                self.table[s, self.held[s]] = self.free.pop()
-                self.held[s] += 1
-        to = self.cache.device
-        return self.cache.batch(torch.from_numpy(self.table).to(to),
-                                torch.from_numpy(self.length).to(to),
-                                torch.tensor(np.concatenate([[0], np.cumsum(new)]),
-                                             dtype=torch.int32, device=to),
-                                int(sum(new)), int(max(new)), int(self.length.max()))
-
-
 def run(device="cuda:0", bits=8, passages=2000, d=64, questions=4, k=5, heads=16, kv_heads=4,
         head_dim=128, generate=8, seed=0):
     """Returns the passages found, what each sequence holds and every output."""
@@ -69,7 +42,7 @@ def run(device="cuda:0", bits=8, passages=2000, d=64, questions=4, k=5, heads=16
              for i, n in zip(np.unique(ids), rng.integers(20, 90, ids.size))}
     cache = jg.KVCache(num_pages=questions * 16, page_size=64, kv_heads=kv_heads,
                        head_dim=head_dim, bits=bits, device=device)
-    pages = Pages(cache, questions, 16 * 64)
+    pages = jg.KVPages(cache, questions, 16 * 64)
     held = [([], []) for _ in range(questions)]
 
     def enter(kk, vv):
@@ -88,7 +61,7 @@ def run(device="cuda:0", bits=8, passages=2000, d=64, questions=4, k=5, heads=16
     for new in [list(rng.integers(5, 40, questions))] + [[1] * questions] * generate:
         batch = enter([rows(n, kv_heads) for n in new], [rows(n, kv_heads) for n in new])
         q = rows(sum(new), heads)
-        steps.append(dict(new=[int(n) for n in new], length=pages.length.copy(), q=q,
+        steps.append(dict(new=[int(n) for n in new], length=[pages.length(s) for s in range(questions)], q=q,
                           out=cache.attend(q.to(device), batch).cpu()))
     return dict(ids=ids, steps=steps, bits=bits,
                 k=[torch.cat(x[0]) for x in held], v=[torch.cat(x[1]) for x in held])
