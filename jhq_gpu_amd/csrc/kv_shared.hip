@@ -384,10 +384,11 @@ Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D,
     r.places = D == 256 ? 256 : r.few && D == 64 && r.lead < 2 ? 768 : 512;
     const int tile = r.lead ? 64 * r.lead : 16, own = r.few ? 16 : tile;
     if (r.waves == 8) r.lead = 1;
-    // steps are numbered with an int
+    // Numbers of tiles, of which first_tile leaves as many; steps are numbered with an int, also where
+    // cu_q does not ascend and every sequence has as many rows as the bounds allow.
     const int64_t tiles = b.n_tokens * G / tile + lead.n_seq, own_tiles = b.n_tokens * G / own + b.n_seq;
-    const __int128 steps = (static_cast<__int128>(tiles) * (lead.max_kv / kStep + 8) +
-                            static_cast<__int128>(own_tiles) * (b.max_kv / kStep + 8)) * c.H;
+    const __int128 steps = (static_cast<__int128>(lead.n_seq) * (before / tile + 1) * (lead.max_kv / kStep + 8) +
+                            static_cast<__int128>(b.n_seq) * (rows / own + 1) * (b.max_kv / kStep + 8)) * c.H;
     r.shared = lead.n_seq > 0 && lead.max_kv > 0 && steps < INT32_MAX / 2 &&
                (once || worth(c, lead, b, D, G));
     if (!r.shared) {

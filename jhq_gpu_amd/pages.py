@@ -29,7 +29,8 @@ class KVPages:
     A page may be held by several sequences: it is then only read, and a sequence that is
     to write into it gets a copy first.  Pages are given out lowest number first.
 
-    Calls enqueue work on the current stream, or `stream`; the device arrays are this
+    Calls enqueue work on the current stream, or `stream` (they are no part of a captured graph, which
+    replays what extend wrote last); the device arrays are this
     object's own and are updated in place, so a batch is good until the next call that changes
     its sequences, and everything that uses them has to be ordered with that stream."""
 
@@ -143,7 +144,8 @@ class KVPages:
 
     def compact(self, keep, stream=None):
         """keep: {sequence: ascending positions}.  Each of these sequences keeps those of its tokens,
-        moved together; keys stay as they are, turned to the positions that they had.
+        moved together; keys stay as they are, turned to the positions that they had (so tokens that
+        come after are turned to positions of their own too: Rotary.apply with a tensor of them).
         Whole pages in front that keep all of their tokens stay; the others' tokens are
         copied into free pages, of which there have to be as many as they fill."""
         P, plan = self.page_size, []
@@ -199,19 +201,23 @@ class KVPages:
             raise RuntimeError("sequences have changed since extend")
         P, groups = self.page_size, []
         least = max(1, operator.index(least))
-        for s in np.nonzero(self._new)[0]:
-            whole = int(self._len[s] - self._new[s]) // P
-            rows = int(self._new[s])
+        live = np.nonzero(self._new)[0]
+        whole = (self._len - self._new)[live] // P
+        # pages that a sequence begins with as the one before it does
+        same = np.zeros(live.size, np.int64)
+        if live.size > 1:
+            width = int(whole.max())
+            equal = self._table[live[1:], :width] == self._table[live[:-1], :width]
+            same[1:] = np.where(equal.all(1), width, equal.argmin(1)) if width else 0
+        for s, m, mine, rows in zip(live.tolist(), same.tolist(), whole.tolist(), self._new[live].tolist()):
             if groups:
-                first, n, same, total = groups[-1]
-                m = min(same, whole)
-                differ = np.nonzero(self._table[s, :m] != self._table[first, :m])[0]
-                m = int(differ[0]) if differ.size else m
+                first, n, shared, total = groups[-1]
+                m = min(m, shared, mine)
                 # a sequence joins where that saves as many pages as it costs the others
-                if m >= least and n * m >= (n - 1) * same:
+                if m >= least and n * m >= (n - 1) * shared:
                     groups[-1] = (first, n + 1, m, total + rows)
                     continue
-            groups.append((int(s), 1, whole, rows))
+            groups.append((s, 1, mine, rows))
         if not any(n > 1 for _, n, _, _ in groups):
             return None
         shared = np.array([m if n > 1 else 0 for _, n, m, _ in groups], np.int64)

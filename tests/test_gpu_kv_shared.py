@@ -307,6 +307,27 @@ def test_contradictions(gpu):
     assert torch.isnan(out[3:]).all() and torch.equal(out[:3], good[:3])
 
 
+@pytest.mark.parametrize("new", [1, 30])
+def test_rows_out_of_order(gpu, new):
+    """cu_q that does not ascend, in the batch and in the prefix: any sequence may be left out, and
+    nothing else is written."""
+    import torch
+    w = Shared(gpu, [(100, [(new, new + 3)] * 6)], 2, 64, 8, 16, "f16", seed=14)
+    T = 6 * new
+    q = w.queries(4)
+    b, p = w.batch(), w.prefix()
+    buf = torch.full((T + 2, 4, 64), 7.0, dtype=q.dtype, device=gpu)
+    data = w.cache.data.clone()
+    for cu in ([0, T, 0, T, 0, T, T], [T, new, 0, 2 * new, T, 0, T], [0, -5, new, 1 << 30, 0, T, 2 * new]):
+        for pcu in ([0, T], [T, 0], [-3, T], [0, 1 << 30]):
+            x = w.cache.batch(b.pages, b.kv_len, w.i32(cu), T, T, b.max_kv)
+            y = w.cache.batch(p.pages, p.kv_len, w.i32(pcu), T, T, p.max_kv)
+            w.cache.attend(q.to(gpu), x, prefix=y, out=buf[1:-1], once=True)
+            assert (buf[0] == 7).all() and (buf[-1] == 7).all()
+    assert torch.equal(w.cache.data, data)
+    w.check(q, w.cache.attend(q.to(gpu), b, prefix=p, once=True))
+
+
 def test_strides_streams_and_graphs(gpu):
     """Queries inside a projection and on no boundary; another stream; a captured call replayed while
     lengths, rows and tables change."""
