@@ -168,8 +168,7 @@ struct Piece {
     }
 };
 template <int BITS, int D, int NC, int W>
-constexpr int ahead_of<Piece, BITS, D, NC, W> = D == 256 ? (NC == 1 && W == 4 ? 2 : 1)
-                                                : 2;
+constexpr int ahead_of<Piece, BITS, D, NC, W> = D == 256 && W == 8 ? 1 : 2;  // registers
 template <class B>
 __device__ inline Share share_of(const KvCache&, const B&, const KvAttend&, const Plan&, const Piece& x) {
     return x.w;
@@ -189,15 +188,19 @@ __device__ inline int dealt(const Deal& d, int lead, int own) {
 }
 
 // Workgroups of a CU.
-template <int D, int LEAD>
-constexpr int kBothWaves = D == 256 ? 1 : D == 64 && LEAD < 2 ? 3 : 2;
+template <int D>
+constexpr int kBothWaves = D == 256 ? 1 : D == 64 ? 3 : 2;
 
 // Prefixes and what stands behind them in one launch: the former, many rows, are bound by vector and matrix
-// instructions, the latter by reading the cache.  LEAD: 0 few rows before, else tiles of 64 LEAD.
+// instructions, the latter by reading the cache.  LEAD: 0 few rows before, else
+// tiles of 64 LEAD.  Tiles of 128 rows are turned to float16 half as often, but leave less beside them; us:
+// 64 tokens of 32 heads on 8 of 128 behind 16003 64.2 and 69.5 with tiles of 64, of heads of 64 48.8 and
+// 44.6, of 32 heads on 4 of 256 behind 12000 96 and 88, 48 of 16 on 4 behind three prefixes 62.3 and 51.5.
+constexpr int most_lead(int D) { return D == 128 ? 2 : 1; }
+
 template <int BITS, int D, int LEAD>
-__global__ __launch_bounds__(256, (kBothWaves<D, LEAD>))
+__global__ __launch_bounds__(256, (kBothWaves<D>))
 void kv_both_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a, KvAttend la, Kept ok, Kept lk, Deal d) {
-    constexpr int NC = LEAD ? LEAD : 1;
     __shared__ __align__(16) float few[4][192];
     const int lane = threadIdx.x & 63, wave = wave_id(), block = blockIdx.x;
     const int lt = all_steps(c, lead, lane, [&](const KvSeq& s) { return tile_steps(lead, s, la, lk); });
@@ -212,7 +215,7 @@ void kv_both_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a, KvAttend la, Ke
     } else {
         JHQ_MANY_LDS(BITS, D, 4);
         each_tile(c, lead, la, lk, lt, n, 1, block, lane, threadIdx.x == 0, [&](const Share& w, int64_t slot) {
-            many_rows<BITS, D, NC, 4>(c, lead, la, Plan{}, Piece{w, lk, slot}, kf, vf, sc, bigs);
+            many_rows<BITS, D, LEAD, 4>(c, lead, la, Plan{}, Piece{w, lk, slot}, kf, vf, sc, bigs);
         });
     }
 }
@@ -379,9 +382,10 @@ Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D,
     const int64_t rows = static_cast<int64_t>(b.max_q) * G, before = static_cast<int64_t>(lead.max_q) * G;
     const int64_t all = b.n_tokens * c.H * G;
     r.few = rows <= 16;
-    r.lead = std::max(rows, before) <= 16 ? 0 : std::max(rows, before) <= 64 ? 1 : 2;
-    r.waves = !r.few && D == 256 && r.lead == 2 ? 8 : 4;
-    r.places = D == 256 ? 256 : r.few && D == 64 && r.lead < 2 ? 768 : 512;
+    const int64_t longest = std::max(rows, before);
+    r.lead = longest <= 16 ? 0 : longest <= 64 ? 1 : r.few ? most_lead(D) : 2;
+    r.waves = D == 256 && r.lead == 2 ? 8 : 4;
+    r.places = D == 256 ? 256 : r.few && D == 64 ? 768 : 512;
     const int tile = r.lead ? 64 * r.lead : 16, own = r.few ? 16 : tile;
     if (r.waves == 8) r.lead = 1;
     // Numbers of tiles, of which first_tile leaves as many; steps are numbered with an int, also where
@@ -422,7 +426,11 @@ hipError_t launch(const KvCache& c, const KvBatch& lead, const KvBatch& b, const
     ob.n_lead = lead.n_seq;
     KvAttend la = a;
     la.causal = 0;
-    const Deal d = {ch.places, 1.0f, !ch.few || ch.lead == 0 ? 1.0f : ch.lead == 1 ? 0.4f : 0.3f};
+    // measured: 64 single tokens behind 16003, 8 bits, 32 heads on 8 of 128: 67.1 us with 0.22, 64.6 with 0.3,
+    // 65.6 with 0.4, 67.1 with 0.5, 71.3 with 0.65; of 64 56.6 with 0.2, 48.4 with 0.3, 45.9 with 0.4, 44.7
+    // with 0.5; 16 on 4 of 256, three prefixes, 59.6, 51.7, 52.9, 53.2
+    const float own = D == 64 || ch.lead == 1 && D == 128 ? 0.4f : 0.3f;
+    const Deal d = {ch.places, 1.0f, ch.few && ch.lead ? own : 1.0f};
     auto go = [&](auto kernel) {
         kernel<<<ch.places, 64 * ch.waves, 0, s>>>(c, ob, lb, a, la, ch.ok, ch.lk, d);
     };
@@ -431,7 +439,7 @@ hipError_t launch(const KvCache& c, const KvBatch& lead, const KvBatch& b, const
     else if (ch.few && ch.lead == 1)
         go(kv_both_kernel<BITS, D, 1>);
     else if (ch.few)
-        go(kv_both_kernel<BITS, D, 2>);
+        go(kv_both_kernel<BITS, D, most_lead(D)>);
     else if (ch.lead == 1 && ch.waves == 4)
         go(kv_tiles_kernel<BITS, D, 1, 4>);
     else if constexpr (D == 256)
