@@ -1,5 +1,5 @@
-// kv_attend.h — attention of new tokens over the quantised key/value cache: its arithmetic, its
-// kernels and the rule that chooses them.  Internal to kv_attend.hip and kv_shared.hip.
+// kv_attend.h — attention of new tokens over the quantised key/value cache: its arithmetic and its
+// kernels.  Internal to kv_attend.hip and kv_shared.hip.
 //
 // Mathematics.  With codes c and scales of the cache, s_ij = scale * ks_j <q_i,
 // ck_j> and o_i = sum_j w_ij vs_j cv_j / sum_j w_ij, w_ij = exp(s_ij).  Both

@@ -1,5 +1,5 @@
 // kv_attend.hip — attention of new tokens over the quantised key/value cache: what joins the parts of
-// rows, and the launches.  Its arithmetic and its kernels are in kv_attend.h.
+// rows, the rules that choose the kernels, and the launches.  The arithmetic and the kernels are in kv_attend.h.
 #include "kv_attend.h"
 
 namespace jhq {

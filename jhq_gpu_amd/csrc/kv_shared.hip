@@ -156,7 +156,9 @@ __device__ inline void few_steps(const KvCache& c, const B& b, const KvAttend& a
     });
 }
 
-// A tile of one of the workgroups that have many rows, for many_rows().
+// A tile of one of the workgroups that have many rows, for many_rows(), which has two steps on their way where
+// the registers suffice: 40 x 2 to 5 tokens of 16 heads of 64 behind four prefixes, 4 bits, 104 us with one,
+// 83 with two and three workgroups a CU in the place of two; leaving out the steps of waves without rows 80.
 struct Piece {
     const Share& w;
     const Kept& k;
@@ -191,11 +193,15 @@ __device__ inline int dealt(const Deal& d, int lead, int own) {
 template <int D>
 constexpr int kBothWaves = D == 256 ? 1 : D == 64 ? 3 : 2;
 
-// Prefixes and what stands behind them in one launch: the former, many rows, are bound by vector and matrix
-// instructions, the latter by reading the cache.  LEAD: 0 few rows before, else
-// tiles of 64 LEAD.  Tiles of 128 rows are turned to float16 half as often, but leave less beside them; us:
-// 64 tokens of 32 heads on 8 of 128 behind 16003 64.2 and 69.5 with tiles of 64, of heads of 64 48.8 and
-// 44.6, of 32 heads on 4 of 256 behind 12000 96 and 88, 48 of 16 on 4 behind three prefixes 62.3 and 51.5.
+// Prefixes and what stands behind them in one launch, so that the former, many rows, which vector and matrix
+// instructions bound, run beside the latter, which reading the cache bounds: 64 tokens of 32 heads on 8 of
+// 128 behind 16003, 50 to 1500 of their own, 8 bits: 55 us, and 40 + 33 in two launches; the join 10 more.
+// Of it 2.5 us go by before the first load of codes, 8 to write the parts; a step of 128 rows takes 3.0 us
+// with two such workgroups on a CU and 3.3 to 3.8 beside waves that read (VALU 40% of the cycles, matrix
+// cores 17%, waves wait in 49% of theirs).  LEAD: 0 few rows before, else tiles of 64 LEAD.  Tiles of 128
+// rows are turned to float16 half as often, but leave less beside them; us: the case above 64.2 a call and
+// 69.5 with tiles of 64, of heads of 64 48.8 and 44.6, 64 tokens of 16 heads on 4 of 256 96 and 88, 48 behind
+// three prefixes 62.3 and 51.5.
 constexpr int most_lead(int D) { return D == 128 ? 2 : 1; }
 
 template <int BITS, int D, int LEAD>
@@ -261,7 +267,8 @@ __device__ inline Parts parts_of(const Kept& k, const KvSeq& s, int seq, int i, 
 }
 
 // Joins what the passes have of a row; latency and reading the parts bound it.  A thread has 4
-// elements of every Y-th part.
+// elements of every Y-th part: 2048 rows of 20 parts of 128 elements 9.9 us with 4, 10.2 with 2, 10.9 with 1,
+// 13.5 with 8.
 template <int D, int Y>
 __global__ __launch_bounds__(256) void kv_shared_join_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a,
                                                              Kept lk, Kept ok) {

@@ -290,7 +290,8 @@ __device__ inline void turn8(const Rotary& r, const void* base, int64_t row, int
 // in 16-bit types.  A large copy moves 4.8 TB/s; 19192 tokens, 8 heads of 128, 8 bits: 119 MB in
 // 31.6 us, 3.8 TB/s, from float32 198 MB in 41.0, 4.8; 4 bits, 8 heads of 64, 16384 tokens 3.1 TB/s and
 // 65536 4.1; 64 single tokens 5.1 us.
-// ROT: keys are turned to their positions first, in float32, and not rounded before they are held.
+// ROT: keys are turned to their positions first, in float32, and not rounded before they are held: 48 single
+// tokens of 4 heads of 256 8.7 us.
 template <int BITS, int D, int DT, bool VEC, bool SEARCH, bool ROT>
 __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatch b, KvRows kr,
                                                                KvRows vr, int sets, Rotary rot) {
@@ -486,7 +487,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvCache c, KvBatch
     }
 }
 
-// Whole pages, 16 bytes a lane and kCopyDeep of them in flight; HBM-bound.  A pair that names a page
+// Whole pages, 16 bytes a lane and kCopyDeep of them in flight; HBM-bound: 63 pages of 135 kB in 4.4 us.  A pair that names a page
 // that the cache does not have is left out.
 constexpr int kCopyDeep = 4;
 constexpr int kCopyRun = 256 * 16 * kCopyDeep;  // bytes of a workgroup
@@ -514,8 +515,12 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(KvCache c, const int
 // token by token within a group of 16: a lane makes the 16 bytes of an element from its 16 bytes in
 // each of the groups that the tokens come from, kMoveDeep of which are on their way at once (half of
 // the tokens at random: three on average).  A slot that the cache does not have counts as a row that
-// is not finite.
+// is not finite.  31187 of 62000 tokens at random, 8 heads of 128, 8 bits: 132 MB in 47 us, 2.8 TB/s (half
+// of each line read is another token's: 80 MB for 66); 213600 in runs, 8 of 64, 4 bits, 246 MB in 71,
+// 3.5 TB/s; 700 tokens 6.4.
 constexpr int kMoveDeep = 4;
+// Waves that a call is cut into by heads at most: the first of these 51.4 us with 8192, 47.1 with 16384, 49.1
+// with one head each; the second 71.2, 75.7, 74.8.
 constexpr int kMoveWaves = 16384;
 
 template <int BITS, int D, bool SEARCH>
