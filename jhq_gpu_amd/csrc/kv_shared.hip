@@ -269,6 +269,9 @@ __device__ inline Parts parts_of(const Kept& k, const KvSeq& s, int seq, int i, 
 // Joins what the passes have of a row; latency and reading the parts bound it.  A thread has 4
 // elements of every Y-th part: 2048 rows of 20 parts of 128 elements 9.9 us with 4, 10.2 with 2, 10.9 with 1,
 // 13.5 with 8.
+constexpr int kJoinWays = 4;
+constexpr int64_t join_rows(int D) { return 256 / (D / 4 * kJoinWays); }  // of a workgroup
+
 template <int D, int Y>
 __global__ __launch_bounds__(256) void kv_shared_join_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a,
                                                              Kept lk, Kept ok) {
@@ -400,19 +403,15 @@ Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D,
     const int64_t tiles = b.n_tokens * G / tile + lead.n_seq, own_tiles = b.n_tokens * G / own + b.n_seq;
     const __int128 steps = (static_cast<__int128>(lead.n_seq) * (before / tile + 1) * (lead.max_kv / kStep + 8) +
                             static_cast<__int128>(b.n_seq) * (rows / own + 1) * (b.max_kv / kStep + 8)) * c.H;
-    r.shared = lead.n_seq > 0 && lead.max_kv > 0 && steps < INT32_MAX / 2 &&
+    // and the join is one launch
+    r.shared = lead.n_seq > 0 && lead.max_kv > 0 && steps < INT32_MAX / 2 && all < join_rows(D) << 23 &&
                (once || worth(c, lead, b, D, G));
     if (!r.shared) {
         r.work = kv_attend_work(c, b, D, G, 0);
         return r;
     }
-    if (all > int64_t(1) << 40) {
-        r.work = -1;
-        return r;
-    }
     const int64_t floats = lay_out(r.lk, work, D, 2 * r.places * (r.lead ? 1 : 4), tile, tiles * c.H, all);
     r.work = (floats + lay_out(r.ok, work + floats, D, 2 * r.places * (r.few ? 4 : 1), own, own_tiles * c.H, all)) * 4;
-    if (r.work > int64_t(1) << 50) r.work = -1;
     r.lk.start = 3;
     r.ok.start = r.few ? 1 : 3;
     return r;
@@ -421,9 +420,7 @@ Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D,
 template <int BITS, int D>
 hipError_t launch(const KvCache& c, const KvBatch& lead, const KvBatch& b, const KvAttend& a,
                   const Both& ch, hipStream_t s) {
-    constexpr int Y = 4;
-    const int64_t joins = (ch.lk.rows + 256 / (D / 4 * Y) - 1) / (256 / (D / 4 * Y));
-    if (joins >= 1 << 23) return hipErrorInvalidValue;
+    const int64_t joins = (ch.lk.rows + join_rows(D) - 1) / join_rows(D);
     KvLead lb;
     static_cast<KvBatch&>(lb) = lead;
     KvOwn ob;
@@ -455,7 +452,7 @@ hipError_t launch(const KvCache& c, const KvBatch& lead, const KvBatch& b, const
         go(kv_tiles_kernel<BITS, D, 2, 4>);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    kv_shared_join_kernel<D, Y><<<static_cast<unsigned>(joins), 256, 0, s>>>(c, ob, lb, a, ch.lk, ch.ok);
+    kv_shared_join_kernel<D, kJoinWays><<<static_cast<unsigned>(joins), 256, 0, s>>>(c, ob, lb, a, ch.lk, ch.ok);
     return hipGetLastError();
 }
 

@@ -135,10 +135,19 @@ class KVCache:
     def _call(self, entry, stream, batch, *args):
         if batch._index != self._index:
             raise ValueError(f"the batch is on cuda:{batch._index}, the cache on {self.device}")
-        self._enqueue(entry, stream, self._ref, self._ptr, batch._ref, *args)
+        if self._device() != self._index:  # kernels are launched on the current device
+            with _torch().cuda.device(self._index):
+                return self._call(entry, stream, batch, *args)
+        if stream is None:
+            s = self._current(self._index)
+        else:
+            s = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+        rc = entry(self._ref, self._ptr, batch._ref, *args, s)
+        if rc:
+            _jg._check(rc)
 
     def _enqueue(self, entry, stream, *args):
-        if self._device() != self._index:  # kernels are launched on the current device
+        if self._device() != self._index:
             with _torch().cuda.device(self._index):
                 return self._enqueue(entry, stream, *args)
         if stream is None:

@@ -69,10 +69,11 @@ class KVPages:
         seq = self._seq(seq)
         return self._table[seq, :self._held(seq)].tolist()
 
-    def extend(self, new, stream=None):
+    def extend(self, new, max_q=None, max_kv=None, stream=None):
         """Room for new[s] more tokens of each sequence s; returns the KVBatch that
         writes and attends with them.  Where a sequence goes on in a page that others hold
-        too, it gets a copy of it."""
+        too, it gets a copy of it.  max_q, max_kv: the batch's bounds, wider than its
+        lengths (the default) where a captured call is replayed as they grow."""
         new = self._counts(new)
         P = self.page_size
         to = self._len + new
@@ -81,6 +82,13 @@ class KVPages:
         if (to > self.max_tokens).any():
             s = int(np.argmax(to > self.max_tokens))
             raise ValueError(f"sequence {s} would have {int(to[s])} tokens, {self.max_tokens} are the most")
+        bounds = []
+        for name, v, least, most in (("max_q", max_q, int(new.max()), 1 << 30),
+                                     ("max_kv", max_kv, int(to.max()), self._width * P)):
+            v = least if v is None else operator.index(v)
+            if not least <= v <= most:
+                raise ValueError(f"{name} must be {least} .. {most}, got {v}")
+            bounds.append(v)
         grow = np.where(new > 0, -(-to // P) - -(-self._len // P), 0)
         split = []
         # a page that k sequences are about to write into is kept by the last of them
@@ -112,8 +120,7 @@ class KVPages:
                 pairs = self._to_device(np.array([src, dst], np.int32))
                 self.cache.copy_pages(pairs[0], pairs[1])
             self._upload()
-        return self.cache.batch(self._pages, self._kv_len, self._cu, int(new.sum()), int(new.max()),
-                                int(to.max()))
+        return self.cache.batch(self._pages, self._kv_len, self._cu, int(new.sum()), *bounds)
 
     def fork(self, src, dst):
         """Sequence dst, which is empty, begins with all tokens of src, in the same pages."""

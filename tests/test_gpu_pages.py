@@ -298,3 +298,42 @@ def test_sequences_that_fork_grow_and_shrink(gpu, bits):
     for s in range(n_seq):
         pages.free(s)
     assert pages.free_pages == 90
+
+
+def test_a_captured_step_is_replayed_as_sequences_grow(gpu):
+    """Positions, write and attention in one graph: extend moves what it reads."""
+    import torch
+    H, D, G, n_seq = 2, 64, 2, 3
+    cache = jg.KVCache(40, 16, H, D, device=gpu)
+    pages = jg.KVPages(cache, n_seq, 200)
+    rope = jg.Rotary(D, device=gpu)
+    g = torch.Generator().manual_seed(5)
+
+    def rows(n, h):
+        return torch.randn(n, h, D, generator=g).bfloat16().to(gpu)
+    prompt = pages.extend([30, 0, 9])
+    cache.write(rows(39, H), rows(39, H), prompt, rotary=rope)
+    pages.fork(0, 1)
+    b = pages.extend([1, 1, 1], max_kv=200)
+    q, k, v = rows(3, H * G), rows(3, H), rows(3, H)
+    turned, out = torch.zeros_like(q), torch.zeros_like(q)
+    work = torch.zeros(cache.work_bytes(b, H * G), dtype=torch.uint8, device=gpu)
+
+    def step():
+        rope.apply(q, b, out=turned)
+        cache.write(k, v, b, rotary=rope)
+        cache.attend(turned, b, out=out, work=work)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(20):  # over the end of a page, and of the page that two hold
+        now = pages.extend([1, 1, 1], max_kv=200)
+        for x, h in ((q, H * G), (k, H), (v, H)):
+            x.copy_(rows(3, h))
+        graph.replay()
+        got, seen = out.clone(), turned.clone()
+        assert torch.equal(rope.apply(q, now), seen)
+        assert torch.equal(cache.attend(seen, now), got)
+    assert pages.length(1) == 51 and torch.isfinite(out).all()

@@ -16,7 +16,7 @@ class Batch:
         self.n_tokens, self.max_q, self.max_kv = n_tokens, max_q, max_kv
         assert max_kv <= self.pages.shape[1] * Cache.page_size
         assert self.cu_q[-1] == n_tokens and (np.diff(self.cu_q) >= 0).all()
-        assert np.diff(self.cu_q).max(initial=0) == max_q and self.kv_len.max(initial=0) == max_kv
+        assert np.diff(self.cu_q).max(initial=0) <= max_q and self.kv_len.max(initial=0) <= max_kv
 
 
 class Cache:
@@ -209,6 +209,18 @@ def test_prefix_groups():
     pages.truncate(1, 7)
     pages.extend([1, 1])
     assert pages.prefix().kv_len.tolist() == [4]
+
+
+def test_bounds():
+    _, pages = _grown([10, 3])
+    b = pages.extend([1, 2])
+    assert (b.max_q, b.max_kv) == (2, 11)
+    b = pages.extend([1, 0], max_q=1, max_kv=100)
+    assert (b.max_q, b.max_kv) == (1, 100)
+    for kw in (dict(max_q=0), dict(max_kv=11), dict(max_kv=101), dict(max_q=(1 << 30) + 1)):
+        with pytest.raises(ValueError, match="max_"):
+            pages.extend([1, 0], **kw)
+    assert pages.length(0) == 12
 
 
 def test_nothing_shared():
