@@ -189,9 +189,9 @@ __device__ inline int dealt(const Deal& d, int lead, int own) {
     return min(d.places - 1, max(1, static_cast<int>(d.places * x / (x + y) + 0.5f)));
 }
 
-// Workgroups of a CU.
-template <int D>
-constexpr int kBothWaves = D == 256 ? 1 : D == 64 ? 3 : 2;
+// Workgroups of a CU, as the registers allow: heads of 64 in 4 bits 85.0 us with three and 81.5 with four
+// (40 x 2 to 5 tokens behind four prefixes), in 8 bits 39.4 and 46.9 (4 behind 50000), with spills.
+constexpr int both_waves(int bits, int D) { return D == 256 ? 1 : D == 128 ? 2 : bits == 4 ? 4 : 3; }
 
 // Prefixes and what stands behind them in one launch, so that the former, many rows, which vector and matrix
 // instructions bound, run beside the latter, which reading the cache bounds: 64 tokens of 32 heads on 8 of
@@ -205,7 +205,7 @@ constexpr int kBothWaves = D == 256 ? 1 : D == 64 ? 3 : 2;
 constexpr int most_lead(int D) { return D == 128 ? 2 : 1; }
 
 template <int BITS, int D, int LEAD>
-__global__ __launch_bounds__(256, (kBothWaves<D>))
+__global__ __launch_bounds__(256, (both_waves(BITS, D)))
 void kv_both_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a, KvAttend la, Kept ok, Kept lk, Deal d) {
     __shared__ __align__(16) float few[4][192];
     const int lane = threadIdx.x & 63, wave = wave_id(), block = blockIdx.x;
@@ -395,7 +395,8 @@ Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D,
     const int64_t longest = std::max(rows, before);
     r.lead = longest <= 16 ? 0 : longest <= 64 ? 1 : r.few ? most_lead(D) : 2;
     r.waves = D == 256 && r.lead == 2 ? 8 : 4;
-    r.places = D == 256 ? 256 : r.few && D == 64 ? 768 : 512;
+    const int bits = (c.codes >> c.shift) * 8 / D;
+    r.places = 256 * (r.few ? both_waves(bits, D) : D == 256 ? 1 : 2);
     const int tile = r.lead ? 64 * r.lead : 16, own = r.few ? 16 : tile;
     if (r.waves == 8) r.lead = 1;
     // Numbers of tiles, of which first_tile leaves as many; steps are numbered with an int, also where
