@@ -70,8 +70,7 @@ constexpr float kHead = 9.0f, kSlack = 6.0f;
 constexpr float kHeadPart = 0x1p-9f;  // 2^-kHead
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Whether a batch's rows are only a part of their tokens': then what a kernel has of them is
-// always kept as a part.
+// Whether a batch's rows see only a part of their tokens in a pass.
 template <class B>
 constexpr bool kParts = !std::is_same<B, KvBatch>::value;
 
@@ -215,16 +214,14 @@ __device__ inline KvSeq lane_seq(const KvCache& c, const B& b, int s) {
 }
 
 // Tiles of sequence s, none past the last.
-template <class B>
-__device__ inline int tiles_of(const KvCache& c, const B& b, const KvAttend& a, const Plan& p,
+__device__ inline int tiles_of(const KvCache& c, const KvBatch& b, const KvAttend& a, const Plan& p,
                                int s) {
     return (lane_seq(c, b, s).q * a.G + p.tile - 1) / p.tile;
 }
 
 // The i-th tile of those that the sequences have, one sequence after the other; false past the
 // last.
-template <class B>
-__device__ inline bool tile_in_order(const KvCache& c, const B& b, const KvAttend& a,
+__device__ inline bool tile_in_order(const KvCache& c, const KvBatch& b, const KvAttend& a,
                                      const Plan& p, int i, int* seq, int* tile) {
     const int lane = threadIdx.x & 63;
     for (int x = 0; x < b.n_seq; x += 256) {
@@ -255,8 +252,7 @@ __device__ inline bool tile_in_order(const KvCache& c, const B& b, const KvAtten
 // The i-th tile of those that the sequences have, in the order of their numbers from each
 // sequence's end, then of the sequences; false past the last.  Tile numbers below t have
 // sum_s min(tiles_s, t) tiles, which is searched for i.
-template <class B>
-__device__ inline bool tile_at(const KvCache& c, const B& b, const KvAttend& a, const Plan& p,
+__device__ inline bool tile_at(const KvCache& c, const KvBatch& b, const KvAttend& a, const Plan& p,
                                int i, int* seq, int* tile) {
     const int lane = threadIdx.x & 63;
     const int first = tiles_of(c, b, a, p, lane);
@@ -292,8 +288,7 @@ __device__ inline bool tile_at(const KvCache& c, const B& b, const KvAttend& a, 
 }
 
 // A workgroup's tile of rows and part of their tokens.
-template <class B>
-__device__ inline Share share_of(const KvCache& c, const B& b, const KvAttend& a,
+__device__ inline Share share_of(const KvCache& c, const KvBatch& b, const KvAttend& a,
                                  const Plan& p, uint32_t block) {
     Share r;
     // Heads vary fastest (workgroups go round the 8 XCDs, whose L2 caches then
@@ -1050,7 +1045,8 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
 template <class X, int BITS, int D, int NC, int W>
 constexpr int ahead_of = 1;
 
-// A workgroup's share, x: the block of a launch or what share_of() and keep() else are overloaded for.
+// A workgroup's share: the block x of a launch, or what share_of() else is overloaded for, which then
+// keeps the rows itself.
 template <int BITS, int D, int NC, int W, class B, class X>
 __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a, const Plan& p,
                                  const X& x, h8 (&kf)[2][4 * Dim<BITS, D>::KS * 64],
@@ -1063,8 +1059,7 @@ __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a
     const Share w = share_of(c, b, a, p, x);
     if (!w.any) return;
     if (!w.s.ok) {
-        if constexpr (!kParts<B>)
-            if (w.split == 0) fail_rows<D>(w, a, threadIdx.x, 64 * W);
+        if (w.split == 0) fail_rows<D>(w, a, threadIdx.x, 64 * W);
         return;
     }
     if (w.split && w.lo >= w.hi) return;  // the join knows which parts there are
@@ -1173,28 +1168,28 @@ __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a
     if (w.lo < w.hi) stage(0, Zero());
     const bool uneven = __syncthreads_or(rows.uneven);
     auto step = [&](int j, int buf, auto uneven) {
-            const bool masked = j < w.full_lo || j + kStep > w.full_hi;
+        const bool masked = j < w.full_lo || j + kStep > w.full_hi;
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                f4 s[NC][2];
+        for (int hf = 0; hf < 2; hf++) {
+            f4 s[NC][2];
 #pragma unroll
-                for (int t = 0; t < 2; t++)
+            for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int q = 0; q < M::KS; q++) {
-                        const h8 x = kf[buf][((hf * 2 + t) * M::KS + q) * 64 + lane];
+                for (int q = 0; q < M::KS; q++) {
+                    const h8 x = kf[buf][((hf * 2 + t) * M::KS + q) * 64 + lane];
 #pragma unroll
-                        for (int k = 0; k < NC; k++)
-                            s[k][t] = mfma(x, rows.q[k][q], q ? s[k][t] : f4{0, 0, 0, 0});
-                    }
-                h8 pr[NC];
-                rows.weigh(s, sc[buf], lane, j, hf, masked, uneven, pr);
-#pragma unroll
-                for (int t = 0; t < M::DT; t++) {
-                    const h8 v = vf[buf][(hf * M::DT + t) * 64 + lane];
-#pragma unroll
-                    for (int k = 0; k < NC; k++) rows.o[k][t] = mfma(v, pr[k], rows.o[k][t]);
+                    for (int k = 0; k < NC; k++)
+                        s[k][t] = mfma(x, rows.q[k][q], q ? s[k][t] : f4{0, 0, 0, 0});
                 }
+            h8 pr[NC];
+            rows.weigh(s, sc[buf], lane, j, hf, masked, uneven, pr);
+#pragma unroll
+            for (int t = 0; t < M::DT; t++) {
+                const h8 v = vf[buf][(hf * M::DT + t) * 64 + lane];
+#pragma unroll
+                for (int k = 0; k < NC; k++) rows.o[k][t] = mfma(v, pr[k], rows.o[k][t]);
             }
+        }
     };
     // In parts, tiles may have few rows: waves without one only bring the others their operands.
     const bool rows_here = std::is_same<X, uint32_t>::value || r0 < w.r0 + w.rn;
@@ -1232,7 +1227,7 @@ __device__ inline void many_rows(const KvCache& c, const B& b, const KvAttend& a
         x.keep(w, a, r0, lane, rows);
         return;
     }
-    if (!kParts<B> && w.alone) return finish<BITS, D, NC>(w, a, r0, lane, rows);
+    if (w.alone) return finish<BITS, D, NC>(w, a, r0, lane, rows);
 #pragma unroll
     for (int k = 0; k < NC; k++) {
         const int row = r0 + k * 16 + r;
