@@ -401,3 +401,37 @@ def test_where_it_pays(gpu, new, P, seqs, G, pays):
     w.new, w.lens, w.kv = w.new[-1:], w.lens[-1:], w.kv[-1:]
     w.check(q[rows].cpu(), once[rows])
     w.check(q[rows].cpu(), alone[rows])
+
+
+def test_two_calls_at_once(gpu):
+    """On two streams, with a workspace each: each its own results, every time."""
+    import torch
+    w = Shared(gpu, [(900, [(1, 40 + i) for i in range(20)]), (300, [(2, 9)] * 3)], 2, 128, 8, 16, "bf16", seed=15)
+    b, p = w.batch(), w.prefix()
+    qs = [w.queries(8, seed=s).to(gpu) for s in (1, 2)]
+    want = [w.cache.attend(q, b, prefix=p, once=True) for q in qs]
+    n = w.cache.work_bytes(b, 8, prefix=p, once=True)
+    streams = [torch.cuda.Stream() for _ in qs]
+    works = [torch.empty(n, dtype=torch.uint8, device=gpu) for _ in qs]
+    outs = [[torch.zeros_like(q) for _ in range(10)] for q in qs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for i in range(10):
+        for q, s, x, o in zip(qs, streams, works, outs):
+            w.cache.attend(q, b, prefix=p, once=True, work=x, out=o[i], stream=s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, y) for os, y in zip(outs, want) for o in os)
+
+
+def test_a_workspace_inside_others(gpu):
+    """No byte outside the workspace is written, and every byte of it may be anything before."""
+    import torch
+    for groups, G in ((GROUPS["many_long"], 4), (GROUPS["few_short"], 1), (GROUPS["wide_chunks"], 4)):
+        w = Shared(gpu, groups, 2, 64, 8, 16, "f16", seed=16)
+        q = w.queries(2 * G).to(gpu)
+        b, p = w.batch(), w.prefix()
+        n = w.cache.work_bytes(b, 2 * G, prefix=p, once=True)
+        buf = torch.full((n + 512,), 0xff, dtype=torch.uint8, device=gpu)
+        out = w.cache.attend(q, b, prefix=p, once=True, work=buf[256:256 + n])
+        assert (buf[:256] == 0xff).all() and (buf[256 + n:] == 0xff).all()
+        w.check(q.cpu(), out)
