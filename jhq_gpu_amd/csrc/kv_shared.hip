@@ -268,14 +268,17 @@ __device__ inline Parts parts_of(const Kept& k, const KvSeq& s, int seq, int i, 
 
 // Joins what the passes have of a row; latency and reading the parts bound it.  A thread has 4
 // elements of every Y-th part: 2048 rows of 20 parts of 128 elements 9.9 us with 4, 10.2 with 2, 10.9 with 1,
-// 13.5 with 8.
+// 13.5 with 8.  Fewer rows have more parts each, and a workgroup of its own each; calls with workgroups of
+// several rows, of one, of one with 512 threads, us (32 heads on 8 of 128, 8 bits): 32 tokens behind 16000
+// (1024 rows) 43.0, 42.4, 46.5; 16 33.2, 31.9, 32.7; 4 behind 50000 45.4, 41.6, 40.4, on heads of 64 36.8,
+// 28.6, 27.9; 4 of 8 heads on 2 behind 100000 56.7, 41.1, 34.7.
 constexpr int kJoinWays = 4;
 constexpr int64_t join_rows(int D) { return 256 / (D / 4 * kJoinWays); }  // of a workgroup
 
-template <int D, int Y>
-__global__ __launch_bounds__(256) void kv_shared_join_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a,
+template <int D, int Y, int N>
+__global__ __launch_bounds__(N) void kv_shared_join_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a,
                                                              Kept lk, Kept ok) {
-    constexpr int T = D / 4, R = 256 / (T * Y);
+    constexpr int T = D / 4, R = N / (T * Y);
     constexpr int WR = 64 > Y * T ? 64 / (Y * T) : 1;  // rows of a wave
     __shared__ __align__(16) float acc[R][Y][D];
     __shared__ float ml[R][Y][2];
@@ -421,7 +424,6 @@ Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D,
 template <int BITS, int D>
 hipError_t launch(const KvCache& c, const KvBatch& lead, const KvBatch& b, const KvAttend& a,
                   const Both& ch, hipStream_t s) {
-    const int64_t joins = (ch.lk.rows + join_rows(D) - 1) / join_rows(D);
     KvLead lb;
     static_cast<KvBatch&>(lb) = lead;
     KvOwn ob;
@@ -453,7 +455,16 @@ hipError_t launch(const KvCache& c, const KvBatch& lead, const KvBatch& b, const
         go(kv_tiles_kernel<BITS, D, 2, 4>);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    kv_shared_join_kernel<D, kJoinWays><<<static_cast<unsigned>(joins), 256, 0, s>>>(c, ob, lb, a, ch.lk, ch.ok);
+    const int64_t rows = ch.lk.rows;
+    auto join = [&](auto kernel, int64_t blocks, int threads) {
+        kernel<<<static_cast<unsigned>(blocks), threads, 0, s>>>(c, ob, lb, a, ch.lk, ch.ok);
+    };
+    if (rows <= 128)
+        join(kv_shared_join_kernel<D, 2048 / D, 512>, rows, 512);
+    else if (rows <= 1024)
+        join(kv_shared_join_kernel<D, 1024 / D, 256>, rows, 256);
+    else
+        join(kv_shared_join_kernel<D, kJoinWays, 256>, (rows + join_rows(D) - 1) / join_rows(D), 256);
     return hipGetLastError();
 }
 
