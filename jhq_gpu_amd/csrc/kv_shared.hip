@@ -367,13 +367,14 @@ struct Both {
 };
 
 // Whether a prefix is read once, by estimates of both ways from the call's bounds (the longest prefix
-// stands for all): reading the cache at 5 TB/s or, over more rows than a wave takes for itself,
-// steps of tiles, whichever is longer; and for the passes' parts 9 us, 150 ns a sequence and, at 128
-// elements, 1.7 ns a row.  Measured, attention of every sequence and with the prefix read once, us (32 heads on
-// 8 of 128, 8 bits, up to 200 tokens of their own): single tokens, 64 behind 900 28.6 and 28.4, behind
-// 4000 65.5 and 37.0; 8 behind 4000 23.5 and 22.0, behind 16000 49.4 and 30.9; 3 behind 16000 25.8
-// and 28.9; chunks of up to 16, 12 behind 2000 31.5 and 43.6, behind 8000 89.6 and 68.2; of up to 80,
-// 32 behind 8000 543 and 501, behind 2000 178 and 256.
+// stands for all): reading the cache at 5 TB/s or, over more rows than a wave takes for itself, steps
+// of tiles, whichever is longer; and for the passes' parts 5.5 us, 150 ns a sequence and, at 128
+// elements, 1.7 ns a row.  Measured, attention of every sequence and with the prefix read once, us (32
+// heads on 8 of 128, 8 bits, up to 200 tokens of their own): single tokens, 64 behind 900 28.6 and
+// 28.4, behind 4000 65.5 and 37.0; 8 behind 2000 19.4 and 20.8, behind 4000 23.5 and 21.6, behind
+// 16000 48.6 and 30.0; 3 behind 4000 16.5 and 19.1, behind 8000 21.3 and 19.9; chunks of up to 16, 12
+// behind 2000 31.5 and 43.6, behind 8000 89.6 and 68.2; of up to 80, 32 behind 8000 543 and 501,
+// behind 2000 178 and 256.
 bool worth(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G) {
     const double step = (D == 64 ? 3.0 : D == 128 ? 5.0 : 15.0) * c.H * (lead.max_kv / kStep + 1);  // ns
     const double read = (2.0 * (c.codes >> c.shift) + 8) * c.H * lead.max_kv / 5000;
@@ -387,7 +388,7 @@ bool worth(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G
     const int groups = static_cast<int>(std::min<int64_t>(lead.n_seq, b.n_tokens));
     const double every = std::max(n * read, tiles(rows, n, rows <= 64 ? 64 : 128) * step);
     const double once = std::max(groups * read, tiles(before, groups, before <= 64 ? 64 : 128) * step);
-    return every > once + 9000 + 150.0 * n + 1.7 * D / 128 * all * c.H;
+    return every > once + 5500 + 150.0 * n + 1.7 * D / 128 * all * c.H;
 }
 
 Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D, int G, bool once, float* work) {

@@ -278,7 +278,7 @@ class KVCache:
         tokens of group g's sequences, kv_len[g] the tokens that they share (0: none), all before
         their new ones, pages[g] the pages of these (KVPages.prefix finds them).  No window then.
         Sequences that contradict their group may come out as NaN.  The bounds choose whether
-        prefixes are read once (from some 50 MB saved on, with single tokens); once=True has them
+        prefixes are read once (from some 35 MB saved on, with single tokens); once=True has them
         read once."""
         window = _window(window)
         if prefix is not None:
