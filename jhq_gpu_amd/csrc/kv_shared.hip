@@ -306,12 +306,16 @@ __global__ __launch_bounds__(N) void kv_shared_join_kernel(KvCache c, KvOwn b, K
         O = parts_of(ok, s, seq, static_cast<int>(i), h, c.H, a, D);
         const KvSeq w = kv_seq(lead, grp, c.shift);
         const int64_t li = tok - w.row;
-        if (tok >= lead.cu_q[grp] && tok < lead.cu_q[grp + 1]) {
-            good = w.ok && li < w.q;
-            if (good && w.n > 0) {
-                sees = true;
-                A = parts_of(lk, w, grp, static_cast<int>(li), h, c.H, a, D);
-            }
+        // What the sequence leaves out in front has to be what its row's group has read: a group with a prefix
+        // has whole sequences, not the end of one that begins before it.
+        if (tok >= lead.cu_q[grp] && tok < lead.cu_q[grp + 1])
+            good = w.ok && li < w.q && s.from == w.n &&
+                   (w.n == 0 || (s.row >= w.row && s.row + s.q <= w.row + w.q));
+        else
+            good = s.from == 0;
+        if (good && s.from) {
+            sees = true;
+            A = parts_of(lk, w, grp, static_cast<int>(li), h, c.H, a, D);
         }
     }
     float m = kNone, l = 0.0f;

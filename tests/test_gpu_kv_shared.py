@@ -435,3 +435,27 @@ def test_a_workspace_inside_others(gpu):
         out = w.cache.attend(q, b, prefix=p, once=True, work=buf[256:256 + n])
         assert (buf[:256] == 0xff).all() and (buf[256 + n:] == 0xff).all()
         w.check(q.cpu(), out)
+
+
+@pytest.mark.parametrize("new,G", [(3, 4), (40, 4)])
+def test_sequences_that_reach_into_a_group(gpu, new, G):
+    """A sequence that begins outside of a group with a prefix and has rows in it: these are NaN, whatever
+    stands in front of the group (a group without a prefix, or none); all other rows are as ever."""
+    import torch
+    w = Shared(gpu, [(0, [(new, 90)]), (64, [(1, 9), (2, 9)])], 2, 64, 8, 16, "f16", seed=17)
+    T = new + 3
+    q = w.queries(2 * G)
+    b, p = w.batch(), w.prefix()
+    first = ref.attend(_np(q[:new]).astype(np.float64), *w.kv[0], 64 ** -0.5, True, 0, ref.UNIT["f16"])
+    table = {0: [-1] * p.pages.shape[1], 64: p.pages[1].tolist()}
+    for cu, lens in (([0, new - 1, T], [0, 64]), ([1, T], [64]), ([0, 1, 2, T], [0, 64, 0])):
+        y = w.cache.batch(w.i32([table[n] for n in lens]), w.i32(lens), w.i32(cu), T, T, 64)
+        lse = torch.zeros(T, 2 * G, device=gpu)
+        out = w.cache.attend(q.to(gpu), b, prefix=y, lse=lse, once=True)
+        g = lens.index(64)
+        cut = np.array([cu[g] <= t < cu[g + 1] for t in range(new)])
+        assert torch.isnan(out[:new][cut]).all() and torch.isnan(lse[:new][cut]).all(), cu
+        o, l, tol, ltol = (x[~cut] for x in first)
+        assert (np.abs(_np(out[:new])[~cut] - o) <= tol).all(), cu
+        assert (np.abs(lse[:new].cpu().numpy()[~cut] - l) <= ltol).all(), cu
+        w.check(q, out, lse, skip=(0,))
