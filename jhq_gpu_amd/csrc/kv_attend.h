@@ -901,26 +901,37 @@ struct Cut {
     KvSeq s;
 };
 
-// Steps of all sequences, of which a head of s has steps(s).
+// The steps of all sequences, of which a head of s has steps(s), and what the sum has seen of the lane's
+// first sequence, which cut_at begins with.
+struct Total {
+    int sum, steps;
+    KvSeq s;
+};
+
 template <class B, class F>
-__device__ inline int all_steps(const KvCache& c, const B& b, int lane, F steps) {
-    int sum = steps(lane_seq(c, b, lane));
+__device__ inline Total all_steps(const KvCache& c, const B& b, int lane, F steps) {
+    Total r;
+    r.s = lane_seq(c, b, lane);
+    r.steps = steps(r.s);
+    int sum = r.steps;
     for (int s = lane + 64; s < b.n_seq; s += 64) sum += steps(lane_seq(c, b, s));
-    return wave_sum(sum) * c.H;
+    r.sum = wave_sum(sum) * c.H;
+    return r;
 }
 
-// The cut of worker's steps where each has `per` of `total`.
+// The cut of worker's steps where each has `per` of the total.
 template <class B, class F>
-__device__ inline Cut cut_at(const KvCache& c, const B& b, int total, int per, int worker, int lane, F steps) {
+__device__ inline Cut cut_at(const KvCache& c, const B& b, const Total& total, int per, int worker, int lane,
+                             F steps) {
     Cut r;
     r.per = per;
-    r.at = min(static_cast<int64_t>(worker) * r.per, static_cast<int64_t>(total));
-    r.end = min(r.at + r.per, total);
+    r.at = min(static_cast<int64_t>(worker) * r.per, static_cast<int64_t>(total.sum));
+    r.end = min(r.at + r.per, total.sum);
     if (r.at >= r.end) return r;
     int base = 0;
     for (int x = 0;; x += 64) {
-        const KvSeq s = lane_seq(c, b, x + lane);
-        const int n = steps(s);
+        const KvSeq s = x ? lane_seq(c, b, x + lane) : total.s;
+        const int n = x ? steps(s) : total.steps;
         int in = n;  // inclusive sum
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -970,8 +981,8 @@ __global__ __launch_bounds__(256, (kStreamWaves<D, NT>)) void kv_stream_kernel(K
         int lo, hi;
         return steps_of(s, a, &lo, &hi);
     };
-    const int total = all_steps(c, b, lane, steps);
-    const Cut cut = cut_at(c, b, total, max(kLeast, (total + (1 << p.log_workers) - 1) >> p.log_workers),
+    const Total total = all_steps(c, b, lane, steps);
+    const Cut cut = cut_at(c, b, total, max(kLeast, (total.sum + (1 << p.log_workers) - 1) >> p.log_workers),
                            worker, lane, steps);
     if (cut.at >= cut.end) return;
     int at = cut.at;

@@ -93,7 +93,11 @@ template <class B, class F>
 __device__ inline void each_tile(const KvCache& c, const B& b, const KvAttend& a, const Kept& k, int total,
                                  int workers, int least, int worker, int lane, bool first_lane, F f) {
     auto steps = [&](const KvSeq& s) { return tile_steps(b, s, a, k); };
-    const Cut cut = cut_at(c, b, total, max(least, (total + workers - 1) / workers), worker, lane, steps);
+    // Loaded anew: kept from both passes' sums, the lane's sequences cost registers (heads of 64 in 4 bits spill
+    // 10 in the place of 6).
+    const KvSeq s0 = lane_seq(c, b, lane);
+    const Cut cut = cut_at(c, b, Total{total, steps(s0), s0}, max(least, (total + workers - 1) / workers), worker,
+                           lane, steps);
     int at = cut.at;
     if (at >= cut.end) return;
     Share w;
@@ -209,8 +213,8 @@ __global__ __launch_bounds__(256, (both_waves(BITS, D)))
 void kv_both_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a, KvAttend la, Kept ok, Kept lk, Deal d) {
     __shared__ __align__(16) float few[4][192];
     const int lane = threadIdx.x & 63, wave = wave_id(), block = blockIdx.x;
-    const int lt = all_steps(c, lead, lane, [&](const KvSeq& s) { return tile_steps(lead, s, la, lk); });
-    const int ot = all_steps(c, b, lane, [&](const KvSeq& s) { return tile_steps(b, s, a, ok); });
+    const int lt = all_steps(c, lead, lane, [&](const KvSeq& s) { return tile_steps(lead, s, la, lk); }).sum;
+    const int ot = all_steps(c, b, lane, [&](const KvSeq& s) { return tile_steps(b, s, a, ok); }).sum;
     const int n = dealt(d, lt, ot);
     if (block >= n) {
         few_steps<BITS, D, 1>(c, b, a, ok, ot, (d.places - n) * 4, (block - n) * 4 + wave, lane, few[wave]);
@@ -232,8 +236,8 @@ __global__ __launch_bounds__(64 * W, W == 8 || D < 256 ? 2 : 1)
 void kv_tiles_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a, KvAttend la, Kept ok, Kept lk, Deal d) {
     JHQ_MANY_LDS(BITS, D, W);
     const int lane = threadIdx.x & 63, block = blockIdx.x;
-    const int lt = all_steps(c, lead, lane, [&](const KvSeq& s) { return tile_steps(lead, s, la, lk); });
-    const int ot = all_steps(c, b, lane, [&](const KvSeq& s) { return tile_steps(b, s, a, ok); });
+    const int lt = all_steps(c, lead, lane, [&](const KvSeq& s) { return tile_steps(lead, s, la, lk); }).sum;
+    const int ot = all_steps(c, b, lane, [&](const KvSeq& s) { return tile_steps(b, s, a, ok); }).sum;
     const int n = dealt(d, lt, ot);
     if (block < n)
         each_tile(c, lead, la, lk, lt, n, 1, block, lane, threadIdx.x == 0, [&](const Share& w, int64_t slot) {

@@ -337,3 +337,69 @@ def test_a_captured_step_is_replayed_as_sequences_grow(gpu):
         assert torch.equal(rope.apply(q, now), seen)
         assert torch.equal(cache.attend(seen, now), got)
     assert pages.length(1) == 51 and torch.isfinite(out).all()
+
+
+def test_a_captured_step_writes_where_extend_says(gpu):
+    """A captured step's replays against lists of rows: every token of every sequence as it reads back, keys
+    at the positions that they had when their replay ran, and attention over them.  Slots that nothing was
+    written into read as NaN."""
+    import torch
+    H, D, G, n_seq = 2, 64, 2, 3
+    cache = jg.KVCache(40, 16, H, D, device=gpu)
+    cache.data.fill_(0xff)
+    pages = jg.KVPages(cache, n_seq, 200)
+    rope = jg.Rotary(D, device=gpu)
+    gen = torch.Generator().manual_seed(6)
+    held = [[np.zeros((0, H, D))] * 2 for _ in range(n_seq)]
+
+    def rows(n, h):
+        return torch.randn(n, h, D, generator=gen).bfloat16().to(gpu)
+
+    plain = jg.KVCache(3, 16, H, D, device=gpu)
+
+    def hold(new, k, v):
+        """The rows as a cache holds them that they enter as one sequence, keys turned before, to positions
+        that are counted here."""
+        T = sum(new)
+        pos = np.concatenate([len(h[0]) + np.arange(a) for h, a in zip(held, new)])
+        b = plain.batch(_i32(gpu, [[2, 0, 1]]), _i32(gpu, [T]), _i32(gpu, [0, T]), T, T, T)
+        plain.write(rope.apply(k.float(), torch.from_numpy(pos).to(gpu)), v.float(), b)
+        at, kv = 0, [x.cpu().numpy() for x in plain.read(b)]
+        for h, a in zip(held, new):
+            h[:] = [np.concatenate([x, y[at:at + a]]) for x, y in zip(h, kv)]
+            at += a
+    k, v = rows(39, H), rows(39, H)
+    cache.write(k, v, pages.extend([30, 0, 9]), rotary=rope)
+    hold([30, 0, 9], k, v)
+    pages.fork(0, 1)
+    held[1] = list(held[0])
+    b = pages.extend([1, 1, 1], max_kv=200)
+    q, k, v = rows(3, H * G), rows(3, H), rows(3, H)
+    turned, out = torch.zeros_like(q), torch.zeros_like(q)
+    work = torch.zeros(cache.work_bytes(b, H * G), dtype=torch.uint8, device=gpu)
+
+    def step():
+        rope.apply(q, b, out=turned)
+        cache.write(k, v, b, rotary=rope)
+        cache.attend(turned, b, out=out, work=work)
+    step()
+    hold([1] * n_seq, k, v)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(20):  # over the end of a page, and of the page that two hold
+        pages.extend([1, 1, 1], max_kv=200)
+        for x, h in ((q, H * G), (k, H), (v, H)):
+            x.copy_(rows(3, h))
+        graph.replay()
+        hold([1] * n_seq, k, v)
+        got = out.clone()
+        at = torch.tensor([len(h[0]) - 1 for h in held], device=gpu)
+        assert torch.equal(rope.apply(q, at), turned)
+        for x, y in zip(cache.read(pages.everything()), zip(*held)):
+            assert np.array_equal(x.cpu().numpy(), np.concatenate(y))
+        for s in range(n_seq):
+            o, _, tol, _ = ref.attend(turned[s:s + 1].double().cpu().numpy(), *held[s], D ** -0.5,
+                                      unit=ref.UNIT["bf16"])
+            assert (np.abs(got[s:s + 1].double().cpu().numpy() - o) <= tol).all()
