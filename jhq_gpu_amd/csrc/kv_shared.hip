@@ -283,23 +283,14 @@ template <int D, int Y, int N>
 __global__ __launch_bounds__(N) void kv_shared_join_kernel(KvCache c, KvOwn b, KvLead lead, KvAttend a,
                                                              Kept lk, Kept ok) {
     constexpr int T = D / 4, R = N / (T * Y);
-    constexpr int WR = 64 > Y * T ? 64 / (Y * T) : 1;  // rows of a wave
+    static_assert(Y > 1 && T * Y % 64 == 0, "a wave's threads have one row");
     __shared__ __align__(16) float acc[R][Y][D];
     __shared__ float ml[R][Y][2];
     const int t = threadIdx.x % T, y = threadIdx.x / T % Y, r = threadIdx.x / (Y * T);
-    const int x = blockIdx.x * R + r;
+    const int x = blockIdx.x * R + __builtin_amdgcn_readfirstlane(r);
     const int tok = x / a.heads, h = x - tok * a.heads;
-    int seq = 0, grp = 0;
-    const int first = __builtin_amdgcn_readfirstlane(x);
-#pragma unroll
-    for (int k = 0; k < WR; k++) {
-        // a wave's rows are mostly one token's
-        const int mine = (first + k) / a.heads;
-        if (k && mine == (first + k - 1) / a.heads) continue;
-        const int s = last_at_most(b.n_seq, mine, [&](int j) { return b.cu_q[j]; });
-        const int g = last_at_most(lead.n_seq, mine, [&](int j) { return lead.cu_q[j]; });
-        if (mine <= tok) seq = s, grp = g;
-    }
+    const int seq = last_at_most(b.n_seq, tok, [&](int j) { return b.cu_q[j]; });
+    const int grp = last_at_most(lead.n_seq, tok, [&](int j) { return lead.cu_q[j]; });
     const KvSeq s = kv_seq(b, seq, c.shift);
     const int64_t i = tok - s.row;
     const bool has = x < lk.rows && i >= 0 && i < s.q;
@@ -337,24 +328,22 @@ __global__ __launch_bounds__(N) void kv_shared_join_kernel(KvCache c, KvOwn b, K
         for (int e = 0; e < 4; e++) o[e] = fmaf(o[e], f0, v[e] * f1);
         m = big;
     }
-    if constexpr (Y > 1) {
-        *reinterpret_cast<f4*>(acc[r][y] + t * 4) = o;
-        if (t == 0) {
-            ml[r][y][0] = m;
-            ml[r][y][1] = l;
-        }
-        __syncthreads();
-        if (y) return;
-        l = 0.0f;
-        o = f4{0, 0, 0, 0};
+    *reinterpret_cast<f4*>(acc[r][y] + t * 4) = o;
+    if (t == 0) {
+        ml[r][y][0] = m;
+        ml[r][y][1] = l;
+    }
+    __syncthreads();
+    if (y) return;
+    l = 0.0f;
+    o = f4{0, 0, 0, 0};
 #pragma unroll
-        for (int z = 0; z < Y; z++) m = fmaxf(m, ml[r][z][0]);
+    for (int z = 0; z < Y; z++) m = fmaxf(m, ml[r][z][0]);
 #pragma unroll
-        for (int z = 0; z < Y; z++) {
-            const float f = __builtin_amdgcn_exp2f(ml[r][z][0] - m);
-            l = fmaf(ml[r][z][1], f, l);
-            o += *reinterpret_cast<const f4*>(acc[r][z] + t * 4) * f;
-        }
+    for (int z = 0; z < Y; z++) {
+        const float f = __builtin_amdgcn_exp2f(ml[r][z][0] - m);
+        l = fmaf(ml[r][z][1], f, l);
+        o += *reinterpret_cast<const f4*>(acc[r][z] + t * 4) * f;
     }
     if (!has) return;
     const int64_t row = static_cast<int64_t>(tok) * a.heads + h;
