@@ -100,27 +100,36 @@ class KVPages:
                 split.append(int(s))
                 refs[page] = left - 1
         self._need(int(grow.sum()) + len(split))
-        src, dst = [], []
+        src, dst, taken = [], [], []
         for s in split:
             at = self._len[s] // P
-            page = int(self._table[s, at])
-            mine = self._take()
-            src.append(page)
-            dst.append(mine)
-            self._refs[page] -= 1
-            self._table[s, at] = mine
+            src.append(int(self._table[s, at]))
+            dst.append(self._take())
+            self._refs[src[-1]] -= 1
+            self._table[s, at] = dst[-1]
         for s in np.nonzero(grow)[0]:
             held = self._held(s)
             for i in range(held, held + int(grow[s])):
-                self._table[s, i] = self._take()
-        self._dirty |= bool(src) or bool(grow.any())
+                taken.append(self._take())
+                self._table[s, i] = taken[-1]
+        self._dirty |= bool(src) or bool(taken)
+        try:
+            with self._on(stream):
+                if src:
+                    pairs = self._to_device(np.array([src, dst], np.int32))
+                    self.cache.copy_pages(pairs[0], pairs[1])
+                self._upload(to, new)
+            batch = self.cache.batch(self._pages, self._kv_len, self._cu, int(new.sum()), *bounds)
+        except BaseException:
+            # no memory, or a launch that failed: sequences and pages are as before, the device's arrays may not be
+            for s, page in zip(split, src):
+                self._table[s, self._len[s] // P] = page
+                self._refs[page] += 1
+            self._release(np.array(dst + taken, np.int64))
+            self._dirty, self._fresh = True, False
+            raise
         self._len, self._new, self._fresh = to, new, True
-        with self._on(stream):
-            if src:
-                pairs = self._to_device(np.array([src, dst], np.int32))
-                self.cache.copy_pages(pairs[0], pairs[1])
-            self._upload()
-        return self.cache.batch(self._pages, self._kv_len, self._cu, int(new.sum()), *bounds)
+        return batch
 
     def fork(self, src, dst):
         """Sequence dst, which is empty, begins with all tokens of src, in the same pages."""
@@ -296,8 +305,8 @@ class KVPages:
     def _to_device(self, a):
         return self._host(a).to(self.cache.device, non_blocking=True)
 
-    def _upload(self):
-        head = np.concatenate([self._len, [0], np.cumsum(self._new)]).astype(np.int32)
+    def _upload(self, lens, new):
+        head = np.concatenate([lens, [0], np.cumsum(new)]).astype(np.int32)
         a = np.concatenate([head, self._table.reshape(-1)]) if self._dirty else head
         self._dev[:a.size].copy_(self._host(a), non_blocking=True)
         self._dirty = False

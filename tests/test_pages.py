@@ -284,3 +284,66 @@ def test_the_copies_refuse():
     err(L.jhq_k_kv_copy(o, F, F, p, F, b, None), "other bits")
     err(L.jhq_k_kv_copy(p, F, None, p, F, b, None), "null slots")
     err(L.jhq_k_kv_copy(None, F, F, p, F, b, None), "null parameters")
+
+
+class Failing(Cache):
+    """A cache whose calls named in `fail` raise, as they do where there is no memory."""
+    fail = ()
+
+    def batch(self, *a):
+        if "batch" in self.fail:
+            raise MemoryError("batch")
+        return super().batch(*a)
+
+    def copy_pages(self, src, dst):
+        if "copy_pages" in self.fail:
+            raise MemoryError("copy_pages")
+        super().copy_pages(src, dst)
+
+    def copy(self, slots, b):
+        if "copy" in self.fail:
+            raise MemoryError("copy")
+        super().copy(slots, b)
+
+
+def _failing(lens, num_pages=60, forks=()):
+    cache = Failing(num_pages)
+    pages = jg.KVPages(cache, len(lens), 100)
+    b = pages.extend(lens)
+    cache.write(list(range(sum(lens))), b)
+    for a, d in forks:
+        pages.fork(a, d)
+    return cache, pages
+
+
+def _model(lens, forks=()):
+    at = np.concatenate([[0], np.cumsum(lens)])
+    model = [list(range(a, b)) for a, b in zip(at[:-1], at[1:])]
+    for a, d in forks:
+        model[d] = list(model[a])
+    return model
+
+
+@pytest.mark.parametrize("fail", ["copy_pages", "batch", "upload"])
+def test_an_extend_that_fails_changes_nothing(fail, monkeypatch):
+    lens, forks = [10, 0, 0, 7], [(0, 1), (0, 2)]
+    cache, pages = _failing(lens, forks=forks)
+    model = _model(lens, forks)
+    before = (pages._table.copy(), pages._refs.copy(), pages._len.copy(), sorted(pages._free))
+    with monkeypatch.context() as m:
+        if fail == "upload":
+            m.setattr(pages, "_upload", lambda *a: (_ for _ in ()).throw(MemoryError("upload")))
+        cache.fail = (fail,)
+        with pytest.raises(MemoryError):
+            pages.extend([1, 9, 1, 30])
+    cache.fail = ()
+    held = [pages.pages_of(s) for s in range(4)]
+    assert held == [before[0][s, :-(-len(m) // 4)].tolist() for s, m in enumerate(model)]
+    for x, y in zip(before[1:], (pages._refs, pages._len, sorted(pages._free))):
+        assert np.array_equal(x, y)
+    _check(pages, cache, model)
+    b = pages.extend([1, 9, 1, 30])
+    cache.write(list(range(100, 141)), b)
+    for m, x in zip(model, np.split(np.arange(100, 141), [1, 10, 11])):
+        m += x.tolist()
+    _check(pages, cache, model)
