@@ -21,6 +21,13 @@ from . import kv as _kv
 __all__ = ["KVPages"]
 
 
+class _Move:
+    """What compact does with a sequence: the tokens `at` stay, moved together from page `stay` on."""
+
+    def __init__(self, seq, at, stay):
+        self.seq, self.at, self.stay = seq, at, stay
+
+
 class KVPages:
     """The pages of `cache` (which nothing else may give out) and the sequences 0 .. n_seq - 1 that
     hold them, of up to max_tokens tokens each.  Which page is whose is the host's
@@ -173,41 +180,62 @@ class KVPages:
             if at.size and (at[0] < 0 or at[-1] >= self._len[s] or (np.diff(at) <= 0).any()):
                 raise ValueError(f"sequence {s}: positions must ascend within its {int(self._len[s])} tokens")
             moved = np.nonzero(at != np.arange(at.size))[0]
-            if moved.size == 0:  # a beginning: no token moves
-                plan.append((s, at, -1))
-                continue
-            plan.append((s, at, int(moved[0]) // P))
-        if len({s for s, _, _ in plan}) != len(plan):
+            # pages in front that stay: of a beginning, where no token moves, all that it fills
+            plan.append(_Move(s, at, int(moved[0]) // P if moved.size else -(-at.size // P)))
+        if len({m.seq for m in plan}) != len(plan):
             raise ValueError("a sequence is named twice")
-        moves = [(s, at, stay) for s, at, stay in plan if stay >= 0]
-        self._need(sum(-(-at.size // P) - stay for s, at, stay in moves))
-        slots, old = [], []
-        for s, at, stay in moves:
-            held = self._held(s)
-            rest = at[stay * P:]
-            slots.append(self._table[s, rest // P].astype(np.int64) * P + rest % P)
-            old.append(self._table[s, stay:held].copy())
-            for i in range(stay, -(-at.size // P)):
-                self._table[s, i] = self._take()
-            self._len[s] = at.size
-        if moves:
-            self._dirty, self._fresh = True, False
-            rows = [s for s, _, _ in moves]
-            lens = self._len[rows]
-            new = np.array([x.size for x in slots], np.int64)
-            width = max(1, int((-(-lens // P)).max()))
-            n = len(rows)
-            arrays = np.concatenate([lens, [0], np.cumsum(new), self._table[rows, :width].reshape(-1)])
+        # everything that can fail comes before what changes this object
+        free, refs = list(self._free), self._refs.copy()
+        rounds = self._rounds(plan, free, refs)
+        if rounds:
             with self._on(stream):
-                dev = self._to_device(arrays.astype(np.int32))
-                batch = self.cache.batch(dev[2 * n + 1:].view(n, width), dev[:n], dev[n:2 * n + 1],
-                                         int(new.sum()), int(new.max()), int(lens.max()))
-                self.cache.copy(self._to_device(np.concatenate(slots)), batch)
-            for pages in old:
-                self._release(pages)
-        for s, at, stay in plan:
-            if stay < 0:
-                self.truncate(s, at.size)
+                for slots, batch in self._copies(rounds):
+                    self.cache.copy(slots, batch)
+        self._free, self._refs = free, refs
+        for m in plan:
+            self._table[m.seq, m.stay:m.stay + len(m.to)] = m.to
+            self._len[m.seq] = m.at.size
+            self._fresh = False
+        self._dirty |= bool(rounds)
+
+    def _rounds(self, plan, free, refs):
+        """Gives the moves pages out of `free` and gives back what they leave; returns the copy that this
+        takes: [(move, first new page, end), ..], where there is one."""
+        P, copies = self.page_size, []
+        self._need(sum(-(-m.at.size // P) - m.stay for m in plan))
+        for m in plan:
+            m.to = [heapq.heappop(free) for _ in range(-(-m.at.size // P) - m.stay)]
+            refs[m.to] = 1
+            if m.to:
+                copies.append((m, 0, len(m.to)))
+        for m in plan:
+            for page in self._table[m.seq, m.stay:self._held(m.seq)].tolist():
+                refs[page] -= 1
+                if refs[page] == 0:
+                    heapq.heappush(free, page)
+        return [copies] if copies else []
+
+    def _copies(self, rounds):
+        """(slots, batch) of each round, all on the device before the first is copied.  A batch's sequences are
+        what fills the new pages alone: where these stand in their sequence does not matter to a copy."""
+        P, arrays, slots, cuts = self.page_size, [], [], []
+        for copies in rounds:
+            n, width = len(copies), max(b - a for _, a, b in copies)
+            table, new = np.zeros((n, width), np.int64), np.zeros(n, np.int64)
+            for i, (m, a, b) in enumerate(copies):
+                at = m.at[(m.stay + a) * P:(m.stay + b) * P]
+                slots.append(self._table[m.seq, at // P].astype(np.int64) * P + at % P)
+                table[i, :b - a], new[i] = m.to[a:b], at.size
+            arrays.append(np.concatenate([new, [0], np.cumsum(new), table.reshape(-1)]))
+            cuts.append((n, width, int(new.sum()), int(new.max())))
+        dev, slots = self._to_device(np.concatenate(arrays).astype(np.int32)), self._to_device(np.concatenate(slots))
+        out = []
+        for n, width, total, most in cuts:
+            end = 2 * n + 1 + n * width
+            out.append((slots[:total], self.cache.batch(dev[2 * n + 1:end].view(n, width), dev[:n],
+                                                        dev[n:2 * n + 1], total, most, most)))
+            dev, slots = dev[end:], slots[total:]
+        return out
 
     def prefix(self, least=1, stream=None):
         """What attend takes as `prefix` beside the batch that extend returned last: neighbouring

@@ -347,3 +347,26 @@ def test_an_extend_that_fails_changes_nothing(fail, monkeypatch):
     for m, x in zip(model, np.split(np.arange(100, 141), [1, 10, 11])):
         m += x.tolist()
     _check(pages, cache, model)
+
+
+@pytest.mark.parametrize("fail", ["copy", "batch", "upload"])
+def test_a_compaction_that_fails_changes_nothing(fail, monkeypatch):
+    lens, forks = [30, 0, 9, 6], [(0, 1)]
+    cache, pages = _failing(lens, forks=forks)
+    model = _model(lens, forks)
+    keep = {0: list(range(1, 30, 2)), 2: [0, 1, 5, 8], 3: [0, 1]}
+    before = (pages._table.copy(), pages._refs.copy(), pages._len.copy(), list(pages._free))
+    with monkeypatch.context() as m:
+        if fail == "upload":
+            m.setattr(pages, "_to_device", lambda *a: (_ for _ in ()).throw(MemoryError("upload")))
+        cache.fail = (fail,)
+        with pytest.raises(MemoryError):
+            pages.compact(keep)
+    cache.fail = ()
+    for x, y in zip(before, (pages._table, pages._refs, pages._len, pages._free)):
+        assert np.array_equal(x, y)
+    _check(pages, cache, model)
+    pages.compact(keep)
+    for s, at in keep.items():
+        model[s] = [model[s][i] for i in at]
+    _check(pages, cache, model)
