@@ -170,7 +170,10 @@ class KVPages:
         moved together; keys stay as they are, turned to the positions that they had (so tokens that
         come after are turned to positions of their own too: Rotary.apply with a tensor of them).
         Whole pages in front that keep all of their tokens stay; the others' tokens are
-        copied into free pages, of which there have to be as many as they fill."""
+        copied into free pages.  Where there are not as many as they fill, pages that have
+        become empty take what follows, in several copies: pages that keep nothing at once, and one free page is
+        enough where nobody else holds the rest.  (Between two of them an error of the device loses what was
+        moved; any other leaves everything as it was.)"""
         P, plan = self.page_size, []
         for s, at in keep.items():
             s, at = self._seq(s), np.asarray(at)
@@ -199,21 +202,50 @@ class KVPages:
         self._dirty |= bool(rounds)
 
     def _rounds(self, plan, free, refs):
-        """Gives the moves pages out of `free` and gives back what they leave; returns the copy that this
-        takes: [(move, first new page, end), ..], where there is one."""
-        P, copies = self.page_size, []
-        self._need(sum(-(-m.at.size // P) - m.stay for m in plan))
-        for m in plan:
-            m.to = [heapq.heappop(free) for _ in range(-(-m.at.size // P) - m.stay)]
-            refs[m.to] = 1
-            if m.to:
-                copies.append((m, 0, len(m.to)))
-        for m in plan:
-            for page in self._table[m.seq, m.stay:self._held(m.seq)].tolist():
+        """Gives the moves pages out of `free` and gives back what they leave; returns the copies that this
+        takes, one after the other: lists of (move, first new page, end).  A copy's pages are read by no
+        move that is not done."""
+        P = self.page_size
+        need = sum(-(-m.at.size // P) - m.stay for m in plan)
+
+        def release(pages):
+            for page in pages.tolist():
                 refs[page] -= 1
                 if refs[page] == 0:
                     heapq.heappush(free, page)
-        return [copies] if copies else []
+        for m in plan:
+            m.old = self._table[m.seq, m.stay:self._held(m.seq)]
+            m.to, m.left = [], 0
+        enough = need <= len(free)
+        if not enough:  # what gives back most, for what it takes, first
+            plan = sorted(plan, key=lambda m: -(-m.at.size // P) - m.stay - int((refs[m.old] == 1).sum()))
+            for m in plan:
+                # how many new pages are full when an old one is empty
+                upto = np.searchsorted(m.at, (m.stay + np.arange(len(m.old) + 1)) * P)
+                m.after = np.where(upto[1:] > upto[:-1], -(-upto[1:] // P) - m.stay, 0)
+        rounds = []
+        while True:
+            if not enough:
+                for m in plan:
+                    done = m.after <= len(m.to)
+                    release(m.old[done])
+                    m.old, m.after = m.old[~done], m.after[~done]
+            copies = []
+            for m in plan:
+                k, at = min(len(free), -(-m.at.size // P) - m.stay - len(m.to)), len(m.to)
+                for _ in range(k):
+                    m.to.append(heapq.heappop(free))
+                    refs[m.to[-1]] = 1
+                if k:
+                    copies.append((m, at, at + k))
+            if not copies:
+                break
+            rounds.append(copies)
+        if sum(len(m.to) for m in plan) < need:
+            raise RuntimeError(f"the cache is full: {need} pages are needed, {len(self._free)} are free")
+        for m in plan:
+            release(m.old)
+        return rounds
 
     def _copies(self, rounds):
         """(slots, batch) of each round, all on the device before the first is copied.  A batch's sequences are

@@ -403,3 +403,24 @@ def test_a_captured_step_writes_where_extend_says(gpu):
             o, _, tol, _ = ref.attend(turned[s:s + 1].double().cpu().numpy(), *held[s], D ** -0.5,
                                       unit=ref.UNIT["bf16"])
             assert (np.abs(got[s:s + 1].double().cpu().numpy() - o) <= tol).all()
+
+
+@pytest.mark.parametrize("bits,D,H", [(8, 128, 2), (4, 64, 3)])
+def test_compaction_in_a_full_cache(gpu, bits, D, H):
+    """In as many copies as the pages that become empty ask for: rows read back as they were."""
+    import torch
+    lens = [600, 333, 50]
+    rng = np.random.default_rng(D)
+    for keep, spare in (([np.arange(300, 600), np.arange(0, 333, 2), np.arange(50)], 0),
+                        ([np.arange(1, 600), np.sort(rng.choice(333, 300, replace=False)), np.arange(20)], 1),
+                        ([np.sort(rng.choice(600, 200, replace=False)), np.arange(3, 333), np.arange(1, 50)], 3)):
+        cache = jg.KVCache(sum(-(-n // 16) for n in lens) + spare, 16, H, D, bits=bits, device=gpu)
+        cache.data.fill_(0xff)
+        pages = jg.KVPages(cache, 3, 700)
+        k, v = torch.randn(2, sum(lens), H, D, generator=torch.Generator().manual_seed(D)).bfloat16().unbind(0)
+        cache.write(k.to(gpu), v.to(gpu), pages.extend(lens))
+        before = cache.read(pages.everything())
+        pages.compact(dict(enumerate(keep)))
+        rows = torch.from_numpy(np.concatenate([a + n for a, n in zip(keep, (0, 600, 933))])).to(gpu)
+        for x, y in zip(before, cache.read(pages.everything())):
+            assert torch.equal(x[rows], y)

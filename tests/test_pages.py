@@ -370,3 +370,66 @@ def test_a_compaction_that_fails_changes_nothing(fail, monkeypatch):
     for s, at in keep.items():
         model[s] = [model[s][i] for i in at]
     _check(pages, cache, model)
+
+
+def _compacted(lens, keep, num_pages, forks=()):
+    cache, pages = _grown(lens, num_pages, forks)
+    model = _model(lens, forks)
+    pages.compact(keep)
+    for s, at in keep.items():
+        model[s] = [model[s][i] for i in at]
+    _check(pages, cache, model)
+    return pages
+
+
+def test_compaction_in_a_full_cache():
+    """Pages that keep nothing take what follows; without one, one free page is enough, over and over."""
+    whole = list(range(32, 64))
+    assert _compacted([64], {0: whole}, 16).free_pages == 8
+    assert _compacted([40, 40], {0: range(20, 40), 1: range(1, 40)}, 20).free_pages == 5
+    # every page keeps something, one page is free
+    assert _compacted([60], {0: np.arange(1, 60)}, 16).free_pages == 1
+    assert _compacted([60], {0: np.arange(0, 60, 2)}, 16).free_pages == 8
+    assert _compacted([28, 28], {0: np.arange(1, 28, 3), 1: np.arange(28)[np.arange(28) % 4 > 0]}, 15).free_pages == 6
+    # what one sequence gives back serves the next, and what is only cut off serves both
+    assert _compacted([30, 30, 0], {0: np.arange(20, 30), 1: np.arange(4, 30, 2)}, 17, forks=[(0, 2)]).free_pages == 2
+    assert _compacted([30, 30], {0: np.arange(1, 30), 1: np.arange(3)}, 16).free_pages == 7
+
+
+def test_a_compaction_that_finds_no_page_changes_nothing():
+    for num_pages, lens, keep, forks in ((15, [60], {0: np.arange(1, 60)}, []),
+                                         (8, [30, 0], {0: np.arange(1, 30)}, [(0, 1)]),
+                                         (12, [30, 0], {0: np.arange(1, 30)}, [(0, 1)]),
+                                         # 8 for what another holds too, 1 + 4 are to be had
+                                         (17, [30, 30, 0], {0: np.arange(1, 30), 1: np.arange(4, 30, 2)}, [(0, 2)])):
+        cache, pages = _grown(lens, num_pages, forks)
+        before = (pages._table.copy(), pages._refs.copy(), pages._len.copy(), list(pages._free))
+        with pytest.raises(RuntimeError, match="full"):
+            pages.compact(keep)
+        for x, y in zip(before, (pages._table, pages._refs, pages._len, pages._free)):
+            assert np.array_equal(x, y)
+        _check(pages, cache, _model(lens, forks))
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_compaction_with_few_free_pages(seed):
+    """Against lists: whatever is shared, with as many pages as are held and a few more."""
+    rng = np.random.default_rng(seed)
+    lens = [int(x) for x in rng.integers(0, 60, 5)]
+    lens[4] = 0
+    forks = [(int(rng.integers(0, 4)), 4)] if rng.random() < 0.6 else []
+    held = sum(-(-n // 4) for n in lens)
+    cache, pages = _grown(lens, max(1, held) + int(rng.integers(0, 3)), forks)
+    model = _model(lens, forks)
+    for _ in range(3):
+        keep = {s: np.nonzero(rng.random(len(m)) < rng.choice([0.1, 0.5, 0.9, 1.0]))[0]
+                for s, m in enumerate(model) if rng.random() < 0.7}
+        try:
+            pages.compact(keep)
+        except RuntimeError:
+            # only pages that others hold, or no free one at all, stand in the way
+            assert forks or pages.free_pages == 0
+        else:
+            for s, at in keep.items():
+                model[s] = [model[s][i] for i in at]
+        _check(pages, cache, model)
