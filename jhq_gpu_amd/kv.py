@@ -23,6 +23,9 @@ __all__ = ["KVCache", "KVBatch"]
 JHQ_BF16, JHQ_F16 = 3, 4
 
 
+_MOVED = ("tokens of the batch's sequences have been moved (KVPages.compact), so that new ones' places are not their "
+          "positions: turn them with Rotary.apply and a tensor of positions")
+
 _DTYPES = {}  # torch type -> element type, filled when torch is first needed
 
 
@@ -67,7 +70,12 @@ class KVBatch:
     tokens, token j in page pages[b, j // page_size]; its last
     cu_q[b+1] - cu_q[b] tokens are new, rows cu_q[b] .. of k, v and q.
     n_tokens rows in all; max_q and max_kv bound one sequence's new tokens and
-    tokens.  Build it with KVCache.batch."""
+    tokens.  Build it with KVCache.batch.
+
+    moved: whether a sequence holds its tokens elsewhere than at their positions
+    (KVPages.compact has moved them), so that nothing is turned to the batch's positions."""
+
+    moved = False
 
     def __init__(self, device, page_size, pages, kv_len, cu_q, n_tokens, max_q, max_kv):
         torch = _torch()
@@ -175,7 +183,7 @@ class KVCache:
         """Quantises the batch's new tokens into the cache: k, v [n_tokens,
         kv_heads, head_dim], float32, bfloat16 or float16, any strides between
         rows.  rotary: a Rotary that turns the keys to their tokens' positions on the
-        way, in float32."""
+        way, in float32 (not where tokens of a sequence have been moved)."""
         dt, kt, kh = self._rows(k, "k", self.kv_heads, batch)
         dv, vt, vh = self._rows(v, "v", self.kv_heads, batch)
         if dt != dv:
@@ -185,6 +193,8 @@ class KVCache:
             return
         if rotary._index != self._index:
             raise ValueError(f"the rotary is on {rotary.device}, the cache on {self.device}")
+        if batch.moved:
+            raise ValueError(_MOVED)
         self._call(self._write_rotary, stream, batch, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, dt,
                    rotary._ref)
 

@@ -20,12 +20,15 @@ from . import kv as _kv
 
 __all__ = ["KVPages"]
 
+_NONE = 1 << 62
+
 
 class _Move:
-    """What compact does with a sequence: the tokens `at` stay, moved together from page `stay` on."""
+    """What compact does with a sequence: the tokens `at` stay, moved together from page `stay` on, of which
+    the first that moves is the one that becomes token `moved`."""
 
-    def __init__(self, seq, at, stay):
-        self.seq, self.at, self.stay = seq, at, stay
+    def __init__(self, seq, at, stay, moved):
+        self.seq, self.at, self.stay, self.moved = seq, at, stay, moved
 
 
 class KVPages:
@@ -54,6 +57,8 @@ class KVPages:
         self._table = np.zeros((n_seq, self._width), np.int32)
         self._len = np.zeros(n_seq, np.int64)
         self._new = np.zeros(n_seq, np.int64)
+        # the first token that compact has moved: from it on, places are not positions
+        self._moved = np.full(n_seq, _NONE, np.int64)
         # lengths, first rows, page table: one array, so that one copy brings them
         head = 2 * n_seq + 1
         self._dev = torch.zeros(head + self._table.size, dtype=torch.int32, device=cache.device)
@@ -135,6 +140,7 @@ class KVPages:
             self._release(np.array(dst + taken, np.int64))
             self._dirty, self._fresh = True, False
             raise
+        batch.moved = bool(((new > 0) & (self._moved < self._len)).any())
         self._len, self._new, self._fresh = to, new, True
         return batch
 
@@ -147,7 +153,7 @@ class KVPages:
         held = self._held(src)
         self._table[dst, :held] = self._table[src, :held]
         np.add.at(self._refs, self._table[src, :held], 1)
-        self._len[dst] = self._len[src]
+        self._len[dst], self._moved[dst] = self._len[src], self._moved[src]
         self._dirty |= held > 0
         self._fresh = False
 
@@ -159,6 +165,8 @@ class KVPages:
         first, held = -(-n // self.page_size), self._held(seq)
         self._release(self._table[seq, first:held])
         self._len[seq] = n
+        if n <= self._moved[seq]:
+            self._moved[seq] = _NONE
         self._fresh = False
 
     def free(self, seq):
@@ -167,8 +175,9 @@ class KVPages:
 
     def compact(self, keep, stream=None):
         """keep: {sequence: ascending positions}.  Each of these sequences keeps those of its tokens,
-        moved together; keys stay as they are, turned to the positions that they had (so tokens that
-        come after are turned to positions of their own too: Rotary.apply with a tensor of them).
+        moved together; keys stay as they are, turned to the positions that they had, so tokens that
+        come after are turned to positions of their own too: Rotary.apply with a tensor of them
+        (it and write(rotary=) refuse a batch of such sequences, whose positions are not their places).
         Whole pages in front that keep all of their tokens stay; the others' tokens are
         copied into free pages.  Where there are not as many as they fill, pages that have
         become empty take what follows, in several copies: pages that keep nothing at once, and one free page is
@@ -184,7 +193,8 @@ class KVPages:
                 raise ValueError(f"sequence {s}: positions must ascend within its {int(self._len[s])} tokens")
             moved = np.nonzero(at != np.arange(at.size))[0]
             # pages in front that stay: of a beginning, where no token moves, all that it fills
-            plan.append(_Move(s, at, int(moved[0]) // P if moved.size else -(-at.size // P)))
+            plan.append(_Move(s, at, int(moved[0]) // P if moved.size else -(-at.size // P),
+                              int(moved[0]) if moved.size else at.size))
         if len({m.seq for m in plan}) != len(plan):
             raise ValueError("a sequence is named twice")
         # everything that can fail comes before what changes this object
@@ -197,6 +207,9 @@ class KVPages:
         self._free, self._refs = free, refs
         for m in plan:
             self._table[m.seq, m.stay:m.stay + len(m.to)] = m.to
+            # what was moved before, and what is now
+            moved = min(int(np.searchsorted(m.at, self._moved[m.seq])), m.moved)
+            self._moved[m.seq] = moved if moved < m.at.size else _NONE
             self._len[m.seq] = m.at.size
             self._fresh = False
         self._dirty |= bool(rounds)
@@ -315,8 +328,10 @@ class KVPages:
         n = self.n_seq
         with self._on(stream):
             dev = self._to_device(arrays.astype(np.int32))
-        return self.cache.batch(dev[2 * n + 1:].view(n, self._width), dev[:n], dev[n:2 * n + 1],
-                                int(self._len.sum()), int(self._len.max()), int(self._len.max()))
+        batch = self.cache.batch(dev[2 * n + 1:].view(n, self._width), dev[:n], dev[n:2 * n + 1],
+                                 int(self._len.sum()), int(self._len.max()), int(self._len.max()))
+        batch.moved = bool((self._moved < self._len).any())
+        return batch
 
     # ---- inside ----
 

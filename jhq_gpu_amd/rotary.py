@@ -143,6 +143,8 @@ class Rotary:
         if type(positions) is _kv.KVBatch:
             if positions._index != self._index:
                 raise ValueError(f"the batch is on cuda:{positions._index}, the rotary on {self.device}")
+            if positions.moved:
+                raise ValueError(_kv._MOVED)
             if positions.n_tokens != n:
                 raise ValueError(f"the batch has {positions.n_tokens} rows, x {n}")
             pp, size, ref = None, 0, positions._ref

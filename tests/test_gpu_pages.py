@@ -424,3 +424,26 @@ def test_compaction_in_a_full_cache(gpu, bits, D, H):
         rows = torch.from_numpy(np.concatenate([a + n for a, n in zip(keep, (0, 600, 933))])).to(gpu)
         for x, y in zip(before, cache.read(pages.everything())):
             assert torch.equal(x[rows], y)
+
+
+def test_moved_tokens_are_not_turned_to_their_places(gpu):
+    """What a compacted sequence holds stands elsewhere than at its positions: write(rotary=) and apply refuse
+    its batches, and nothing is written."""
+    import torch
+    cache = jg.KVCache(9, 16, 1, 64, device=gpu)
+    pages, rope = jg.KVPages(cache, 2, 60), jg.Rotary(64, device=gpu)
+    x = torch.randn(50, 1, 64, generator=torch.Generator().manual_seed(7)).bfloat16().to(gpu)
+    cache.write(x, x, pages.extend([30, 20]), rotary=rope)
+    pages.compact({0: np.arange(4, 30)})
+    b = pages.extend([1, 1])
+    before = cache.data.clone()
+    with pytest.raises(ValueError, match="moved"):
+        cache.write(x[:2], x[:2], b, rotary=rope)
+    with pytest.raises(ValueError, match="moved"):
+        rope.apply(x[:2], b)
+    assert torch.equal(cache.data, before)
+    turned = rope.apply(x[:2], torch.tensor([30, 20], device=gpu))
+    cache.write(turned, x[:2], b)
+    b = pages.extend([0, 1])  # the other sequence's places are its positions
+    cache.write(x[:1], x[:1], b, rotary=rope)
+    assert torch.equal(rope.apply(x[:1], b), rope.apply(x[:1], torch.tensor([21], device=gpu)))

@@ -433,3 +433,32 @@ def test_compaction_with_few_free_pages(seed):
             for s, at in keep.items():
                 model[s] = [model[s][i] for i in at]
         _check(pages, cache, model)
+
+
+def test_batches_say_where_places_are_not_positions():
+    cache, pages = _grown([20, 10, 6, 0])
+    assert not pages.extend([1, 1, 1, 0]).moved and not pages.everything().moved
+    pages.compact({0: np.arange(15), 2: np.arange(7)})  # beginnings: nothing moves
+    assert not pages.extend([1, 1, 1, 0]).moved
+    pages.compact({0: np.r_[0:9, 11:16]})  # token 11 becomes 9
+    assert pages.everything().moved
+    assert not pages.extend([0, 1, 1, 0]).moved  # of sequences without new tokens nothing is turned
+    assert pages.extend([1, 0, 0, 0]).moved
+    pages.fork(0, 3)
+    assert pages.extend([0, 0, 0, 1]).moved
+    pages.truncate(0, 10)
+    assert pages.extend([1, 0, 0, 0]).moved
+    pages.truncate(0, 9)  # the last token that was moved goes
+    assert not pages.extend([1, 0, 0, 0]).moved
+    pages.compact({3: np.arange(5, 16)})
+    pages.compact({3: np.arange(0)})
+    assert not pages.extend([1, 1, 1, 1]).moved
+    # moved once, and compacted again: in front of it, behind it, cut off before it
+    for keep, moved in ((np.r_[0:20, 22:26], True), (np.r_[0:2, 3:26], True), (np.arange(26), True),
+                        (np.arange(11), True), (np.arange(10), False)):
+        cache, pages = _grown([30])
+        pages.compact({0: np.r_[0:10, 14:30]})
+        pages.compact({0: keep})
+        assert pages.extend([1]).moved == moved
+    pages.free(0)
+    assert not pages.extend([3]).moved
