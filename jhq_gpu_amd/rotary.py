@@ -47,6 +47,8 @@ def _scaled(rot_dim, base, scaling):
         if rot_dim == 2:
             raise ValueError("scaling ntk needs rot_dim > 2")
         base = base * f ** (rot_dim / (rot_dim - 2.0))
+        if not math.isfinite(base):
+            raise OverflowError
     w = [base ** (-2.0 * i / rot_dim) for i in pairs]
     if kind == "ntk":
         return w, 1.0
@@ -63,11 +65,14 @@ def _scaled(rot_dim, base, scaling):
     # yarn: the same by a pair's number, between those that turn `fast` and `slow` times
     if base == 1.0:
         raise ValueError("scaling yarn needs a base other than 1")
+    fast, slow = s.get("fast", 32.0), s.get("slow", 1.0)
+    if fast <= slow:
+        raise ValueError(f"scaling fast must be above slow, got {fast} and {slow}")
 
     def place(turns):
         return rot_dim * math.log(s["length"] / (turns * 2 * math.pi)) / (2 * math.log(base))
-    lo = max(math.floor(place(s.get("fast", 32.0))), 0)
-    hi = min(math.ceil(place(s.get("slow", 1.0))), rot_dim - 1)
+    lo = max(math.floor(place(fast)), 0)
+    hi = min(math.ceil(place(slow)), rot_dim - 1)
     mix = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in pairs]
     return ([x * (1.0 - m + m / f) for x, m in zip(w, mix)],
             0.1 * math.log(f) + 1.0 if f > 1.0 else 1.0)
@@ -102,7 +107,10 @@ class Rotary:
         if not (math.isfinite(base) and base > 0):
             raise ValueError(f"base must be positive, got {base}")
         if frequencies is None:
-            freq, amp = _scaled(rot_dim, base, scaling)
+            try:
+                freq, amp = _scaled(rot_dim, base, scaling)
+            except OverflowError:
+                raise ValueError(f"frequencies of base {base} and scaling {scaling} pass float64's range") from None
         else:
             if scaling is not None:
                 raise ValueError("frequencies are given: scaling does not apply")

@@ -122,3 +122,16 @@ def test_write_refuses_a_rotary_of_other_heads():
     assert call(None) == jg.JHQ_EINVAL and "null rotary" in _err()
     assert call(_rot(head_dim=64, rot_dim=64)) == jg.JHQ_EINVAL and "another" in _err()
     assert call(_rot(rot_dim=129)) == jg.JHQ_EINVAL and "rot_dim" in _err()
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(scaling=dict(kind="ntk", factor=1e308)), "range"), (dict(base=1e308, scaling=dict(kind="ntk", factor=100)), "range"),
+    (dict(base=5e-324), "range"), (dict(scaling=dict(kind="yarn", factor=2, length=1e308, fast=1e-10, slow=1e-11)), "range"),
+    (dict(scaling=dict(kind="linear", factor=5e-324)), "finite"), (dict(scaling=dict(kind="bands", factor=5e-324, length=9)), "finite"),
+    (dict(scaling=dict(kind="yarn", factor=2, length=4096, fast=1, slow=32)), "fast must be above slow"),
+    (dict(scaling=dict(kind="yarn", factor=2, length=4096, fast=0.5)), "fast must be above slow"),
+])
+def test_extreme_scalings_are_refused(kw, msg):
+    """As any other argument that is not valid, instead of a frequency of 0 or a ramp the wrong way round."""
+    with pytest.raises(ValueError, match=msg):
+        jg.Rotary(**{**dict(head_dim=64, device="cpu"), **kw})
