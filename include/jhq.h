@@ -503,7 +503,8 @@ int jhq_k_kv_attend(const jhq_kv_params* p, const void* d_cache, const jhq_kv_ba
  * rows, max_kv a prefix.  The sequences in b are as without a prefix: their first kv_len[g] tokens
  * are those of the prefix, and all of their new tokens stand behind them.  What the call computes is
  * jhq_k_kv_attend of b: the bounds choose whether prefixes are read once or by every
- * sequence, or once = 1 has them read once.
+ * sequence, or once = 1 has them read once, where a call can: n_tokens * q_heads below 2^31 / head_dim, and
+ * the bounds' steps of 64 tokens, over all tiles of rows and key heads, below 2^30.
  * Rows that no group has are those of sequences without one.  Where the host's
  * bounds, a sequence or its length contradict a group, its rows may come out as NaN.  There is no
  * window here: behind one, sequences share little. */

@@ -360,7 +360,7 @@ struct Both {
     int waves;      // of a workgroup
     int places;     // workgroups of the launch
     Kept lk, ok;
-    int64_t work;   // bytes, -1: more than 2^50
+    int64_t work;   // bytes, -1: more than 2^50 (of attention as without a prefix)
 };
 
 // Whether a prefix is read once, by estimates of both ways from the call's bounds (the longest prefix
@@ -405,7 +405,7 @@ Both choose_both(const KvCache& c, const KvBatch& lead, const KvBatch& b, int D,
     const int64_t tiles = b.n_tokens * G / tile + lead.n_seq, own_tiles = b.n_tokens * G / own + b.n_seq;
     const __int128 steps = (static_cast<__int128>(lead.n_seq) * (before / tile + 1) * (lead.max_kv / kStep + 8) +
                             static_cast<__int128>(b.n_seq) * (rows / own + 1) * (b.max_kv / kStep + 8)) * c.H;
-    // and the join is one launch
+    // and the join is one launch: all below 2^31 / D
     r.shared = lead.n_seq > 0 && lead.max_kv > 0 && steps < INT32_MAX / 2 && all < join_rows(D) << 23 &&
                (once || worth(c, lead, b, D, G));
     if (!r.shared) {

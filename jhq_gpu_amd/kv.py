@@ -289,7 +289,8 @@ class KVCache:
         their new ones, pages[g] the pages of these (KVPages.prefix finds them).  No window then.
         Sequences that contradict their group may come out as NaN.  The bounds choose whether
         prefixes are read once (from some 35 MB saved on, with single tokens); once=True has them
-        read once."""
+        read once wherever a call can (n_tokens * q_heads below 2^31 / head_dim, and less than 2^30 steps of 64
+        tokens by the bounds): past that every sequence reads them, with the same results."""
         window = _window(window)
         if prefix is not None:
             self._no_window(window)

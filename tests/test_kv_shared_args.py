@@ -74,3 +74,64 @@ def test_workspaces(n_tokens, max_q, rows):
                 assert -1 <= n <= 1 << 50
                 if n < 0:
                     assert "2^50" in _err() or n_tokens > 1 << 30
+
+
+def _work(b, p, once, heads=4, D=128, bits=8, H=2):
+    """Bytes with the prefix and without it, and what the former says."""
+    L, P = jg.lib(), ctypes.byref(jg._KvParams(bits, H, D, 64, 10))
+    n = L.jhq_kv_shared_work_bytes(P, ctypes.byref(b), ctypes.byref(p), once, heads)
+    msg = _err()
+    return n, L.jhq_kv_work_bytes(P, ctypes.byref(b), heads, 0), msg
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_once_ends_where_a_call_does(D):
+    """Read once up to the documented rows and steps; past them it is attention of every sequence, whose
+    workspace it then has."""
+    def call(tokens, max_kv=5000, n_seq=3, heads=4):
+        return _work(_batch(n_tokens=tokens, n_seq=n_seq), _batch(n_tokens=tokens, max_q=tokens, max_kv=max_kv, n_seq=1),
+                     1, heads=heads, D=D)
+    most = (1 << 31) // D // 4
+    n, plain, _ = call(most - 1)
+    # every row has a place of its own in both passes: sums of values, maximum and sum
+    assert n >= 2 * (most - 1) * 4 * (D + 2) * 4 and n > plain
+    n, plain, _ = call(most)
+    assert n == plain
+    # 1000 rows of 2 key heads, 2 query heads each, in tiles of 64 at least: 64 tokens a step
+    n, plain, _ = call(1000, max_kv=1 << 24)
+    assert n > plain
+    n, plain, _ = call(100000, max_kv=1 << 30)
+    assert n == plain
+    n, plain, _ = call(1000, max_kv=0)
+    assert n == plain
+
+
+@pytest.mark.parametrize("n_tokens", [1, 9, 1000, 1 << 19])
+@pytest.mark.parametrize("bits,D,H", [(8, 64, 8), (4, 128, 2), (8, 256, 1)])
+@pytest.mark.parametrize("max_q,G", [(1, 1), (1, 8), (4, 4), (100, 2)])
+def test_workspaces_have_room(n_tokens, bits, D, H, max_q, G):
+    """For every row's place in both passes, for two parts of 16 rows of each workgroup, and for 8 bytes a
+    key head of every tile that the rows can be cut into; no more than a hundred times that of the parts."""
+    b = _batch(n_tokens=n_tokens, max_q=max_q, max_kv=9000, n_seq=5)
+    p = _batch(n_tokens=n_tokens, max_q=min(n_tokens, 5 * max_q), max_kv=5000, n_seq=2)
+    n, plain, _ = _work(b, p, 1, heads=H * G, D=D, bits=bits, H=H)
+    rows = n_tokens * H * G
+    if rows >= (1 << 31) // D:
+        assert n == plain
+        return
+    each = (D + 2) * 4
+    tiles = (n_tokens * G // 128 + 2 + n_tokens * G // 128 + 5) * H * 8
+    parts = 2 * 2 * 256 * 16 * each
+    assert n >= 2 * rows * each + parts + tiles
+    most = (n_tokens * G // 16 + 2 + n_tokens * G // 16 + 5) * H * 8
+    assert n <= 2 * rows * each + 100 * parts + most + 64
+
+
+def test_workspaces_past_2_50_bytes_are_refused():
+    """Attention of every sequence, which keeps every row of the call (2^31 x 64 of 130 floats, 2^50 bytes) for
+    each of its parts: one sequence's few tiles over a context of 2^30 have many."""
+    b = _batch(n_tokens=1 << 31, n_seq=1, max_q=16, max_kv=1 << 30, max_pages=1 << 24)
+    p = _batch(n_tokens=1 << 31, n_seq=1, max_q=16, max_kv=5000)
+    for once in (0, 1):
+        n, plain, msg = _work(b, p, once, heads=64)
+        assert n == plain == -1 and "2^50" in msg
