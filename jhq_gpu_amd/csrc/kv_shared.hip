@@ -194,13 +194,14 @@ __device__ inline int dealt(const Deal& d, int lead, int own) {
 }
 
 // Workgroups of a CU, as the registers allow: heads of 64 in 4 bits 85.0 us with three and 81.5 with four
-// (40 x 2 to 5 tokens behind four prefixes), in 8 bits 39.4 and 46.9 (4 behind 50000), with spills.
+// (40 x 2 to 5 tokens behind four prefixes), which spill 6 registers; in 8 bits, where four spill more,
+// 39.4 and 46.9 (4 behind 50000).  Two of heads of 128 in 8 bits spill one.
 constexpr int both_waves(int bits, int D) { return D == 256 ? 1 : D == 128 ? 2 : bits == 4 ? 4 : 3; }
 
 // Prefixes and what stands behind them in one launch, so that the former, many rows, which vector and matrix
 // instructions bound, run beside the latter, which reading the cache bounds: 64 tokens of 32 heads on 8 of
-// 128 behind 16003, 50 to 1500 of their own, 8 bits: 55 us, and 40 + 33 in two launches; the join 10 more.
-// Of it 2.5 us go by before the first load of codes, 8 to write the parts; a step of 128 rows takes 3.0 us
+// 128 behind 16003, 50 to 1500 of their own, 8 bits: 66.5 us a call, join included, and 80 in two launches
+// (64 now; in a trace, one by one, 62 and 10 the join).  Of it 2.5 us go by before the first load of codes, 8 to write the parts; a step of 128 rows takes 3.0 us
 // with two such workgroups on a CU and 3.3 to 3.8 beside waves that read (VALU 40% of the cycles, matrix
 // cores 17%, waves wait in 49% of theirs).  LEAD: 0 few rows before, else tiles of 64 LEAD.  Tiles of 128
 // rows are turned to float16 half as often, but leave less beside them; us: the case above 64.2 a call and
@@ -271,8 +272,8 @@ __device__ inline Parts parts_of(const Kept& k, const KvSeq& s, int seq, int i, 
 }
 
 // Joins what the passes have of a row; latency and reading the parts bound it.  A thread has 4
-// elements of every Y-th part: 2048 rows of 20 parts of 128 elements 9.9 us with 4, 10.2 with 2, 10.9 with 1,
-// 13.5 with 8.  Fewer rows have more parts each, and a workgroup of its own each; calls with workgroups of
+// elements of every Y-th part: 2048 rows of 20 parts of 128 elements 9.9 us with 4 (9.7 now), 10.2 with 2, 10.9
+// with 1, 13.5 with 8.  Fewer rows have more parts each, and a workgroup of its own each; calls with workgroups of
 // several rows, of one, of one with 512 threads, us (32 heads on 8 of 128, 8 bits): 32 tokens behind 16000
 // (1024 rows) 43.0, 42.4, 46.5; 16 33.2, 31.9, 32.7; 4 behind 50000 45.4, 41.6, 40.4, on heads of 64 36.8,
 // 28.6, 27.9; 4 of 8 heads on 2 behind 100000 56.7, 41.1, 34.7.

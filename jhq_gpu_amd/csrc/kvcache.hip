@@ -291,7 +291,9 @@ __device__ inline void turn8(const Rotary& r, const void* base, int64_t row, int
 // 31.6 us, 3.8 TB/s, from float32 198 MB in 41.0, 4.8; 4 bits, 8 heads of 64, 16384 tokens 3.1 TB/s and
 // 65536 4.1; 64 single tokens 5.1 us.
 // ROT: keys are turned to their positions first, in float32, and not rounded before they are held: 48 single
-// tokens of 4 heads of 256 6.3 us (8.7 with every row of their runs made into codes).
+// tokens of 4 heads of 256 6.5 us (8.7 with every row of their runs made into codes).  Over prompts the angles
+// bound it, which a lane computes for its 8 elements of each token and head: 4096 tokens, 8 heads of
+// 128, 8 bits 14.6 us (9.3 without), 19192 48.1 (30.8), side by side, which has half as many, 38.9.
 template <int BITS, int D, int DT, bool VEC, bool SEARCH, bool ROT>
 __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvCache c, KvBatch b, KvRows kr,
                                                                KvRows vr, int sets, Rotary rot) {
@@ -489,8 +491,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvCache c, KvBatch
     }
 }
 
-// Whole pages, 16 bytes a lane and kCopyDeep of them in flight; HBM-bound: 63 pages of 135 kB in 4.4 us.  A pair that names a page
-// that the cache does not have is left out.
+// Whole pages, 16 bytes a lane and kCopyDeep of them in flight; HBM-bound: 63 pages of 135 kB, 17 MB, in 5.5 us.
+// A pair that names a page that the cache does not have is left out.
 constexpr int kCopyDeep = 4;
 constexpr int kCopyRun = 256 * 16 * kCopyDeep;  // bytes of a workgroup
 
@@ -512,14 +514,15 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(KvCache c, const int
 }
 
 // Tokens as they are held, from any slots (page * page_size + place) of cache f to the batch's new
-// tokens; HBM-bound.  A wave has a run's keys or values in `per` heads: where its tokens lie is the
+// tokens; latency bounds it: of a head at a time, its loads, then its stores, with three quarters of the
+// waves' time spent waiting.  A wave has a run's keys or values in `per` heads: where its tokens lie is the
 // same for each.  Keys move 16 bytes a lane, a piece of a token, to where they lie in order.  Values stand
 // token by token within a group of 16: a lane makes the 16 bytes of an element from its 16 bytes in
 // each of the groups that the tokens come from, kMoveDeep of which are on their way at once (half of
 // the tokens at random: three on average).  A slot that the cache does not have counts as a row that
-// is not finite.  31187 of 62000 tokens at random, 8 heads of 128, 8 bits: 132 MB in 47 us, 2.8 TB/s (half
-// of each line read is another token's: 80 MB for 66); 213600 in runs, 8 of 64, 4 bits, 246 MB in 71,
-// 3.5 TB/s; 700 tokens 6.4.
+// is not finite.  31187 of 62000 tokens at random, 8 heads of 128, 8 bits: 132 MB in 55 us, 2.4 TB/s (47 where
+// calls follow each other; lines of which a part is another token's: 80 MB read for 66, 3 us of a copy);
+// 213600 in runs, 8 of 64, 4 bits, 246 MB in 85, 2.9 TB/s (76); 700 tokens 6.4.
 constexpr int kMoveDeep = 4;
 // Waves that a call is cut into by heads at most: the first of these 51.4 us with 8192, 47.1 with 16384, 49.1
 // with one head each; the second 71.2, 75.7, 74.8.

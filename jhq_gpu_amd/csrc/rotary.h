@@ -23,9 +23,10 @@ Rotary rotary_of(const jhq_rotary& r, bool inverse);
 
 #ifdef __HIPCC__
 // Cosine and sine of pos * turn 2^-64 of a turn.  The product modulo 2^64 is exact whatever the
-// position, which no float product is (2^20 radians have 2^-4 of error in float32): what is left of
-// the error is the frequency's own rounding, |pos| 2^-65 turns.  The upper 32 bits are cut into a
-// quarter and a rest of at most pi / 4, whose sine and cosine are their series up to x^9 and
+// position, which no float product is (2^20 radians have 2^-4 of error in float32): of the position only
+// the frequency's own rounding is left, |pos| 2^-65 turns.  The upper 32 bits (what is cut off is below
+// 2^-32 turns, 2^-29.3 radians) are cut into a quarter and a rest of at most pi / 4, which float32 leaves
+// within 3 2^-24 of itself and whose sine and cosine are their series up to x^9 and
 // x^10 (the next terms are below 2^-27 of the result).
 __device__ inline void turn_of(uint64_t turn, int64_t pos, float& c, float& s) {
     const uint32_t ph = static_cast<uint32_t>(static_cast<uint64_t>(pos) * turn >> 32);

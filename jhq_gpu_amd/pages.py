@@ -284,8 +284,10 @@ class KVPages:
 
     def prefix(self, least=1, stream=None):
         """What attend takes as `prefix` beside the batch that extend returned last: neighbouring
-        sequences whose tables begin with the same pages, least pages of them at the
-        least, all before their new tokens.  None where no two do."""
+        sequences (those that share pages are best given numbers in a row) whose tables begin with the
+        same pages, least pages of them at the least, all before their new tokens.  None where no two
+        do.  Its arrays are new ones, for this step: a captured call would replay those that it was captured
+        with."""
         if not self._fresh:
             raise RuntimeError("sequences have changed since extend")
         P, groups = self.page_size, []

@@ -143,7 +143,8 @@ class Rotary:
         whose new tokens' positions they are (rows that no sequence has keep what out
         had, zero where out is None).  Computed in float32 and rounded once.  out: a tensor
         of x's shape and type, x itself among them; it must not share memory with x
-        otherwise.  inverse turns back: the gradient's pass."""
+        otherwise.  inverse turns back: the gradient's pass, which is the caller's to run, as
+        autograd does not record the call (a result that it allocates requires no gradient)."""
         n, heads, xt, xh = self._rows(x, "x")
         dt = _DTYPES.get(x.dtype)
         if dt is None:
