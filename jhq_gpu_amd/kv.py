@@ -155,6 +155,7 @@ class KVCache:
             _jg._check(rc)
 
     def _enqueue(self, entry, stream, *args):
+        # not called by _call: 0.3 us of a single token's 10
         if self._device() != self._index:
             with _torch().cuda.device(self._index):
                 return self._enqueue(entry, stream, *args)
